@@ -32,6 +32,7 @@ EXPORTS = [
     "dkv_gather_cold", "dkv_refine_rows", "dkv_wire_pack", "dkv_wire_unpack", "dkv_attend_layer_noalloc",
     "dkv_quantize8", "dkv_quantize8_rungs", "dkv_centered_rows", "dkv_matmul_f32_workspace_bytes", "dkv_matmul_f32",
     "dkv_ladder_errors", "dkv_ladder_code", "dkv_rows_to_caches", "dkv_copy_tokens", "dkv_outside_tokens", "dkv_project_caches", "dkv_live_groups",
+    "dkv_page_assign", "dkv_page_trim", "dkv_fp4_store", "dkv_fp4_load",
 ]
 NOALLOC_MAX_BYTES = 64 << 20  # DKV_NOALLOC_MAX_BYTES: the static workspace of dkv_attend_layer_noalloc
 
@@ -74,6 +75,18 @@ class AttendArgs(ctypes.Structure):
     ]
 
 
+class Fp4Cache(ctypes.Structure):
+    """One layer of a paged 4-bit cache (dkv_fp4_cache_t)."""
+    _fields_ = [("key_codes", c_vp), ("key_scales", c_vp), ("value_codes", c_vp), ("value_scales", c_vp),
+                ("pages", c_i32), ("kv_heads", c_i32), ("page", c_i32), ("head_dim", c_i32)]
+
+
+class Pages(ctypes.Structure):
+    """Block tables and free pages of a paged cache (dkv_pages_t)."""
+    _fields_ = [("lengths", c_vp), ("table", c_vp), ("free_pages", c_vp), ("free_count", c_vp), ("state", c_vp),
+                ("requests", c_i32), ("width", c_i32), ("page", c_i32), ("pages", c_i32)]
+
+
 class DkvError(RuntimeError):
     pass
 
@@ -95,6 +108,10 @@ def lib() -> ctypes.CDLL:
                      "dkv_matmul_f32_workspace_bytes"):
             getattr(handle, name).restype = c_sz
         handle.dkv_topk_workspace_bytes.argtypes = [c_i32]
+        handle.dkv_page_assign.argtypes = [c_vp, c_vp, c_i32, c_vp, c_vp, c_vp, c_vp]
+        handle.dkv_page_trim.argtypes = [c_vp, c_vp, c_vp]
+        handle.dkv_fp4_store.argtypes = [c_vp, c_vp, c_vp, c_i32, c_i64, c_i64, c_i64, c_i64, c_vp, c_i32, c_vp]
+        handle.dkv_fp4_load.argtypes = [c_vp, c_vp, c_i32, c_vp, c_vp, c_i32, c_vp]
         if handle.dkv_abi_version() != ABI_VERSION:
             raise RuntimeError(f"{LIB_PATH} has ABI {handle.dkv_abi_version()}, expected {ABI_VERSION}")
         _lib = handle
@@ -521,3 +538,58 @@ def gather_cold(stream: Stream, cold, cold_tok_off, idx, refined_base_off: int, 
     _check(lib().dkv_gather_cold(ctypes.byref(stream), c_vp(ptr(cold)), c_vp(ptr(cold_tok_off)), c_vp(ptr(idx)),
                                  c_i32(k), c_vp(refined_ptr), c_i64(refined_base_off), c_vp(ptr(tok_off)),
                                  c_vp(ptr(pieces)), c_vp(stream_handle())), "dkv_gather_cold")
+
+
+# ----------------------------------------------------------------- paged 4-bit cache
+
+def page_assign(pages: Pages, new, rows: int, slots, positions, cu) -> None:
+    """Pages for ``new`` int32 [requests] more tokens; slots and positions int64 [rows], cu int32 [requests + 1]."""
+    _expect("page_assign", cu.device, (new, "new", torch.int32, (pages.requests,)), (slots, "slots", torch.int64, (rows,)),
+            (positions, "positions", torch.int64, (rows,)), (cu, "cu", torch.int32, (pages.requests + 1,)))
+    with _on_device_of(cu):
+        _check(lib().dkv_page_assign(ctypes.addressof(pages), ptr(new), rows, ptr(slots), ptr(positions), ptr(cu),
+                                     stream_handle()), "dkv_page_assign")
+
+
+def page_trim(pages: Pages, keep) -> None:
+    """Requests cut back to at most ``keep`` int32 [requests] tokens, their other pages free again."""
+    _expect("page_trim", keep.device, (keep, "keep", torch.int32, (pages.requests,)))
+    with _on_device_of(keep):
+        _check(lib().dkv_page_trim(ctypes.addressof(pages), ptr(keep), stream_handle()), "dkv_page_trim")
+
+
+def _fp4_rows(t: torch.Tensor) -> torch.Tensor:
+    """Rows as dkv_fp4_store reads them: any 16-byte strides over contiguous dimensions, else a copy."""
+    unit = 4 if t.dtype == torch.float32 else 8
+    if t.stride(2) != 1 or t.stride(0) % unit or t.stride(1) % unit or t.data_ptr() % 16:
+        return t.contiguous().clone() if t.is_contiguous() else t.contiguous()
+    return t
+
+
+def fp4_store(cache: Fp4Cache, key, value, slots) -> None:
+    """Rows key and value [n, kv_heads, head_dim] (f32, f16 or bf16) into slots int64 [n]; rows whose slot is negative
+    are left out."""
+    n, shape = slots.shape[0], (slots.shape[0], cache.kv_heads, cache.head_dim)
+    code = dtype_code(key.dtype)
+    _expect("fp4_store", slots.device, (slots, "slots", torch.int64, (n,)), (key, "key", key.dtype, shape),
+            (value, "value", key.dtype, shape))
+    if n == 0:
+        return
+    key, value = _fp4_rows(key), _fp4_rows(value)
+    with _on_device_of(slots):
+        _check(lib().dkv_fp4_store(ctypes.addressof(cache), key.data_ptr(), value.data_ptr(), code, key.stride(0),
+                                   key.stride(1), value.stride(0), value.stride(1), ptr(slots), n, stream_handle()),
+               "dkv_fp4_store")
+
+
+def fp4_load(cache: Fp4Cache, slots, key, value) -> None:
+    """The values of slots int64 [n] into key and value [n, kv_heads, head_dim]; zeros where a slot is negative."""
+    n, shape = slots.shape[0], (slots.shape[0], cache.kv_heads, cache.head_dim)
+    code = dtype_code(key.dtype)
+    _expect("fp4_load", slots.device, (slots, "slots", torch.int64, (n,)), (key, "key", key.dtype, shape),
+            (value, "value", key.dtype, shape))
+    if n == 0:
+        return
+    with _on_device_of(slots):
+        _check(lib().dkv_fp4_load(ctypes.addressof(cache), ptr(slots), n, ptr(key), ptr(value), code, stream_handle()),
+               "dkv_fp4_load")

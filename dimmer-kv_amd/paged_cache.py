@@ -1,0 +1,155 @@
+"""A paged KV cache in 4 bits for many requests, attended to as it lies (MI355X HIP path).
+
+Next to the calibrated codecs (kvtc.py, progressive.py), which compress a finished prefill, this cache needs no
+calibration and grows while it serves: every new token's keys and values (RoPE applied) are quantized into pages, 32
+dimensions to a power of two and 4 bits each (4.25 bits a value), and attention reads the pages.  include/dimmerkv.h
+states the values, the pages' form and the tables.
+
+``PagedCache`` holds the pages of every layer, the block tables and the free pages, all on the GPU; no call waits for
+the GPU or reads from it, so a step can be captured in a HIP graph.  A step of a serving loop is
+
+    step = cache.assign(new, rows)                    # pages, slots and positions of the step's tokens
+    cache.store(layer, key, value, step)              # in every layer: the new rows into the pages
+    cache.trim(keep)                                  # finished requests, refused drafts
+
+Calls on one cache share its tables and belong on one stream (or on streams the caller orders).
+"""
+
+from __future__ import annotations
+
+from dataclasses import dataclass
+
+import torch
+
+import dkv_hip
+
+
+@dataclass
+class Step:
+    """The rows of one step: requests one after another, ``cu`` the rows before each, -1 slots behind the last."""
+    slots: torch.Tensor      # int64 [rows]
+    positions: torch.Tensor  # int64 [rows]
+    cu: torch.Tensor         # int32 [requests + 1]
+    rows: int
+    longest: int             # a bound on the requests' lengths, new tokens included: it shapes launches, not results
+    most: int                # the same for the new tokens of a request
+
+
+REFUSED = {1: "more new tokens than rows", 2: "a request passes its row of the block table", 3: "too few free pages"}
+
+
+class PagedCache:
+    def __init__(self, layers: int, kv_heads: int, head_dim: int, pages: int, page: int = 64, requests: int = 1,
+                 table_pages: int | None = None, device="cuda"):
+        """``pages`` pages of ``page`` tokens (a power of two, 16 to 4096) in every layer, shared by ``requests``
+        requests of at most ``table_pages`` pages each (all of them by default)."""
+        table_pages = pages if table_pages is None else table_pages
+        if head_dim not in (64, 128, 256):
+            raise ValueError(f"head_dim {head_dim} is not 64, 128 or 256")
+        if page < 16 or page > 4096 or page & (page - 1):
+            raise ValueError(f"page {page} must be a power of two from 16 to 4096")
+        if layers < 0 or kv_heads < 1 or pages < 1 or table_pages < 1 or not 1 <= requests <= 8192:
+            raise ValueError(f"bad cache: {layers} layers, {kv_heads} KV heads, {pages} pages, {requests} requests of "
+                             f"{table_pages} pages")
+        if table_pages * page >= 1 << 31 or pages * page >= 1 << 40:
+            raise ValueError(f"{table_pages} pages of {page} tokens pass 2^31 tokens a request")
+        if torch.device(device).type != "cuda":
+            raise ValueError("PagedCache needs a GPU (the HIP path has no CPU fallback)")
+        self.layers, self.kv_heads, self.head_dim = layers, kv_heads, head_dim
+        self.pages, self.page, self.requests, self.table_pages = pages, page, requests, table_pages
+
+        def blank(width):
+            return torch.zeros(layers, pages, kv_heads, page * width, dtype=torch.uint8, device=device)
+
+        self.key_codes, self.value_codes = blank(head_dim // 2), blank(head_dim // 2)
+        self.key_scales, self.value_scales = blank(head_dim // 32), blank(head_dim // 32)
+        self.table = torch.full((requests, table_pages), -1, dtype=torch.int32, device=device)
+        self.lengths = torch.zeros(requests, dtype=torch.int32, device=device)
+        self.free = torch.arange(pages - 1, -1, -1, dtype=torch.int32, device=device)
+        self.free_count = torch.full((1,), pages, dtype=torch.int32, device=device)
+        self._state = torch.zeros(3, dtype=torch.int32, device=device)
+        self.device = self.table.device
+        self._pages = dkv_hip.Pages(self.lengths.data_ptr(), self.table.data_ptr(), self.free.data_ptr(),
+                                    self.free_count.data_ptr(), self._state.data_ptr(), requests, table_pages, page, pages)
+        self._layers = [dkv_hip.Fp4Cache(self.key_codes[i].data_ptr(), self.key_scales[i].data_ptr(),
+                                         self.value_codes[i].data_ptr(), self.value_scales[i].data_ptr(), pages,
+                                         kv_heads, page, head_dim) for i in range(layers)]
+
+    # ----- tables -----
+    def _counts(self, counts) -> torch.Tensor:
+        if not torch.is_tensor(counts):
+            counts = dkv_hip.to_device(list(counts), torch.int32, self.device)
+        return counts
+
+    def assign(self, new, rows: int | None = None, longest: int | None = None, most: int | None = None) -> Step:
+        """Pages for ``new`` tokens of each request (int32 [requests] on the GPU, or host numbers) and the slots and
+        positions of the step's ``rows`` rows (needed with a GPU tensor; more than the new tokens for a padded step).
+        ``longest`` and ``most`` bound the lengths and new tokens a request may have; they only shape later launches.
+        If the pages, a table row or the rows do not suffice, nothing is assigned and every slot is -1; ``check``
+        tells."""
+        if not torch.is_tensor(new):
+            new = [int(n) for n in new]
+            rows = sum(max(n, 0) for n in new) if rows is None else rows
+            most = max(0, *new) if most is None else most
+        if rows is None:
+            raise ValueError("assign: a GPU tensor of new tokens needs rows, the step's number of rows")
+        if rows < 0:
+            raise ValueError(f"assign: {rows} rows")
+        places = torch.empty(2, rows, dtype=torch.int64, device=self.device)
+        step = Step(places[0], places[1], torch.empty(self.requests + 1, dtype=torch.int32, device=self.device), rows,
+                    self.table_pages * self.page if longest is None else longest, rows if most is None else most)
+        dkv_hip.page_assign(self._pages, self._counts(new), rows, step.slots, step.positions, step.cu)
+        return step
+
+    def trim(self, keep) -> None:
+        """Cut every request back to at most ``keep`` tokens (int32 [requests] on the GPU, or host numbers; 0 ends a
+        request) and free the pages behind that."""
+        dkv_hip.page_trim(self._pages, self._counts(keep))
+
+    def check(self) -> None:
+        """Wait for the GPU and raise if the last ``assign`` or ``trim`` was refused."""
+        state = self._state.tolist()
+        if state[0]:
+            raise dkv_hip.DkvError(f"assign: {REFUSED.get(state[0], state[0])}; nothing was assigned")
+        if state[2]:
+            raise dkv_hip.DkvError("trim: more pages given back than the cache has (a page in two requests?)")
+
+    def slots(self, request: int, start: int, stop: int) -> torch.Tensor:
+        """Slots int64 of tokens start..stop - 1 that a request holds."""
+        at = torch.arange(start, stop, device=self.device)
+        return self.table[request].long()[at // self.page] * self.page + at % self.page
+
+    # ----- rows -----
+    def _layer(self, layer: int) -> dkv_hip.Fp4Cache:
+        if not 0 <= layer < self.layers:
+            raise ValueError(f"layer {layer} of {self.layers}")
+        return self._layers[layer]
+
+    def _here(self, t: torch.Tensor, what: str) -> None:
+        if t.device != self.device:
+            raise ValueError(f"{what}: tensors must be on {self.device} (got {t.device})")
+
+    def store(self, layer: int, key: torch.Tensor, value: torch.Tensor, step: Step) -> None:
+        """The step's keys and values [rows, kv_heads, head_dim] (float32, float16 or bfloat16, any strides) into the
+        pages of ``layer``; rows without a slot are left out."""
+        self._here(step.slots, "store")
+        dkv_hip.fp4_store(self._layer(layer), key, value, step.slots)
+
+    def load(self, layer: int, slots: torch.Tensor, dtype: torch.dtype = torch.float16):
+        """(keys, values) [n, kv_heads, head_dim] held in ``slots`` (int64 [n]); zeros for negative slots.  Every value
+        is exact in the three types."""
+        self._here(slots, "load")
+        shape = (slots.shape[0], self.kv_heads, self.head_dim)
+        key = torch.empty(shape, dtype=dtype, device=self.device)
+        value = torch.empty_like(key)
+        dkv_hip.fp4_load(self._layer(layer), slots, key, value)
+        return key, value
+
+    def held_bytes(self) -> int:
+        """GPU memory of the pages of all layers, the tables and the free list."""
+        return sum(t.numel() * t.element_size() for t in (
+            self.key_codes, self.key_scales, self.value_codes, self.value_scales, self.table, self.lengths, self.free,
+            self.free_count, self._state))
+
+
+__all__ = ["PagedCache", "Step"]

@@ -422,6 +422,85 @@ int dkv_refine_rows(const dkv_stream_t* s, int32_t n, const uint8_t* cold, const
                     const int32_t* rows, int32_t k, uint8_t* refined, int64_t refined_base_off, int64_t* tok_off,
                     int16_t* pieces, int64_t* owner, int32_t version, int64_t* fetched, void* stream);
 
+/* ---- a paged KV cache in 4 bits --------------------------------------------
+ * No counterpart in the reference: the full cache of many requests, kept in 4
+ * bits, that grows token by token and is attended to as it lies.
+ *
+ * Values: 32 consecutive dimensions of a token and head (a block) share 2^e,
+ * and each is a code times it: sign bit 3, then 0, 0.5, 1, 1.5, 2, 3, 4, 6 for
+ * 0..7.  e = floor(log2 amax) - 2 of the block's largest magnitude, one more if
+ * amax >= 1.75 * 2^floor(log2 amax), clamped to DKV_FP4_EXP_MIN..MAX (so every
+ * value is an fp16 value; larger magnitudes than 49152 become it).  Rounding is
+ * to the nearest code, ties to the even one.  A block that holds an infinity or
+ * a NaN is stored as NaN in all 32.
+ *
+ * Pages: `page` tokens (a power of two, 16..4096) of every KV head.  For page p,
+ * head h, hp = p * kv_heads + h:
+ *   key codes    byte (hp * page + t) * D/2 + i: dimension 2i low, 2i+1 high
+ *   key scales   byte (hp * page + t) * D/32 + block: e + 127, or 255 for NaN
+ *   value codes  hp * page * D/2, then fours of tokens: 16 lanes of D/16
+ *                dimensions, each [token of the four][D/32 bytes]
+ *   value scales hp * page * D/32, then fours of tokens: [block][token]
+ * (a value lane's bytes are one load of the attention's operand).  A slot is
+ * page id * page + token; a negative slot, or one past the pages, is no slot. */
+#define DKV_FP4_EXP_MIN (-22)
+#define DKV_FP4_EXP_MAX 13
+#define DKV_FP4_NAN 255
+
+typedef struct dkv_fp4_cache {  /* one layer; arrays 16-byte aligned */
+  uint8_t* key_codes;     /* [pages][kv_heads][page * head_dim/2] */
+  uint8_t* key_scales;    /* [pages][kv_heads][page * head_dim/32] */
+  uint8_t* value_codes;
+  uint8_t* value_scales;
+  int32_t pages;
+  int32_t kv_heads;
+  int32_t page;
+  int32_t head_dim;       /* 64, 128 or 256 */
+} dkv_fp4_cache_t;
+
+typedef struct dkv_pages {  /* the requests' block tables and the free pages */
+  int32_t* lengths;     /* [requests] tokens held */
+  int32_t* table;       /* [requests][width] page ids; entries past a request's pages are not read */
+  int32_t* free_pages;  /* [pages] a stack of free page ids, the next one at free_count - 1 */
+  int32_t* free_count;  /* [1] */
+  int32_t* state;       /* [3] zero at first: why the last assign was refused, scratch, the last trim's */
+  int32_t requests;     /* at most 8192 */
+  int32_t width;        /* width * page < 2^31 */
+  int32_t page;
+  int32_t pages;        /* ids the free stack has room for */
+} dkv_pages_t;
+
+#define DKV_PAGES_ROWS 1   /* more new tokens than rows */
+#define DKV_PAGES_WIDTH 2  /* a request would pass its table row */
+#define DKV_PAGES_FREE 3   /* too few free pages (assign), or more given back than the stack holds (trim) */
+
+/* Pages for new_tokens [requests] (negative: none) more tokens: free pages into
+ * the table in request order, lengths advanced, and for each of the `rows` rows
+ * (requests one after another) its slot and position, -1 behind the last one;
+ * cu [requests + 1] gets the rows before each request.  If anything does not fit,
+ * nothing changes but the outputs: cu is all 0, every slot -1, state[0] says why.
+ * Calls on one cache are ordered by the caller (they share state). */
+int dkv_page_assign(const dkv_pages_t* p, const int32_t* new_tokens, int32_t rows, int64_t* slots, int64_t* positions,
+                    int32_t* cu, void* stream);
+
+/* Requests cut back to at most keep [requests] tokens (0: a finished request;
+ * negative as 0), the pages behind that returned to the stack in the order that
+ * undoes an assign, their table entries set to -1.  Each page must belong to one
+ * request only. */
+int dkv_page_trim(const dkv_pages_t* p, const int32_t* keep, void* stream);
+
+/* Keys and values (f32, f16 or bf16; one type) of n rows into their slots.  Row t
+ * of head h lies at key + t * key_token + h * key_head elements (strides that are
+ * multiples of 16 bytes, 16-byte aligned rows, dimensions contiguous).  Rows
+ * without a slot are left out; two rows must not share a slot. */
+int dkv_fp4_store(const dkv_fp4_cache_t* c, const void* key, const void* value, int32_t dtype, int64_t key_token,
+                  int64_t key_head, int64_t value_token, int64_t value_head, const int64_t* slots, int32_t n, void* stream);
+
+/* The values of n slots as rows [n][kv_heads][head_dim] of f32, f16 or bf16 (each
+ * exact); rows without a slot become zeros. */
+int dkv_fp4_load(const dkv_fp4_cache_t* c, const int64_t* slots, int32_t n, void* key, void* value, int32_t dtype,
+                 void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,132 @@
+"""The paged 4-bit cache's refusals, before anything is launched (no GPU needed), and its oracle against closed forms."""
+
+from __future__ import annotations
+
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+import dkv_hip
+from oracle import paged_ref
+
+P = 64  # a stand-in for a device pointer: 16-byte aligned and never read here
+
+
+def pages(**change):
+    fields = dict(lengths=P, table=P, free_pages=P, free_count=P, state=P, requests=3, width=4, page=16, pages=12)
+    fields.update(change)
+    return dkv_hip.Pages(**fields)
+
+
+def cache(**change):
+    fields = dict(key_codes=P, key_scales=P, value_codes=P, value_scales=P, pages=4, kv_heads=2, page=16, head_dim=64)
+    fields.update(change)
+    return dkv_hip.Fp4Cache(**fields)
+
+
+def refused(rc, code, words):
+    assert rc == code and words in dkv_hip.lib().dkv_last_error().decode()
+
+
+def assign(p, new=P, rows=4, slots=P, positions=P, cu=P):
+    return dkv_hip.lib().dkv_page_assign(None if p is None else ctypes.addressof(p), new, rows, slots, positions, cu, None)
+
+
+@pytest.mark.parametrize("change,code,words", [
+    (dict(requests=0), -2, "bad shape"), (dict(requests=8193), -2, "at most 8192"), (dict(width=0), -2, "bad shape"),
+    (dict(pages=-1), -2, "bad shape"), (dict(page=8), -2, "power of two"), (dict(page=48), -2, "power of two"),
+    (dict(page=8192), -2, "power of two"), (dict(page=4096, width=1 << 19), -2, "2^31"),
+    (dict(lengths=None), -1, "null"), (dict(table=None), -1, "null"), (dict(free_pages=None), -1, "null"),
+    (dict(free_count=None), -1, "null"), (dict(state=None), -1, "null")])
+def test_page_tables_refused(change, code, words):
+    p = pages(**change)
+    refused(assign(p), code, words)
+    refused(dkv_hip.lib().dkv_page_trim(ctypes.addressof(p), P, None), code, words)
+
+
+def test_page_calls_refused():
+    refused(assign(None), -1, "null pages")
+    refused(assign(pages(), rows=-1), -2, "-1 rows")
+    for name in ("new", "slots", "positions", "cu"):
+        refused(assign(pages(), **{name: None}), -1, "null pointer")
+    refused(dkv_hip.lib().dkv_page_trim(ctypes.addressof(pages()), None, None), -1, "null pointer")
+
+
+def store(c, key=P, value=P, dtype=1, strides=(128, 64, 128, 64), slots=P, n=5):
+    return dkv_hip.lib().dkv_fp4_store(None if c is None else ctypes.addressof(c), key, value, dtype, *strides, slots, n, None)
+
+
+@pytest.mark.parametrize("change,code,words", [
+    (dict(key_codes=None), -1, "null cache"), (dict(value_scales=None), -1, "null cache"), (dict(value_codes=72), -1, "aligned"),
+    (dict(key_scales=65), -1, "aligned"), (dict(head_dim=96), -2, "head_dim"), (dict(head_dim=32), -2, "head_dim"),
+    (dict(pages=0), -2, "bad cache"), (dict(kv_heads=0), -2, "bad cache"), (dict(kv_heads=65536), -2, "bad cache"),
+    (dict(page=24), -2, "bad cache")])
+def test_caches_refused(change, code, words):
+    c = cache(**change)
+    refused(store(c), code, words)
+    refused(dkv_hip.lib().dkv_fp4_load(ctypes.addressof(c), P, 5, P, P, 1, None), code, words)
+
+
+def test_rows_refused():
+    refused(store(None), -1, "null cache")
+    refused(store(cache(), dtype=3), -1, "dtype 3")
+    refused(store(cache(), n=-1), -2, "-1 rows")
+    for name in ("key", "value", "slots"):
+        refused(store(cache(), **{name: None}), -1, "null pointer")
+    refused(store(cache(), key=72), -1, "aligned")
+    refused(store(cache(), strides=(128, 60, 128, 64)), -1, "multiples")
+    refused(store(cache(), dtype=0, strides=(128, 62, 128, 64)), -1, "multiples")
+    assert store(cache(), key=None, n=0) == 0  # nothing to do
+
+
+def test_python_refusals():
+    from paged_cache import PagedCache
+
+    for bad in (dict(head_dim=96), dict(page=24), dict(page=8), dict(pages=0), dict(requests=0), dict(requests=9000),
+                dict(kv_heads=0), dict(table_pages=1 << 26), dict(device="cpu")):
+        kwargs = dict(layers=1, kv_heads=2, head_dim=64, pages=4, page=64, device="cuda") | bad
+        with pytest.raises(ValueError):
+            PagedCache(**kwargs)
+    rows, slots = torch.zeros(3, 2, 64), torch.zeros(3, dtype=torch.int64)
+    for key, value, where in ((rows, rows, slots), (rows.double(), rows.double(), slots), (rows, rows.half(), slots),
+                              (rows[:, :1], rows, slots), (rows, rows, slots.int()), (rows[:2], rows[:2], slots)):
+        with pytest.raises(ValueError):
+            dkv_hip.fp4_store(cache(), key, value, where)
+    with pytest.raises(ValueError):
+        dkv_hip.page_trim(pages(), torch.zeros(3, dtype=torch.int64))
+
+
+def test_oracle_quantize():
+    grid = np.concatenate([paged_ref.GRID, -paged_ref.GRID])
+    for e in (-22, -3, 0, 13):
+        row = np.resize(grid, 32) * 2.0 ** e
+        assert np.array_equal(paged_ref.quantize(row)[2], row)  # the cache's own values stay
+        assert paged_ref.quantize(row)[1].tolist() == [e + 127]
+    rng = np.random.RandomState(0)
+    x = rng.randn(50, 64) * np.exp(rng.randn(50, 1) * 3)
+    codes, scales, values = paged_ref.quantize(x)
+    unit = np.repeat(2.0 ** (scales.astype(float) - 127), 32, axis=-1)
+    # half a step of the largest codes (4 to 6), but for what lies between 6 and 7 units
+    assert (np.abs(values - x) <= unit * 1.0).all() and np.abs(x / unit).max() < 7.0
+    assert (codes >> 3 == np.signbit(x)).all()
+
+
+def test_oracle_attend_against_softmax():
+    rng = np.random.RandomState(1)
+    q, k, v = rng.randn(4, 6, 8), rng.randn(9, 2, 8), rng.randn(9, 2, 8)
+    want = torch.nn.functional.scaled_dot_product_attention(
+        torch.tensor(q).transpose(0, 1), torch.tensor(k).transpose(0, 1).repeat_interleave(3, 0),
+        torch.tensor(v).transpose(0, 1).repeat_interleave(3, 0),
+        attn_mask=torch.ones(4, 9).tril(5).bool(), scale=0.3).transpose(0, 1).numpy()
+    assert np.allclose(paged_ref.attend(q, k, v, 0.3), want, atol=1e-12)
+    assert not paged_ref.attend(q[:1], k[:0], v[:0], 0.3).any()
+
+
+def test_oracle_tables():
+    t = paged_ref.Tables(2, 3, 5, 16)
+    assert t.assign([17, 1], 20)[0] == [0 * 16 + i for i in range(16)] + [16, 32, -1, -1] and t.free == [4, 3]
+    t.trim([16, 1])
+    assert t.free == [4, 3, 1] and t.table == [[0], [2]]
+    assert t.assign([33, 0], 33)[3] == 2 and t.assign([32, 33], 65)[3] == 3 and t.lengths == [16, 1]
