@@ -546,16 +546,17 @@ def page_assign(pages: Pages, new, rows: int, slots, positions, cu) -> None:
     """Pages for ``new`` int32 [requests] more tokens; slots and positions int64 [rows], cu int32 [requests + 1]."""
     _expect("page_assign", cu.device, (new, "new", torch.int32, (pages.requests,)), (slots, "slots", torch.int64, (rows,)),
             (positions, "positions", torch.int64, (rows,)), (cu, "cu", torch.int32, (pages.requests + 1,)))
+    args = ptr(new), rows, ptr(slots), ptr(positions), ptr(cu)
     with _on_device_of(cu):
-        _check(lib().dkv_page_assign(ctypes.addressof(pages), ptr(new), rows, ptr(slots), ptr(positions), ptr(cu),
-                                     stream_handle()), "dkv_page_assign")
+        _check(lib().dkv_page_assign(ctypes.addressof(pages), *args, stream_handle()), "dkv_page_assign")
 
 
 def page_trim(pages: Pages, keep) -> None:
     """Requests cut back to at most ``keep`` int32 [requests] tokens, their other pages free again."""
     _expect("page_trim", keep.device, (keep, "keep", torch.int32, (pages.requests,)))
+    where = ptr(keep)
     with _on_device_of(keep):
-        _check(lib().dkv_page_trim(ctypes.addressof(pages), ptr(keep), stream_handle()), "dkv_page_trim")
+        _check(lib().dkv_page_trim(ctypes.addressof(pages), where, stream_handle()), "dkv_page_trim")
 
 
 def _fp4_rows(t: torch.Tensor) -> torch.Tensor:
@@ -575,10 +576,10 @@ def fp4_store(cache: Fp4Cache, key, value, slots) -> None:
             (value, "value", key.dtype, shape))
     if n == 0:
         return
-    key, value = _fp4_rows(key), _fp4_rows(value)
+    where, key, value = ptr(slots), _fp4_rows(key), _fp4_rows(value)
     with _on_device_of(slots):
         _check(lib().dkv_fp4_store(ctypes.addressof(cache), key.data_ptr(), value.data_ptr(), code, key.stride(0),
-                                   key.stride(1), value.stride(0), value.stride(1), ptr(slots), n, stream_handle()),
+                                   key.stride(1), value.stride(0), value.stride(1), where, n, stream_handle()),
                "dkv_fp4_store")
 
 
@@ -590,6 +591,6 @@ def fp4_load(cache: Fp4Cache, slots, key, value) -> None:
             (value, "value", key.dtype, shape))
     if n == 0:
         return
+    where, keys, values = ptr(slots), ptr(key), ptr(value)
     with _on_device_of(slots):
-        _check(lib().dkv_fp4_load(ctypes.addressof(cache), ptr(slots), n, ptr(key), ptr(value), code, stream_handle()),
-               "dkv_fp4_load")
+        _check(lib().dkv_fp4_load(ctypes.addressof(cache), where, n, keys, values, code, stream_handle()), "dkv_fp4_load")

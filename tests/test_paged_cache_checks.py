@@ -51,7 +51,8 @@ def test_page_calls_refused():
     refused(assign(pages(), rows=-1), -2, "-1 rows")
     for name in ("new", "slots", "positions", "cu"):
         refused(assign(pages(), **{name: None}), -1, "null pointer")
-    refused(dkv_hip.lib().dkv_page_trim(ctypes.addressof(pages()), None, None), -1, "null pointer")
+    p = pages()
+    refused(dkv_hip.lib().dkv_page_trim(ctypes.addressof(p), None, None), -1, "null pointer")
 
 
 def store(c, key=P, value=P, dtype=1, strides=(128, 64, 128, 64), slots=P, n=5):
@@ -94,8 +95,9 @@ def test_python_refusals():
                               (rows[:, :1], rows, slots), (rows, rows, slots.int()), (rows[:2], rows[:2], slots)):
         with pytest.raises(ValueError):
             dkv_hip.fp4_store(cache(), key, value, where)
-    with pytest.raises(ValueError):
-        dkv_hip.page_trim(pages(), torch.zeros(3, dtype=torch.int64))
+    for keep in (torch.zeros(3, dtype=torch.int64), torch.zeros(2, dtype=torch.int32), torch.zeros(3, dtype=torch.int32)):
+        with pytest.raises(ValueError):
+            dkv_hip.page_trim(pages(), keep)
 
 
 def test_oracle_quantize():
