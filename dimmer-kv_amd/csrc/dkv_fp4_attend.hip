@@ -1,0 +1,558 @@
+// Attention over the paged 4-bit cache (include/dimmerkv.h states the cache): softmax(scaling * q k^T) v for the newest
+// tokens of many requests, causal, optionally within a sliding window, query heads sharing KV heads.
+//
+// One pass over the pages with the running maximum and sum of a softmax.  The rows of a workgroup are query heads that
+// share a KV head, times consecutive tokens; its four waves take chunks of tokens in turn and join at the end, so nothing
+// is shared between them on the way: no barrier, no staging.  Codes become matrix operands in registers, one conversion
+// for two values:
+//   scores^T = K q^T: operand A is 16 tokens x 32 dimensions, a lane's part of a row being 16 consecutive bytes (D = 128)
+//     of one block, so one load and one exponent; the dimensions' order in the products is the queries' own.
+//   out^T = V^T p^T: the scores leave the first product with a lane holding tokens 4g..4g+3 of its query row, which is
+//     what operand B of the second wants if V's lanes take the same tokens: the weights never change lanes, and the
+//     pages keep values in fours of tokens so that a lane's share is one load.
+// K is exact in bfloat16 and float16 alike, V in float16 (the exponents are clamped for that).  Queries go in as they are
+// (float32 as three bfloat16 pieces that add up to it).  The weights are rounded to float16, 2^-12 relative and shifted by
+// 2^15 so that weights down to 2^-29 of the largest keep that: an eighth of the rounding of a bfloat16 result; float32
+// results take a second piece.  Sums, maxima and accumulators are float32.
+#include <math.h>
+
+#include "dkv_device.h"
+#include "dkv_fp4.h"
+#include "dkv_host.h"
+
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+
+constexpr int kWaves = 4;
+constexpr float kWeightShift = 15.0f;  // weights are held times 2^15
+
+struct AttendArgs {
+  dkv_fp4_cache_t c;
+  const int32_t* table;
+  const int32_t* lengths;
+  const int32_t* cu;
+  const void* query;
+  void* out;
+  float* part;      // [rows * q_heads][splits][D] sums when the tokens are split over workgroups
+  float2* part_ml;  // [rows * q_heads][splits] maximum and sum
+  int64_t query_token, query_head;
+  int requests, width, shift, rows, groups, window, splits, fill;
+  float scale;  // |scaling| * log2 e
+  int negate;   // scaling < 0: the queries change sign
+};
+
+template <typename T>
+struct Operand;  // what a query type's products are made of
+template <>
+struct Operand<half_t> {
+  typedef half8 frag;
+  static constexpr int kPieces = 1;
+  static DKV_DEVICE half2_t pair(uint32_t word, float scale, int sel) {
+    switch (sel) {
+      case 0: return __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word, scale, 0);
+      case 1: return __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word, scale, 1);
+      case 2: return __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word, scale, 2);
+      default: return __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word, scale, 3);
+    }
+  }
+  static DKV_DEVICE floatx4 mfma(frag a, frag b, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+template <>
+struct Operand<dkv_bf16> {
+  typedef bf16x8 frag;
+  static constexpr int kPieces = 1;
+  static DKV_DEVICE bf16x2 pair(uint32_t word, float scale, int sel) {
+    switch (sel) {
+      case 0: return __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 0);
+      case 1: return __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 1);
+      case 2: return __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 2);
+      default: return __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, 3);
+    }
+  }
+  static DKV_DEVICE floatx4 mfma(frag a, frag b, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+template <>
+struct Operand<float> : Operand<dkv_bf16> {
+  static constexpr int kPieces = 3;
+};
+
+// 8 query values into kPieces operands.
+DKV_DEVICE void query_pieces(const half_t* p, bool negate, half8 (&out)[1]) {
+  out[0] = *(const half8*)p;
+  if (negate) out[0] = -out[0];
+}
+DKV_DEVICE void query_pieces(const dkv_bf16* p, bool negate, bf16x8 (&out)[1]) {
+  uint4 w = *(const uint4*)p;
+  if (negate) { w.x ^= 0x80008000u; w.y ^= 0x80008000u; w.z ^= 0x80008000u; w.w ^= 0x80008000u; }
+  __builtin_memcpy(&out[0], &w, 16);
+}
+DKV_DEVICE void query_pieces(const float* p, bool negate, bf16x8 (&out)[3]) {
+  // upper halves of the value, of what they leave, and the rest: 8 bits each of the 24
+  uint32_t words[3][4] = {};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float x = p[i];
+    if (negate) x = -x;
+    const uint32_t a = __float_as_uint(x) & 0xffff0000u;
+    const float left = x - __uint_as_float(a);
+    const uint32_t b = __float_as_uint(left) & 0xffff0000u;
+    const uint32_t c = __float_as_uint(left - __uint_as_float(b));
+    const bool finite = (a & 0x7f800000u) != 0x7f800000u;  // an infinity or NaN is one piece
+    words[0][i >> 1] |= (a >> 16 | (finite || !(__float_as_uint(x) & 0x7fffffu) ? 0u : 0x40u)) << (16 * (i & 1));
+    words[1][i >> 1] |= (finite ? b >> 16 : 0u) << (16 * (i & 1));
+    words[2][i >> 1] |= (finite ? c >> 16 : 0u) << (16 * (i & 1));
+  }
+#pragma unroll
+  for (int k = 0; k < 3; ++k) __builtin_memcpy(&out[k], words[k], 16);
+}
+
+DKV_DEVICE float exponent(uint32_t byte) { return __uint_as_float(byte << 23); }
+
+// The codes and exponents of one chunk in this lane: CH tiles of 16 tokens.
+template <int D, int CH>
+struct Chunk {
+  static constexpr int kWords = D / 32;
+  uint32_t k[CH][kWords], ks[CH], v[CH][kWords], vs[CH];
+  bool valid[CH];  // the same in every lane
+  bool whole;
+};
+
+template <int N>
+DKV_DEVICE void load_words(const uint8_t* p, uint32_t (&w)[N]) {
+  if constexpr (N == 2) {
+    const uint2 x = *(const uint2*)p;
+    w[0] = x.x; w[1] = x.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const uint4 x = ((const uint4*)p)[i / 4];
+      w[i] = x.x; w[i + 1] = x.y; w[i + 2] = x.z; w[i + 3] = x.w;
+    }
+  }
+}
+
+template <int D, int CH>
+DKV_DEVICE void load_chunk(const AttendArgs& a, const int32_t* row, int len, int h, int chunk, Chunk<D, CH>& c) {
+  const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+  const int page = a.c.page;
+  c.whole = true;
+#pragma unroll
+  for (int t = 0; t < CH; ++t) {
+    const int token = (chunk * CH + t) * 16;
+    int id = token < len ? row[token >> a.shift] : -1;
+    c.valid[t] = (uint32_t)id < (uint32_t)a.c.pages;  // entries that are no page are read as none
+    c.whole = c.whole && c.valid[t];
+    id = c.valid[t] ? id : 0;
+    const long first = ((long)id * a.c.kv_heads + h) * page + (token & (page - 1));  // token of the arrays
+    load_words(a.c.key_codes + (first + i) * (D / 2) + g * (D / 8), c.k[t]);
+    const uint8_t* ks = a.c.key_scales + (first + i) * (D / 32);
+    if constexpr (D == 64) c.ks[t] = ks[g >> 1];
+    else if constexpr (D == 128) c.ks[t] = ks[g];
+    else c.ks[t] = *(const uint16_t*)(ks + 2 * g);
+    load_words(a.c.value_codes + (first / 4 + g) * (2 * D) + i * (D / 8), c.v[t]);
+    c.vs[t] = *(const uint32_t*)(a.c.value_scales + (first / 4 + g) * (D / 8) + (i * (D / 16) / 32) * 4);
+  }
+}
+
+template <int D, typename T, int NT, int CH>
+__global__ __launch_bounds__(kWaves * 64, NT == 1 ? 2 : 1) void fp4_attend_kernel(AttendArgs a) {
+  using Op = Operand<T>;
+  using frag = typename Op::frag;
+  constexpr int kRows = 16 * NT, kSteps = D / 32, kLane = D / 16, kPieces = Op::kPieces;
+  constexpr int kWeights = kPieces == 1 ? 1 : 2;  // float16 pieces of a weight
+  constexpr int kStride = D + 4;                  // a row of sums in LDS
+  __shared__ float sums[kWaves * 16 * kStride];
+  __shared__ float stat[2][kWaves][kRows];
+
+  const int h = blockIdx.x, b = blockIdx.z, split = blockIdx.y % a.splits, blocks = gridDim.y / a.splits;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+  const int q_heads = a.c.kv_heads * a.groups;
+  const int q0 = min(max(a.cu[b], 0), a.rows), q1 = min(max(a.cu[b + 1], q0), a.rows);
+  const int n_rows = (q1 - q0) * a.groups;
+  const int len = min(max(a.lengths[b], 0), a.width << a.shift);
+  const int32_t* table = a.table + (long)b * a.width;
+  const int first_position = len - (q1 - q0);  // of the request's first query token; below 0 it sees nothing
+
+  if (a.fill && b == 0 && blockIdx.y == 0) {  // rows behind the last request
+    T* out = (T*)a.out;
+    const int end = min(max(a.cu[a.requests], 0), a.rows);
+    const long n = (long)(a.rows - end) * a.groups * D;
+    for (long x = threadIdx.x; x < n; x += kWaves * 64)
+      __builtin_memset(out + ((end + x / (a.groups * D)) * q_heads + h * a.groups) * D + x % (a.groups * D), 0, sizeof(T));
+  }
+
+  for (int block = blockIdx.y / a.splits; block * (long)kRows < n_rows; block += blocks) {
+    const int row0 = block * kRows, row1 = min(row0 + kRows, n_rows);
+    // queries: operand B, lane i a row, 8 dimensions of g * D/4 + 8 * step
+    frag q[NT][kSteps][kPieces];
+    int position[NT], before[NT];  // the last token a row sees, and the one before the first
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int r = row0 + nt * 16 + i;
+      const int token = r / a.groups;
+      position[nt] = r < n_rows ? first_position + token : -1;
+      before[nt] = (int)max((long)position[nt] - a.window, -1L);
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        if (r < n_rows) {
+          const T* p = (const T*)a.query + (q0 + token) * a.query_token + (h * a.groups + r - token * a.groups) * a.query_head;
+          query_pieces(p + g * (D / 4) + s * 8, a.negate, q[nt][s]);
+        } else {
+          __builtin_memset(q[nt][s], 0, sizeof(q[nt][s]));
+        }
+      }
+    }
+    const int low_position = first_position + row0 / a.groups, high_position = first_position + (row1 - 1) / a.groups;
+    const int begin = (int)max((long)low_position - a.window + 1, 0L), end = high_position + 1;  // tokens some row sees
+    const int all_from = (int)max((long)high_position - a.window + 1, 0L);                       // and all rows, from here
+    const int chunk_begin = begin / (16 * CH), chunk_end = max((end + 16 * CH - 1) / (16 * CH), chunk_begin);
+    const long chunks = end > begin ? chunk_end - chunk_begin : 0;
+    const int c0 = chunk_begin + (int)(chunks * split / a.splits), c1 = chunk_begin + (int)(chunks * (split + 1) / a.splits);
+
+    floatx4 o[NT][kLane];
+    float m[NT], l[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      m[nt] = -INFINITY;
+      l[nt] = 0.0f;
+#pragma unroll
+      for (int j = 0; j < kLane; ++j) o[nt][j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+
+    Chunk<D, CH> now, next;
+    int chunk = __builtin_amdgcn_readfirstlane(c0 + wave);
+    if (chunk < c1) load_chunk<D, CH>(a, table, len, h, chunk, now);
+    for (; chunk < c1; chunk += kWaves) {
+      if (chunk + kWaves < c1) load_chunk<D, CH>(a, table, len, h, chunk + kWaves, next);
+
+      // scores^T: lane i a row, tokens 4g..4g+3 of each tile
+      floatx4 s[NT][CH];
+#pragma unroll
+      for (int t = 0; t < CH; ++t) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) s[nt][t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int st = 0; st < kSteps; ++st) {
+          const float e = exponent(D == 256 ? (st < 4 ? now.ks[t] & 255 : now.ks[t] >> 8) : now.ks[t]);
+          frag key;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const auto two = Op::pair(now.k[t][st], e, x);
+            key[2 * x] = two[0];
+            key[2 * x + 1] = two[1];
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int p = kPieces - 1; p >= 0; --p) s[nt][t] = Op::mfma(key, q[nt][st][p], s[nt][t]);
+        }
+      }
+
+      const int base = chunk * CH * 16;
+      const bool masked = !now.whole || base + CH * 16 > low_position + 1 || base < all_from;
+      if (masked) {
+#pragma unroll
+        for (int t = 0; t < CH; ++t) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int token = base + t * 16 + g * 4 + r;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              if (!now.valid[t] || token > position[nt] || token <= before[nt]) s[nt][t][r] = -INFINITY;
+            // what lies behind the request is stale: its values become zeros
+            if (!now.valid[t] || token >= len) now.vs[t] &= ~(255u << (8 * r));
+          }
+        }
+      }
+
+      half8 w[NT][CH / 2][kWeights];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < CH; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) top = fmaxf(top, s[nt][t][r]);
+        top = max_xor32(max_xor16(top));
+        const float higher = fmaxf(m[nt], top * a.scale);
+        if (__any(higher > m[nt])) {
+          const float factor = __builtin_amdgcn_exp2f(m[nt] - (higher == -INFINITY ? 0.0f : higher));
+          l[nt] *= factor;
+#pragma unroll
+          for (int j = 0; j < kLane; ++j) o[nt][j] *= factor;
+          m[nt] = higher;
+        }
+        const float shift = kWeightShift - (m[nt] == -INFINITY ? 0.0f : m[nt]);
+#pragma unroll
+        for (int t = 0; t < CH; ++t) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float p = __builtin_amdgcn_exp2f(fmaf(s[nt][t][r], a.scale, shift));
+            l[nt] += p;
+            w[nt][t / 2][0][(t & 1) * 4 + r] = (half_t)p;
+            if constexpr (kWeights == 2) w[nt][t / 2][1][(t & 1) * 4 + r] = (half_t)(p - (float)(half_t)p);
+          }
+        }
+      }
+
+      if (masked) {
+        // A block of NaN belongs to the rows that see its token, and a product would give it (0 * NaN) to all: where a
+        // chunk has rows that do not see all of it, such blocks become zeros and the rows that see them NaN by hand.
+#pragma unroll
+        for (int u = 0; u < CH / 2; ++u) {
+          uint32_t bad[2];
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            uint32_t& vs = now.vs[2 * u + x];
+            bad[x] = ((vs & 0x7f7f7f7fu) + 0x01010101u) & vs & 0x80808080u;  // the bytes that are 255
+            vs &= ~((bad[x] >> 7) * 255u);
+          }
+          if (__any((bad[0] | bad[1]) != 0)) {
+            half8 is_bad;
+#pragma unroll
+            for (int x = 0; x < 8; ++x) is_bad[x] = (bad[x >> 2] >> (8 * (x & 3) + 7)) & 1 ? (half_t)1.0f : (half_t)0.0f;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              half8 sees;
+#pragma unroll
+              for (int x = 0; x < 8; ++x) {
+                const int token = base + (2 * u + (x >> 2)) * 16 + g * 4 + (x & 3);
+                sees[x] = token <= position[nt] && token > before[nt] ? (half_t)1.0f : (half_t)0.0f;
+              }
+              const floatx4 hit = __builtin_amdgcn_mfma_f32_16x16x32_f16(is_bad, sees, floatx4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+#pragma unroll
+              for (int j = 0; j < kLane; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                  if (hit[r] > 0.0f) o[nt][j][r] = __builtin_nanf("");
+            }
+          }
+        }
+      }
+
+      // out^T: operand A is 16 lanes' dimensions i * kLane + j over the 32 tokens of two tiles
+#pragma unroll
+      for (int u = 0; u < CH / 2; ++u) {
+        float e[8];
+#pragma unroll
+        for (int x = 0; x < 8; ++x) e[x] = exponent((now.vs[2 * u + (x >> 2)] >> (8 * (x & 3))) & 255);
+#pragma unroll
+        for (int j = 0; j < kLane; j += 2) {
+          half8 even, odd;
+#pragma unroll
+          for (int x = 0; x < 8; ++x) {
+            const int byte = (x & 3) * (D / 32) + j / 2;
+            const half2_t two = Operand<half_t>::pair(now.v[2 * u + (x >> 2)][byte / 4], e[x], byte % 4);
+            even[x] = two[0];
+            odd[x] = two[1];
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int p = kWeights - 1; p >= 0; --p) {
+              o[nt][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, w[nt][u][p], o[nt][j], 0, 0, 0);
+              o[nt][j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, w[nt][u][p], o[nt][j + 1], 0, 0, 0);
+            }
+        }
+      }
+      now = next;
+    }
+
+    // the four waves' sums, 16 rows at a time
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const float total = sum_xor32(sum_xor16(l[nt]));
+      if (g == 0) {
+        stat[0][wave][nt * 16 + i] = m[nt];
+        stat[1][wave][nt * 16 + i] = total;
+      }
+    }
+    __syncthreads();
+    const int row = threadIdx.x >> 4, part = threadIdx.x & 15;  // in the join: a row, and kLane of its dimensions
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int x = 0; x < kWaves; ++x) top = fmaxf(top, stat[0][x][nt * 16 + i]);
+      const float factor = m[nt] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[nt] - top);
+      float* mine = sums + (wave * 16 + i) * kStride + g * (D / 4);
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int j = 0; j < kLane; ++j) mine[r * kLane + j] = o[nt][j][r] * factor;
+      __syncthreads();
+      const int r = row0 + nt * 16 + row;
+      if (r < n_rows) {
+        float highest = -INFINITY, total = 0.0f, acc[kLane] = {};
+#pragma unroll
+        for (int x = 0; x < kWaves; ++x) highest = fmaxf(highest, stat[0][x][nt * 16 + row]);
+#pragma unroll
+        for (int x = 0; x < kWaves; ++x) {
+          const float mx = stat[0][x][nt * 16 + row];
+          total += mx == -INFINITY ? 0.0f : stat[1][x][nt * 16 + row] * __builtin_amdgcn_exp2f(mx - highest);
+#pragma unroll
+          for (int j = 0; j < kLane; ++j) acc[j] += sums[(x * 16 + row) * kStride + part * kLane + j];
+        }
+        const int token = r / a.groups;
+        const long out_row = (long)(q0 + token) * q_heads + h * a.groups + (r - token * a.groups);
+        if (a.splits == 1) {
+          T* out = (T*)a.out + out_row * D + part * kLane;
+          const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+          for (int j = 0; j < kLane; ++j) {
+            const float v = total == 0.0f ? 0.0f : acc[j] * inverse;
+            if constexpr (sizeof(T) == 4) out[j] = v;
+            else if constexpr (kPieces == 1 && __is_same(T, half_t)) out[j] = (half_t)v;
+            else out[j].bits = float_to_bf16_bits(v);
+          }
+        } else {
+          float* out = a.part + (out_row * a.splits + split) * D + part * kLane;
+#pragma unroll
+          for (int j = 0; j < kLane; ++j) out[j] = acc[j];
+          if (part == 0) a.part_ml[out_row * a.splits + split] = make_float2(highest, total);
+        }
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// The splits of a row joined: a wave per row, D / 64 dimensions a lane.
+template <int D, typename T>
+__global__ __launch_bounds__(256) void fp4_join_kernel(AttendArgs a, int q_heads) {
+  constexpr int kLane = D / 64;
+  const int lane = threadIdx.x & 63;
+  const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= (long)min(max(a.cu[a.requests], 0), a.rows) * q_heads) return;
+  const float2* ml = a.part_ml + row * a.splits;
+  float top = -INFINITY;
+  for (int s = lane; s < a.splits; s += 64) top = fmaxf(top, ml[s].x);
+  top = wave_max(top);
+  float acc[kLane] = {}, total = 0.0f;
+  for (int s = 0; s < a.splits; ++s) {
+    const float2 x = ml[s];
+    if (x.x == -INFINITY) continue;  // nothing seen there
+    const float factor = __builtin_amdgcn_exp2f(x.x - top);
+    total += x.y * factor;
+    const float* p = a.part + (row * a.splits + s) * D + lane * kLane;
+#pragma unroll
+    for (int j = 0; j < kLane; ++j) acc[j] += p[j] * factor;
+  }
+  T* out = (T*)a.out + row * D + lane * kLane;
+#pragma unroll
+  for (int j = 0; j < kLane; ++j) {
+    const float v = total == 0.0f ? 0.0f : acc[j] / total;
+    if constexpr (sizeof(T) == 4) out[j] = v;
+    else if constexpr (__is_same(T, half_t)) out[j] = (half_t)v;
+    else out[j].bits = float_to_bf16_bits(v);
+  }
+}
+
+struct Plan {
+  int tiles;   // 16-row tiles a workgroup takes
+  int blocks;  // row blocks a request is given
+  int splits;
+};
+
+Plan plan_of(const dkv_fp4_attend_args_t& p) {
+  Plan plan;
+  const long groups = p.q_heads / p.cache.kv_heads, rows = (long)(p.most < 1 ? 1 : p.most) * groups;
+  const bool narrow = p.query_dtype == DKV_F32 || p.cache.head_dim == 256;
+  plan.tiles = rows <= 16 || (p.query_dtype == DKV_F32 && p.cache.head_dim == 256) ? 1 : rows <= 32 || narrow ? 2 : 4;
+  const long blocks = (rows + plan.tiles * 16 - 1) / (plan.tiles * 16);
+  plan.blocks = (int)(blocks < 4096 ? blocks : 4096);
+  const long groups_of_work = (long)p.requests * p.cache.kv_heads * plan.blocks, longest = p.longest < 1 ? 1 : p.longest;
+  const long wanted = (512 + groups_of_work - 1) / groups_of_work, most = (longest + 255) / 256;
+  plan.splits = (int)(wanted < most ? wanted : most);
+  if (plan.splits > 256) plan.splits = 256;
+  while ((long)plan.blocks * plan.splits > 65535) plan.blocks /= 2;
+  return plan;
+}
+
+int check_attend(const dkv_fp4_attend_args_t* p, const char* what) {
+  DKV_REQUIRE(p, DKV_EINVAL, "%s: null arguments", what);
+  const int rc = dkv::check_fp4_cache(&p->cache, what);
+  if (rc) return rc;
+  DKV_REQUIRE(p->query_dtype == DKV_F32 || p->query_dtype == DKV_F16 || p->query_dtype == DKV_BF16, DKV_EINVAL,
+              "%s: query dtype %d not supported", what, p->query_dtype);
+  DKV_REQUIRE(p->requests > 0 && p->requests <= 8192 && p->width > 0 && (int64_t)p->width * p->cache.page < (1L << 31) && p->rows >= 0,
+              DKV_ESHAPE, "%s: bad shape (requests=%d width=%d rows=%d)", what, p->requests, p->width, p->rows);
+  DKV_REQUIRE(p->q_heads > 0 && p->q_heads % p->cache.kv_heads == 0, DKV_ESHAPE,
+              "%s: %d query heads over %d KV heads", what, p->q_heads, p->cache.kv_heads);
+  DKV_REQUIRE((int64_t)p->rows * p->q_heads < (1L << 31) - 65536, DKV_ESHAPE, "%s: %d rows of %d heads pass 2^31", what, p->rows, p->q_heads);
+  DKV_REQUIRE(p->window >= 0, DKV_ESHAPE, "%s: window %d", what, p->window);
+  return DKV_OK;
+}
+
+size_t part_bytes(const dkv_fp4_attend_args_t& p, const Plan& plan) {
+  if (plan.splits == 1) return 0;
+  return (size_t)p.rows * p.q_heads * plan.splits * (p.cache.head_dim * sizeof(float) + sizeof(float2));
+}
+
+template <int D, typename T>
+void launch(const AttendArgs& a, const Plan& plan, int q_heads, hipStream_t st) {
+  const dim3 grid(a.c.kv_heads, plan.blocks * plan.splits, a.requests), block(kWaves * 64);
+  constexpr bool wide = D < 256 && sizeof(T) == 2;
+  if (plan.tiles == 1) {
+    hipLaunchKernelGGL((fp4_attend_kernel<D, T, 1, D == 256 ? 2 : 4>), grid, block, 0, st, a);
+  } else if (plan.tiles == 2) {
+    if constexpr (D < 256 || sizeof(T) == 2) hipLaunchKernelGGL((fp4_attend_kernel<D, T, 2, 2>), grid, block, 0, st, a);
+  } else {
+    if constexpr (wide) hipLaunchKernelGGL((fp4_attend_kernel<D, T, 4, 2>), grid, block, 0, st, a);
+  }
+  if (plan.splits > 1) {
+    const long rows = (long)a.rows * q_heads;
+    hipLaunchKernelGGL((fp4_join_kernel<D, T>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a, q_heads);
+  }
+}
+
+template <int D>
+void launch_type(const AttendArgs& a, const Plan& plan, int q_heads, int dtype, hipStream_t st) {
+  if (dtype == DKV_F32) launch<D, float>(a, plan, q_heads, st);
+  else if (dtype == DKV_F16) launch<D, half_t>(a, plan, q_heads, st);
+  else launch<D, dkv_bf16>(a, plan, q_heads, st);
+}
+
+}  // namespace
+
+extern "C" size_t dkv_fp4_attend_workspace_bytes(const dkv_fp4_attend_args_t* p) {
+  if (check_attend(p, "dkv_fp4_attend_workspace_bytes")) return 0;
+  return part_bytes(*p, plan_of(*p)) + 16;
+}
+
+extern "C" int dkv_fp4_attend(const dkv_fp4_attend_args_t* p, void* workspace, size_t workspace_bytes, void* stream) {
+  const int rc = check_attend(p, "dkv_fp4_attend");
+  if (rc) return rc;
+  if (p->rows == 0) return DKV_OK;
+  DKV_REQUIRE(p->table && p->lengths && p->cu && p->query && p->out, DKV_EINVAL, "dkv_fp4_attend: null pointer");
+  const int unit = p->query_dtype == DKV_F32 ? 4 : 8;
+  DKV_REQUIRE((((uintptr_t)p->query | (uintptr_t)p->out) & 15) == 0 && p->query_token % unit == 0 && p->query_head % unit == 0,
+              DKV_EINVAL, "dkv_fp4_attend: query rows and out must be 16-byte aligned");
+  const Plan plan = plan_of(*p);
+  const size_t need = part_bytes(*p, plan);
+  DKV_REQUIRE(need == 0 || workspace, DKV_EINVAL, "dkv_fp4_attend: null workspace");
+  DKV_REQUIRE(need <= workspace_bytes, DKV_EWORKSPACE, "dkv_fp4_attend: workspace %zu < %zu bytes", workspace_bytes, need);
+  DKV_REQUIRE(((uintptr_t)workspace & 15) == 0, DKV_EINVAL, "dkv_fp4_attend: workspace must be 16-byte aligned");
+  AttendArgs a{};
+  a.c = p->cache;
+  a.table = p->table; a.lengths = p->lengths; a.cu = p->cu; a.query = p->query; a.out = p->out;
+  a.part = (float*)workspace;
+  a.part_ml = (float2*)(a.part + (size_t)p->rows * p->q_heads * plan.splits * p->cache.head_dim);
+  a.query_token = p->query_token; a.query_head = p->query_head;
+  a.requests = p->requests; a.width = p->width; a.shift = dkv::page_shift(p->cache.page); a.rows = p->rows;
+  a.groups = p->q_heads / p->cache.kv_heads;
+  a.window = p->window ? p->window : INT32_MAX;
+  a.splits = plan.splits; a.fill = p->fill;
+  // a positive factor keeps the order of the scores; one of 0 weighs every token the same, as the smallest does
+  a.scale = fmaxf(fabsf(p->scaling) * 1.44269504088896340736f, 1.1754944e-38f);
+  if (p->scaling != p->scaling) a.scale = p->scaling;
+  a.negate = p->scaling < 0.0f;
+  hipStream_t st = dkv::as_stream(stream);
+  if (a.c.head_dim == 64) launch_type<64>(a, plan, p->q_heads, p->query_dtype, st);
+  else if (a.c.head_dim == 128) launch_type<128>(a, plan, p->q_heads, p->query_dtype, st);
+  else launch_type<256>(a, plan, p->q_heads, p->query_dtype, st);
+  return dkv::check_launch("dkv_fp4_attend");
+}

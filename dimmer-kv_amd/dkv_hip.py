@@ -33,6 +33,7 @@ EXPORTS = [
     "dkv_quantize8", "dkv_quantize8_rungs", "dkv_centered_rows", "dkv_matmul_f32_workspace_bytes", "dkv_matmul_f32",
     "dkv_ladder_errors", "dkv_ladder_code", "dkv_rows_to_caches", "dkv_copy_tokens", "dkv_outside_tokens", "dkv_project_caches", "dkv_live_groups",
     "dkv_page_assign", "dkv_page_trim", "dkv_fp4_store", "dkv_fp4_load",
+    "dkv_fp4_attend_workspace_bytes", "dkv_fp4_attend",
 ]
 NOALLOC_MAX_BYTES = 64 << 20  # DKV_NOALLOC_MAX_BYTES: the static workspace of dkv_attend_layer_noalloc
 
@@ -87,6 +88,14 @@ class Pages(ctypes.Structure):
                 ("requests", c_i32), ("width", c_i32), ("page", c_i32), ("pages", c_i32)]
 
 
+class Fp4AttendArgs(ctypes.Structure):
+    """dkv_fp4_attend_args_t."""
+    _fields_ = [("cache", Fp4Cache), ("table", c_vp), ("lengths", c_vp), ("cu", c_vp), ("query", c_vp), ("out", c_vp),
+                ("query_token", c_i64), ("query_head", c_i64), ("requests", c_i32), ("width", c_i32), ("rows", c_i32),
+                ("q_heads", c_i32), ("query_dtype", c_i32), ("window", c_i32), ("longest", c_i32), ("most", c_i32),
+                ("scaling", c_f32), ("fill", c_i32)]
+
+
 class DkvError(RuntimeError):
     pass
 
@@ -105,12 +114,14 @@ def lib() -> ctypes.CDLL:
         handle.dkv_abi_version.restype = c_i32
         handle.dkv_last_error.restype = ctypes.c_char_p
         for name in ("dkv_attend_workspace_bytes", "dkv_score_workspace_bytes", "dkv_topk_workspace_bytes",
-                     "dkv_matmul_f32_workspace_bytes"):
+                     "dkv_matmul_f32_workspace_bytes", "dkv_fp4_attend_workspace_bytes"):
             getattr(handle, name).restype = c_sz
         handle.dkv_topk_workspace_bytes.argtypes = [c_i32]
         handle.dkv_page_assign.argtypes = [c_vp, c_vp, c_i32, c_vp, c_vp, c_vp, c_vp]
         handle.dkv_page_trim.argtypes = [c_vp, c_vp, c_vp]
         handle.dkv_fp4_store.argtypes = [c_vp, c_vp, c_vp, c_i32, c_i64, c_i64, c_i64, c_i64, c_vp, c_i32, c_vp]
+        handle.dkv_fp4_attend_workspace_bytes.argtypes = [c_vp]
+        handle.dkv_fp4_attend.argtypes = [c_vp, c_vp, c_sz, c_vp]
         handle.dkv_fp4_load.argtypes = [c_vp, c_vp, c_i32, c_vp, c_vp, c_i32, c_vp]
         if handle.dkv_abi_version() != ABI_VERSION:
             raise RuntimeError(f"{LIB_PATH} has ABI {handle.dkv_abi_version()}, expected {ABI_VERSION}")
@@ -560,7 +571,7 @@ def page_trim(pages: Pages, keep) -> None:
 
 
 def _fp4_rows(t: torch.Tensor) -> torch.Tensor:
-    """Rows as dkv_fp4_store reads them: any 16-byte strides over contiguous dimensions, else a copy."""
+    """Rows as dkv_fp4_store and dkv_fp4_attend read them: any 16-byte strides over contiguous dimensions, else a copy."""
     unit = 4 if t.dtype == torch.float32 else 8
     if t.stride(2) != 1 or t.stride(0) % unit or t.stride(1) % unit or t.data_ptr() % 16:
         return t.contiguous().clone() if t.is_contiguous() else t.contiguous()
@@ -594,3 +605,34 @@ def fp4_load(cache: Fp4Cache, slots, key, value) -> None:
     where, keys, values = ptr(slots), ptr(key), ptr(value)
     with _on_device_of(slots):
         _check(lib().dkv_fp4_load(ctypes.addressof(cache), where, n, keys, values, code, stream_handle()), "dkv_fp4_load")
+
+
+def fp4_attend(args: Fp4AttendArgs, query, cu, out=None) -> torch.Tensor:
+    """Attention of query [rows, q_heads, head_dim] (f32, f16 or bf16) over the pages of ``args`` (its cache, table and
+    lengths, requests, width, scaling, window, longest and most set): out of the same shape and type, whose rows behind
+    cu[requests] are left as they are; a new one, with zeros there, if it is None."""
+    rows, q_heads, dim = query.shape
+    args.query_dtype = dtype_code(query.dtype)
+    _expect("fp4_attend", cu.device, (cu, "cu", torch.int32, (args.requests + 1,)),
+            (query, "query", query.dtype, (rows, q_heads, args.cache.head_dim)))
+    args.cu = ptr(cu)
+    args.fill = out is None
+    if out is None:
+        out = torch.empty(rows, q_heads, dim, dtype=query.dtype, device=query.device)
+    else:
+        _expect("fp4_attend", cu.device, (out, "out", query.dtype, (rows, q_heads, dim)))
+        if not out.is_contiguous() or out.data_ptr() % 16:
+            raise ValueError("fp4_attend: out must be contiguous and 16-byte aligned")
+    if rows == 0:
+        return out
+    query = _fp4_rows(query)
+    args.query, args.query_token, args.query_head = query.data_ptr(), query.stride(0), query.stride(1)
+    args.out, args.rows, args.q_heads = out.data_ptr(), rows, q_heads
+    where = ctypes.addressof(args)
+    need = lib().dkv_fp4_attend_workspace_bytes(where)
+    if need == 0:
+        _check(-2, "dkv_fp4_attend_workspace_bytes")
+    with _on_device_of(cu):
+        workspace = torch.empty(need, dtype=torch.uint8, device=query.device)
+        _check(lib().dkv_fp4_attend(where, workspace.data_ptr(), need, stream_handle()), "dkv_fp4_attend")
+    return out

@@ -9,7 +9,8 @@ states the values, the pages' form and the tables.
 the GPU or reads from it, so a step can be captured in a HIP graph.  A step of a serving loop is
 
     step = cache.assign(new, rows)                    # pages, slots and positions of the step's tokens
-    cache.store(layer, key, value, step)              # in every layer: the new rows into the pages
+    cache.store(layer, key, value, step)              # in every layer: the new rows into the pages,
+    out = cache.attend_rows(layer, query, step)       # and the queries over all of them
     cache.trim(keep)                                  # finished requests, refused drafts
 
 Calls on one cache share its tables and belong on one stream (or on streams the caller orders).
@@ -74,6 +75,12 @@ class PagedCache:
         self._layers = [dkv_hip.Fp4Cache(self.key_codes[i].data_ptr(), self.key_scales[i].data_ptr(),
                                          self.value_codes[i].data_ptr(), self.value_scales[i].data_ptr(), pages,
                                          kv_heads, page, head_dim) for i in range(layers)]
+        self._attend = []
+        for cache in self._layers:
+            a = dkv_hip.Fp4AttendArgs()
+            a.cache, a.table, a.lengths = cache, self.table.data_ptr(), self.lengths.data_ptr()
+            a.requests, a.width = requests, table_pages
+            self._attend.append(a)
 
     # ----- tables -----
     def _counts(self, counts) -> torch.Tensor:
@@ -144,6 +151,26 @@ class PagedCache:
         value = torch.empty_like(key)
         dkv_hip.fp4_load(self._layer(layer), slots, key, value)
         return key, value
+
+    def attend_rows(self, layer: int, query: torch.Tensor, step: Step, scaling: float | None = None,
+                    window: int | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+        """Attention of the step's queries [rows, q_heads, head_dim] (float32, float16 or bfloat16, any strides) over
+        the pages of ``layer``, where the step's own keys and values lie already: causal, and over the last ``window``
+        tokens of each query's if given.  ``out`` (same shape and type, contiguous) keeps its rows behind the last
+        request; without it they are zeros."""
+        if not 0 <= layer < self.layers:
+            raise ValueError(f"layer {layer} of {self.layers}")
+        if query.dim() != 3 or query.shape[1] % self.kv_heads or query.shape[0] != step.rows:
+            raise ValueError(f"attend_rows: query must be [{step.rows}, a multiple of {self.kv_heads}, {self.head_dim}] "
+                             f"(got {list(query.shape)})")
+        if window is not None and not 1 <= window < 1 << 31:
+            raise ValueError(f"attend_rows: window {window}")
+        self._here(step.cu, "attend_rows")
+        args = self._attend[layer]
+        args.scaling = self.head_dim ** -0.5 if scaling is None else scaling
+        args.window = window or 0
+        args.longest, args.most = min(max(step.longest, 1), (1 << 31) - 1), min(max(step.most, 1), (1 << 31) - 1)
+        return dkv_hip.fp4_attend(args, query, step.cu, out)
 
     def held_bytes(self) -> int:
         """GPU memory of the pages of all layers, the tables and the free list."""

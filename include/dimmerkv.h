@@ -501,6 +501,38 @@ int dkv_fp4_store(const dkv_fp4_cache_t* c, const void* key, const void* value, 
 int dkv_fp4_load(const dkv_fp4_cache_t* c, const int64_t* slots, int32_t n, void* key, void* value, int32_t dtype,
                  void* stream);
 
+/* Attention of the newest tokens of every request over its pages: request b's
+ * rows cu[b] .. cu[b+1]-1 of query are its last tokens (stored before), row i of n
+ * at position lengths[b] - n + i, and sees tokens up to its own and, with a window,
+ * the last `window` of them.  out = softmax(scaling * q k^T) v per row and head,
+ * query head x reading KV head x / (q_heads / kv_heads); a row that sees nothing
+ * is 0; a token a row does not see has no part in it, whatever its values.  Rows
+ * behind cu[requests] are left as they are, or zeroed with `fill`.  Entries of the
+ * table that are no page count as tokens not seen. */
+typedef struct dkv_fp4_attend_args {
+  dkv_fp4_cache_t cache;
+  const int32_t* table;    /* [requests][width] */
+  const int32_t* lengths;  /* [requests] */
+  const int32_t* cu;       /* [requests + 1] */
+  const void* query;       /* row t, head x at query + t * query_token + x * query_head elements, 16-byte aligned */
+  void* out;               /* [rows][q_heads][head_dim], the query's type */
+  int64_t query_token;
+  int64_t query_head;
+  int32_t requests;
+  int32_t width;
+  int32_t rows;
+  int32_t q_heads;
+  int32_t query_dtype;
+  int32_t window;          /* 0: all tokens */
+  int32_t longest;         /* bounds on the lengths and on the rows of a request: they shape the launch, not the result */
+  int32_t most;
+  float scaling;
+  int32_t fill;
+} dkv_fp4_attend_args_t;
+
+size_t dkv_fp4_attend_workspace_bytes(const dkv_fp4_attend_args_t* p);
+int dkv_fp4_attend(const dkv_fp4_attend_args_t* p, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -132,3 +132,43 @@ def test_oracle_tables():
     t.trim([16, 1])
     assert t.free == [4, 3, 1] and t.table == [[0], [2]]
     assert t.assign([33, 0], 33)[3] == 2 and t.assign([32, 33], 65)[3] == 3 and t.lengths == [16, 1]
+
+
+def attend_args(**change):
+    a = dkv_hip.Fp4AttendArgs()
+    fields = dict(cache=cache(), table=P, lengths=P, cu=P, query=P, out=P, query_token=256, query_head=64, requests=2,
+                  width=4, rows=3, q_heads=4, query_dtype=2, window=0, longest=64, most=2, scaling=0.125, fill=0)
+    fields.update(change)
+    for name, value in fields.items():
+        setattr(a, name, value)
+    return a
+
+
+@pytest.mark.parametrize("change,code,words", [
+    (dict(cache=cache(head_dim=80)), -2, "head_dim"), (dict(cache=cache(page=20)), -2, "bad cache"),
+    (dict(cache=cache(key_codes=None)), -1, "null cache"), (dict(query_dtype=5), -1, "dtype 5"),
+    (dict(requests=0), -2, "bad shape"), (dict(requests=8193), -2, "bad shape"), (dict(width=0), -2, "bad shape"),
+    (dict(width=1 << 27), -2, "bad shape"), (dict(rows=-1), -2, "bad shape"), (dict(q_heads=3), -2, "3 query heads"),
+    (dict(q_heads=0), -2, "query heads"), (dict(rows=1 << 30), -2, "2^31"), (dict(window=-1), -2, "window"),
+    (dict(table=None), -1, "null pointer"), (dict(lengths=None), -1, "null pointer"), (dict(cu=None), -1, "null pointer"),
+    (dict(query=None), -1, "null pointer"), (dict(out=None), -1, "null pointer"), (dict(query=72), -1, "aligned"),
+    (dict(out=72), -1, "aligned"), (dict(query_token=100), -1, "aligned"), (dict(query_dtype=0, query_head=66), -1, "aligned")])
+def test_attention_refused(change, code, words):
+    a = attend_args(**change)
+    refused(dkv_hip.lib().dkv_fp4_attend(ctypes.addressof(a), P, 1 << 20, None), code, words)
+
+
+def test_attention_workspace():
+    lib = dkv_hip.lib()
+    lib.dkv_fp4_attend_workspace_bytes.restype = ctypes.c_size_t
+    bad = attend_args(q_heads=3)
+    assert lib.dkv_fp4_attend_workspace_bytes(ctypes.addressof(bad)) == 0
+    long = attend_args(longest=1 << 16, rows=1, most=1, requests=1)
+    need = lib.dkv_fp4_attend_workspace_bytes(ctypes.addressof(long))
+    assert need > 16
+    refused(lib.dkv_fp4_attend(ctypes.addressof(long), P, 16, None), -3, "workspace")
+    refused(lib.dkv_fp4_attend(ctypes.addressof(long), None, need, None), -1, "workspace")
+    refused(lib.dkv_fp4_attend(ctypes.addressof(long), 72, need, None), -1, "aligned")
+    none = attend_args(rows=0)
+    assert lib.dkv_fp4_attend(ctypes.addressof(none), None, 0, None) == 0
+    refused(lib.dkv_fp4_attend(None, None, 0, None), -1, "null arguments")
