@@ -24,7 +24,7 @@ CSRC = HERE / "csrc"
 INCLUDE = ROOT / "include"
 LIB = HERE / "libdimmerkv_hip.so"
 SOURCES = ["dkv_pack.hip", "dkv_attend.hip", "dkv_gemm.hip", "dkv_codec.hip", "dkv_pages.hip",
-           "dkv_fp4_attend.hip"]
+           "dkv_fp4_attend.hip", "dkv_logits.hip"]
 ARCH = os.environ.get("DKV_OFFLOAD_ARCH", "gfx950")
 
 

@@ -33,7 +33,7 @@ EXPORTS = [
     "dkv_quantize8", "dkv_quantize8_rungs", "dkv_centered_rows", "dkv_matmul_f32_workspace_bytes", "dkv_matmul_f32",
     "dkv_ladder_errors", "dkv_ladder_code", "dkv_rows_to_caches", "dkv_copy_tokens", "dkv_outside_tokens", "dkv_project_caches", "dkv_live_groups",
     "dkv_page_assign", "dkv_page_trim", "dkv_fp4_store", "dkv_fp4_load",
-    "dkv_fp4_attend_workspace_bytes", "dkv_fp4_attend",
+    "dkv_fp4_attend_workspace_bytes", "dkv_fp4_attend", "dkv_adjust_logits_workspace_bytes", "dkv_adjust_logits",
 ]
 NOALLOC_MAX_BYTES = 64 << 20  # DKV_NOALLOC_MAX_BYTES: the static workspace of dkv_attend_layer_noalloc
 
@@ -96,6 +96,14 @@ class Fp4AttendArgs(ctypes.Structure):
                 ("scaling", c_f32), ("fill", c_i32)]
 
 
+class LogitsArgs(ctypes.Structure):
+    """dkv_logits_args_t."""
+    _fields_ = [(name, c_vp) for name in ("logits", "out", "tokens", "lengths", "reply", "repetition", "presence", "frequency",
+                                          "bias_ids", "bias_values", "bias_cu", "allowed", "allowed_row", "pick")]
+    _fields_ += [("logits_row", c_i64), ("out_row", c_i64), ("tokens_row", c_i64)]
+    _fields_ += [(name, c_i32) for name in ("dtype", "rows", "vocab", "history", "token_bytes", "biases", "masks", "words")]
+
+
 class DkvError(RuntimeError):
     pass
 
@@ -114,7 +122,8 @@ def lib() -> ctypes.CDLL:
         handle.dkv_abi_version.restype = c_i32
         handle.dkv_last_error.restype = ctypes.c_char_p
         for name in ("dkv_attend_workspace_bytes", "dkv_score_workspace_bytes", "dkv_topk_workspace_bytes",
-                     "dkv_matmul_f32_workspace_bytes", "dkv_fp4_attend_workspace_bytes"):
+                     "dkv_matmul_f32_workspace_bytes", "dkv_fp4_attend_workspace_bytes",
+                     "dkv_adjust_logits_workspace_bytes"):
             getattr(handle, name).restype = c_sz
         handle.dkv_topk_workspace_bytes.argtypes = [c_i32]
         handle.dkv_page_assign.argtypes = [c_vp, c_vp, c_i32, c_vp, c_vp, c_vp, c_vp]
@@ -122,6 +131,8 @@ def lib() -> ctypes.CDLL:
         handle.dkv_fp4_store.argtypes = [c_vp, c_vp, c_vp, c_i32, c_i64, c_i64, c_i64, c_i64, c_vp, c_i32, c_vp]
         handle.dkv_fp4_attend_workspace_bytes.argtypes = [c_vp]
         handle.dkv_fp4_attend.argtypes = [c_vp, c_vp, c_sz, c_vp]
+        handle.dkv_adjust_logits_workspace_bytes.argtypes = [c_vp]
+        handle.dkv_adjust_logits.argtypes = [c_vp, c_vp, c_sz, c_vp]
         handle.dkv_fp4_load.argtypes = [c_vp, c_vp, c_i32, c_vp, c_vp, c_i32, c_vp]
         if handle.dkv_abi_version() != ABI_VERSION:
             raise RuntimeError(f"{LIB_PATH} has ABI {handle.dkv_abi_version()}, expected {ABI_VERSION}")
@@ -636,3 +647,50 @@ def fp4_attend(args: Fp4AttendArgs, query, cu, out=None) -> torch.Tensor:
         workspace = torch.empty(need, dtype=torch.uint8, device=query.device)
         _check(lib().dkv_fp4_attend(where, workspace.data_ptr(), need, stream_handle()), "dkv_fp4_attend")
     return out
+
+
+def adjust_logits(args: LogitsArgs, logits, tokens=None, lengths=None, reply=None, out=None):
+    """logits [rows, vocab] (f32, f16 or bf16) under the controls of ``args`` (its penalties, biases and masks set) ->
+    (out of the same shape and type, pick int64 [rows]).  ``tokens`` [rows, history] int32 or int64 with lengths and
+    reply int32 [rows]; ``out`` may be the logits."""
+    rows, vocab = args.rows, args.vocab
+    args.dtype = dtype_code(logits.dtype)
+    _expect("adjust_logits", logits.device, (logits, "logits", logits.dtype, (rows, vocab)))
+    if not logits.is_cuda:
+        raise ValueError("dimmer-kv HIP kernels need GPU tensors (no CPU path)")
+    if logits.stride(1) != 1 or (rows > 1 and logits.stride(0) < vocab):
+        if out is logits:
+            raise ValueError("adjust_logits: logits changed in place need rows of unit stride that do not overlap")
+        logits = logits.contiguous()
+    if out is None:
+        out = torch.empty(rows, vocab, dtype=logits.dtype, device=logits.device)
+    elif out is not logits:
+        _expect("adjust_logits", logits.device, (out, "out", logits.dtype, (rows, vocab)))
+        if out.stride(1) != 1 or (rows > 1 and out.stride(0) < vocab):
+            raise ValueError("adjust_logits: out needs rows of unit stride that do not overlap")
+    args.tokens = args.lengths = args.reply = None
+    if tokens is not None:
+        if tokens.dtype not in (torch.int32, torch.int64) or tokens.dim() != 2 or (
+                tokens.shape[1] > 1 and tokens.stride(1) != 1):
+            raise ValueError("adjust_logits: tokens must be int32 or int64 [rows, history] with contiguous rows")
+        _expect("adjust_logits", logits.device, (tokens, "tokens", tokens.dtype, (rows, tokens.shape[1])),
+                (lengths, "lengths", torch.int32, (rows,)))
+        args.tokens, args.lengths, args.tokens_row = addr(tokens), ptr(lengths), tokens.stride(0)
+        args.history, args.token_bytes = tokens.shape[1], tokens.element_size()
+        if reply is not None:
+            _expect("adjust_logits", logits.device, (reply, "reply", torch.int32, (rows,)))
+            args.reply = ptr(reply)
+    pick = torch.empty(rows, dtype=torch.int64, device=logits.device)
+    if rows == 0:
+        return out, pick
+    args.logits, args.out, args.pick = logits.data_ptr(), out.data_ptr(), pick.data_ptr()
+    # (the stride of a single row says nothing)
+    args.logits_row, args.out_row = max(logits.stride(0), vocab), max(out.stride(0), vocab)
+    where = ctypes.addressof(args)
+    need = lib().dkv_adjust_logits_workspace_bytes(where)
+    if need == 0:
+        _check(-2, "dkv_adjust_logits_workspace_bytes")
+    with _on_device_of(logits):
+        workspace = torch.empty(need, dtype=torch.uint8, device=logits.device)
+        _check(lib().dkv_adjust_logits(where, workspace.data_ptr(), need, stream_handle()), "dkv_adjust_logits")
+    return out, pick

@@ -533,6 +533,50 @@ typedef struct dkv_fp4_attend_args {
 size_t dkv_fp4_attend_workspace_bytes(const dkv_fp4_attend_args_t* p);
 int dkv_fp4_attend(const dkv_fp4_attend_args_t* p, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- logits of replies ------------------------------------------------------
+ * No counterpart in the reference, whose answers take the argmax as it is.  For
+ * every row (a reply) and token of the vocabulary, in float32, each operation
+ * rounded on its own:
+ *   x = x > 0 ? x / repetition : x * repetition   if the row's history holds it
+ *   x = x - (frequency * count + presence)        if its reply does, count times
+ *   x = x + bias                                  (an id listed twice: the last)
+ *   x = -infinity                                 if the row's mask has no bit for it
+ * and out = x in the logits' type.  pick is the token of the largest x before that
+ * last rounding, the lowest one of equals (a NaN counts as largest, as in
+ * torch.argmax), -1 if no token is above -infinity.  History and reply: tokens
+ * [row][0 .. lengths) and from reply[row] on; ids outside 0 .. vocab - 1 are
+ * skipped.  out may be logits itself. */
+typedef struct dkv_logits_args {
+  const void* logits;        /* [rows], logits_row elements apart */
+  void* out;                 /* [rows], out_row elements apart */
+  const void* tokens;        /* int32 or int64 (token_bytes 4 or 8) [rows][history], tokens_row apart; null: no history */
+  const int32_t* lengths;    /* [rows] */
+  const int32_t* reply;      /* [rows] or null: the reply begins at 0 */
+  const float* repetition;   /* [rows] or null: 1 */
+  const float* presence;     /* [rows] or null: 0 */
+  const float* frequency;    /* [rows] or null: 0 */
+  const int32_t* bias_ids;   /* [biases] */
+  const float* bias_values;  /* [biases] */
+  const int32_t* bias_cu;    /* [rows + 1] where each row's biases begin */
+  const int32_t* allowed;    /* [masks][words] bit t % 32 of word t / 32: token t may be picked; null: no mask */
+  const int32_t* allowed_row;/* [rows] which mask, -1 none; null: row r takes mask r */
+  int64_t* pick;             /* [rows] or null */
+  int64_t logits_row;
+  int64_t out_row;
+  int64_t tokens_row;
+  int32_t dtype;
+  int32_t rows;              /* at most 65535 */
+  int32_t vocab;
+  int32_t history;
+  int32_t token_bytes;
+  int32_t biases;            /* 0: no biases */
+  int32_t masks;
+  int32_t words;
+} dkv_logits_args_t;
+
+size_t dkv_adjust_logits_workspace_bytes(const dkv_logits_args_t* p);
+int dkv_adjust_logits(const dkv_logits_args_t* p, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

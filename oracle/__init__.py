@@ -18,6 +18,7 @@ answer-time path so that the HIP kernels can be checked against it:
                     ladder layout this build defines (byte totals follow
                     scripts/progressive.py:185-194, 232 and scripts/kvtc.py:82-85;
                     ladder code bits LSB-first as scripts/kvtc_storage.py:21-27)
+- ``logits_ref``    reply logits under penalties, biases and masks (no counterpart in the reference)
 - ``paged_ref``     the paged 4-bit cache: values, block tables and attention (no counterpart in
                     the reference)
 - ``storage_ref``   the kvtc byte-storage layout, encode_bytes / decode_bytes
