@@ -27,6 +27,7 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 
 constexpr int kWaves = 4;
+constexpr int kMaxSplits = 256;
 constexpr float kWeightShift = 15.0f;  // weights are held times 2^15
 
 struct AttendArgs {
@@ -39,10 +40,14 @@ struct AttendArgs {
   float* part;      // [rows * q_heads][splits][D] sums when the tokens are split over workgroups
   float2* part_ml;  // [rows * q_heads][splits] maximum and sum
   int64_t query_token, query_head;
-  int requests, width, shift, rows, groups, window, splits, fill;
+  int requests, width, shift, rows, groups, window, splits, share, fill;
   float scale;  // |scaling| * log2 e
   int negate;   // scaling < 0: the queries change sign
 };
+
+DKV_DEVICE void set_result(float& y, float x) { y = x; }
+DKV_DEVICE void set_result(half_t& y, float x) { y = (half_t)x; }
+DKV_DEVICE void set_result(dkv_bf16& y, float x) { y.bits = float_to_bf16_bits(x); }
 
 template <typename T>
 struct Operand;  // what a query type's products are made of
@@ -80,22 +85,27 @@ struct Operand<float> : Operand<dkv_bf16> {
 };
 
 // 8 query values into kPieces operands.
+DKV_DEVICE uint4 signed_words(const void* p, uint32_t sign) {
+  const uint4 w = *(const uint4*)p;
+  return make_uint4(w.x ^ sign, w.y ^ sign, w.z ^ sign, w.w ^ sign);
+}
 DKV_DEVICE void query_pieces(const half_t* p, bool negate, half8 (&out)[1]) {
-  out[0] = *(const half8*)p;
-  if (negate) out[0] = -out[0];
+  const uint4 w = signed_words(p, negate ? 0x80008000u : 0u);
+  __builtin_memcpy(&out[0], &w, 16);
 }
 DKV_DEVICE void query_pieces(const dkv_bf16* p, bool negate, bf16x8 (&out)[1]) {
-  uint4 w = *(const uint4*)p;
-  if (negate) { w.x ^= 0x80008000u; w.y ^= 0x80008000u; w.z ^= 0x80008000u; w.w ^= 0x80008000u; }
+  const uint4 w = signed_words(p, negate ? 0x80008000u : 0u);
   __builtin_memcpy(&out[0], &w, 16);
 }
 DKV_DEVICE void query_pieces(const float* p, bool negate, bf16x8 (&out)[3]) {
+  const uint32_t sign = negate ? 0x80000000u : 0u;
+  const uint4 first = signed_words(p, sign), second = signed_words(p + 4, sign);
+  const uint32_t value[8] = {first.x, first.y, first.z, first.w, second.x, second.y, second.z, second.w};
   // upper halves of the value, of what they leave, and the rest: 8 bits each of the 24
   uint32_t words[3][4] = {};
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    float x = p[i];
-    if (negate) x = -x;
+    const float x = __uint_as_float(value[i]);
     const uint32_t a = __float_as_uint(x) & 0xffff0000u;
     const float left = x - __uint_as_float(a);
     const uint32_t b = __float_as_uint(left) & 0xffff0000u;
@@ -110,6 +120,11 @@ DKV_DEVICE void query_pieces(const float* p, bool negate, bf16x8 (&out)[3]) {
 }
 
 DKV_DEVICE float exponent(uint32_t byte) { return __uint_as_float(byte << 23); }
+
+// The tables are read through the scalar cache: an index the same in every lane costs no vector load, and no wait for the
+// page loads on their way.
+typedef const __attribute__((address_space(4))) int32_t* scalar_ints;
+DKV_DEVICE scalar_ints as_scalar(const int32_t* p) { return (scalar_ints)(uintptr_t)p; }
 
 // The codes and exponents of one chunk in this lane: CH tiles of 16 tokens.
 template <int D, int CH>
@@ -134,26 +149,48 @@ DKV_DEVICE void load_words(const uint8_t* p, uint32_t (&w)[N]) {
   }
 }
 
+// A lane's bytes inside a tile, behind the tile's first byte of codes (16 tokens of D / 2) and of exponents.
+template <int D>
+struct LaneOffsets {
+  uint32_t key, key_scale, value, value_scale;
+  DKV_DEVICE LaneOffsets() {
+    const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+    key = i * (D / 2) + g * (D / 8);
+    key_scale = i * (D / 32) + (D == 64 ? g >> 1 : D == 128 ? g : 2 * g);
+    value = g * (2 * D) + i * (D / 8);
+    value_scale = g * (D / 8) + (i * (D / 16) / 32) * 4;
+  }
+};
+
+// The table entries of a chunk's tiles, one a lane (lane t, and every 16th from it, tile t).  They are loaded a chunk
+// ahead of the pages, so that no page load waits for its address.
+template <int CH>
+DKV_DEVICE int load_entries(const AttendArgs& a, const int32_t* row, int len, int chunk) {
+  const int token = (chunk * CH + (int)(threadIdx.x & 15) % CH) * 16;
+  return row[token < len ? token >> a.shift : 0];  // (checked where it is used, so that nothing waits for it here)
+}
+
+// Loads are made for every tile, so that the ones on their way are the same count on every path: a tile that holds nothing
+// (behind the request, or an entry that is no page) reads the arrays' first bytes in all lanes.
 template <int D, int CH>
-DKV_DEVICE void load_chunk(const AttendArgs& a, const int32_t* row, int len, int h, int chunk, Chunk<D, CH>& c) {
-  const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+DKV_DEVICE void load_chunk(const AttendArgs& a, int entries, int len, int h, int chunk, const LaneOffsets<D>& at,
+                           Chunk<D, CH>& c) {
   const int page = a.c.page;
   c.whole = true;
 #pragma unroll
   for (int t = 0; t < CH; ++t) {
-    const int token = (chunk * CH + t) * 16;
-    int id = token < len ? row[token >> a.shift] : -1;
-    c.valid[t] = (uint32_t)id < (uint32_t)a.c.pages;  // entries that are no page are read as none
+    const uint32_t id = (uint32_t)__builtin_amdgcn_readlane(entries, t), token = (uint32_t)(chunk * CH + t) * 16;
+    c.valid[t] = token < (uint32_t)len && id < (uint32_t)a.c.pages;
     c.whole = c.whole && c.valid[t];
-    id = c.valid[t] ? id : 0;
-    const long first = ((long)id * a.c.kv_heads + h) * page + (token & (page - 1));  // token of the arrays
-    load_words(a.c.key_codes + (first + i) * (D / 2) + g * (D / 8), c.k[t]);
-    const uint8_t* ks = a.c.key_scales + (first + i) * (D / 32);
-    if constexpr (D == 64) c.ks[t] = ks[g >> 1];
-    else if constexpr (D == 128) c.ks[t] = ks[g];
-    else c.ks[t] = *(const uint16_t*)(ks + 2 * g);
-    load_words(a.c.value_codes + (first / 4 + g) * (2 * D) + i * (D / 8), c.v[t]);
-    c.vs[t] = *(const uint32_t*)(a.c.value_scales + (first / 4 + g) * (D / 8) + (i * (D / 16) / 32) * 4);
+    const uint32_t mask = c.valid[t] ? ~0u : 0u, within = token & (uint32_t)(page - 1);
+    const uint64_t first = ((uint64_t)(id & mask) * a.c.kv_heads + (h & mask)) * page + (within & mask);
+    const uint64_t codes = first * (D / 2), scales = first * (D / 32);
+    load_words(a.c.key_codes + codes + (at.key & mask), c.k[t]);
+    const uint8_t* ks = a.c.key_scales + scales + (at.key_scale & mask);
+    if constexpr (D == 256) c.ks[t] = *(const uint16_t*)ks;
+    else c.ks[t] = *ks;
+    load_words(a.c.value_codes + codes + (at.value & mask), c.v[t]);
+    c.vs[t] = *(const uint32_t*)(a.c.value_scales + scales + (at.value_scale & mask));
   }
 }
 
@@ -170,10 +207,12 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 ? 2 : 1) void fp4_attend_kerne
   const int h = blockIdx.x, b = blockIdx.z, split = blockIdx.y % a.splits, blocks = gridDim.y / a.splits;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
   const int q_heads = a.c.kv_heads * a.groups;
-  const int q0 = min(max(a.cu[b], 0), a.rows), q1 = min(max(a.cu[b + 1], q0), a.rows);
-  const int n_rows = (q1 - q0) * a.groups;
-  const int len = min(max(a.lengths[b], 0), a.width << a.shift);
+  const scalar_ints cu = as_scalar(a.cu) + b;
   const int32_t* table = a.table + (long)b * a.width;
+  const int q0 = min(max(cu[0], 0), a.rows), q1 = min(max(cu[1], q0), a.rows);
+  const int n_rows = (q1 - q0) * a.groups;
+  const int len = min(max(as_scalar(a.lengths)[b], 0), a.width << a.shift);
+  const LaneOffsets<D> at;
   const int first_position = len - (q1 - q0);  // of the request's first query token; below 0 it sees nothing
 
   if (a.fill && b == 0 && blockIdx.y == 0) {  // rows behind the last request
@@ -191,26 +230,22 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 ? 2 : 1) void fp4_attend_kerne
     int position[NT], before[NT];  // the last token a row sees, and the one before the first
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int r = row0 + nt * 16 + i;
+      const int r = min(row0 + nt * 16 + i, n_rows - 1);  // (rows past the last one repeat it, and go nowhere)
       const int token = r / a.groups;
-      position[nt] = r < n_rows ? first_position + token : -1;
+      position[nt] = first_position + token;
       before[nt] = (int)max((long)position[nt] - a.window, -1L);
+      const T* p = (const T*)a.query + (q0 + token) * a.query_token + (h * a.groups + r - token * a.groups) * a.query_head;
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        if (r < n_rows) {
-          const T* p = (const T*)a.query + (q0 + token) * a.query_token + (h * a.groups + r - token * a.groups) * a.query_head;
-          query_pieces(p + g * (D / 4) + s * 8, a.negate, q[nt][s]);
-        } else {
-          __builtin_memset(q[nt][s], 0, sizeof(q[nt][s]));
-        }
-      }
+      for (int s = 0; s < kSteps; ++s) query_pieces(p + g * (D / 4) + s * 8, a.negate, q[nt][s]);
     }
     const int low_position = first_position + row0 / a.groups, high_position = first_position + (row1 - 1) / a.groups;
     const int begin = (int)max((long)low_position - a.window + 1, 0L), end = high_position + 1;  // tokens some row sees
     const int all_from = (int)max((long)high_position - a.window + 1, 0L);                       // and all rows, from here
     const int chunk_begin = begin / (16 * CH), chunk_end = max((end + 16 * CH - 1) / (16 * CH), chunk_begin);
     const long chunks = end > begin ? chunk_end - chunk_begin : 0;
-    const int c0 = chunk_begin + (int)(chunks * split / a.splits), c1 = chunk_begin + (int)(chunks * (split + 1) / a.splits);
+    // as many chunks a split as the plan gives (so that a short request takes few), or what covers them all
+    const long share = max((long)a.share / CH, (chunks + a.splits - 1) / a.splits);
+    const int c0 = chunk_begin + (int)min(split * share, chunks), c1 = chunk_begin + (int)min((split + 1) * share, chunks);
 
     floatx4 o[NT][kLane];
     float m[NT], l[NT];
@@ -224,9 +259,13 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 ? 2 : 1) void fp4_attend_kerne
 
     Chunk<D, CH> now, next;
     int chunk = __builtin_amdgcn_readfirstlane(c0 + wave);
-    if (chunk < c1) load_chunk<D, CH>(a, table, len, h, chunk, now);
+    int entries = load_entries<CH>(a, table, chunk < c1 ? len : 0, chunk);
+    load_chunk<D, CH>(a, entries, chunk < c1 ? len : 0, h, chunk, at, now);
+    entries = load_entries<CH>(a, table, chunk + kWaves < c1 ? len : 0, chunk + kWaves);
     for (; chunk < c1; chunk += kWaves) {
-      if (chunk + kWaves < c1) load_chunk<D, CH>(a, table, len, h, chunk + kWaves, next);
+      const int later = load_entries<CH>(a, table, chunk + 2 * kWaves < c1 ? len : 0, chunk + 2 * kWaves);
+      load_chunk<D, CH>(a, entries, chunk + kWaves < c1 ? len : 0, h, chunk + kWaves, at, next);
+      entries = later;
 
       // scores^T: lane i a row, tokens 4g..4g+3 of each tile
       floatx4 s[NT][CH];
@@ -403,15 +442,14 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 ? 2 : 1) void fp4_attend_kerne
           const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
 #pragma unroll
           for (int j = 0; j < kLane; ++j) {
-            const float v = total == 0.0f ? 0.0f : acc[j] * inverse;
-            if constexpr (sizeof(T) == 4) out[j] = v;
-            else if constexpr (kPieces == 1 && __is_same(T, half_t)) out[j] = (half_t)v;
-            else out[j].bits = float_to_bf16_bits(v);
+            set_result(out[j], total == 0.0f ? 0.0f : acc[j] * inverse);
           }
         } else {
-          float* out = a.part + (out_row * a.splits + split) * D + part * kLane;
+          if (highest != -INFINITY) {
+            float* out = a.part + (out_row * a.splits + split) * D + part * kLane;
 #pragma unroll
-          for (int j = 0; j < kLane; ++j) out[j] = acc[j];
+            for (int j = 0; j < kLane; ++j) out[j] = acc[j];
+          }
           if (part == 0) a.part_ml[out_row * a.splits + split] = make_float2(highest, total);
         }
       }
@@ -420,42 +458,69 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 ? 2 : 1) void fp4_attend_kerne
   }
 }
 
-// The splits of a row joined: a wave per row, D / 64 dimensions a lane.
+// The splits of a row joined: a workgroup per row, D / 4 threads for its dimensions in fours, the splits dealt out to the
+// 256 / (D / 4) sets of them and their sums added in LDS.
 template <int D, typename T>
 __global__ __launch_bounds__(256) void fp4_join_kernel(AttendArgs a, int q_heads) {
-  constexpr int kLane = D / 64;
-  const int lane = threadIdx.x & 63;
-  const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  constexpr int kSet = D / 4, kSets = 256 / kSet;
+  __shared__ float weight[kMaxSplits];
+  __shared__ float4 sums[kSets][kSet];
+  __shared__ float whole;
+  const long row = blockIdx.x;
   if (row >= (long)min(max(a.cu[a.requests], 0), a.rows) * q_heads) return;
   const float2* ml = a.part_ml + row * a.splits;
-  float top = -INFINITY;
-  for (int s = lane; s < a.splits; s += 64) top = fmaxf(top, ml[s].x);
-  top = wave_max(top);
-  float acc[kLane] = {}, total = 0.0f;
-  for (int s = 0; s < a.splits; ++s) {
-    const float2 x = ml[s];
-    if (x.x == -INFINITY) continue;  // nothing seen there
-    const float factor = __builtin_amdgcn_exp2f(x.x - top);
-    total += x.y * factor;
-    const float* p = a.part + (row * a.splits + s) * D + lane * kLane;
+  if (threadIdx.x < 64) {
+    float top = -INFINITY, total = 0.0f;
+    float2 x[kMaxSplits / 64];
 #pragma unroll
-    for (int j = 0; j < kLane; ++j) acc[j] += p[j] * factor;
-  }
-  T* out = (T*)a.out + row * D + lane * kLane;
+    for (int k = 0; k < kMaxSplits / 64; ++k) {
+      const int s = k * 64 + (int)threadIdx.x;
+      x[k] = s < a.splits ? ml[s] : make_float2(-INFINITY, 0.0f);
+      top = fmaxf(top, x[k].x);
+    }
+    top = wave_max(top);
 #pragma unroll
-  for (int j = 0; j < kLane; ++j) {
-    const float v = total == 0.0f ? 0.0f : acc[j] / total;
-    if constexpr (sizeof(T) == 4) out[j] = v;
-    else if constexpr (__is_same(T, half_t)) out[j] = (half_t)v;
-    else out[j].bits = float_to_bf16_bits(v);
+    for (int k = 0; k < kMaxSplits / 64; ++k) {
+      const float factor = x[k].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x[k].x - top);
+      weight[k * 64 + threadIdx.x] = factor;
+      total += x[k].x == -INFINITY ? 0.0f : x[k].y * factor;
+    }
+    total = wave_sum(total);
+    if (threadIdx.x == 0) whole = total;
   }
+  __syncthreads();
+  const int at = threadIdx.x % kSet, set = threadIdx.x / kSet;
+  const float4* part = (const float4*)(a.part + row * a.splits * D) + at;
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+  for (int s = set; s < a.splits; s += kSets) {
+    const float w = weight[s];
+    if (w == 0.0f) continue;  // nothing seen there, and nothing written
+    const float4 v = part[s * kSet];
+    acc.x = fmaf(v.x, w, acc.x); acc.y = fmaf(v.y, w, acc.y); acc.z = fmaf(v.z, w, acc.z); acc.w = fmaf(v.w, w, acc.w);
+  }
+  sums[set][at] = acc;
+  __syncthreads();
+  if (set) return;
+#pragma unroll
+  for (int x = 1; x < kSets; ++x) {
+    const float4 v = sums[x][at];
+    acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
+  }
+  T* out = (T*)a.out + row * D + at * 4;
+  const float v[4] = {acc.x, acc.y, acc.z, acc.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) set_result(out[j], whole == 0.0f ? 0.0f : v[j] / whole);
 }
 
 struct Plan {
   int tiles;   // 16-row tiles a workgroup takes
   int blocks;  // row blocks a request is given
   int splits;
+  int share;   // 16-token tiles a split takes at the least
 };
+
+constexpr long kWorkgroups = 512;
 
 Plan plan_of(const dkv_fp4_attend_args_t& p) {
   Plan plan;
@@ -464,11 +529,17 @@ Plan plan_of(const dkv_fp4_attend_args_t& p) {
   plan.tiles = rows <= 16 || (p.query_dtype == DKV_F32 && p.cache.head_dim == 256) ? 1 : rows <= 32 || narrow ? 2 : 4;
   const long blocks = (rows + plan.tiles * 16 - 1) / (plan.tiles * 16);
   plan.blocks = (int)(blocks < 4096 ? blocks : 4096);
-  const long groups_of_work = (long)p.requests * p.cache.kv_heads * plan.blocks, longest = p.longest < 1 ? 1 : p.longest;
-  const long wanted = (512 + groups_of_work - 1) / groups_of_work, most = (longest + 255) / 256;
-  plan.splits = (int)(wanted < most ? wanted : most);
-  if (plan.splits > 256) plan.splits = 256;
+  // Workgroups enough for the card, of 256 tokens at the least; of 1,024 where that makes more than the card holds at
+  // once, so that requests of different lengths even out.
+  const long each = (long)p.requests * p.cache.kv_heads * plan.blocks;
+  long longest = p.longest < 1 ? 1 : p.longest;  // the tokens a row block may see
+  if (p.window) longest = min(longest, (long)p.window + plan.tiles * 16 / groups + 16);
+  const long fill = (kWorkgroups + each - 1) / each, even = p.requests > 1 ? (8 * kWorkgroups + each - 1) / each : 1;
+  const long wanted = max(min(fill, (longest + 255) / 256), min(even, (longest + 1023) / 1024));
+  plan.splits = (int)min(max(wanted, 1L), (long)kMaxSplits);
   while ((long)plan.blocks * plan.splits > 65535) plan.blocks /= 2;
+  const long tiles = (longest + 15) / 16;
+  plan.share = (int)(((tiles + plan.splits - 1) / plan.splits + 15) / 16 * 16);
   return plan;
 }
 
@@ -505,7 +576,7 @@ void launch(const AttendArgs& a, const Plan& plan, int q_heads, hipStream_t st) 
   }
   if (plan.splits > 1) {
     const long rows = (long)a.rows * q_heads;
-    hipLaunchKernelGGL((fp4_join_kernel<D, T>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a, q_heads);
+    hipLaunchKernelGGL((fp4_join_kernel<D, T>), dim3((unsigned)rows), dim3(256), 0, st, a, q_heads);
   }
 }
 
@@ -545,7 +616,7 @@ extern "C" int dkv_fp4_attend(const dkv_fp4_attend_args_t* p, void* workspace, s
   a.requests = p->requests; a.width = p->width; a.shift = dkv::page_shift(p->cache.page); a.rows = p->rows;
   a.groups = p->q_heads / p->cache.kv_heads;
   a.window = p->window ? p->window : INT32_MAX;
-  a.splits = plan.splits; a.fill = p->fill;
+  a.splits = plan.splits; a.share = plan.share; a.fill = p->fill;
   // a positive factor keeps the order of the scores; one of 0 weighs every token the same, as the smallest does
   a.scale = fmaxf(fabsf(p->scaling) * 1.44269504088896340736f, 1.1754944e-38f);
   if (p->scaling != p->scaling) a.scale = p->scaling;
