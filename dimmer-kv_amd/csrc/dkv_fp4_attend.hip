@@ -126,12 +126,16 @@ DKV_DEVICE float exponent(uint32_t byte) { return __uint_as_float(byte << 23); }
 typedef const __attribute__((address_space(4))) int32_t* scalar_ints;
 DKV_DEVICE scalar_ints as_scalar(const int32_t* p) { return (scalar_ints)(uintptr_t)p; }
 
-// The codes and exponents of one chunk in this lane: CH tiles of 16 tokens.
+// One chunk in this lane, CH tiles of 16 tokens: codes and exponents, and which tiles hold something (the same in every
+// lane).
 template <int D, int CH>
-struct Chunk {
-  static constexpr int kWords = D / 32;
-  uint32_t k[CH][kWords], ks[CH], v[CH][kWords], vs[CH];
-  bool valid[CH];  // the same in every lane
+struct Codes {
+  uint32_t words[CH][D / 32], scales[CH];
+};
+template <int CH>
+struct Tiles {
+  uint64_t first[CH];  // token of the arrays where the tile begins
+  bool valid[CH];
   bool whole;
 };
 
@@ -170,37 +174,53 @@ DKV_DEVICE int load_entries(const AttendArgs& a, const int32_t* row, int len, in
   return row[token < len ? token >> a.shift : 0];  // (checked where it is used, so that nothing waits for it here)
 }
 
-// Loads are made for every tile, so that the ones on their way are the same count on every path: a tile that holds nothing
-// (behind the request, or an entry that is no page) reads the arrays' first bytes in all lanes.
-template <int D, int CH>
-DKV_DEVICE void load_chunk(const AttendArgs& a, int entries, int len, int h, int chunk, const LaneOffsets<D>& at,
-                           Chunk<D, CH>& c) {
-  const int page = a.c.page;
-  c.whole = true;
+template <int CH>
+DKV_DEVICE void find_tiles(const AttendArgs& a, int entries, int len, int h, int chunk, Tiles<CH>& tiles) {
+  const uint32_t page = a.c.page;
+  tiles.whole = true;
 #pragma unroll
   for (int t = 0; t < CH; ++t) {
     const uint32_t id = (uint32_t)__builtin_amdgcn_readlane(entries, t), token = (uint32_t)(chunk * CH + t) * 16;
-    c.valid[t] = token < (uint32_t)len && id < (uint32_t)a.c.pages;
-    c.whole = c.whole && c.valid[t];
-    const uint32_t mask = c.valid[t] ? ~0u : 0u, within = token & (uint32_t)(page - 1);
-    const uint64_t first = ((uint64_t)(id & mask) * a.c.kv_heads + (h & mask)) * page + (within & mask);
-    const uint64_t codes = first * (D / 2), scales = first * (D / 32);
-    load_words(a.c.key_codes + codes + (at.key & mask), c.k[t]);
-    const uint8_t* ks = a.c.key_scales + scales + (at.key_scale & mask);
-    if constexpr (D == 256) c.ks[t] = *(const uint16_t*)ks;
-    else c.ks[t] = *ks;
-    load_words(a.c.value_codes + codes + (at.value & mask), c.v[t]);
-    c.vs[t] = *(const uint32_t*)(a.c.value_scales + scales + (at.value_scale & mask));
+    tiles.valid[t] = token < (uint32_t)len && id < (uint32_t)a.c.pages;
+    tiles.whole = tiles.whole && tiles.valid[t];
+    tiles.first[t] = tiles.valid[t] ? ((uint64_t)id * a.c.kv_heads + h) * page + (token & (page - 1)) : 0;
+  }
+}
+
+// Loads are made for every tile, so that the ones on their way are the same count on every path: a tile that holds nothing
+// (behind the request, or an entry that is no page) reads the arrays' first bytes in all lanes.
+template <int D, int CH>
+DKV_DEVICE void load_keys(const AttendArgs& a, const Tiles<CH>& tiles, const LaneOffsets<D>& at, Codes<D, CH>& c) {
+#pragma unroll
+  for (int t = 0; t < CH; ++t) {
+    const uint32_t mask = tiles.valid[t] ? ~0u : 0u;
+    load_words(a.c.key_codes + tiles.first[t] * (D / 2) + (at.key & mask), c.words[t]);
+    const uint8_t* scale = a.c.key_scales + tiles.first[t] * (D / 32) + (at.key_scale & mask);
+    if constexpr (D == 256) c.scales[t] = *(const uint16_t*)scale;
+    else c.scales[t] = *scale;
+  }
+}
+template <int D, int CH>
+DKV_DEVICE void load_values(const AttendArgs& a, const Tiles<CH>& tiles, const LaneOffsets<D>& at, Codes<D, CH>& c) {
+#pragma unroll
+  for (int t = 0; t < CH; ++t) {
+    const uint32_t mask = tiles.valid[t] ? ~0u : 0u;
+    load_words(a.c.value_codes + tiles.first[t] * (D / 2) + (at.value & mask), c.words[t]);
+    c.scales[t] = *(const uint32_t*)(a.c.value_scales + tiles.first[t] * (D / 32) + (at.value_scale & mask));
   }
 }
 
 template <int D, typename T, int NT, int CH>
-__global__ __launch_bounds__(kWaves * 64, NT == 1 ? 2 : 1) void fp4_attend_kernel(AttendArgs a) {
+__global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_attend_kernel(AttendArgs a) {
   using Op = Operand<T>;
   using frag = typename Op::frag;
   constexpr int kRows = 16 * NT, kSteps = D / 32, kLane = D / 16, kPieces = Op::kPieces;
   constexpr int kWeights = kPieces == 1 ? 1 : 2;  // float16 pieces of a weight
   constexpr int kStride = D + 4;                  // a row of sums in LDS
+  // With 64 rows the accumulators leave no registers for the queries and a second chunk, and two waves a SIMD matter more
+  // (one fills the other's waits): queries lie in LDS, and a chunk's loads follow the last use of the one before.
+  constexpr bool kLean = NT == 4;
+  __shared__ frag held[kLean ? NT * kSteps * 64 : 1];
   __shared__ float sums[kWaves * 16 * kStride];
   __shared__ float stat[2][kWaves][kRows];
 
@@ -226,18 +246,29 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 ? 2 : 1) void fp4_attend_kerne
   for (int block = blockIdx.y / a.splits; block * (long)kRows < n_rows; block += blocks) {
     const int row0 = block * kRows, row1 = min(row0 + kRows, n_rows);
     // queries: operand B, lane i a row, 8 dimensions of g * D/4 + 8 * step
-    frag q[NT][kSteps][kPieces];
-    int position[NT], before[NT];  // the last token a row sees, and the one before the first
+    frag q[kLean ? 1 : NT][kSteps][kPieces];
+    // the last token a row sees, and the one before the first (made where a chunk has a mask, and not held)
+    auto last_seen = [&](int nt) { return first_position + min(row0 + nt * 16 + i, n_rows - 1) / a.groups; };
+    auto before_first = [&](int last) { return (int)max((long)last - a.window, -1L); };
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int r = min(row0 + nt * 16 + i, n_rows - 1);  // (rows past the last one repeat it, and go nowhere)
       const int token = r / a.groups;
-      position[nt] = first_position + token;
-      before[nt] = (int)max((long)position[nt] - a.window, -1L);
       const T* p = (const T*)a.query + (q0 + token) * a.query_token + (h * a.groups + r - token * a.groups) * a.query_head;
+      if constexpr (kLean) {
+        if (nt == wave) {
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) query_pieces(p + g * (D / 4) + s * 8, a.negate, q[nt][s]);
+          for (int s = 0; s < kSteps; ++s) {
+            query_pieces(p + g * (D / 4) + s * 8, a.negate, q[0][0]);
+            held[(nt * kSteps + s) * 64 + lane] = q[0][0][0];
+          }
+        }
+      } else {
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) query_pieces(p + g * (D / 4) + s * 8, a.negate, q[nt][s]);
+      }
     }
+    if constexpr (kLean) __syncthreads();
     const int low_position = first_position + row0 / a.groups, high_position = first_position + (row1 - 1) / a.groups;
     const int begin = (int)max((long)low_position - a.window + 1, 0L), end = high_position + 1;  // tokens some row sees
     const int all_from = (int)max((long)high_position - a.window + 1, 0L);                       // and all rows, from here
@@ -257,54 +288,77 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 ? 2 : 1) void fp4_attend_kerne
       for (int j = 0; j < kLane; ++j) o[nt][j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
     }
 
-    Chunk<D, CH> now, next;
+    Codes<D, CH> keys, values, next_keys, next_values;
+    Tiles<CH> tiles, next_tiles;
     int chunk = __builtin_amdgcn_readfirstlane(c0 + wave);
     int entries = load_entries<CH>(a, table, chunk < c1 ? len : 0, chunk);
-    load_chunk<D, CH>(a, entries, chunk < c1 ? len : 0, h, chunk, at, now);
+    find_tiles<CH>(a, entries, chunk < c1 ? len : 0, h, chunk, tiles);
+    load_keys<D, CH>(a, tiles, at, keys);
+    load_values<D, CH>(a, tiles, at, values);
     entries = load_entries<CH>(a, table, chunk + kWaves < c1 ? len : 0, chunk + kWaves);
     for (; chunk < c1; chunk += kWaves) {
       const int later = load_entries<CH>(a, table, chunk + 2 * kWaves < c1 ? len : 0, chunk + 2 * kWaves);
-      load_chunk<D, CH>(a, entries, chunk + kWaves < c1 ? len : 0, h, chunk + kWaves, at, next);
+      find_tiles<CH>(a, entries, chunk + kWaves < c1 ? len : 0, h, chunk + kWaves, next_tiles);
       entries = later;
+      if constexpr (!kLean) {
+        load_keys<D, CH>(a, next_tiles, at, next_keys);
+        load_values<D, CH>(a, next_tiles, at, next_values);
+      }
 
       // scores^T: lane i a row, tokens 4g..4g+3 of each tile
       floatx4 s[NT][CH];
 #pragma unroll
-      for (int t = 0; t < CH; ++t) {
+      for (int t = 0; t < CH; ++t)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) s[nt][t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int st = 0; st < kSteps; ++st) {
-          const float e = exponent(D == 256 ? (st < 4 ? now.ks[t] & 255 : now.ks[t] >> 8) : now.ks[t]);
-          frag key;
+      for (int st = 0; st < kSteps; ++st) {
+        frag key[CH];
+#pragma unroll
+        for (int t = 0; t < CH; ++t) {
+          const float e = exponent(D == 256 ? (st < 4 ? keys.scales[t] & 255 : keys.scales[t] >> 8) : keys.scales[t]);
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
-            const auto two = Op::pair(now.k[t][st], e, x);
-            key[2 * x] = two[0];
-            key[2 * x + 1] = two[1];
+            const auto two = Op::pair(keys.words[t][st], e, x);
+            key[t][2 * x] = two[0];
+            key[t][2 * x + 1] = two[1];
           }
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int p = kPieces - 1; p >= 0; --p) s[nt][t] = Op::mfma(key, q[nt][st][p], s[nt][t]);
         }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          if constexpr (kLean) { if (nt == 0) __builtin_amdgcn_sched_barrier(0); }
+          if constexpr (kLean) q[0][0][0] = held[(nt * kSteps + st) * 64 + lane];
+#pragma unroll
+          for (int p = kPieces - 1; p >= 0; --p)
+#pragma unroll
+            for (int t = 0; t < CH; ++t) s[nt][t] = Op::mfma(key[t], kLean ? q[0][0][0] : q[kLean ? 0 : nt][kLean ? 0 : st][p], s[nt][t]);
+        }
+      }
+      if constexpr (kLean) {
+        load_keys<D, CH>(a, next_tiles, at, keys);
+        __builtin_amdgcn_sched_barrier(0);
       }
 
       const int base = chunk * CH * 16;
-      const bool masked = !now.whole || base + CH * 16 > low_position + 1 || base < all_from;
+      const bool masked = !tiles.whole || base + CH * 16 > low_position + 1 || base < all_from;
       if (masked) {
 #pragma unroll
-        for (int t = 0; t < CH; ++t) {
+        for (int nt = 0; nt < NT; ++nt) {
+          const int last = last_seen(nt), before = before_first(last);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int token = base + t * 16 + g * 4 + r;
+          for (int t = 0; t < CH; ++t)
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-              if (!now.valid[t] || token > position[nt] || token <= before[nt]) s[nt][t][r] = -INFINITY;
-            // what lies behind the request is stale: its values become zeros
-            if (!now.valid[t] || token >= len) now.vs[t] &= ~(255u << (8 * r));
-          }
+            for (int r = 0; r < 4; ++r) {
+              const int token = base + t * 16 + g * 4 + r;
+              if (!tiles.valid[t] || token > last || token <= before) s[nt][t][r] = -INFINITY;
+            }
         }
+        // what lies behind the request is stale: its values become zeros
+#pragma unroll
+        for (int t = 0; t < CH; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (!tiles.valid[t] || base + t * 16 + g * 4 + r >= len) values.scales[t] &= ~(255u << (8 * r));
       }
 
       half8 w[NT][CH / 2][kWeights];
@@ -345,7 +399,7 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 ? 2 : 1) void fp4_attend_kerne
           uint32_t bad[2];
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            uint32_t& vs = now.vs[2 * u + x];
+            uint32_t& vs = values.scales[2 * u + x];
             bad[x] = ((vs & 0x7f7f7f7fu) + 0x01010101u) & vs & 0x80808080u;  // the bytes that are 255
             vs &= ~((bad[x] >> 7) * 255u);
           }
@@ -355,11 +409,12 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 ? 2 : 1) void fp4_attend_kerne
             for (int x = 0; x < 8; ++x) is_bad[x] = (bad[x >> 2] >> (8 * (x & 3) + 7)) & 1 ? (half_t)1.0f : (half_t)0.0f;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
+              const int last = last_seen(nt), before = before_first(last);
               half8 sees;
 #pragma unroll
               for (int x = 0; x < 8; ++x) {
                 const int token = base + (2 * u + (x >> 2)) * 16 + g * 4 + (x & 3);
-                sees[x] = token <= position[nt] && token > before[nt] ? (half_t)1.0f : (half_t)0.0f;
+                sees[x] = token <= last && token > before ? (half_t)1.0f : (half_t)0.0f;
               }
               const floatx4 hit = __builtin_amdgcn_mfma_f32_16x16x32_f16(is_bad, sees, floatx4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
 #pragma unroll
@@ -377,14 +432,15 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 ? 2 : 1) void fp4_attend_kerne
       for (int u = 0; u < CH / 2; ++u) {
         float e[8];
 #pragma unroll
-        for (int x = 0; x < 8; ++x) e[x] = exponent((now.vs[2 * u + (x >> 2)] >> (8 * (x & 3))) & 255);
+        for (int x = 0; x < 8; ++x) e[x] = exponent((values.scales[2 * u + (x >> 2)] >> (8 * (x & 3))) & 255);
 #pragma unroll
         for (int j = 0; j < kLane; j += 2) {
+          if constexpr (kLean) __builtin_amdgcn_sched_barrier(0);
           half8 even, odd;
 #pragma unroll
           for (int x = 0; x < 8; ++x) {
             const int byte = (x & 3) * (D / 32) + j / 2;
-            const half2_t two = Operand<half_t>::pair(now.v[2 * u + (x >> 2)][byte / 4], e[x], byte % 4);
+            const half2_t two = Operand<half_t>::pair(values.words[2 * u + (x >> 2)][byte / 4], e[x], byte % 4);
             even[x] = two[0];
             odd[x] = two[1];
           }
@@ -397,7 +453,13 @@ __global__ __launch_bounds__(kWaves * 64, NT == 1 ? 2 : 1) void fp4_attend_kerne
             }
         }
       }
-      now = next;
+      tiles = next_tiles;
+      if constexpr (kLean) {
+        load_values<D, CH>(a, tiles, at, values);
+      } else {
+        keys = next_keys;
+        values = next_values;
+      }
     }
 
     // the four waves' sums, 16 rows at a time
