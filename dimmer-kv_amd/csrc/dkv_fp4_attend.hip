@@ -11,9 +11,10 @@
 //     what operand B of the second wants if V's lanes take the same tokens: the weights never change lanes, and the
 //     pages keep values in fours of tokens so that a lane's share is one load.
 // K is exact in bfloat16 and float16 alike, V in float16 (the exponents are clamped for that).  Queries go in as they are
-// (float32 as three bfloat16 pieces that add up to it).  The weights are rounded to float16, 2^-12 relative and shifted by
-// 2^15 so that weights down to 2^-29 of the largest keep that: an eighth of the rounding of a bfloat16 result; float32
-// results take a second piece.  Sums, maxima and accumulators are float32.
+// (float32 as three bfloat16 pieces that add up to it).  The weights are rounded to float16, 2^-11 relative, and are held
+// times 2^8 so that weights down to 2^-22 of the row's reference keep that (smaller ones are off by 2^-33 of it): an eighth
+// of a bfloat16 result's own rounding.  Float32 results take a second piece of the weights, held times 2^15.  Sums, maxima
+// and accumulators are float32.
 #include <math.h>
 
 #include "dkv_device.h"
@@ -27,8 +28,7 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 
 constexpr int kWaves = 4;
-constexpr int kMaxSplits = 256;
-constexpr float kWeightShift = 15.0f;  // weights are held times 2^15
+constexpr int kMaxSplits = 256, kFewSplits = 4;
 
 struct AttendArgs {
   dkv_fp4_cache_t c;
@@ -119,6 +119,19 @@ DKV_DEVICE void query_pieces(const float* p, bool negate, bf16x8 (&out)[3]) {
   for (int k = 0; k < 3; ++k) __builtin_memcpy(&out[k], words[k], 16);
 }
 
+// The larger of two floats (a NaN loses), without the quieting that the compiler puts before fmaxf.
+DKV_DEVICE float larger(float a, float b) {
+  float c;
+  asm("v_max_f32 %0, %1, %2" : "=v"(c) : "v"(a), "v"(b));
+  return c;
+}
+
+DKV_DEVICE float larger(float a, float b, float c) {
+  float d;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));
+  return d;
+}
+
 DKV_DEVICE float exponent(uint32_t byte) { return __uint_as_float(byte << 23); }
 
 // The tables are read through the scalar cache: an index the same in every lane costs no vector load, and no wait for the
@@ -139,16 +152,23 @@ struct Tiles {
   bool whole;
 };
 
+// Loads through a buffer descriptor: a base in scalar registers and the lane's offset, and nothing read past `bytes`.
+typedef __amdgpu_buffer_rsrc_t buffer;
+DKV_DEVICE buffer buffer_of(const uint8_t* base, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, bytes, 0x00020000);
+}
+typedef uint32_t uint2_t __attribute__((ext_vector_type(2)));
+typedef uint32_t uint4_t __attribute__((ext_vector_type(4)));
 template <int N>
-DKV_DEVICE void load_words(const uint8_t* p, uint32_t (&w)[N]) {
+DKV_DEVICE void load_words(buffer from, uint32_t at, uint32_t (&w)[N]) {
   if constexpr (N == 2) {
-    const uint2 x = *(const uint2*)p;
-    w[0] = x.x; w[1] = x.y;
+    const uint2_t x = __builtin_amdgcn_raw_buffer_load_b64(from, at, 0, 0);
+    w[0] = x[0]; w[1] = x[1];
   } else {
 #pragma unroll
     for (int i = 0; i < N; i += 4) {
-      const uint4 x = ((const uint4*)p)[i / 4];
-      w[i] = x.x; w[i + 1] = x.y; w[i + 2] = x.z; w[i + 3] = x.w;
+      const uint4_t x = __builtin_amdgcn_raw_buffer_load_b128(from, at + i * 4, 0, 0);
+      w[i] = x[0]; w[i + 1] = x[1]; w[i + 2] = x[2]; w[i + 3] = x[3];
     }
   }
 }
@@ -187,26 +207,25 @@ DKV_DEVICE void find_tiles(const AttendArgs& a, int entries, int len, int h, int
   }
 }
 
-// Loads are made for every tile, so that the ones on their way are the same count on every path: a tile that holds nothing
-// (behind the request, or an entry that is no page) reads the arrays' first bytes in all lanes.
+// Loads are made for every tile, so that the ones on their way are the same count on every path; of a tile that holds
+// nothing (behind the request, or an entry that is no page) no byte is read, and its codes and exponents are 0.
 template <int D, int CH>
 DKV_DEVICE void load_keys(const AttendArgs& a, const Tiles<CH>& tiles, const LaneOffsets<D>& at, Codes<D, CH>& c) {
 #pragma unroll
   for (int t = 0; t < CH; ++t) {
-    const uint32_t mask = tiles.valid[t] ? ~0u : 0u;
-    load_words(a.c.key_codes + tiles.first[t] * (D / 2) + (at.key & mask), c.words[t]);
-    const uint8_t* scale = a.c.key_scales + tiles.first[t] * (D / 32) + (at.key_scale & mask);
-    if constexpr (D == 256) c.scales[t] = *(const uint16_t*)scale;
-    else c.scales[t] = *scale;
+    load_words(buffer_of(a.c.key_codes + tiles.first[t] * (D / 2), tiles.valid[t] ? 8 * D : 0), at.key, c.words[t]);
+    const buffer scales = buffer_of(a.c.key_scales + tiles.first[t] * (D / 32), tiles.valid[t] ? D / 2 : 0);
+    if constexpr (D == 256) c.scales[t] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(scales, at.key_scale, 0, 0);
+    else c.scales[t] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(scales, at.key_scale, 0, 0);
   }
 }
 template <int D, int CH>
 DKV_DEVICE void load_values(const AttendArgs& a, const Tiles<CH>& tiles, const LaneOffsets<D>& at, Codes<D, CH>& c) {
 #pragma unroll
   for (int t = 0; t < CH; ++t) {
-    const uint32_t mask = tiles.valid[t] ? ~0u : 0u;
-    load_words(a.c.value_codes + tiles.first[t] * (D / 2) + (at.value & mask), c.words[t]);
-    c.scales[t] = *(const uint32_t*)(a.c.value_scales + tiles.first[t] * (D / 32) + (at.value_scale & mask));
+    load_words(buffer_of(a.c.value_codes + tiles.first[t] * (D / 2), tiles.valid[t] ? 8 * D : 0), at.value, c.words[t]);
+    c.scales[t] = __builtin_amdgcn_raw_buffer_load_b32(
+        buffer_of(a.c.value_scales + tiles.first[t] * (D / 32), tiles.valid[t] ? D / 2 : 0), at.value_scale, 0, 0);
   }
 }
 
@@ -216,6 +235,9 @@ __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_at
   using frag = typename Op::frag;
   constexpr int kRows = 16 * NT, kSteps = D / 32, kLane = D / 16, kPieces = Op::kPieces;
   constexpr int kWeights = kPieces == 1 ? 1 : 2;  // float16 pieces of a weight
+  // Weights are held times 2^kShift, against a reference that scores may pass by kSlack: 2^15 at the most, below the
+  // largest float16.
+  constexpr float kSlack = kWeights == 1 ? 7.0f : 0.0f, kShift = 15.0f - kSlack;
   constexpr int kStride = D + 4;                  // a row of sums in LDS
   // With 64 rows the accumulators leave no registers for the queries and a second chunk, and two waves a SIMD matter more
   // (one fills the other's waits): queries lie in LDS, and a chunk's loads follow the last use of the one before.
@@ -311,28 +333,39 @@ __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_at
       for (int t = 0; t < CH; ++t)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) s[nt][t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int st = 0; st < kSteps; ++st) {
-        frag key[CH];
+      frag key[CH];
+      auto convert_keys = [&](int st, frag (&out)[CH]) {
 #pragma unroll
         for (int t = 0; t < CH; ++t) {
           const float e = exponent(D == 256 ? (st < 4 ? keys.scales[t] & 255 : keys.scales[t] >> 8) : keys.scales[t]);
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
             const auto two = Op::pair(keys.words[t][st], e, x);
-            key[t][2 * x] = two[0];
-            key[t][2 * x + 1] = two[1];
+            out[t][2 * x] = two[0];
+            out[t][2 * x + 1] = two[1];
           }
         }
+      };
+      frag lean[2][kLean ? NT : 1];
+      if constexpr (kLean)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          if constexpr (kLean) { if (nt == 0) __builtin_amdgcn_sched_barrier(0); }
-          if constexpr (kLean) q[0][0][0] = held[(nt * kSteps + st) * 64 + lane];
+        for (int nt = 0; nt < NT; ++nt) lean[0][nt] = held[(nt * kSteps) * 64 + lane];
+#pragma unroll
+      for (int st = 0; st < kSteps; ++st) {
+        if constexpr (kLean) __builtin_amdgcn_sched_barrier(0);
+        convert_keys(st, key);
+        if (st + 1 < kSteps) {  // (an LDS read takes as long as a step's products)
+          if constexpr (kLean)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) lean[(st + 1) & 1][nt] = held[(nt * kSteps + st + 1) * 64 + lane];
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int p = kPieces - 1; p >= 0; --p)
 #pragma unroll
-            for (int t = 0; t < CH; ++t) s[nt][t] = Op::mfma(key[t], kLean ? q[0][0][0] : q[kLean ? 0 : nt][kLean ? 0 : st][p], s[nt][t]);
-        }
+            for (int t = 0; t < CH; ++t)
+              s[nt][t] = Op::mfma(key[t], kLean ? lean[st & 1][kLean ? nt : 0] : q[kLean ? 0 : nt][kLean ? 0 : st][p], s[nt][t]);
       }
       if constexpr (kLean) {
         load_keys<D, CH>(a, next_tiles, at, keys);
@@ -364,21 +397,20 @@ __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_at
       half8 w[NT][CH / 2][kWeights];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        float top = -INFINITY;
+        // The reference m of a row follows its maximum only when a score passes it by kSlack: most chunks then need no
+        // exchange between the four lanes of a row, and no rescaling.
+        float top = s[nt][0][0];
 #pragma unroll
-        for (int t = 0; t < CH; ++t)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) top = fmaxf(top, s[nt][t][r]);
-        top = max_xor32(max_xor16(top));
-        const float higher = fmaxf(m[nt], top * a.scale);
-        if (__any(higher > m[nt])) {
+        for (int t = 0; t < CH; ++t) top = larger(larger(top, s[nt][t][0], s[nt][t][1]), s[nt][t][2], s[nt][t][3]);
+        if (__any(top * a.scale > m[nt] + kSlack)) {
+          const float higher = larger(m[nt], max_xor32(max_xor16(top)) * a.scale);
           const float factor = __builtin_amdgcn_exp2f(m[nt] - (higher == -INFINITY ? 0.0f : higher));
           l[nt] *= factor;
 #pragma unroll
           for (int j = 0; j < kLane; ++j) o[nt][j] *= factor;
           m[nt] = higher;
         }
-        const float shift = kWeightShift - (m[nt] == -INFINITY ? 0.0f : m[nt]);
+        const float shift = kShift - (m[nt] == -INFINITY ? 0.0f : m[nt]);
 #pragma unroll
         for (int t = 0; t < CH; ++t) {
 #pragma unroll
@@ -428,30 +460,31 @@ __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_at
       }
 
       // out^T: operand A is 16 lanes' dimensions i * kLane + j over the 32 tokens of two tiles
+      constexpr int kPairs = kLane / 2, kTurns = CH / 2 * kPairs;
+      auto convert_values = [&](int turn, half8& even, half8& odd) {
+        const int u = turn / kPairs, pair = turn % kPairs;
 #pragma unroll
-      for (int u = 0; u < CH / 2; ++u) {
-        float e[8];
-#pragma unroll
-        for (int x = 0; x < 8; ++x) e[x] = exponent((values.scales[2 * u + (x >> 2)] >> (8 * (x & 3))) & 255);
-#pragma unroll
-        for (int j = 0; j < kLane; j += 2) {
-          if constexpr (kLean) __builtin_amdgcn_sched_barrier(0);
-          half8 even, odd;
-#pragma unroll
-          for (int x = 0; x < 8; ++x) {
-            const int byte = (x & 3) * (D / 32) + j / 2;
-            const half2_t two = Operand<half_t>::pair(values.words[2 * u + (x >> 2)][byte / 4], e[x], byte % 4);
-            even[x] = two[0];
-            odd[x] = two[1];
-          }
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int p = kWeights - 1; p >= 0; --p) {
-              o[nt][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, w[nt][u][p], o[nt][j], 0, 0, 0);
-              o[nt][j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, w[nt][u][p], o[nt][j + 1], 0, 0, 0);
-            }
+        for (int x = 0; x < 8; ++x) {
+          const float e = exponent((values.scales[2 * u + (x >> 2)] >> (8 * (x & 3))) & 255);
+          const int byte = (x & 3) * (D / 32) + pair;
+          const half2_t two = Operand<half_t>::pair(values.words[2 * u + (x >> 2)][byte / 4], e, byte % 4);
+          even[x] = two[0];
+          odd[x] = two[1];
         }
+      };
+#pragma unroll
+      for (int turn = 0; turn < kTurns; ++turn) {
+        if constexpr (kLean) __builtin_amdgcn_sched_barrier(0);
+        const int u = turn / kPairs, j = turn % kPairs * 2;
+        half8 even, odd;
+        convert_values(turn, even, odd);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int p = kWeights - 1; p >= 0; --p) {
+            o[nt][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, w[nt][u][p], o[nt][j], 0, 0, 0);
+            o[nt][j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, w[nt][u][p], o[nt][j + 1], 0, 0, 0);
+          }
       }
       tiles = next_tiles;
       if constexpr (kLean) {
@@ -575,6 +608,32 @@ __global__ __launch_bounds__(256) void fp4_join_kernel(AttendArgs a, int q_heads
   for (int j = 0; j < 4; ++j) set_result(out[j], whole == 0.0f ? 0.0f : v[j] / whole);
 }
 
+// The same for few splits: a set of D / 4 threads per row.  49,152 rows of two splits: 40 us a workgroup a row, XX here.
+template <int D, typename T>
+__global__ __launch_bounds__(256) void fp4_join_few_kernel(AttendArgs a, int q_heads) {
+  constexpr int kSet = D / 4, kSets = 256 / kSet;
+  const int at = threadIdx.x % kSet;
+  const long row = (long)blockIdx.x * kSets + threadIdx.x / kSet;
+  if (row >= (long)min(max(a.cu[a.requests], 0), a.rows) * q_heads) return;
+  const float2* ml = a.part_ml + row * a.splits;
+  const float4* part = (const float4*)(a.part + row * a.splits * D) + at;
+  float top = -INFINITY, whole = 0.0f;
+  for (int s = 0; s < a.splits; ++s) top = fmaxf(top, ml[s].x);
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int s = 0; s < a.splits; ++s) {
+    const float2 x = ml[s];
+    if (x.x == -INFINITY) continue;  // nothing seen there, and nothing written
+    const float w = __builtin_amdgcn_exp2f(x.x - top);
+    const float4 v = part[s * kSet];
+    whole += x.y * w;
+    acc.x = fmaf(v.x, w, acc.x); acc.y = fmaf(v.y, w, acc.y); acc.z = fmaf(v.z, w, acc.z); acc.w = fmaf(v.w, w, acc.w);
+  }
+  T* out = (T*)a.out + row * D + at * 4;
+  const float v[4] = {acc.x, acc.y, acc.z, acc.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) set_result(out[j], whole == 0.0f ? 0.0f : v[j] / whole);
+}
+
 struct Plan {
   int tiles;   // 16-row tiles a workgroup takes
   int blocks;  // row blocks a request is given
@@ -599,6 +658,13 @@ Plan plan_of(const dkv_fp4_attend_args_t& p) {
   const long fill = (kWorkgroups + each - 1) / each, even = p.requests > 1 ? (8 * kWorkgroups + each - 1) / each : 1;
   const long wanted = max(min(fill, (longest + 255) / 256), min(even, (longest + 1023) / 1024));
   plan.splits = (int)min(max(wanted, 1L), (long)kMaxSplits);
+  // Blocks of 64 rows that fill the card once and a half leave half of it idle at the end: two or three splits where that
+  // makes fuller rounds, by more than the join costs.
+  if (plan.splits == 1 && plan.tiles == 4 && longest >= 4096) {
+    const auto rounds = [&](long x) { return (double)((each * x + kWorkgroups - 1) / kWorkgroups) / x; };
+    for (int x = 2; x <= 3; ++x)
+      if (rounds(x) < 0.85 * rounds(plan.splits)) plan.splits = x;
+  }
   while ((long)plan.blocks * plan.splits > 65535) plan.blocks /= 2;
   const long tiles = (longest + 15) / 16;
   plan.share = (int)(((tiles + plan.splits - 1) / plan.splits + 15) / 16 * 16);
@@ -636,9 +702,12 @@ void launch(const AttendArgs& a, const Plan& plan, int q_heads, hipStream_t st) 
   } else {
     if constexpr (wide) hipLaunchKernelGGL((fp4_attend_kernel<D, T, 4, 2>), grid, block, 0, st, a);
   }
-  if (plan.splits > 1) {
-    const long rows = (long)a.rows * q_heads;
+  const long rows = (long)a.rows * q_heads;
+  if (plan.splits > kFewSplits) {
     hipLaunchKernelGGL((fp4_join_kernel<D, T>), dim3((unsigned)rows), dim3(256), 0, st, a, q_heads);
+  } else if (plan.splits > 1) {
+    constexpr int kSets = 1024 / D;
+    hipLaunchKernelGGL((fp4_join_few_kernel<D, T>), dim3((unsigned)((rows + kSets - 1) / kSets)), dim3(256), 0, st, a, q_heads);
   }
 }
 
