@@ -265,7 +265,10 @@ __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_at
       __builtin_memset(out + ((end + x / (a.groups * D)) * q_heads + h * a.groups) * D + x % (a.groups * D), 0, sizeof(T));
   }
 
-  for (int block = blockIdx.y / a.splits; block * (long)kRows < n_rows; block += blocks) {
+  // (the last rows first: they see the most tokens, and the card is left with short work at the end)
+  const long row_blocks = ((long)n_rows + kRows - 1) / kRows;
+  for (long turn = blockIdx.y / a.splits; turn < row_blocks; turn += blocks) {
+    const int block = (int)(row_blocks - 1 - turn);
     const int row0 = block * kRows, row1 = min(row0 + kRows, n_rows);
     // queries: operand B, lane i a row, 8 dimensions of g * D/4 + 8 * step
     frag q[kLean ? 1 : NT][kSteps][kPieces];
