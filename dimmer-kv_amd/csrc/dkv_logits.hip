@@ -1,9 +1,12 @@
 // The logits of replies under penalties for repeated tokens, biases and a grammar's masks, and the token picked
 // (include/dimmerkv.h states the arithmetic).
 //
-// One pass over the logits: a workgroup takes a stretch of a row's vocabulary, counts the history's tokens that fall into
-// it in LDS (integer atomics: the order does not matter), and then streams the stretch once.  Every float32 operation is
-// rounded on its own, in the stated order, so equal inputs stay equal and ties are ties.
+// One pass over the logits: a workgroup takes a stretch of a row's vocabulary.  It loads the stretch into registers, counts
+// meanwhile the history's tokens that fall into it in LDS (integer atomics that return nothing: the order does not matter and
+// nothing waits for them), and writes the stretch, masked.  Each wave lists the counted tokens of its lines as it meets them
+// and takes them 64 at a time, one a lane: there is a division for each, and taken where they stand in the lines, a few
+// lanes of the wave would make it at every place.
+// Every float32 operation is rounded on its own, in the stated order, so equal inputs stay equal and ties are ties.
 #include <math.h>
 
 #include "dkv_device.h"
@@ -12,13 +15,12 @@
 
 namespace {
 
-constexpr uint32_t kSeen = 0x80000000u;  // in a count: the prompt holds the token
-constexpr int kThreads = 512;
+constexpr int kThreads = 1024;
 
 struct LogitsArgs {
   dkv_logits_args_t p;
   uint64_t* partial;  // [rows][chunks] keys of the best token of each stretch; null when there is one stretch
-  int chunk, chunks;  // elements of a stretch, and how many there are
+  int chunks;         // stretches of a row
 };
 
 // Float order as unsigned order; a NaN above all, both zeros the same.
@@ -47,111 +49,212 @@ DKV_DEVICE float logit_value(half_t x) { return (float)x; }
 DKV_DEVICE float logit_value(dkv_bf16 x) { return bf16_bits_to_float(x.bits); }
 DKV_DEVICE void set_logit(float& y, float x) { y = x; }
 DKV_DEVICE void set_logit(half_t& y, float x) { y = (half_t)x; }
-DKV_DEVICE void set_logit(dkv_bf16& y, float x) { y.bits = float_to_bf16_bits(x); }
+DKV_DEVICE void set_logit(dkv_bf16& y, float x) {
+  const __bf16 z = (__bf16)x;
+  __builtin_memcpy(&y.bits, &z, 2);
+}
 
-template <typename T, typename ID, bool BIAS>
-__global__ __launch_bounds__(kThreads) void adjust_logits_kernel(LogitsArgs a) {
+// How often the stretch's tokens occur.  A token takes 16 bits where the history is short enough for 15 of count (the
+// highest bit: the prompt holds it), 32 otherwise.
+template <bool SHORT>
+struct Counts {
+  static constexpr uint32_t kSeen = SHORT ? 0x8000u : 0x80000000u;
+  static DKV_DEVICE uint32_t get(const uint32_t* counts, int at) {
+    return SHORT ? (counts[at >> 1] >> (16 * (at & 1))) & 0xffffu : counts[at];
+  }
+  static DKV_DEVICE void add(uint32_t* counts, int at, bool reply) {
+    uint32_t* word = counts + (SHORT ? at >> 1 : at);
+    const int shift = SHORT ? 16 * (at & 1) : 0;
+    if (reply) atomicAdd(word, 1u << shift);
+    else atomicOr(word, kSeen << shift);
+  }
+};
+
+// A stretch is kThreads * N lines of 16 bytes.  LDS: counts, and a bit a token for those with a bias.
+template <typename T, int N, bool SHORT>
+struct Stretch {
+  static constexpr int V = 16 / sizeof(T), kTokens = kThreads * N * V;
+  static constexpr int kCountWords = SHORT ? kTokens / 2 : kTokens, kBitWords = kTokens / 32;
+  static constexpr int kBytes = 4 * (kCountWords + kBitWords);
+};
+
+template <typename T, typename ID, int N, bool SHORT>
+__global__ __launch_bounds__(kThreads, 8) void adjust_logits_kernel(LogitsArgs a) {
 #pragma clang fp contract(off)
-  constexpr int V = 16 / sizeof(T);
+  using S = Stretch<T, N, SHORT>;
+  using Count = Counts<SHORT>;
+  constexpr int V = S::V, kTokens = S::kTokens;
   extern __shared__ uint32_t lds[];
-  uint32_t* counts = lds;           // [chunk]
-  uint32_t* last = lds + a.chunk;   // [chunk] with biases: place in the row's list, from 1
+  uint32_t* counts = lds;
+  uint32_t* biased = lds + S::kCountWords;
   __shared__ uint64_t bests[kThreads / 64];
   const dkv_logits_args_t& p = a.p;
-  const int row = blockIdx.y, tid = threadIdx.x, vocab = p.vocab;
+  const int row = blockIdx.y, tid = threadIdx.x, lane = tid & 63, vocab = p.vocab;
   const T* logits = (const T*)p.logits + row * p.logits_row;
   T* out = (T*)p.out + row * p.out_row;
-  // Elements are numbered from the 16-byte line the row begins in; a row of any alignment is read in whole lines if its
-  // out row begins alike.
+  // Elements are numbered from the 16-byte line the row begins in; a row of any alignment is read in whole lines, and
+  // written so if its out row begins alike.
   const int shift = (int)((uintptr_t)logits / sizeof(T) % V);
   const bool alike = shift == (int)((uintptr_t)out / sizeof(T) % V);
-  const long first = (long)blockIdx.x * a.chunk - shift;  // token of the stretch's element 0
+  const long first = (long)blockIdx.x * kTokens - shift;  // token of the stretch's element 0
 
-  for (int x = tid * 4; x < a.chunk * (BIAS ? 2 : 1); x += kThreads * 4) *(uint4*)(lds + x) = make_uint4(0, 0, 0, 0);
-  __syncthreads();
-  if (p.tokens) {
-    const int length = min(max(p.lengths[row], 0), p.history), reply = p.reply ? max(p.reply[row], 0) : 0;
-    const ID* tokens = (const ID*)p.tokens + row * p.tokens_row;
-    for (int j = tid; j < length; j += kThreads) {
-      const long id = tokens[j], at = id - first;
-      if (id >= 0 && id < vocab && at >= 0 && at < a.chunk) {
-        if (j >= reply) atomicAdd(counts + at, 1u);
-        else if (!(counts[at] & kSeen)) atomicOr(counts + at, kSeen);
-      }
-    }
+  uint4 lines[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const long token = first + (k * kThreads + tid) * V;
+    if (token >= 0 && token + V <= vocab) lines[k] = *(const uint4*)(logits + token);
   }
-  if (BIAS) {
-    const int lo = max(p.bias_cu[row], 0), hi = min(p.bias_cu[row + 1], p.biases);
-    for (int j = lo + tid; j < hi; j += kThreads) {
-      const long id = p.bias_ids[j], at = id - first;
-      if (id >= 0 && id < vocab && at >= 0 && at < a.chunk) atomicMax(last + at, (uint32_t)(j - lo) + 1);
+  // the history eight tokens a thread at a time, the first of them on their way while LDS is cleared
+  const int length = p.tokens ? min(max(p.lengths[row], 0), p.history) : 0, reply = p.tokens && p.reply ? max(p.reply[row], 0) : 0;
+  const ID* tokens = (const ID*)p.tokens + row * p.tokens_row;
+  constexpr int kBatch = 8;
+  ID id[kBatch];
+  const auto fetch = [&](int j0) {
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const int j = j0 + k * kThreads + tid;
+      id[k] = j < length ? tokens[j] : (ID)-1;
     }
+  };
+  fetch(0);
+  for (int x = tid * 4; x < S::kCountWords + S::kBitWords; x += kThreads * 4) *(uint4*)(lds + x) = make_uint4(0, 0, 0, 0);
+  __syncthreads();
+  for (int j0 = 0; j0 < length; j0 += kBatch * kThreads) {
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const long at = (long)id[k] - first;
+      if (id[k] >= 0 && id[k] < vocab && (uint64_t)at < (uint64_t)kTokens)
+        Count::add(counts, (int)at, j0 + k * kThreads + tid >= reply);
+    }
+    fetch(j0 + kBatch * kThreads);
+  }
+  const int bias0 = p.biases ? max(p.bias_cu[row], 0) : 0, bias1 = p.biases ? min(p.bias_cu[row + 1], p.biases) : 0;
+  for (int j = bias0 + tid; j < bias1; j += kThreads) {
+    const long token = p.bias_ids[j], at = token - first;
+    if (token < 0 || token >= vocab || at < 0 || at >= kTokens) continue;
+    atomicOr(biased + (at >> 5), 1u << (at & 31));
   }
   __syncthreads();
 
-  const float repetition = p.repetition ? p.repetition[row] : 1.0f, presence = p.presence ? p.presence[row] : 0.0f,
-              frequency = p.frequency ? p.frequency[row] : 0.0f;
   const uint32_t* allowed = nullptr;
   if (p.allowed) {
     const int mask = p.allowed_row ? p.allowed_row[row] : row;
     if (mask >= 0 && mask < p.masks) allowed = (const uint32_t*)p.allowed + (long)mask * p.words;
   }
+  const auto may = [&](int token) { return !allowed || ((allowed[token >> 5] >> (token & 31)) & 1); };
   uint64_t best = 0;
-  auto adjust = [&](float x, int at, int token, bool allow) {
-    const uint32_t count = counts[at];
+  float highest = -INFINITY;  // of best; above it all once that is a NaN
+  const auto seen = [&](float x, int token) {
+    best = best_of(best, (uint64_t)order_key(x) << 32 | (uint32_t)~token);
+    highest = x != x ? INFINITY : fmaxf(highest, x);
+  };
+  const float repetition = p.repetition ? p.repetition[row] : 1.0f, presence = p.presence ? p.presence[row] : 0.0f,
+              frequency = p.frequency ? p.frequency[row] : 0.0f;
+  const auto penalized = [&](float x, uint32_t count) {
     if (count) {
       x = x > 0.0f ? x / repetition : x * repetition;
-      const uint32_t n = count & ~kSeen;
-      if (n) {
-        const float less = frequency * (float)n;
+      const uint32_t mentions = count & (Count::kSeen - 1);
+      if (mentions) {
+        const float less = frequency * (float)mentions;
         x = x - (less + presence);
       }
     }
-    if (BIAS) {
-      const uint32_t place = last[at];
-      if (place) x = x + p.bias_values[max(p.bias_cu[row], 0) + (int)place - 1];
-    }
-    if (!allow) x = -INFINITY;
-    best = best_of(best, (uint64_t)order_key(x) << 32 | (uint32_t)~token);
     return x;
   };
-  for (int at = tid * V; at < a.chunk; at += kThreads * V) {
+  // Tokens with a bias keep their logit at first and are taken from there at the end (out may be the logits).
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const int at = (k * kThreads + tid) * V;
     const long token = first + at;
     if (token >= vocab) break;
+    const uint32_t with_bias = p.biases ? biased[at >> 5] >> (at & 31) : 0;
     if (token >= 0 && token + V <= vocab) {
-      uint64_t bits = ~0ull;
+      uint32_t held[SHORT ? V / 2 : V], any = 0, bits = ~0u;
+#pragma unroll
+      for (int v = 0; v < (SHORT ? V / 2 : V); ++v) any |= held[v] = counts[(SHORT ? at / 2 : at) + v];
+      T x[V];
+      float z[V];
+      __builtin_memcpy(x, &lines[k], 16);
       if (allowed) {
         const int word = (int)token >> 5, in = (int)token & 31;
         bits = allowed[word] >> in;
-        if (in + V > 32) bits |= (uint64_t)allowed[word + 1] << (32 - in);
-      }
-      T x[V], y[V];
-      __builtin_memcpy(x, __builtin_assume_aligned(logits + token, 16), 16);
+        if (in + V > 32) bits |= allowed[word + 1] << (32 - in);
 #pragma unroll
-      for (int k = 0; k < V; ++k) set_logit(y[k], adjust(logit_value(x[k]), at + k, (int)token + k, (bits >> k) & 1));
+        for (int v = 0; v < V; ++v)
+          if (!(((bits | with_bias) >> v) & 1)) set_logit(x[v], -INFINITY);
+      }
+#pragma unroll
+      for (int v = 0; v < V; ++v) z[v] = logit_value(x[v]);
+      if (any) {
+        const uint32_t free = bits & ~with_bias;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const uint32_t count = SHORT ? (held[v >> 1] >> (16 * (v & 1))) & 0xffffu : held[v];
+          if (count && (free >> v) & 1) {
+            z[v] = penalized(z[v], count);
+            set_logit(x[v], z[v]);
+          }
+        }
+      }
+      if (with_bias) {
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+          if ((with_bias >> v) & 1) z[v] = -INFINITY;
+      }
+      float top = -INFINITY;  // of the line, whose tokens come after those of best: an equal one does not matter
+      bool odd = false;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        top = fmaxf(top, z[v]);
+        odd = odd || z[v] != z[v];
+      }
+      if (odd || top > highest) {
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+          if (!(z[v] < highest)) seen(z[v], (int)token + v);
+      }
       if (alike) {
-        __builtin_memcpy(__builtin_assume_aligned(out + token, 16), y, 16);
+        __builtin_memcpy(__builtin_assume_aligned(out + token, 16), x, 16);
       } else {
 #pragma unroll
-        for (int k = 0; k < V; ++k) out[token + k] = y[k];
+        for (int v = 0; v < V; ++v) out[token + v] = x[v];
       }
     } else {
-      for (int k = 0; k < V; ++k) {
-        const long t = token + k;
+      for (int v = 0; v < V; ++v) {
+        const long t = token + v;
         if (t < 0 || t >= vocab) continue;
-        const bool allow = !allowed || ((allowed[t >> 5] >> (t & 31)) & 1);
-        set_logit(out[t], adjust(logit_value(logits[t]), at + k, (int)t, allow));
+        if ((with_bias >> v) & 1) {
+          out[t] = logits[t];
+          continue;
+        }
+        const float z = may((int)t) ? penalized(logit_value(logits[t]), Count::get(counts, at + v)) : -INFINITY;
+        seen(z, (int)t);
+        set_logit(out[t], z);
       }
+    }
+  }
+  if (bias1 > bias0) {
+    __syncthreads();
+    for (int j = bias0 + tid; j < bias1; j += kThreads) {
+      const long token = p.bias_ids[j], at = token - first;
+      if (token < 0 || token >= vocab || at < 0 || at >= kTokens) continue;
+      float x = penalized(logit_value(out[token]), Count::get(counts, (int)at));
+      x = x + p.bias_values[j];
+      if (!may((int)token)) x = -INFINITY;
+      seen(x, (int)token);
+      set_logit(out[token], x);
     }
   }
   if (!p.pick) return;
   best = wave_best(best);
-  if ((tid & 63) == 0) bests[tid >> 6] = best;
+  if (lane == 0) bests[tid >> 6] = best;
   __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < kThreads / 64; ++w) best = best_of(best, bests[w]);
-    if (a.partial) a.partial[(long)row * a.chunks + blockIdx.x] = best;
-    else p.pick[row] = picked(best);
+  if (tid < 64) {
+    best = wave_best(tid < kThreads / 64 ? bests[tid] : 0);
+    if (tid == 0) {
+      if (a.partial) a.partial[(long)row * a.chunks + blockIdx.x] = best;
+      else p.pick[row] = picked(best);
+    }
   }
 }
 
@@ -165,11 +268,22 @@ __global__ __launch_bounds__(256) void pick_kernel(const uint64_t* partial, int 
   if (lane == 0) pick[row] = picked(best);
 }
 
-// 32 KB of LDS either way
-int chunk_of(const dkv_logits_args_t& p) { return p.biases ? 4096 : 8192; }
+// Stretches of 16,384 tokens (two or four lines a thread) where that makes two workgroups a CU, as each of them reads the
+// whole history; one line a thread otherwise, for more workgroups.
+struct Plan {
+  bool counts16;
+  int lines, chunks;
+};
 
-// one element of a line at the most in front of a row's first
-int chunks_of(const dkv_logits_args_t& p, int chunk) { return (int)(((long)p.vocab + 8 + chunk - 1) / chunk); }
+Plan plan_of(const dkv_logits_args_t& p) {
+  Plan plan;
+  const int line = p.dtype == DKV_F32 ? 4 : 8, most = 16 / line;  // elements of a line; lines of 16,384
+  const auto chunks = [&](int lines) { return (int)(((long)p.vocab + line - 1 + kThreads * lines * line - 1) / (kThreads * lines * line)); };
+  plan.counts16 = !p.tokens || p.history < 0x8000;
+  plan.lines = plan.counts16 && (long)chunks(most) * p.rows >= 512 ? most : 1;
+  plan.chunks = chunks(plan.lines);
+  return plan;
+}
 
 int check_logits(const dkv_logits_args_t* p, const char* what) {
   DKV_REQUIRE(p, DKV_EINVAL, "%s: null arguments", what);
@@ -186,26 +300,37 @@ int check_logits(const dkv_logits_args_t* p, const char* what) {
   return DKV_OK;
 }
 
+template <typename T, typename ID, int N, bool SHORT>
+int launch(const LogitsArgs& a, hipStream_t st) {
+  constexpr int kBytes = Stretch<T, N, SHORT>::kBytes;
+  if constexpr (kBytes > 64000) {  // past what a kernel may ask for without saying so
+    if (hipFuncSetAttribute((const void*)adjust_logits_kernel<T, ID, N, SHORT>, hipFuncAttributeMaxDynamicSharedMemorySize, kBytes) !=
+        hipSuccess) {
+      (void)hipGetLastError();
+      dkv::set_error("dkv_adjust_logits: no %d bytes of LDS", kBytes);
+      return DKV_ELAUNCH;
+    }
+  }
+  hipLaunchKernelGGL((adjust_logits_kernel<T, ID, N, SHORT>), dim3(a.chunks, a.p.rows), dim3(kThreads), kBytes, st, a);
+  return DKV_OK;
+}
+
 template <typename T, typename ID>
-void launch(const LogitsArgs& a, hipStream_t st) {
-  const dim3 grid(a.chunks, a.p.rows);
-  if (a.p.biases)
-    hipLaunchKernelGGL((adjust_logits_kernel<T, ID, true>), grid, dim3(kThreads), a.chunk * 8, st, a);
-  else
-    hipLaunchKernelGGL((adjust_logits_kernel<T, ID, false>), grid, dim3(kThreads), a.chunk * 4, st, a);
+int launch_plan(const LogitsArgs& a, const Plan& plan, hipStream_t st) {
+  if (plan.lines > 1) return launch<T, ID, (int)sizeof(T), true>(a, st);
+  return plan.counts16 ? launch<T, ID, 1, true>(a, st) : launch<T, ID, 1, false>(a, st);
 }
 
 template <typename T>
-void launch_type(const LogitsArgs& a, hipStream_t st) {
-  if (a.p.token_bytes == 4) launch<T, int32_t>(a, st);
-  else launch<T, int64_t>(a, st);
+int launch_type(const LogitsArgs& a, const Plan& plan, hipStream_t st) {
+  return a.p.token_bytes == 4 ? launch_plan<T, int32_t>(a, plan, st) : launch_plan<T, int64_t>(a, plan, st);
 }
 
 }  // namespace
 
 extern "C" size_t dkv_adjust_logits_workspace_bytes(const dkv_logits_args_t* p) {
   if (check_logits(p, "dkv_adjust_logits_workspace_bytes")) return 0;
-  return (size_t)p->rows * chunks_of(*p, chunk_of(*p)) * sizeof(uint64_t) + 16;
+  return (size_t)p->rows * plan_of(*p).chunks * sizeof(uint64_t) + 16;
 }
 
 extern "C" int dkv_adjust_logits(const dkv_logits_args_t* p, void* workspace, size_t workspace_bytes, void* stream) {
@@ -218,8 +343,8 @@ extern "C" int dkv_adjust_logits(const dkv_logits_args_t* p, void* workspace, si
   DKV_REQUIRE(p->logits_row >= p->vocab && p->out_row >= p->vocab, DKV_ESHAPE, "dkv_adjust_logits: rows overlap");
   LogitsArgs a{};
   a.p = *p;
-  a.chunk = chunk_of(*p);
-  a.chunks = chunks_of(*p, a.chunk);
+  const Plan plan = plan_of(*p);
+  a.chunks = plan.chunks;
   if (p->pick && a.chunks > 1) {
     const size_t need = (size_t)p->rows * a.chunks * sizeof(uint64_t);
     DKV_REQUIRE(workspace && ((uintptr_t)workspace & 15) == 0, DKV_EINVAL, "dkv_adjust_logits: null or misaligned workspace");
@@ -227,9 +352,9 @@ extern "C" int dkv_adjust_logits(const dkv_logits_args_t* p, void* workspace, si
     a.partial = (uint64_t*)workspace;
   }
   hipStream_t st = dkv::as_stream(stream);
-  if (p->dtype == DKV_F32) launch_type<float>(a, st);
-  else if (p->dtype == DKV_F16) launch_type<half_t>(a, st);
-  else launch_type<dkv_bf16>(a, st);
+  const int launched = p->dtype == DKV_F32 ? launch_type<float>(a, plan, st)
+                       : p->dtype == DKV_F16 ? launch_type<half_t>(a, plan, st) : launch_type<dkv_bf16>(a, plan, st);
+  if (launched) return launched;
   if (a.partial)
     hipLaunchKernelGGL(pick_kernel, dim3((p->rows + 3) / 4), dim3(256), 0, st, a.partial, a.chunks, p->rows, p->pick);
   return dkv::check_launch("dkv_adjust_logits");

@@ -29,7 +29,7 @@ class ReplyControls:
           holds, ``presence`` and ``frequency`` are subtracted once and per occurrence in the reply: numbers, or float32
           [rows];
         - ``bias``: added to logits; {token: value} for every row, a list of such dicts by row, or (ids int32,
-          values float32, cu int32 [rows + 1]);
+          values float32, cu int32 [rows + 1]); of an id that a row lists twice the last value counts;
         - ``allowed``: bool [rows, vocab] or [1, vocab] (every row), or (words int32 [masks, ceil(vocab / 32)],
           mask of each row int32 [rows], -1 for none).  ``allow`` changes it later."""
         if rows < 0 or rows > 65535 or vocab < 1:
@@ -79,9 +79,19 @@ class ReplyControls:
         if (ids.dtype != torch.int32 or values.dtype != torch.float32 or cu.dtype != torch.int32 or ids.dim() != 1
                 or ids.shape != values.shape or cu.shape != (self.rows + 1,)):
             raise ValueError(f"ReplyControls: bias must be (int32 [n], float32 [n], int32 [{self.rows + 1}])")
-        for name, t in (("bias_ids", ids), ("bias_values", values), ("bias_cu", cu)):
-            self._hold(name, t.to(self.device).contiguous())
+        ids, values, cu = (t.to(self.device).contiguous() for t in (ids, values, cu))
+        for name, t in (("bias_ids", self._last_of_each(ids, cu)), ("bias_values", values), ("bias_cu", cu)):
+            self._hold(name, t)
         self._args.biases = ids.shape[0]
+
+    def _last_of_each(self, ids: torch.Tensor, cu: torch.Tensor) -> torch.Tensor:
+        """The ids with -1 for all but a row's last mention of each: a stable sort by row and id puts that one last."""
+        if ids.numel() == 0:
+            return ids
+        row = torch.searchsorted(cu, torch.arange(ids.numel(), dtype=torch.int32, device=self.device), right=True)
+        key, place = torch.sort(row * (1 << 32) + ids, stable=True)
+        last = torch.nn.functional.pad(key[1:] != key[:-1], (0, 1), value=True)
+        return torch.empty_like(ids).scatter_(0, place, torch.where(last, ids[place], torch.full_like(ids, -1)))
 
     def allow(self, allowed) -> None:
         """The tokens that may be picked from now on (as ``allowed`` of the constructor, or None for all)."""

@@ -539,7 +539,7 @@ int dkv_fp4_attend(const dkv_fp4_attend_args_t* p, void* workspace, size_t works
  * rounded on its own:
  *   x = x > 0 ? x / repetition : x * repetition   if the row's history holds it
  *   x = x - (frequency * count + presence)        if its reply does, count times
- *   x = x + bias                                  (an id listed twice: the last)
+ *   x = x + bias                                  (the ids of a row's list differ)
  *   x = -infinity                                 if the row's mask has no bit for it
  * and out = x in the logits' type.  pick is the token of the largest x before that
  * last rounding, the lowest one of equals (a NaN counts as largest, as in
@@ -555,7 +555,7 @@ typedef struct dkv_logits_args {
   const float* repetition;   /* [rows] or null: 1 */
   const float* presence;     /* [rows] or null: 0 */
   const float* frequency;    /* [rows] or null: 0 */
-  const int32_t* bias_ids;   /* [biases] */
+  const int32_t* bias_ids;   /* [biases], each once in a row; skipped outside 0 .. vocab - 1 */
   const float* bias_values;  /* [biases] */
   const int32_t* bias_cu;    /* [rows + 1] where each row's biases begin */
   const int32_t* allowed;    /* [masks][words] bit t % 32 of word t / 32: token t may be picked; null: no mask */
