@@ -28,13 +28,9 @@ struct PageArgs {
   int requests, width, shift, pages, rows;
 };
 
+// Running sum of counts below 2^31 over a wave, in two 32-bit scans of 16 bits each.
 DKV_DEVICE long wave_scan_long(long v) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const long other = __shfl_up(v, d);
-    if ((int)__lane_id() >= d) v += other;
-  }
-  return v;
+  return ((long)wave_scan((int)(v >> 16)) << 16) + wave_scan((int)(v & 0xffff));
 }
 
 DKV_DEVICE long pages_of(long tokens, int shift) { return (tokens + (1L << shift) - 1) >> shift; }
@@ -137,7 +133,7 @@ __global__ __launch_bounds__(kPageThreads) void pages_kernel(PageArgs a) {
     }
   }
   if (gridDim.x > 1) {
-    __threadfence();
+    // (what the last one must not overtake are the others' reads, and those have returned; nothing they wrote is read)
     __syncthreads();
     if (tid == 0) last = atomicAdd(a.state + 1, 1) == (int)gridDim.x - 1;
     __syncthreads();
@@ -390,7 +386,7 @@ extern "C" int dkv_page_trim(const dkv_pages_t* p, const int32_t* keep, void* st
   DKV_REQUIRE(keep, DKV_EINVAL, "dkv_page_trim: null pointer");
   // a page a thread at the most: the pages the table can hold
   const long most = min((long)p->requests * p->width, (long)p->pages);
-  const int blocks = (int)min(max((most + kPageThreads - 1) / kPageThreads, 1L), 64L);
+  const int blocks = (int)min(max((most + kPageThreads - 1) / kPageThreads, 1L), 16L);
   hipLaunchKernelGGL(pages_kernel<false>, dim3(blocks), dim3(kPageThreads), p->requests * 2 * sizeof(int),
                      dkv::as_stream(stream), page_args(*p, keep));
   return dkv::check_launch("dkv_page_trim");
