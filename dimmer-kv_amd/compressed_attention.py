@@ -460,8 +460,31 @@ def _stops(token: int, tokenizer) -> bool:
     return token == tokenizer.eos_token_id or token in tokenizer.all_special_ids
 
 
+class _Picker:
+    """The choice of a reply's tokens under controls: the history so far on the GPU, a token longer at each choice."""
+
+    def __init__(self, controls, history: torch.Tensor | None, input_ids: torch.Tensor, max_new_tokens: int):
+        if controls.rows != 1:
+            raise ValueError(f"greedy_answer takes controls of one row (got {controls.rows})")
+        before = [input_ids.reshape(-1)] if history is None else [history.to(input_ids.device).reshape(-1), input_ids.reshape(-1)]
+        prompt = torch.cat(before).to(torch.int64)
+        self.controls, self.length = controls, prompt.numel()
+        self.tokens = torch.cat([prompt, prompt.new_zeros(max_new_tokens)]).unsqueeze(0)
+        self.start = torch.full((1,), self.length, dtype=torch.int32, device=prompt.device)
+
+    def pick(self, logits: torch.Tensor, reply: list[int], grammar) -> int:
+        if grammar is not None:
+            mask = grammar(reply)
+            self.controls.allow(None if mask is None else mask.reshape(1, -1))
+        if reply:
+            self.tokens[0, self.length + len(reply) - 1] = reply[-1]
+        _, pick = self.controls.apply(logits.unsqueeze(0), self.tokens, self.start + len(reply), self.start)
+        return int(pick)
+
+
 def greedy_answer(model, tokenizer, context: CompressedContext | None, cache, input_ids: torch.Tensor,
-                  start_position: int, max_new_tokens: int = 12, evicted=None, stop_at_eos: bool = True):
+                  start_position: int, max_new_tokens: int = 12, evicted=None, stop_at_eos: bool = True, controls=None,
+                  history: torch.Tensor | None = None, grammar=None):
     """Greedy decoding on top of a prefilled cache (scripts/compressed_attention.py:140-169): at most
     ``max_new_tokens`` forward passes, the first over ``input_ids`` (the question) at positions from
     ``start_position``, each later one over the token the previous pass chose; an end-of-sequence or
@@ -469,8 +492,18 @@ def greedy_answer(model, tokenizer, context: CompressedContext | None, cache, in
 
     With ``context`` set, every attention call of the model runs over the compressed tokens directly
     (the HIP decode kernels) and ``cache`` must be ``context.exact_cache``; otherwise ``cache`` is a
-    full cache with optional per-layer ``evicted`` masks.  Returns (text, first-step logits)."""
+    full cache with optional per-layer ``evicted`` masks.  Returns (text, first-step logits).
+
+    ``controls`` (a ``reply_controls.ReplyControls`` of one row) chooses each token under its penalties, biases and
+    masks instead of the plain argmax: the penalties' history is ``history`` (the context's token ids, if wanted), the
+    question and the reply, and the reply's own tokens are the ones counted.  ``grammar`` (with controls) is called with
+    the reply's tokens before each choice and returns a bool [vocabulary] mask of the tokens that may follow, or None
+    for all; the reply ends where it allows none."""
     import dimmer
+
+    if grammar is not None and controls is None:
+        raise ValueError("greedy_answer: a grammar needs controls")
+    picker = None if controls is None else _Picker(controls, history, input_ids, max_new_tokens)
 
     device = input_ids.device
     reply: list[int] = []
@@ -486,7 +519,9 @@ def greedy_answer(model, tokenizer, context: CompressedContext | None, cache, in
                          use_cache=True).logits[0, -1]
             if first_logits is None:
                 first_logits = last.float()
-            token = int(torch.argmax(last))
+            token = int(torch.argmax(last)) if picker is None else picker.pick(last, reply, grammar)
+            if token < 0:
+                break
             if stop_at_eos and _stops(token, tokenizer):
                 break
             reply.append(token)

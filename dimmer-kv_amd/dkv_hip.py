@@ -564,88 +564,117 @@ def gather_cold(stream: Stream, cold, cold_tok_off, idx, refined_base_off: int, 
 
 # ----------------------------------------------------------------- paged 4-bit cache
 
+def _like(t, shape, dtype, index: int) -> bool:
+    """Whether ``t`` is a contiguous ``dtype`` tensor of ``shape`` on GPU ``index``: the quick form of _expect and ptr, for
+    calls whose kernels take a few microseconds."""
+    return t.dtype == dtype and t.shape == shape and t.get_device() == index and t.is_contiguous()
+
+
+def _on_gpu(index: int):
+    """GPU ``index`` as the current device."""
+    return _HERE if _current_device is not None and index == _current_device() else torch.cuda.device(index)
+
+
 def page_assign(pages: Pages, new, rows: int, slots, positions, cu) -> None:
     """Pages for ``new`` int32 [requests] more tokens; slots and positions int64 [rows], cu int32 [requests + 1]."""
-    _expect("page_assign", cu.device, (new, "new", torch.int32, (pages.requests,)), (slots, "slots", torch.int64, (rows,)),
-            (positions, "positions", torch.int64, (rows,)), (cu, "cu", torch.int32, (pages.requests + 1,)))
-    args = ptr(new), rows, ptr(slots), ptr(positions), ptr(cu)
-    with _on_device_of(cu):
-        _check(lib().dkv_page_assign(ctypes.addressof(pages), *args, stream_handle()), "dkv_page_assign")
+    index, requests = cu.get_device(), pages.requests
+    if not (index >= 0 and _like(new, (requests,), torch.int32, index) and _like(slots, (rows,), torch.int64, index)
+            and _like(positions, (rows,), torch.int64, index) and _like(cu, (requests + 1,), torch.int32, index)):
+        _expect("page_assign", cu.device, (new, "new", torch.int32, (requests,)), (slots, "slots", torch.int64, (rows,)),
+                (positions, "positions", torch.int64, (rows,)), (cu, "cu", torch.int32, (requests + 1,)))
+        ptr(new), ptr(slots), ptr(positions), ptr(cu)
+    with _on_gpu(index):
+        _check(lib().dkv_page_assign(ctypes.addressof(pages), addr(new), rows, addr(slots), addr(positions), addr(cu),
+                                     stream_handle()), "dkv_page_assign")
 
 
 def page_trim(pages: Pages, keep) -> None:
     """Requests cut back to at most ``keep`` int32 [requests] tokens, their other pages free again."""
-    _expect("page_trim", keep.device, (keep, "keep", torch.int32, (pages.requests,)))
-    where = ptr(keep)
-    with _on_device_of(keep):
-        _check(lib().dkv_page_trim(ctypes.addressof(pages), where, stream_handle()), "dkv_page_trim")
+    index = keep.get_device()
+    if index < 0 or not _like(keep, (pages.requests,), torch.int32, index):
+        _expect("page_trim", keep.device, (keep, "keep", torch.int32, (pages.requests,)))
+        ptr(keep)
+    with _on_gpu(index):
+        _check(lib().dkv_page_trim(ctypes.addressof(pages), keep.data_ptr(), stream_handle()), "dkv_page_trim")
 
 
-def _fp4_rows(t: torch.Tensor) -> torch.Tensor:
-    """Rows as dkv_fp4_store and dkv_fp4_attend read them: any 16-byte strides over contiguous dimensions, else a copy."""
-    unit = 4 if t.dtype == torch.float32 else 8
-    if t.stride(2) != 1 or t.stride(0) % unit or t.stride(1) % unit or t.data_ptr() % 16:
-        return t.contiguous().clone() if t.is_contiguous() else t.contiguous()
-    return t
+def _strided_rows(t: torch.Tensor):
+    """Rows [n, heads, dim] as dkv_fp4_store and dkv_fp4_attend read them (any 16-byte strides over contiguous dimensions,
+    else a copy): (tensor, address, row stride, head stride)."""
+    row, head, one = t.stride()
+    where = t.data_ptr()
+    if one != 1 or (row | head) % (4 if t.dtype == torch.float32 else 8) or where % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+        row, head, _ = t.stride()
+        where = t.data_ptr()
+    return t, where, row, head
 
 
 def fp4_store(cache: Fp4Cache, key, value, slots) -> None:
     """Rows key and value [n, kv_heads, head_dim] (f32, f16 or bf16) into slots int64 [n]; rows whose slot is negative
     are left out."""
-    n, shape = slots.shape[0], (slots.shape[0], cache.kv_heads, cache.head_dim)
-    code = dtype_code(key.dtype)
-    _expect("fp4_store", slots.device, (slots, "slots", torch.int64, (n,)), (key, "key", key.dtype, shape),
-            (value, "value", key.dtype, shape))
+    index, n, dtype = slots.get_device(), slots.shape[0], key.dtype
+    shape, code = (n, cache.kv_heads, cache.head_dim), dtype_code(dtype)
+    if not (index >= 0 and _like(slots, (n,), torch.int64, index) and key.shape == shape and value.shape == shape
+            and value.dtype == dtype and key.get_device() == index and value.get_device() == index):
+        _expect("fp4_store", slots.device, (slots, "slots", torch.int64, (n,)), (key, "key", dtype, shape),
+                (value, "value", dtype, shape))
+        ptr(slots)
     if n == 0:
         return
-    where, key, value = ptr(slots), _fp4_rows(key), _fp4_rows(value)
-    with _on_device_of(slots):
-        _check(lib().dkv_fp4_store(ctypes.addressof(cache), key.data_ptr(), value.data_ptr(), code, key.stride(0),
-                                   key.stride(1), value.stride(0), value.stride(1), where, n, stream_handle()),
-               "dkv_fp4_store")
+    key, key_at, key_row, key_head = _strided_rows(key)
+    value, value_at, value_row, value_head = _strided_rows(value)
+    with _on_gpu(index):
+        _check(lib().dkv_fp4_store(ctypes.addressof(cache), key_at, value_at, code, key_row, key_head, value_row, value_head,
+                                   slots.data_ptr(), n, stream_handle()), "dkv_fp4_store")
 
 
 def fp4_load(cache: Fp4Cache, slots, key, value) -> None:
     """The values of slots int64 [n] into key and value [n, kv_heads, head_dim]; zeros where a slot is negative."""
-    n, shape = slots.shape[0], (slots.shape[0], cache.kv_heads, cache.head_dim)
-    code = dtype_code(key.dtype)
-    _expect("fp4_load", slots.device, (slots, "slots", torch.int64, (n,)), (key, "key", key.dtype, shape),
-            (value, "value", key.dtype, shape))
+    index, n, dtype = slots.get_device(), slots.shape[0], key.dtype
+    shape, code = (n, cache.kv_heads, cache.head_dim), dtype_code(dtype)
+    if not (index >= 0 and _like(slots, (n,), torch.int64, index) and _like(key, shape, dtype, index)
+            and _like(value, shape, dtype, index)):
+        _expect("fp4_load", slots.device, (slots, "slots", torch.int64, (n,)), (key, "key", dtype, shape),
+                (value, "value", dtype, shape))
+        ptr(slots), ptr(key), ptr(value)
     if n == 0:
         return
-    where, keys, values = ptr(slots), ptr(key), ptr(value)
-    with _on_device_of(slots):
-        _check(lib().dkv_fp4_load(ctypes.addressof(cache), where, n, keys, values, code, stream_handle()), "dkv_fp4_load")
+    with _on_gpu(index):
+        _check(lib().dkv_fp4_load(ctypes.addressof(cache), slots.data_ptr(), n, key.data_ptr(), value.data_ptr(), code,
+                                  stream_handle()), "dkv_fp4_load")
 
 
 def fp4_attend(args: Fp4AttendArgs, query, cu, out=None) -> torch.Tensor:
     """Attention of query [rows, q_heads, head_dim] (f32, f16 or bf16) over the pages of ``args`` (its cache, table and
     lengths, requests, width, scaling, window, longest and most set): out of the same shape and type, whose rows behind
     cu[requests] are left as they are; a new one, with zeros there, if it is None."""
-    rows, q_heads, dim = query.shape
-    args.query_dtype = dtype_code(query.dtype)
-    _expect("fp4_attend", cu.device, (cu, "cu", torch.int32, (args.requests + 1,)),
-            (query, "query", query.dtype, (rows, q_heads, args.cache.head_dim)))
-    args.cu = ptr(cu)
+    index, dtype, shape = cu.get_device(), query.dtype, query.shape
+    rows, q_heads, dim = shape
+    args.query_dtype = dtype_code(dtype)
+    if not (index >= 0 and _like(cu, (args.requests + 1,), torch.int32, index) and query.get_device() == index
+            and dim == args.cache.head_dim):
+        _expect("fp4_attend", cu.device, (cu, "cu", torch.int32, (args.requests + 1,)),
+                (query, "query", dtype, (rows, q_heads, args.cache.head_dim)))
+        ptr(cu)
     args.fill = out is None
     if out is None:
-        out = torch.empty(rows, q_heads, dim, dtype=query.dtype, device=query.device)
-    else:
-        _expect("fp4_attend", cu.device, (out, "out", query.dtype, (rows, q_heads, dim)))
-        if not out.is_contiguous() or out.data_ptr() % 16:
-            raise ValueError("fp4_attend: out must be contiguous and 16-byte aligned")
+        out = torch.empty(shape, dtype=dtype, device=query.device)
+    elif not _like(out, shape, dtype, index) or out.data_ptr() % 16:
+        _expect("fp4_attend", cu.device, (out, "out", dtype, shape))
+        raise ValueError("fp4_attend: out must be contiguous and 16-byte aligned")
     if rows == 0:
         return out
-    query = _fp4_rows(query)
-    args.query, args.query_token, args.query_head = query.data_ptr(), query.stride(0), query.stride(1)
-    args.out, args.rows, args.q_heads = out.data_ptr(), rows, q_heads
-    where = ctypes.addressof(args)
-    need = lib().dkv_fp4_attend_workspace_bytes(where)
+    query, args.query, args.query_token, args.query_head = _strided_rows(query)
+    args.cu, args.out, args.rows, args.q_heads = cu.data_ptr(), out.data_ptr(), rows, q_heads
+    where, library = ctypes.addressof(args), lib()
+    need = library.dkv_fp4_attend_workspace_bytes(where)
     if need == 0:
         _check(-2, "dkv_fp4_attend_workspace_bytes")
-    with _on_device_of(cu):
-        workspace = torch.empty(need, dtype=torch.uint8, device=query.device)
-        _check(lib().dkv_fp4_attend(where, workspace.data_ptr(), need, stream_handle()), "dkv_fp4_attend")
+    with _on_gpu(index):
+        workspace = torch.empty(need, dtype=torch.uint8, device=query.device) if need > 16 else None
+        _check(library.dkv_fp4_attend(where, workspace.data_ptr() if need > 16 else None, need, stream_handle()),
+               "dkv_fp4_attend")
     return out
 
 
@@ -653,44 +682,56 @@ def adjust_logits(args: LogitsArgs, logits, tokens=None, lengths=None, reply=Non
     """logits [rows, vocab] (f32, f16 or bf16) under the controls of ``args`` (its penalties, biases and masks set) ->
     (out of the same shape and type, pick int64 [rows]).  ``tokens`` [rows, history] int32 or int64 with lengths and
     reply int32 [rows]; ``out`` may be the logits."""
-    rows, vocab = args.rows, args.vocab
-    args.dtype = dtype_code(logits.dtype)
-    _expect("adjust_logits", logits.device, (logits, "logits", logits.dtype, (rows, vocab)))
-    if not logits.is_cuda:
+    index, dtype, rows, vocab = logits.get_device(), logits.dtype, args.rows, args.vocab
+    args.dtype = dtype_code(dtype)
+    if index < 0 or logits.shape != (rows, vocab):
+        _expect("adjust_logits", logits.device, (logits, "logits", dtype, (rows, vocab)))
         raise ValueError("dimmer-kv HIP kernels need GPU tensors (no CPU path)")
-    if logits.stride(1) != 1 or (rows > 1 and logits.stride(0) < vocab):
+    row, one = logits.stride()
+    if one != 1 or (rows > 1 and row < vocab):
         if out is logits:
             raise ValueError("adjust_logits: logits changed in place need rows of unit stride that do not overlap")
-        logits = logits.contiguous()
+        logits = logits.clone(memory_format=torch.contiguous_format)
+        row = vocab
+    # (the stride of a single row says nothing)
+    args.logits, args.logits_row = logits.data_ptr(), max(row, vocab)
     if out is None:
-        out = torch.empty(rows, vocab, dtype=logits.dtype, device=logits.device)
-    elif out is not logits:
-        _expect("adjust_logits", logits.device, (out, "out", logits.dtype, (rows, vocab)))
-        if out.stride(1) != 1 or (rows > 1 and out.stride(0) < vocab):
+        out = torch.empty(rows, vocab, dtype=dtype, device=logits.device)
+        args.out_row = vocab
+    else:
+        out_row, one = out.stride() if out.dim() == 2 else (0, 0)
+        if out.shape != (rows, vocab) or out.dtype != dtype or out.get_device() != index:
+            _expect("adjust_logits", logits.device, (out, "out", dtype, (rows, vocab)))
+        if one != 1 or (rows > 1 and out_row < vocab):
             raise ValueError("adjust_logits: out needs rows of unit stride that do not overlap")
+        args.out_row = max(out_row, vocab)
+    args.out = out.data_ptr()
     args.tokens = args.lengths = args.reply = None
     if tokens is not None:
         if tokens.dtype not in (torch.int32, torch.int64) or tokens.dim() != 2 or (
                 tokens.shape[1] > 1 and tokens.stride(1) != 1):
             raise ValueError("adjust_logits: tokens must be int32 or int64 [rows, history] with contiguous rows")
-        _expect("adjust_logits", logits.device, (tokens, "tokens", tokens.dtype, (rows, tokens.shape[1])),
-                (lengths, "lengths", torch.int32, (rows,)))
-        args.tokens, args.lengths, args.tokens_row = addr(tokens), ptr(lengths), tokens.stride(0)
-        args.history, args.token_bytes = tokens.shape[1], tokens.element_size()
+        history = tokens.shape[1]
+        if tokens.shape[0] != rows or tokens.get_device() != index or not _like(lengths, (rows,), torch.int32, index):
+            _expect("adjust_logits", logits.device, (tokens, "tokens", tokens.dtype, (rows, history)),
+                    (lengths, "lengths", torch.int32, (rows,)))
+            ptr(lengths)
+        args.tokens, args.lengths, args.tokens_row = addr(tokens), addr(lengths), tokens.stride(0)
+        args.history, args.token_bytes = history, tokens.element_size()
         if reply is not None:
-            _expect("adjust_logits", logits.device, (reply, "reply", torch.int32, (rows,)))
-            args.reply = ptr(reply)
+            if not _like(reply, (rows,), torch.int32, index):
+                _expect("adjust_logits", logits.device, (reply, "reply", torch.int32, (rows,)))
+                ptr(reply)
+            args.reply = addr(reply)
+    where, library = ctypes.addressof(args), lib()
+    need = library.dkv_adjust_logits_workspace_bytes(where)
+    if need == 0:
+        _check(-2, "dkv_adjust_logits_workspace_bytes")
     pick = torch.empty(rows, dtype=torch.int64, device=logits.device)
     if rows == 0:
         return out, pick
-    args.logits, args.out, args.pick = logits.data_ptr(), out.data_ptr(), pick.data_ptr()
-    # (the stride of a single row says nothing)
-    args.logits_row, args.out_row = max(logits.stride(0), vocab), max(out.stride(0), vocab)
-    where = ctypes.addressof(args)
-    need = lib().dkv_adjust_logits_workspace_bytes(where)
-    if need == 0:
-        _check(-2, "dkv_adjust_logits_workspace_bytes")
-    with _on_device_of(logits):
+    args.pick = pick.data_ptr()
+    with _on_gpu(index):
         workspace = torch.empty(need, dtype=torch.uint8, device=logits.device)
-        _check(lib().dkv_adjust_logits(where, workspace.data_ptr(), need, stream_handle()), "dkv_adjust_logits")
+        _check(library.dkv_adjust_logits(where, workspace.data_ptr(), need, stream_handle()), "dkv_adjust_logits")
     return out, pick

@@ -5,6 +5,9 @@ method-name mini-language and its error messages).
 Served names (scripts/methods.py:1-33):
 
 - ``full``: the uncompressed cache (control).
+- ``fp4``: every token in 4 bits (paged_cache.PagedContext, 4.25 bits a value; no counterpart in the reference).  ``stored``
+  is the context: ``greedy_answer(model, tokenizer, stored, stored.exact_cache, ...)`` answers over its pages; ``keys`` /
+  ``values`` are rebuilt from them on first access.
 - ``prog@<budget>[:snap][:r<frac>]``: progressive bit-plane kvtc with a hot tier of ``budget``
   and question-time refinement of the top ``frac`` tokens (scripts/methods.py:227-254).  The
   returned ``Compressed`` carries ``stored`` (the packed cache: ``stored.context(q_heads,
@@ -63,10 +66,12 @@ class Compressed:
 
 
 def budget_of(name: str) -> float:
-    """Nominal memory budget of a method name: 1.0 for ``full``, the number after ``@`` (or after
+    """Nominal memory budget of a method name: 1.0 for ``full``, 4.25 of 16 bits for ``fp4``, the number after ``@`` (or after
     the first ``:`` of ``h2o:``/``dkv:`` names), NaN when the name implies none."""
     if name == "full":
         return 1.0
+    if name == "fp4":
+        return 4.25 / 16
     head, sep, rest = name.partition("@")
     if sep:
         return float(rest.split(":", 1)[0])
@@ -166,11 +171,24 @@ class Methods:
             total = 2 * 2 * len(keys) * keys[0].numel()  # FP16 keys and values
             return Compressed(keys, values, None, total, 0.0,
                               token_bytes=torch.full((tokens,), total / tokens, device=self.device))
+        if name == "fp4":
+            return self._fp4(keys, values)
         if name.startswith("prog@"):
             return self._progressive(name, keys, values, scores)
         if name.startswith(KVTC_PREFIXES):
             return self._kvtc(name, keys, values, scores)
-        raise ValueError(f"method {name!r} is not served by this package (full, prog@, kvtc@, kvtcf@, dkvtc@ are)")
+        raise ValueError(f"method {name!r} is not served by this package (full, fp4, prog@, kvtc@, kvtcf@, dkvtc@ are)")
+
+    def _fp4(self, keys, values) -> Compressed:
+        if self._model is None:
+            raise ValueError("fp4 needs Methods(..., model=model) for the model's cache configuration.")
+        from paged_cache import PagedContext
+
+        stored, seconds = self._timed(lambda: PagedContext(keys, values, self._model))
+        tokens, dtype = keys[0].shape[2], keys[0].dtype
+        per_token = torch.full((tokens,), float(stored.token_bytes()), device=self.device)
+        return Compressed(None, None, None, tokens * stored.token_bytes(), seconds, token_bytes=per_token, stored=stored,
+                          rebuild=lambda: stored.rebuilt(dtype))
 
     def _kvtc(self, name: str, keys, values, scores) -> Compressed:
         plan = _kvtc_plan(name, scores)

@@ -14,6 +14,9 @@ the GPU or reads from it, so a step can be captured in a HIP graph.  A step of a
     cache.trim(keep)                                  # finished requests, refused drafts
 
 Calls on one cache share its tables and belong on one stream (or on streams the caller orders).
+
+``PagedContext`` is the cache of one conversation behind a Hugging Face model: an attention context like
+``CompressedContext`` (``dimmer.STATE.compressed``, ``greedy_answer``), whose new tokens go into the pages too.
 """
 
 from __future__ import annotations
@@ -102,8 +105,8 @@ class PagedCache:
             raise ValueError("assign: a GPU tensor of new tokens needs rows, the step's number of rows")
         if rows < 0:
             raise ValueError(f"assign: {rows} rows")
-        places = torch.empty(2, rows, dtype=torch.int64, device=self.device)
-        step = Step(places[0], places[1], torch.empty(self.requests + 1, dtype=torch.int32, device=self.device), rows,
+        slots, positions = torch.empty(2, rows, dtype=torch.int64, device=self.device).unbind()
+        step = Step(slots, positions, torch.empty(self.requests + 1, dtype=torch.int32, device=self.device), rows,
                     self.table_pages * self.page if longest is None else longest, rows if most is None else most)
         dkv_hip.page_assign(self._pages, self._counts(new), rows, step.slots, step.positions, step.cu)
         return step
@@ -166,7 +169,7 @@ class PagedCache:
         if window is not None and not 1 <= window < 1 << 31:
             raise ValueError(f"attend_rows: window {window}")
         self._here(step.cu, "attend_rows")
-        args = self._attend[layer]
+        args = dkv_hip.Fp4AttendArgs.from_buffer_copy(self._attend[layer])
         args.scaling = self.head_dim ** -0.5 if scaling is None else scaling
         args.window = window or 0
         args.longest, args.most = min(max(step.longest, 1), (1 << 31) - 1), min(max(step.most, 1), (1 << 31) - 1)
@@ -179,4 +182,81 @@ class PagedCache:
             self.free_count, self._state))
 
 
-__all__ = ["PagedCache", "Step"]
+class PagedContext:
+    """One conversation in a paged 4-bit cache, attended to directly: the ``attend`` contract of
+    ``compressed_attention.CompressedContext`` for the ``dimmer`` hook.  Every forward's new keys and values are stored
+    before they are attended to, in 4 bits as all others, so ``exact_cache`` (the cache the model updates) only carries
+    them here: it starts empty.  Attention is causal over all tokens; the model's additive mask is not read."""
+
+    def __init__(self, keys: list[torch.Tensor], values: list[torch.Tensor], model, page: int = 64, room: int = 1024):
+        """Per-layer [1, kv_heads, tokens, head_dim] keys (RoPE applied) and values on the GPU, with room for ``room`` more
+        tokens."""
+        first = keys[0]
+        shape = first.shape
+        if len(keys) != len(values) or len(shape) != 4 or shape[0] != 1:
+            raise ValueError(f"PagedContext takes one conversation's per-layer [1, heads, tokens, head_dim] caches "
+                             f"(got {len(keys)} and {len(values)} of {list(shape)})")
+        if room < 0:
+            raise ValueError(f"PagedContext: room {room}")
+        _, heads, tokens, dim = shape
+        pages = max(1, -(-(tokens + room) // page))
+        self.cache = PagedCache(len(keys), heads, dim, pages, page=page, device=first.device)
+        self.capacity, self.tokens = pages * page, tokens
+        self._model = model
+        step = self.cache.assign([tokens], longest=tokens)
+        for layer, (key, value) in enumerate(zip(keys, values)):
+            if key.shape != shape or value.shape != shape:
+                raise ValueError(f"layer {layer}: keys {list(key.shape)} and values {list(value.shape)}, not {list(shape)}")
+            self.cache.store(layer, key[0].transpose(0, 1), value[0].transpose(0, 1), step)
+        self._step = None
+        self.exact_cache = self.fresh_cache()
+
+    def fresh_cache(self):
+        """An empty cache for the model to update: one for every answer."""
+        from transformers import DynamicCache
+
+        return DynamicCache(config=self._model.config)
+
+    def token_bytes(self) -> int:
+        """Bytes of codes and exponents a token takes over all layers."""
+        c = self.cache
+        return 2 * c.layers * c.kv_heads * (c.head_dim // 2 + c.head_dim // 32)
+
+    def rewind(self, tokens: int) -> None:
+        """Forget everything behind the first ``tokens`` tokens (an answered question, say)."""
+        if not 0 <= tokens <= self.tokens:
+            raise ValueError(f"rewind to {tokens} of {self.tokens} tokens")
+        self.cache.trim([tokens])
+        self.tokens, self._step = tokens, None
+        self.exact_cache = self.fresh_cache()
+
+    def rebuilt(self, dtype: torch.dtype = torch.float16):
+        """(keys, values): per-layer [1, kv_heads, tokens, head_dim] caches of the values held."""
+        slots = self.cache.slots(0, 0, self.tokens)
+        rows = [self.cache.load(layer, slots, dtype) for layer in range(self.cache.layers)]
+        return ([key.transpose(0, 1).contiguous().unsqueeze(0) for key, _ in rows],
+                [value.transpose(0, 1).contiguous().unsqueeze(0) for _, value in rows])
+
+    def attend(self, module, query, key, value, attention_mask, scaling):
+        """Same contract as an HF attention function: returns (output [1, T, H, D], None)."""
+        layer, c = module.layer_idx, self.cache
+        batch, q_heads, new, _ = query.shape
+        if batch != 1:
+            raise ValueError("PagedContext takes one conversation")
+        if module.num_key_value_groups * c.kv_heads != q_heads:
+            raise ValueError("module.num_key_value_groups does not match the cache's KV heads")
+        if key is None or key.shape[2] < new:
+            raise ValueError("PagedContext needs the new tokens' keys in the model's cache")
+        if layer == 0:  # a forward begins: pages for its tokens
+            if self.tokens + new > self.capacity:
+                raise ValueError(f"{self.tokens} + {new} tokens pass the {self.capacity} the context has pages for")
+            self._step = c.assign([new], longest=self.tokens + new)
+            self.tokens += new
+        elif self._step is None or self._step.rows != new:
+            raise ValueError("PagedContext: a forward starts at layer 0")
+        past = key.shape[2] - new
+        c.store(layer, key[0, :, past:].transpose(0, 1), value[0, :, past:].transpose(0, 1), self._step)
+        return c.attend_rows(layer, query[0].transpose(0, 1), self._step, scaling=scaling).unsqueeze(0), None
+
+
+__all__ = ["PagedCache", "PagedContext", "Step"]

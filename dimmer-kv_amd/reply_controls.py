@@ -131,7 +131,7 @@ class ReplyControls:
             raise ValueError(f"ReplyControls: logits must be on {self.device} (got {logits.device})")
         if tokens is not None and lengths is None:
             lengths = torch.full((self.rows,), tokens.shape[1], dtype=torch.int32, device=self.device)
-        return dkv_hip.adjust_logits(self._args, logits, tokens, lengths, reply_start, out)
+        return dkv_hip.adjust_logits(dkv_hip.LogitsArgs.from_buffer_copy(self._args), logits, tokens, lengths, reply_start, out)
 
 
 __all__ = ["ReplyControls", "pack_allowed"]
