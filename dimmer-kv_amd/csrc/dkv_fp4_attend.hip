@@ -27,7 +27,6 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 
-constexpr int kWaves = 4;
 constexpr int kMaxSplits = 256, kFewSplits = 4;
 
 struct AttendArgs {
@@ -229,7 +228,7 @@ DKV_DEVICE void load_values(const AttendArgs& a, const Tiles<CH>& tiles, const L
   }
 }
 
-template <int D, typename T, int NT, int CH>
+template <int D, typename T, int NT, int CH, int kWaves>
 __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_attend_kernel(AttendArgs a) {
   using Op = Operand<T>;
   using frag = typename Op::frag;
@@ -243,7 +242,7 @@ __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_at
   // (one fills the other's waits): queries lie in LDS, and a chunk's loads follow the last use of the one before.
   constexpr bool kLean = NT == 4;
   __shared__ frag held[kLean ? NT * kSteps * 64 : 1];
-  __shared__ float sums[kWaves * 16 * kStride];
+  __shared__ float sums[4 * 16 * kStride];
   __shared__ float stat[2][kWaves][kRows];
 
   const int h = blockIdx.x, b = blockIdx.z, split = blockIdx.y % a.splits, blocks = gridDim.y / a.splits;
@@ -498,7 +497,7 @@ __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_at
       }
     }
 
-    // the four waves' sums, 16 rows at a time
+    // the waves' sums, 16 rows at a time and four waves at a time
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const float total = sum_xor32(sum_xor16(l[nt]));
@@ -508,45 +507,64 @@ __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_at
       }
     }
     __syncthreads();
-    const int row = threadIdx.x >> 4, part = threadIdx.x & 15;  // in the join: a row, and kLane of its dimensions
+    constexpr int kParts = kWaves * 4, kPart = D / kParts;
+    const int row = threadIdx.x / kParts, part = threadIdx.x % kParts;  // in the join: a row, and kPart of its dimensions
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       float top = -INFINITY;
 #pragma unroll
       for (int x = 0; x < kWaves; ++x) top = fmaxf(top, stat[0][x][nt * 16 + i]);
       const float factor = m[nt] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[nt] - top);
-      float* mine = sums + (wave * 16 + i) * kStride + g * (D / 4);
+      float* mine = sums + ((wave & 3) * 16 + i) * kStride + g * (D / 4);
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
+      for (int j = 0; j < kLane; ++j) o[nt][j] *= factor;
+      if constexpr (kWaves == 8) {
+        if (wave >= 4) {
 #pragma unroll
-        for (int j = 0; j < kLane; ++j) mine[r * kLane + j] = o[nt][j][r] * factor;
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int j = 0; j < kLane; ++j) mine[r * kLane + j] = o[nt][j][r];
+        }
+        __syncthreads();
+        if (wave < 4) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int j = 0; j < kLane; ++j) mine[r * kLane + j] += o[nt][j][r];
+        }
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int j = 0; j < kLane; ++j) mine[r * kLane + j] = o[nt][j][r];
+      }
       __syncthreads();
       const int r = row0 + nt * 16 + row;
       if (r < n_rows) {
-        float highest = -INFINITY, total = 0.0f, acc[kLane] = {};
+        float highest = -INFINITY, total = 0.0f, acc[kPart] = {};
 #pragma unroll
         for (int x = 0; x < kWaves; ++x) highest = fmaxf(highest, stat[0][x][nt * 16 + row]);
 #pragma unroll
         for (int x = 0; x < kWaves; ++x) {
           const float mx = stat[0][x][nt * 16 + row];
           total += mx == -INFINITY ? 0.0f : stat[1][x][nt * 16 + row] * __builtin_amdgcn_exp2f(mx - highest);
-#pragma unroll
-          for (int j = 0; j < kLane; ++j) acc[j] += sums[(x * 16 + row) * kStride + part * kLane + j];
         }
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+#pragma unroll
+          for (int j = 0; j < kPart; ++j) acc[j] += sums[(x * 16 + row) * kStride + part * kPart + j];
         const int token = r / a.groups;
         const long out_row = (long)(q0 + token) * q_heads + h * a.groups + (r - token * a.groups);
         if (a.splits == 1) {
-          T* out = (T*)a.out + out_row * D + part * kLane;
+          T* out = (T*)a.out + out_row * D + part * kPart;
           const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
 #pragma unroll
-          for (int j = 0; j < kLane; ++j) {
-            set_result(out[j], total == 0.0f ? 0.0f : acc[j] * inverse);
-          }
+          for (int j = 0; j < kPart; ++j) set_result(out[j], total == 0.0f ? 0.0f : acc[j] * inverse);
         } else {
           if (highest != -INFINITY) {
-            float* out = a.part + (out_row * a.splits + split) * D + part * kLane;
+            float* out = a.part + (out_row * a.splits + split) * D + part * kPart;
 #pragma unroll
-            for (int j = 0; j < kLane; ++j) out[j] = acc[j];
+            for (int j = 0; j < kPart; ++j) out[j] = acc[j];
           }
           if (part == 0) a.part_ml[out_row * a.splits + split] = make_float2(highest, total);
         }
@@ -639,12 +657,13 @@ __global__ __launch_bounds__(256) void fp4_join_few_kernel(AttendArgs a, int q_h
 
 struct Plan {
   int tiles;   // 16-row tiles a workgroup takes
+  int waves;   // of a workgroup
   int blocks;  // row blocks a request is given
   int splits;
   int share;   // 16-token tiles a split takes at the least
 };
 
-constexpr long kWorkgroups = 512;
+constexpr long kWorkgroups = 512;  // of four waves: what the card holds at two waves a SIMD
 
 Plan plan_of(const dkv_fp4_attend_args_t& p) {
   Plan plan;
@@ -653,14 +672,20 @@ Plan plan_of(const dkv_fp4_attend_args_t& p) {
   plan.tiles = rows <= 16 || (p.query_dtype == DKV_F32 && p.cache.head_dim == 256) ? 1 : rows <= 32 || narrow ? 2 : 4;
   const long blocks = (rows + plan.tiles * 16 - 1) / (plan.tiles * 16);
   plan.blocks = (int)(blocks < 4096 ? blocks : 4096);
-  // Workgroups enough for the card, of 256 tokens at the least; of 1,024 where that makes more than the card holds at
-  // once, so that requests of different lengths even out.
   const long each = (long)p.requests * p.cache.kv_heads * plan.blocks;
   long longest = p.longest < 1 ? 1 : p.longest;  // the tokens a row block may see
   if (p.window) longest = min(longest, (long)p.window + plan.tiles * 16 / groups + 16);
+  // Workgroups enough for the card, of 256 tokens at the least; of 1,024 where that makes more than the card holds at
+  // once, so that requests of different lengths even out.
   const long fill = (kWorkgroups + each - 1) / each, even = p.requests > 1 ? (8 * kWorkgroups + each - 1) / each : 1;
   const long wanted = max(min(fill, (longest + 255) / 256), min(even, (longest + 1023) / 1024));
-  plan.splits = (int)min(max(wanted, 1L), (long)kMaxSplits);
+  // Short requests of few rows are not split: eight waves take them in two turns, four where requests alone fill the card.
+  // In a captured graph, 8 KV heads of 128 bfloat16 dimensions: 700 tokens of 32 requests 9.1 us against 13.5 split and
+  // joined, 2,000 of them 16.5 against 18.8; one request of 500 tokens 8.2 against 9.0, of 1,000 10.3 against 9.7, of 2,000
+  // 14.1 against 9.0.  Called from Python the second launch costs 3 us more.
+  const long brief = p.cache.head_dim < 256 ? 1024 : p.query_dtype == DKV_F32 ? 256 : 512;
+  plan.waves = plan.tiles == 1 && longest <= (each >= 256 ? 2 * brief : brief) ? 8 : 4;
+  plan.splits = plan.waves == 8 ? 1 : (int)min(max(wanted, 1L), (long)kMaxSplits);
   // Blocks of 64 rows that fill the card once and a half leave half of it idle at the end: two or three splits where that
   // makes fuller rounds, by more than the join costs.
   if (plan.splits == 1 && plan.tiles == 4 && longest >= 4096) {
@@ -696,14 +721,15 @@ size_t part_bytes(const dkv_fp4_attend_args_t& p, const Plan& plan) {
 
 template <int D, typename T>
 void launch(const AttendArgs& a, const Plan& plan, int q_heads, hipStream_t st) {
-  const dim3 grid(a.c.kv_heads, plan.blocks * plan.splits, a.requests), block(kWaves * 64);
+  const dim3 grid(a.c.kv_heads, plan.blocks * plan.splits, a.requests), block(plan.waves * 64);
   constexpr bool wide = D < 256 && sizeof(T) == 2;
   if (plan.tiles == 1) {
-    hipLaunchKernelGGL((fp4_attend_kernel<D, T, 1, D == 256 ? 2 : 4>), grid, block, 0, st, a);
+    if (plan.waves == 8) hipLaunchKernelGGL((fp4_attend_kernel<D, T, 1, D == 256 ? 2 : 4, 8>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((fp4_attend_kernel<D, T, 1, D == 256 ? 2 : 4, 4>), grid, block, 0, st, a);
   } else if (plan.tiles == 2) {
-    if constexpr (D < 256 || sizeof(T) == 2) hipLaunchKernelGGL((fp4_attend_kernel<D, T, 2, 2>), grid, block, 0, st, a);
+    if constexpr (D < 256 || sizeof(T) == 2) hipLaunchKernelGGL((fp4_attend_kernel<D, T, 2, 2, 4>), grid, block, 0, st, a);
   } else {
-    if constexpr (wide) hipLaunchKernelGGL((fp4_attend_kernel<D, T, 4, 2>), grid, block, 0, st, a);
+    if constexpr (wide) hipLaunchKernelGGL((fp4_attend_kernel<D, T, 4, 2, 4>), grid, block, 0, st, a);
   }
   const long rows = (long)a.rows * q_heads;
   if (plan.splits > kFewSplits) {
