@@ -13,8 +13,8 @@
 // K is exact in bfloat16 and float16 alike, V in float16 (the exponents are clamped for that).  Queries go in as they are
 // (float32 as three bfloat16 pieces that add up to it).  The weights are rounded to float16, 2^-11 relative, and are held
 // times 2^8 so that weights down to 2^-22 of the row's reference keep that (smaller ones are off by 2^-33 of it): an eighth
-// of a bfloat16 result's own rounding.  Float32 results take a second piece of the weights, held times 2^15.  Sums, maxima
-// and accumulators are float32.
+// of a bfloat16 result's own rounding, as much as a float16 one's.  Float16 results of up to 32 rows take a second piece of
+// the weights, and so do float32 results, held times 2^15.  Sums, maxima and accumulators are float32.
 #include <math.h>
 
 #include "dkv_device.h"
@@ -233,10 +233,12 @@ __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_at
   using Op = Operand<T>;
   using frag = typename Op::frag;
   constexpr int kRows = 16 * NT, kSteps = D / 32, kLane = D / 16, kPieces = Op::kPieces;
-  constexpr int kWeights = kPieces == 1 ? 1 : 2;  // float16 pieces of a weight
+  // float16 pieces of a weight: a second one for float32 results, and for float16 ones where the memory is what bounds
+  // (the products of up to 32 rows are free there)
+  constexpr int kWeights = kPieces > 1 || (__is_same(T, half_t) && NT <= 2) ? 2 : 1;
   // Weights are held times 2^kShift, against a reference that scores may pass by kSlack: 2^15 at the most, below the
   // largest float16.
-  constexpr float kSlack = kWeights == 1 ? 7.0f : 0.0f, kShift = 15.0f - kSlack;
+  constexpr float kSlack = kPieces == 1 ? 7.0f : 0.0f, kShift = 15.0f - kSlack;
   constexpr int kStride = D + 4;                  // a row of sums in LDS
   // With 64 rows the accumulators leave no registers for the queries and a second chunk, and two waves a SIMD matter more
   // (one fills the other's waits): queries lie in LDS, and a chunk's loads follow the last use of the one before.
