@@ -3,11 +3,36 @@
 
 #include <stdint.h>
 
+#include "dkv_device.h"
 #include "dkv_host.h"
 #include "dimmerkv.h"
 
 typedef float floatx2 __attribute__((ext_vector_type(2)));
 struct dkv_bf16 { uint16_t bits; };
+
+#ifdef __HIPCC__
+// Results that one workgroup leaves for another of the same launch, on whatever die.  They are written and read at the
+// device's scope, past the dies' own caches, so that neither side has to flush or drop a cache; `left_behind` waits until a
+// wave's are there, and after a barrier one thread of the workgroup may announce them.
+DKV_DEVICE void leave(uint64_t* at, uint64_t v) { __hip_atomic_store(at, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+DKV_DEVICE uint64_t pick_up(const uint64_t* at) {
+  return __hip_atomic_load((uint64_t*)at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+DKV_DEVICE void leave2(float* at, float a, float b) {
+  leave((uint64_t*)at, (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a));
+}
+DKV_DEVICE float2 pick_up2(const float* at) {
+  const uint64_t v = pick_up((const uint64_t*)at);
+  return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
+}
+DKV_DEVICE void left_behind() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// Whether this is the last of `all` announcements on a word that is 0 before the first one, and 0 again after the last.
+DKV_DEVICE bool last_of(uint32_t* word, uint32_t all) {
+  if (__hip_atomic_fetch_add(word, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != all - 1) return false;
+  __hip_atomic_store(word, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return true;
+}
+#endif
 
 namespace dkv {
 

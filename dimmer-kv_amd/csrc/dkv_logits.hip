@@ -251,10 +251,26 @@ __global__ __launch_bounds__(kThreads, 8) void adjust_logits_kernel(LogitsArgs a
   __syncthreads();
   if (tid < 64) {
     best = wave_best(tid < kThreads / 64 ? bests[tid] : 0);
-    if (tid == 0) {
-      if (a.partial) a.partial[(long)row * a.chunks + blockIdx.x] = best;
-      else p.pick[row] = picked(best);
+    if (!a.partial) {
+      if (tid == 0) p.pick[row] = picked(best);
+      return;
     }
+    uint64_t* partial = a.partial + (long)row * a.chunks;
+    if (!p.arrivals) {
+      if (tid == 0) partial[blockIdx.x] = best;
+      return;
+    }
+    bool last = false;
+    if (tid == 0) {
+      leave(partial + blockIdx.x, best);
+      left_behind();
+      last = last_of(p.arrivals + row, a.chunks);
+    }
+    if (!__any(last)) return;
+    best = 0;
+    for (int c = tid; c < a.chunks; c += 64) best = best_of(best, pick_up(partial + c));
+    best = wave_best(best);
+    if (tid == 0) p.pick[row] = picked(best);
   }
 }
 
@@ -293,6 +309,7 @@ int check_logits(const dkv_logits_args_t* p, const char* what) {
   DKV_REQUIRE(p->history >= 0 && p->biases >= 0 && p->masks >= 0, DKV_ESHAPE, "%s: bad shape (history=%d biases=%d masks=%d)",
               what, p->history, p->biases, p->masks);
   DKV_REQUIRE(p->token_bytes == 4 || p->token_bytes == 8 || !p->tokens, DKV_EINVAL, "%s: tokens of %d bytes", what, p->token_bytes);
+  DKV_REQUIRE((uintptr_t)p->arrivals % 4 == 0, DKV_EINVAL, "%s: misaligned arrivals", what);
   DKV_REQUIRE(!p->tokens || p->lengths, DKV_EINVAL, "%s: tokens without lengths", what);
   DKV_REQUIRE(!p->biases || (p->bias_ids && p->bias_values && p->bias_cu), DKV_EINVAL, "%s: null bias pointer", what);
   DKV_REQUIRE(!p->allowed || p->words >= ((int64_t)p->vocab + 31) / 32, DKV_ESHAPE, "%s: %d mask words for %d tokens", what, p->words, p->vocab);
@@ -355,7 +372,7 @@ extern "C" int dkv_adjust_logits(const dkv_logits_args_t* p, void* workspace, si
   const int launched = p->dtype == DKV_F32 ? launch_type<float>(a, plan, st)
                        : p->dtype == DKV_F16 ? launch_type<half_t>(a, plan, st) : launch_type<dkv_bf16>(a, plan, st);
   if (launched) return launched;
-  if (a.partial)
+  if (a.partial && !p->arrivals)
     hipLaunchKernelGGL(pick_kernel, dim3((p->rows + 3) / 4), dim3(256), 0, st, a.partial, a.chunks, p->rows, p->pick);
   return dkv::check_launch("dkv_adjust_logits");
 }

@@ -93,13 +93,14 @@ class Fp4AttendArgs(ctypes.Structure):
     _fields_ = [("cache", Fp4Cache), ("table", c_vp), ("lengths", c_vp), ("cu", c_vp), ("query", c_vp), ("out", c_vp),
                 ("query_token", c_i64), ("query_head", c_i64), ("requests", c_i32), ("width", c_i32), ("rows", c_i32),
                 ("q_heads", c_i32), ("query_dtype", c_i32), ("window", c_i32), ("longest", c_i32), ("most", c_i32),
-                ("scaling", c_f32), ("fill", c_i32)]
+                ("scaling", c_f32), ("fill", c_i32), ("arrivals", c_vp), ("arrivals_count", c_i32)]
 
 
 class LogitsArgs(ctypes.Structure):
     """dkv_logits_args_t."""
     _fields_ = [(name, c_vp) for name in ("logits", "out", "tokens", "lengths", "reply", "repetition", "presence", "frequency",
-                                          "bias_ids", "bias_values", "bias_cu", "allowed", "allowed_row", "pick")]
+                                          "bias_ids", "bias_values", "bias_cu", "allowed", "allowed_row", "pick",
+                                          "arrivals")]
     _fields_ += [("logits_row", c_i64), ("out_row", c_i64), ("tokens_row", c_i64)]
     _fields_ += [(name, c_i32) for name in ("dtype", "rows", "vocab", "history", "token_bytes", "biases", "masks", "words")]
 

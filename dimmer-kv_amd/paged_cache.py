@@ -21,6 +21,7 @@ Calls on one cache share its tables and belong on one stream (or on streams the 
 
 from __future__ import annotations
 
+import itertools
 from dataclasses import dataclass
 
 import torch
@@ -39,6 +40,7 @@ class Step:
     most: int                # the same for the new tokens of a request
 
 
+ARRIVAL_SETS = 32
 REFUSED = {1: "more new tokens than rows", 2: "a request passes its row of the block table", 3: "too few free pages"}
 
 
@@ -78,11 +80,17 @@ class PagedCache:
         self._layers = [dkv_hip.Fp4Cache(self.key_codes[i].data_ptr(), self.key_scales[i].data_ptr(),
                                          self.value_codes[i].data_ptr(), self.value_scales[i].data_ptr(), pages,
                                          kv_heads, page, head_dim) for i in range(layers)]
+        # Words that the workgroups of one attention call count themselves on (zero between calls): calls take turns over
+        # several sets, so that ones captured in graphs or queued on other streams do not meet on one.
+        self._set = max(1024, 2 * requests * kv_heads)
+        self._arrivals = torch.zeros(ARRIVAL_SETS, self._set, dtype=torch.int32, device=device)
+        self._turns = itertools.cycle(range(self._arrivals.data_ptr(), self._arrivals.data_ptr() + ARRIVAL_SETS * self._set * 4,
+                                            self._set * 4))
         self._attend = []
         for cache in self._layers:
             a = dkv_hip.Fp4AttendArgs()
             a.cache, a.table, a.lengths = cache, self.table.data_ptr(), self.lengths.data_ptr()
-            a.requests, a.width = requests, table_pages
+            a.requests, a.width, a.arrivals_count = requests, table_pages, self._set
             self._attend.append(a)
 
     # ----- tables -----
@@ -172,6 +180,7 @@ class PagedCache:
         args = dkv_hip.Fp4AttendArgs.from_buffer_copy(self._attend[layer])
         args.scaling = self.head_dim ** -0.5 if scaling is None else scaling
         args.window = window or 0
+        args.arrivals = next(self._turns)
         args.longest, args.most = min(max(step.longest, 1), (1 << 31) - 1), min(max(step.most, 1), (1 << 31) - 1)
         return dkv_hip.fp4_attend(args, query, step.cu, out)
 
@@ -179,7 +188,7 @@ class PagedCache:
         """GPU memory of the pages of all layers, the tables and the free list."""
         return sum(t.numel() * t.element_size() for t in (
             self.key_codes, self.key_scales, self.value_codes, self.value_scales, self.table, self.lengths, self.free,
-            self.free_count, self._state))
+            self.free_count, self._state, self._arrivals))
 
 
 class PagedContext:

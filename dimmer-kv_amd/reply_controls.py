@@ -7,9 +7,13 @@ tokens so far.  ``greedy_answer(..., controls=...)`` answers under them.
 
 from __future__ import annotations
 
+import itertools
+
 import torch
 
 import dkv_hip
+
+ARRIVAL_SETS = 32
 
 
 def pack_allowed(mask: torch.Tensor) -> torch.Tensor:
@@ -40,6 +44,10 @@ class ReplyControls:
         self.device = torch.empty(0, device=device).device
         self._args = dkv_hip.LogitsArgs()
         self._args.rows, self._args.vocab = rows, vocab
+        # words that a call's workgroups count themselves on (zero between calls); calls take turns over several sets
+        self._arrivals = torch.zeros(ARRIVAL_SETS, max(rows, 1), dtype=torch.int32, device=device)
+        start, step = self._arrivals.data_ptr(), self._arrivals.stride(0) * 4
+        self._turns = itertools.cycle(range(start, start + ARRIVAL_SETS * step, step))
         self._held = {}  # the tensors whose addresses the arguments hold
         for name, value in (("repetition", repetition), ("presence", presence), ("frequency", frequency)):
             if value is not None:
@@ -131,7 +139,9 @@ class ReplyControls:
             raise ValueError(f"ReplyControls: logits must be on {self.device} (got {logits.device})")
         if tokens is not None and lengths is None:
             lengths = torch.full((self.rows,), tokens.shape[1], dtype=torch.int32, device=self.device)
-        return dkv_hip.adjust_logits(dkv_hip.LogitsArgs.from_buffer_copy(self._args), logits, tokens, lengths, reply_start, out)
+        args = dkv_hip.LogitsArgs.from_buffer_copy(self._args)
+        args.arrivals = next(self._turns)
+        return dkv_hip.adjust_logits(args, logits, tokens, lengths, reply_start, out)
 
 
 __all__ = ["ReplyControls", "pack_allowed"]

@@ -528,6 +528,8 @@ typedef struct dkv_fp4_attend_args {
   int32_t most;
   float scaling;
   int32_t fill;
+  uint32_t* arrivals;      /* [arrivals_count] zero at first and left so, or null: with it, requests split over workgroups */
+  int32_t arrivals_count;  /* are joined in the same launch.  Calls that overlap need words of their own. */
 } dkv_fp4_attend_args_t;
 
 size_t dkv_fp4_attend_workspace_bytes(const dkv_fp4_attend_args_t* p);
@@ -561,6 +563,8 @@ typedef struct dkv_logits_args {
   const int32_t* allowed;    /* [masks][words] bit t % 32 of word t / 32: token t may be picked; null: no mask */
   const int32_t* allowed_row;/* [rows] which mask, -1 none; null: row r takes mask r */
   int64_t* pick;             /* [rows] or null */
+  uint32_t* arrivals;        /* [rows] zero at first and left so, or null: with it the pick takes no second launch.  Calls */
+                             /* that overlap need words of their own. */
   int64_t logits_row;
   int64_t out_row;
   int64_t tokens_row;
