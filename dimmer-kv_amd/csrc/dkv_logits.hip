@@ -117,7 +117,7 @@ __global__ __launch_bounds__(kThreads, 8) void adjust_logits_kernel(LogitsArgs a
     }
   };
   fetch(0);
-  for (int x = tid * 4; x < S::kCountWords + S::kBitWords; x += kThreads * 4) *(uint4*)(lds + x) = make_uint4(0, 0, 0, 0);
+  for (int x = tid * 4; x < S::kCountWords + (p.biases ? S::kBitWords : 0); x += kThreads * 4) *(uint4*)(lds + x) = make_uint4(0, 0, 0, 0);
   __syncthreads();
   for (int j0 = 0; j0 < length; j0 += kBatch * kThreads) {
 #pragma unroll
@@ -318,29 +318,23 @@ int check_logits(const dkv_logits_args_t* p, const char* what) {
 }
 
 template <typename T, typename ID, int N, bool SHORT>
-int launch(const LogitsArgs& a, hipStream_t st) {
-  constexpr int kBytes = Stretch<T, N, SHORT>::kBytes;
-  if constexpr (kBytes > 64000) {  // past what a kernel may ask for without saying so
-    if (hipFuncSetAttribute((const void*)adjust_logits_kernel<T, ID, N, SHORT>, hipFuncAttributeMaxDynamicSharedMemorySize, kBytes) !=
-        hipSuccess) {
-      (void)hipGetLastError();
-      dkv::set_error("dkv_adjust_logits: no %d bytes of LDS", kBytes);
-      return DKV_ELAUNCH;
-    }
-  }
-  hipLaunchKernelGGL((adjust_logits_kernel<T, ID, N, SHORT>), dim3(a.chunks, a.p.rows), dim3(kThreads), kBytes, st, a);
-  return DKV_OK;
+void launch(const LogitsArgs& a, hipStream_t st) {
+  using S = Stretch<T, N, SHORT>;  // (the bits come last: without biases they are not asked for)
+  hipLaunchKernelGGL((adjust_logits_kernel<T, ID, N, SHORT>), dim3(a.chunks, a.p.rows), dim3(kThreads),
+                     a.p.biases ? S::kBytes : 4 * S::kCountWords, st, a);
 }
 
 template <typename T, typename ID>
-int launch_plan(const LogitsArgs& a, const Plan& plan, hipStream_t st) {
-  if (plan.lines > 1) return launch<T, ID, (int)sizeof(T), true>(a, st);
-  return plan.counts16 ? launch<T, ID, 1, true>(a, st) : launch<T, ID, 1, false>(a, st);
+void launch_plan(const LogitsArgs& a, const Plan& plan, hipStream_t st) {
+  if (plan.lines > 1) launch<T, ID, (int)sizeof(T), true>(a, st);
+  else if (plan.counts16) launch<T, ID, 1, true>(a, st);
+  else launch<T, ID, 1, false>(a, st);
 }
 
 template <typename T>
-int launch_type(const LogitsArgs& a, const Plan& plan, hipStream_t st) {
-  return a.p.token_bytes == 4 ? launch_plan<T, int32_t>(a, plan, st) : launch_plan<T, int64_t>(a, plan, st);
+void launch_type(const LogitsArgs& a, const Plan& plan, hipStream_t st) {
+  if (a.p.token_bytes == 4) launch_plan<T, int32_t>(a, plan, st);
+  else launch_plan<T, int64_t>(a, plan, st);
 }
 
 }  // namespace
@@ -369,9 +363,9 @@ extern "C" int dkv_adjust_logits(const dkv_logits_args_t* p, void* workspace, si
     a.partial = (uint64_t*)workspace;
   }
   hipStream_t st = dkv::as_stream(stream);
-  const int launched = p->dtype == DKV_F32 ? launch_type<float>(a, plan, st)
-                       : p->dtype == DKV_F16 ? launch_type<half_t>(a, plan, st) : launch_type<dkv_bf16>(a, plan, st);
-  if (launched) return launched;
+  if (p->dtype == DKV_F32) launch_type<float>(a, plan, st);
+  else if (p->dtype == DKV_F16) launch_type<half_t>(a, plan, st);
+  else launch_type<dkv_bf16>(a, plan, st);
   if (a.partial && !p->arrivals)
     hipLaunchKernelGGL(pick_kernel, dim3((p->rows + 3) / 4), dim3(256), 0, st, a.partial, a.chunks, p->rows, p->pick);
   return dkv::check_launch("dkv_adjust_logits");

@@ -40,7 +40,7 @@ class Step:
     most: int                # the same for the new tokens of a request
 
 
-ARRIVAL_SETS = 32
+ARRIVAL_SETS = 256
 REFUSED = {1: "more new tokens than rows", 2: "a request passes its row of the block table", 3: "too few free pages"}
 
 
@@ -100,8 +100,8 @@ class PagedCache:
         return counts
 
     def assign(self, new, rows: int | None = None, longest: int | None = None, most: int | None = None) -> Step:
-        """Pages for ``new`` tokens of each request (int32 [requests] on the GPU, or host numbers) and the slots and
-        positions of the step's ``rows`` rows (needed with a GPU tensor; more than the new tokens for a padded step).
+        """Pages for ``new`` tokens of each request (int32 [requests] on the GPU, as a captured step needs, or host numbers)
+        and the slots and positions of the step's ``rows`` rows (needed with a GPU tensor; more than the new tokens for a padded step).
         ``longest`` and ``most`` bound the lengths and new tokens a request may have; they only shape later launches.
         If the pages, a table row or the rows do not suffice, nothing is assigned and every slot is -1; ``check``
         tells."""

@@ -13,7 +13,7 @@ import torch
 
 import dkv_hip
 
-ARRIVAL_SETS = 32
+ARRIVAL_SETS = 256
 
 
 def pack_allowed(mask: torch.Tensor) -> torch.Tensor:

@@ -41,7 +41,7 @@ def check_step(step, want):
     assert step.cu.tolist() == cu
 
 
-@pytest.mark.parametrize("requests,page", [(1, 16), (3, 32), (64, 16), (65, 64), (1025, 16), (2500, 128)])
+@pytest.mark.parametrize("requests,page", [(1, 16), (3, 32), (64, 16), (65, 64), (1025, 16), (2500, 128), (8192, 16)])
 def test_assign_and_trim(requests, page):
     """Admissions, single tokens, ends and cuts in any order, the tables equal after each."""
     rng = np.random.RandomState(requests)
@@ -252,3 +252,29 @@ def test_other_stream_and_graph():
         check_tables(cache, ref)
         want = paged_ref.quantize(key.double().cpu().numpy())[2]
         assert np.array_equal(out[0].double().cpu().numpy(), want), turn
+
+
+def test_past_32_bits():
+    """Pages whose bytes lie past 2^32: stored, loaded and attended to like any other."""
+    from paged_cache import PagedCache
+
+    heads, dim, page, pages = 8, 256, 4096, 1100
+    cache = PagedCache(1, heads, dim, pages, page=page, table_pages=4, device=DEV)
+    assert cache.key_codes.numel() > 1 << 32
+    cache.free.copy_(torch.arange(pages))  # the last pages first
+    step = cache.assign([4100])
+    rows = torch.randn(2, 4100, heads, dim, device=DEV)
+    cache.store(0, rows[0], rows[1], step)
+    assert int(step.slots[0]) == (pages - 1) * page and int(step.slots[-1]) == (pages - 2) * page + 3
+    key, value = cache.load(0, step.slots, torch.float32)
+    pick = [0, 7, 4095, 4096, 4099]
+    for have, given in ((key, rows[0]), (value, rows[1])):
+        assert np.array_equal(have[pick].double().cpu().numpy(), paged_ref.quantize(given[pick].double().cpu().numpy())[2])
+    query = torch.randn(4100, heads, dim, device=DEV)[-1:].contiguous()
+    one = cache.assign([1])
+    cache.store(0, rows[0][:1], rows[1][:1], one)
+    out = cache.attend_rows(0, query, one)
+    weights = torch.softmax(torch.einsum("hd,thd->ht", query[0].double(), torch.cat([key, key[:1]]).double()) * dim ** -0.5, -1)
+    want = torch.einsum("ht,thd->hd", weights, torch.cat([value, value[:1]]).double())
+    # float32: the weights' error, some 2^-17 (256 products of order 1, 4,101 sums), on values below 8
+    assert (out[0].double() - want).abs().max() < 8 * 2.0 ** -17

@@ -101,6 +101,26 @@ def test_large_vocabulary():
     check(c, *apply(c))
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_many_rows(dtype):
+    """Enough rows for the long stretches, two lines or four a thread."""
+    c = make_case(70, 128256, 400, 9, True, dtype)
+    out, pick = apply(c)
+    for r in (0, 1, 33, 68, 69):
+        one = {k: (v[r:r + 1] if k != "bias" else [v[r]]) for k, v in c.items()}
+        check(one, out[r:r + 1], pick[r:r + 1])
+
+
+def test_long_history():
+    """More mentions than 15 bits count: 40,000 tokens, 35,000 of them one."""
+    c = make_case(2, 9000, 40000, 3, False, "f32")
+    c["tokens"][0, 2000:37000] = 17
+    c["reply"][:] = [1000, 39000]
+    c["lengths"][:] = 40000
+    check(c, *apply(c))
+    check(c, *apply(c, ids=torch.int32))
+
+
 def test_in_place_and_strided():
     """Logits changed in place, rows that lie apart and begin anywhere, a given out of another alignment."""
     c = make_case(4, 777, 50, 5, True, "bf16")
