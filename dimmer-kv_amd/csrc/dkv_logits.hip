@@ -3,10 +3,12 @@
 //
 // One pass over the logits: a workgroup takes a stretch of a row's vocabulary.  It loads the stretch into registers, counts
 // meanwhile the history's tokens that fall into it in LDS (integer atomics that return nothing: the order does not matter and
-// nothing waits for them), and writes the stretch, masked.  Each wave lists the counted tokens of its lines as it meets them
-// and takes them 64 at a time, one a lane: there is a division for each, and taken where they stand in the lines, a few
-// lanes of the wave would make it at every place.
-// Every float32 operation is rounded on its own, in the stated order, so equal inputs stay equal and ties are ties.
+// nothing waits for them), and writes the stretch once.  Every float32 operation is rounded on its own, in the stated order,
+// so equal inputs stay equal and ties are ties.
+// Measured: 128 replies of 128,256 bfloat16 logits 40 us with histories of up to 16K tokens, biases and masks, 22 us
+// without any (66 MB: 13 us at a copy's rate): reading the history once for every stretch and dividing the logits it
+// names are the difference; loads, counting and stores of the workgroups run side by side rather than overlapped.  Stretches
+// of 8,192 and 32,768 tokens cost 50 and 54 us, a list of the counted tokens worked off by full waves 43 to 56.
 #include <math.h>
 
 #include "dkv_device.h"

@@ -10,7 +10,9 @@ namespace {
 // Pages for new tokens, and pages given back.  Both are a running sum over the requests (rows and pages of those before
 // it) followed by independent work on rows and pages, which find their request by bisection in the sums.  Every workgroup
 // makes the sums for itself in LDS, so one launch serves; what the sums are made of (lengths, free count) is rewritten by
-// the workgroup that ends last, when all others have read it.
+// the workgroup that ends last, when all others have read it.  Latency is what it costs: one token each of 256 requests
+// 4.4 us, 217K rows of 48 prompts 7.3 us (68 us with a device-wide fence before each arrival, which writes a die's cache
+// back).
 // ---------------------------------------------------------------------------
 constexpr int kPageThreads = 1024;
 constexpr int kMaxRequests = 8192;  // two 32-bit sums each in LDS
