@@ -36,6 +36,9 @@ DKV_DEVICE bool last_of(uint32_t* word, uint32_t all) {
 
 namespace dkv {
 
+// Tokens a request may have: what the kernels round up to whole chunks stays below 2^31.
+constexpr int64_t kMostTokens = (1L << 31) - (1 << 16);
+
 // log2 of a page's tokens; -1 for a page that is not a power of two from 16 (an attention tile) to 4096.
 inline int page_shift(int32_t page) {
   for (int s = 4; s <= 12; ++s)

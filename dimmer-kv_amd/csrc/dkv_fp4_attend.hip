@@ -194,8 +194,8 @@ struct LaneOffsets {
 // ahead of the pages, so that no page load waits for its address.
 template <int CH>
 DKV_DEVICE int load_entries(const AttendArgs& a, const int32_t* row, int len, int chunk) {
-  const int token = (chunk * CH + (int)(threadIdx.x & 15) % CH) * 16;
-  return row[token < len ? token >> a.shift : 0];  // (checked where it is used, so that nothing waits for it here)
+  const uint32_t token = (uint32_t)(chunk * CH + (int)(threadIdx.x & 15) % CH) * 16;
+  return row[token < (uint32_t)len ? token >> a.shift : 0];  // (checked where it is used, so that nothing waits for it here)
 }
 
 template <int CH>
@@ -515,6 +515,8 @@ __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_at
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const float total = sum_xor32(sum_xor16(l[nt]));
+      // a row whose scores are all NaN has no maximum, but is not one that sees nothing
+      if (m[nt] == -INFINITY && total != 0.0f) m[nt] = 0.0f;
       if (g == 0) {
         stat[0][wave][nt * 16 + i] = m[nt];
         stat[1][wave][nt * 16 + i] = total;
@@ -691,9 +693,10 @@ __global__ __launch_bounds__(256) void fp4_join_kernel(AttendArgs a, int q_heads
     top = wave_max(top);
 #pragma unroll
     for (int k = 0; k < kMaxSplits / 64; ++k) {
-      const float factor = x[k].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x[k].x - top);
+      // (a split that saw nothing wrote nothing; one whose weight is 0 did, and may hold a NaN)
+      const float factor = x[k].x == -INFINITY ? -1.0f : __builtin_amdgcn_exp2f(x[k].x - top);
       weight[k * 64 + threadIdx.x] = factor;
-      total += x[k].x == -INFINITY ? 0.0f : x[k].y * factor;
+      total += factor < 0.0f ? 0.0f : x[k].y * factor;
     }
     total = wave_sum(total);
     if (threadIdx.x == 0) whole = total;
@@ -705,7 +708,7 @@ __global__ __launch_bounds__(256) void fp4_join_kernel(AttendArgs a, int q_heads
 #pragma unroll 4
   for (int s = set; s < a.splits; s += kSets) {
     const float w = weight[s];
-    if (w == 0.0f) continue;  // nothing seen there, and nothing written
+    if (w < 0.0f) continue;
     const float4 v = part[s * kSet];
     acc.x = fmaf(v.x, w, acc.x); acc.y = fmaf(v.y, w, acc.y); acc.z = fmaf(v.z, w, acc.z); acc.w = fmaf(v.w, w, acc.w);
   }
@@ -800,7 +803,7 @@ int check_attend(const dkv_fp4_attend_args_t* p, const char* what) {
   if (rc) return rc;
   DKV_REQUIRE(p->query_dtype == DKV_F32 || p->query_dtype == DKV_F16 || p->query_dtype == DKV_BF16, DKV_EINVAL,
               "%s: query dtype %d not supported", what, p->query_dtype);
-  DKV_REQUIRE(p->requests > 0 && p->requests <= 8192 && p->width > 0 && (int64_t)p->width * p->cache.page < (1L << 31) && p->rows >= 0,
+  DKV_REQUIRE(p->requests > 0 && p->requests <= 8192 && p->width > 0 && (int64_t)p->width * p->cache.page < dkv::kMostTokens && p->rows >= 0,
               DKV_ESHAPE, "%s: bad shape (requests=%d width=%d rows=%d)", what, p->requests, p->width, p->rows);
   DKV_REQUIRE(p->q_heads > 0 && p->q_heads % p->cache.kv_heads == 0, DKV_ESHAPE,
               "%s: %d query heads over %d KV heads", what, p->q_heads, p->cache.kv_heads);

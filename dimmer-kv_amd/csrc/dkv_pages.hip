@@ -163,7 +163,7 @@ int check_pages(const dkv_pages_t* p, const char* what) {
   DKV_REQUIRE(p->requests > 0 && p->requests <= kMaxRequests && p->width > 0 && p->pages > 0, DKV_ESHAPE,
               "%s: bad shape (requests=%d, at most %d; width=%d pages=%d)", what, p->requests, kMaxRequests, p->width, p->pages);
   DKV_REQUIRE(dkv::page_shift(p->page) >= 0, DKV_ESHAPE, "%s: page %d must be a power of two from 16 to 4096", what, p->page);
-  DKV_REQUIRE((int64_t)p->width * p->page < (1L << 31), DKV_ESHAPE, "%s: %d pages of %d tokens pass 2^31 tokens a request",
+  DKV_REQUIRE((int64_t)p->width * p->page < dkv::kMostTokens, DKV_ESHAPE, "%s: %d pages of %d tokens pass 2^31 - 2^16 tokens a request",
               what, p->width, p->page);
   DKV_REQUIRE(p->lengths && p->table && p->free_pages && p->free_count && p->state, DKV_EINVAL, "%s: null pointer", what);
   return DKV_OK;

@@ -57,8 +57,8 @@ class PagedCache:
         if layers < 0 or kv_heads < 1 or pages < 1 or table_pages < 1 or not 1 <= requests <= 8192:
             raise ValueError(f"bad cache: {layers} layers, {kv_heads} KV heads, {pages} pages, {requests} requests of "
                              f"{table_pages} pages")
-        if table_pages * page >= 1 << 31 or pages * page >= 1 << 40:
-            raise ValueError(f"{table_pages} pages of {page} tokens pass 2^31 tokens a request")
+        if table_pages * page >= (1 << 31) - (1 << 16):
+            raise ValueError(f"{table_pages} pages of {page} tokens pass 2^31 - 2^16 tokens a request")
         if torch.device(device).type != "cuda":
             raise ValueError("PagedCache needs a GPU (the HIP path has no CPU fallback)")
         self.layers, self.kv_heads, self.head_dim = layers, kv_heads, head_dim

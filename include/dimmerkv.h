@@ -465,7 +465,7 @@ typedef struct dkv_pages {  /* the requests' block tables and the free pages */
   int32_t* free_count;  /* [1] */
   int32_t* state;       /* [3] zero at first: why the last assign was refused, scratch, the last trim's */
   int32_t requests;     /* at most 8192 */
-  int32_t width;        /* width * page < 2^31 */
+  int32_t width;        /* width * page < 2^31 - 2^16 */
   int32_t page;
   int32_t pages;        /* ids the free stack has room for */
 } dkv_pages_t;

@@ -204,6 +204,49 @@ def test_nan_reaches_only_rows_that_see_it():
         assert got[sees][..., 32:].isnan().all() and torch.equal(got[sees][..., :32], want[sees][..., :32])
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("total,new", [(1, 1), (40, 3), (700, 1), (3000, 2), (200, 50)])
+def test_nan_keys_and_queries(total, new, dtype):
+    """A NaN query makes its own row NaN; a NaN key every row that sees it, also where a row sees nothing else, and in one
+    split of many."""
+    cache, step = build([total - new], [new], 1, 64, 16)
+    query = torch.randn(new, 3, 64, device=DEV).to(TYPES[dtype])
+    clean = cache.attend_rows(0, query, step)
+    assert clean.isfinite().all()
+    dirty = query.clone()
+    dirty[-1, 1, 5] = float("nan")
+    got = cache.attend_rows(0, dirty, step)
+    assert got[-1, 1].isnan().all()
+    got[-1, 1] = clean[-1, 1]
+    assert torch.equal(got, clean)
+    from paged_cache import Step
+
+    slot = cache.slots(0, total - new, total - new + 1)  # the first of the new tokens
+    key, value = cache.load(0, slot, torch.float32)
+    key[0, 0, 3] = float("nan")
+    cache.store(0, key, value, Step(slot, slot, step.cu, 1, 1, 1))
+    assert cache.attend_rows(0, query, step).isnan().all()
+    seen = cache.attend_rows(0, query, step, window=1)
+    assert seen[0].isnan().all() and seen[1:].isfinite().all()
+
+
+@pytest.mark.parametrize("total", [900, 1500, 20000])
+def test_nan_value_of_no_weight(total):
+    """A value of NaN that the softmax weighs by less than the smallest float32 makes its block NaN all the same, in one
+    launch, joined in it or by another."""
+    from paged_cache import Step
+
+    cache, step = build([total - 1], [1], 1, 64, 16)
+    query = torch.ones(1, 2, 64, device=DEV)
+    key, value = torch.full((1, 1, 64), 6.0, device=DEV), torch.ones(1, 1, 64, device=DEV)
+    value[0, 0, 33] = float("nan")
+    for at, k in ((total - 1, key), (5, -key)):  # scores of 48 and -48, times 4: e^-384
+        slot = cache.slots(0, at, at + 1)
+        cache.store(0, k, value if at == 5 else torch.ones_like(value), Step(slot, slot, step.cu, 1, 1, 1))
+    out = cache.attend_rows(0, query, step, scaling=0.5)
+    assert out[..., 32:].isnan().all() and (out[..., :32] == 1.0).all()
+
+
 def test_no_rows_and_no_tokens():
     cache, step = build([5, 0], [0, 0], 2, 64, 16)
     assert cache.attend_rows(0, torch.empty(0, 4, 64, device=DEV), step).shape == (0, 4, 64)
