@@ -759,6 +759,7 @@ struct Plan {
   int blocks;  // row blocks a request is given
   int splits;
   int share;   // 16-token tiles a split takes at the least
+  bool joins;  // the launch joins its splits itself
 };
 
 constexpr long kWorkgroups = 512;  // of four waves: what the card holds at two waves a SIMD
@@ -790,6 +791,21 @@ Plan plan_of(const dkv_fp4_attend_args_t& p) {
     const auto rounds = [&](long x) { return (double)((each * x + kWorkgroups - 1) / kWorkgroups) / x; };
     for (int x = 2; x <= 3; ++x)
       if (rounds(x) < 0.85 * rounds(plan.splits)) plan.splits = x;
+  }
+  // A row block whose rows times splits are few is joined by the last of its workgroups to arrive, others by a launch of
+  // their own, which costs the caller 3 us.  Fewer splits are made for that where a wave then takes one more chunk at most.
+  // 8 KV heads of 128 bfloat16 dimensions, 3 query heads each: 3,000 tokens 9.3 us in a graph and 11.2 a call against 9.5
+  // and 13.8 by two launches, 6,000 tokens 11.5 and 11.3 against 9.8 and 13.9; 16K tokens stay with 64 splits (13.0 and
+  // 13.9; 14.5 and 14.4 with the 21 that one workgroup would join).  A launch that fills the card is not joined in itself
+  // (4 requests of 12,000 tokens, 64 dimensions, 16 splits: 13.5 and 14.0 against 14.6 and 14.4), and at 256 dimensions
+  // fewer rows are (8 rows, 12 splits of 3,000 tokens, 2 KV heads: 10.7 and 13.8 against 14.7 and 14.7).
+  const long row_block = min(rows, plan.tiles * 16L), joined = p.cache.head_dim < 256 ? 64 : 32;
+  plan.joins = false;
+  if (p.arrivals && plan.tiles <= 2 && plan.splits > 1 && each <= p.arrivals_count && row_block <= joined / 2) {
+    const long fewer = min((long)plan.splits, joined / row_block), chunk = plan.tiles == 1 && p.cache.head_dim < 256 ? 256 : 128;
+    const auto turns = [&](long splits) { return (longest + chunk * splits - 1) / (chunk * splits); };
+    plan.joins = each * fewer < kWorkgroups && turns(fewer) - turns(plan.splits) <= (p.cache.head_dim < 256 ? 1 : 0);
+    if (plan.joins) plan.splits = (int)fewer;
   }
   while ((long)plan.blocks * plan.splits > 65535) plan.blocks /= 2;
   const long tiles = (longest + 15) / 16;
@@ -873,14 +889,7 @@ extern "C" int dkv_fp4_attend(const dkv_fp4_attend_args_t* p, void* workspace, s
   a.table = p->table; a.lengths = p->lengths; a.cu = p->cu; a.query = p->query; a.out = p->out;
   a.part = (float*)workspace;
   a.part_ml = (float2*)(a.part + (size_t)p->rows * p->q_heads * plan.splits * p->cache.head_dim);
-  // A row block whose rows times splits are few is joined by the last of its workgroups to arrive, others by a launch of
-  // their own.  1,500 tokens of 8 KV heads (4 rows, 6 splits): 9.3 us against 8.8 and the 3 us that a launch costs the
-  // caller; 16K tokens (3 rows, 64 splits): 17.3 against 13, as one workgroup reads all of it.
-  const long row_block = min((long)(p->most < 1 ? 1 : p->most) * (p->q_heads / p->cache.kv_heads), plan.tiles * 16L);
-  const long counted = (long)p->requests * plan.blocks * p->cache.kv_heads;
-  if (p->arrivals && plan.tiles <= 2 && counted <= p->arrivals_count && row_block * plan.splits <= 64 &&
-      counted * plan.splits <= 2 * kWorkgroups)
-    a.arrivals = p->arrivals;
+  if (plan.joins) a.arrivals = p->arrivals;
   a.query_token = p->query_token; a.query_head = p->query_head;
   a.requests = p->requests; a.width = p->width; a.shift = dkv::page_shift(p->cache.page); a.rows = p->rows;
   a.groups = p->q_heads / p->cache.kv_heads;
