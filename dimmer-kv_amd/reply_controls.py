@@ -35,7 +35,11 @@ class ReplyControls:
         - ``bias``: added to logits; {token: value} for every row, a list of such dicts by row, or (ids int32,
           values float32, cu int32 [rows + 1]); of an id that a row lists twice the last value counts;
         - ``allowed``: bool [rows, vocab] or [1, vocab] (every row), or (words int32 [masks, ceil(vocab / 32)],
-          mask of each row int32 [rows], -1 for none).  ``allow`` changes it later."""
+          mask of each row int32 [rows], -1 for none).  ``allow`` changes it later.
+
+        A captured ``apply`` reads the memory of its capture: bool masks given to ``allow`` later go into the memory of
+        the first of their shape, so replays see them; tensors of a tuple on the GPU are read where they are, and theirs
+        to change is the caller's."""
         if rows < 0 or rows > 65535 or vocab < 1:
             raise ValueError(f"ReplyControls: {rows} rows (at most 65535) of {vocab} tokens")
         if torch.device(device).type != "cuda":
@@ -49,6 +53,7 @@ class ReplyControls:
         start, step = self._arrivals.data_ptr(), self._arrivals.stride(0) * 4
         self._turns = itertools.cycle(range(start, start + ARRIVAL_SETS * step, step))
         self._held = {}  # the tensors whose addresses the arguments hold
+        self._masks, self._first = {}, None  # words of bool masks by their number, and the row of zeros for a single one
         for name, value in (("repetition", repetition), ("presence", presence), ("frequency", frequency)):
             if value is not None:
                 self._hold(name, self._per_row(name, value))
@@ -115,7 +120,9 @@ class ReplyControls:
                 raise ValueError(f"ReplyControls: allowed must be bool [rows, {self.vocab}] or (words, mask of each row)")
             words = pack_allowed(allowed)
             if allowed.shape[0] == 1:
-                row = torch.zeros(self.rows, dtype=torch.int32)
+                if self._first is None:
+                    self._first = torch.zeros(self.rows, dtype=torch.int32, device=self.device)
+                row = self._first
         need = -(-self.vocab // 32)
         if words.dtype != torch.int32 or words.dim() != 2 or words.shape[1] < need:
             raise ValueError(f"ReplyControls: mask words must be int32 [masks, {need}]")
@@ -123,6 +130,9 @@ class ReplyControls:
             raise ValueError(f"ReplyControls: {words.shape[0]} masks for {self.rows} rows")
         if row is not None and (row.dtype != torch.int32 or row.shape != (self.rows,)):
             raise ValueError(f"ReplyControls: the mask of each row must be int32 [{self.rows}]")
+        if not isinstance(allowed, tuple):  # into the words that captured calls may be reading
+            held = self._masks.get(words.shape[0])
+            words = self._masks.setdefault(words.shape[0], words.to(self.device)) if held is None else held.copy_(words)
         self._hold("allowed", words.to(self.device).contiguous())
         self._args.masks, self._args.words = words.shape
         self._args.allowed_row = None

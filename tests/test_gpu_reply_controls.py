@@ -205,3 +205,30 @@ def test_graph_and_stream():
         torch.cuda.synchronize()
         check(c, out, pick)
         controls.apply(c["logits"])
+
+
+@pytest.mark.parametrize("masks", [1, 3])
+def test_masks_change_under_a_graph(masks):
+    """Replays of a captured call see the bool masks given since, also with masks of another shape or none between."""
+    from reply_controls import ReplyControls
+
+    rows, vocab = 3, 1000
+    generator = torch.Generator(DEV).manual_seed(4)
+    logits = torch.randn(rows, vocab, generator=generator, device=DEV)
+    mask = lambda n: torch.rand(n, vocab, generator=generator, device=DEV) < 0.1
+    controls = ReplyControls(rows, vocab, allowed=mask(masks), device=DEV)
+    controls.apply(logits)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        _, pick = controls.apply(logits)
+    for turn in range(4):
+        if turn == 2:
+            controls.allow(None)
+            controls.allow(mask(4 - masks))
+        may = mask(masks)
+        controls.allow(may.cpu() if turn == 1 else may)
+        torch.full((1 << 16,), -1, dtype=torch.int32, device=DEV)  # what memory given back would hold
+        graph.replay()
+        want = torch.where(may, logits, -float("inf")).argmax(1)
+        assert torch.equal(pick, want) and torch.equal(controls.apply(logits)[1], want)
