@@ -31,6 +31,8 @@ after ``update``, additive attention_mask or None, scaling) ->
 
 from __future__ import annotations
 
+import copy
+
 import torch
 
 import dkv_hip
@@ -468,7 +470,8 @@ class _Picker:
             raise ValueError(f"greedy_answer takes controls of one row (got {controls.rows})")
         before = [input_ids.reshape(-1)] if history is None else [history.to(input_ids.device).reshape(-1), input_ids.reshape(-1)]
         prompt = torch.cat(before).to(torch.int64)
-        self.controls, self.length = controls, prompt.numel()
+        # (a copy: a grammar's masks end with the answer)
+        self.controls, self.length = copy.copy(controls), prompt.numel()
         self.tokens = torch.cat([prompt, prompt.new_zeros(max_new_tokens)]).unsqueeze(0)
         self.start = torch.full((1,), self.length, dtype=torch.int32, device=prompt.device)
 

@@ -62,6 +62,14 @@ class ReplyControls:
         if allowed is not None:
             self.allow(allowed)
 
+    def __copy__(self) -> "ReplyControls":
+        """The same controls, with masks of its own from now on."""
+        other = ReplyControls.__new__(ReplyControls)
+        other.__dict__.update(self.__dict__)
+        other._args = dkv_hip.LogitsArgs.from_buffer_copy(self._args)
+        other._held, other._masks = dict(self._held), {}
+        return other
+
     def _hold(self, name: str, t: torch.Tensor) -> None:
         self._held[name] = t
         setattr(self._args, name, dkv_hip.ptr(t) if t.numel() else None)

@@ -193,3 +193,21 @@ def test_serving_loop():
                     for x in range(2):
                         del held[layer][b][x][tables.lengths[b]:]
     cache.check()
+
+
+def test_grammar_ends_with_the_answer():
+    """The masks that controls were made with hold again after an answer under a grammar."""
+    from compressed_attention import greedy_answer
+    from reply_controls import ReplyControls
+
+    model, keys, values, m, question = setup()
+    vocab = model.config.vocab_size
+    context = m.apply("fp4", keys, values, {}).stored
+    only = lambda token: torch.arange(vocab, device=DEV) == token
+    controls = ReplyControls(1, vocab, allowed=only(7).unsqueeze(0))
+    for grammar, want in ((None, "7 7"), (lambda reply: only(11), "11 11"), (None, "7 7"), (lambda reply: ~only(11) & only(11), ""),
+                          (lambda reply: None, "%s"), (None, "7 7")):
+        text, first = greedy_answer(model, _Tokenizer(), context, context.exact_cache, question, 300, max_new_tokens=2,
+                                    controls=controls, grammar=grammar)
+        assert text.split()[:1] == [str(int(first.argmax()))] if want == "%s" else text == want
+        context.rewind(300)
