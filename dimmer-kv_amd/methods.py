@@ -188,7 +188,7 @@ class Methods:
         tokens, dtype = keys[0].shape[2], keys[0].dtype
         per_token = torch.full((tokens,), float(stored.token_bytes()), device=self.device)
         return Compressed(None, None, None, tokens * stored.token_bytes(), seconds, token_bytes=per_token, stored=stored,
-                          rebuild=lambda: stored.rebuilt(dtype))
+                          rebuild=lambda: stored.rebuilt(dtype, tokens))
 
     def _kvtc(self, name: str, keys, values, scores) -> Compressed:
         plan = _kvtc_plan(name, scores)

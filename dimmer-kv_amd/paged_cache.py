@@ -195,7 +195,8 @@ class PagedContext:
     """One conversation in a paged 4-bit cache, attended to directly: the ``attend`` contract of
     ``compressed_attention.CompressedContext`` for the ``dimmer`` hook.  Every forward's new keys and values are stored
     before they are attended to, in 4 bits as all others, so ``exact_cache`` (the cache the model updates) only carries
-    them here: it starts empty.  Attention is causal over all tokens; the model's additive mask is not read."""
+    them here: it starts empty.  Attention is causal, over all tokens or a layer's sliding window as the model's
+    configuration has it; the model's additive mask is not read."""
 
     def __init__(self, keys: list[torch.Tensor], values: list[torch.Tensor], model, page: int = 64, room: int = 1024):
         """Per-layer [1, kv_heads, tokens, head_dim] keys (RoPE applied) and values on the GPU, with room for ``room`` more
@@ -212,6 +213,7 @@ class PagedContext:
         self.cache = PagedCache(len(keys), heads, dim, pages, page=page, device=first.device)
         self.capacity, self.tokens = pages * page, tokens
         self._model = model
+        self._windows = self._layer_windows(model.config, len(keys))
         step = self.cache.assign([tokens], longest=tokens)
         for layer, (key, value) in enumerate(zip(keys, values)):
             if key.shape != shape or value.shape != shape:
@@ -219,6 +221,16 @@ class PagedContext:
             self.cache.store(layer, key[0].transpose(0, 1), value[0].transpose(0, 1), step)
         self._step = None
         self.exact_cache = self.fresh_cache()
+
+    @staticmethod
+    def _layer_windows(config, layers: int) -> list[int | None]:
+        config = config.get_text_config(decoder=True)
+        window = getattr(config, "sliding_window", None)
+        kinds = getattr(config, "layer_types", None) or ["sliding_attention" if window else "full_attention"] * layers
+        for kind in kinds:
+            if kind not in ("full_attention", "sliding_attention"):
+                raise ValueError(f"PagedContext: layers of {kind}")
+        return [window if kind == "sliding_attention" else None for kind in kinds]
 
     def fresh_cache(self):
         """An empty cache for the model to update: one for every answer."""
@@ -239,9 +251,10 @@ class PagedContext:
         self.tokens, self._step = tokens, None
         self.exact_cache = self.fresh_cache()
 
-    def rebuilt(self, dtype: torch.dtype = torch.float16):
-        """(keys, values): per-layer [1, kv_heads, tokens, head_dim] caches of the values held."""
-        slots = self.cache.slots(0, 0, self.tokens)
+    def rebuilt(self, dtype: torch.dtype = torch.float16, tokens: int | None = None):
+        """(keys, values): per-layer [1, kv_heads, tokens, head_dim] caches of the values held, of the first ``tokens``
+        if given."""
+        slots = self.cache.slots(0, 0, self.tokens if tokens is None else min(tokens, self.tokens))
         rows = [self.cache.load(layer, slots, dtype) for layer in range(self.cache.layers)]
         return ([key.transpose(0, 1).contiguous().unsqueeze(0) for key, _ in rows],
                 [value.transpose(0, 1).contiguous().unsqueeze(0) for _, value in rows])
@@ -265,7 +278,8 @@ class PagedContext:
             raise ValueError("PagedContext: a forward starts at layer 0")
         past = key.shape[2] - new
         c.store(layer, key[0, :, past:].transpose(0, 1), value[0, :, past:].transpose(0, 1), self._step)
-        return c.attend_rows(layer, query[0].transpose(0, 1), self._step, scaling=scaling).unsqueeze(0), None
+        return c.attend_rows(layer, query[0].transpose(0, 1), self._step, scaling=scaling,
+                             window=self._windows[layer]).unsqueeze(0), None
 
 
 __all__ = ["PagedCache", "PagedContext", "Step"]

@@ -211,3 +211,46 @@ def test_grammar_ends_with_the_answer():
                                     controls=controls, grammar=grammar)
         assert text.split()[:1] == [str(int(first.argmax()))] if want == "%s" else text == want
         context.rewind(300)
+
+
+def test_rebuilt_after_an_answer():
+    """A compressed cache's keys and values are the prefill's, also when an answer lies behind them by then."""
+    from compressed_attention import greedy_answer
+
+    model, keys, values, m, question = setup()
+    packed = m.apply("fp4", keys, values, {})
+    greedy_answer(model, _Tokenizer(), packed.stored, packed.stored.exact_cache, question, 300, max_new_tokens=2)
+    assert packed.stored.tokens == 313 and packed.token_bytes.shape == (300,)
+    for have, given in ((packed.keys[0], keys[0]), (packed.values[1], values[1])):
+        assert have.shape == given.shape
+        want = paged_ref.quantize(given[0, :, 280:].double().cpu().numpy())[2]
+        assert np.array_equal(have[0, :, 280:].double().cpu().numpy(), want)
+    assert packed.stored.rebuilt()[0][0].shape[2] == 313
+
+
+def test_sliding_window_layers():
+    """Layers that the model's configuration gives a sliding window attend over it, the others over all tokens."""
+    from types import SimpleNamespace
+
+    from paged_cache import PagedContext
+    from transformers import LlamaConfig
+
+    heads, groups, dim, tokens, new, window = 2, 2, 64, 150, 20, 33
+    shape = dict(num_hidden_layers=2, hidden_size=heads * groups * dim, num_attention_heads=heads * groups,
+                 num_key_value_heads=heads, head_dim=dim)
+    g = torch.Generator(DEV).manual_seed(5)
+    rand = lambda *s: torch.randn(*s, generator=g, device=DEV)
+    keys, values = ([rand(1, heads, tokens, dim) for _ in range(2)] for _ in range(2))
+    config = LlamaConfig(sliding_window=window, layer_types=["full_attention", "sliding_attention"], **shape)
+    context = PagedContext(keys, values, SimpleNamespace(config=config))
+    for layer in range(2):
+        module = SimpleNamespace(layer_idx=layer, num_key_value_groups=groups)
+        query, key, value = rand(1, heads * groups, new, dim), rand(1, heads, new, dim), rand(1, heads, new, dim)
+        have, _ = context.attend(module, query, *context.exact_cache.update(key, value, layer), None, dim ** -0.5)
+        rows = [t.double().cpu().numpy() for t in context.cache.load(layer, context.cache.slots(0, 0, tokens + new), torch.float32)]
+        want = paged_ref.attend(query[0].transpose(0, 1).double().cpu().numpy(), *rows, dim ** -0.5, window if layer else None)
+        # float32 sums of at most 170 terms of order 1
+        assert np.abs(have[0].double().cpu().numpy() - want).max() < 170 * 2.0 ** -22
+    config = LlamaConfig(layer_types=["full_attention", "chunked_attention"], attention_chunk_size=64, **shape)
+    with pytest.raises(ValueError, match="chunked"):
+        PagedContext(keys, values, SimpleNamespace(config=config))
