@@ -308,6 +308,9 @@ int check_logits(const dkv_logits_args_t* p, const char* what) {
   DKV_REQUIRE(p->dtype == DKV_F32 || p->dtype == DKV_F16 || p->dtype == DKV_BF16, DKV_EINVAL, "%s: dtype %d not supported", what, p->dtype);
   DKV_REQUIRE(p->rows >= 0 && p->rows <= 65535 && p->vocab > 0 && p->vocab <= INT32_MAX - 65536, DKV_ESHAPE,
               "%s: bad shape (rows=%d, at most 65535; vocab=%d)", what, p->rows, p->vocab);
+  // (32-bit indexes that run a batch of the history and a workgroup of the biases past their ends)
+  DKV_REQUIRE(p->history <= INT32_MAX - 65536 && p->biases <= INT32_MAX - 65536, DKV_ESHAPE, "%s: history=%d or biases=%d pass 2^31 - 2^16",
+              what, p->history, p->biases);
   DKV_REQUIRE(p->history >= 0 && p->biases >= 0 && p->masks >= 0, DKV_ESHAPE, "%s: bad shape (history=%d biases=%d masks=%d)",
               what, p->history, p->biases, p->masks);
   DKV_REQUIRE(p->token_bytes == 4 || p->token_bytes == 8 || !p->tokens, DKV_EINVAL, "%s: tokens of %d bytes", what, p->token_bytes);

@@ -360,7 +360,7 @@ int check_rows(const dkv_fp4_cache_t* c, const void* key, const void* value, int
   const int rc = dkv::check_fp4_cache(c, what);
   if (rc) return rc;
   DKV_REQUIRE(dtype == DKV_F32 || dtype == DKV_F16 || dtype == DKV_BF16, DKV_EINVAL, "%s: dtype %d not supported", what, dtype);
-  DKV_REQUIRE(n >= 0, DKV_ESHAPE, "%s: %d rows", what, n);
+  DKV_REQUIRE(n >= 0 && n <= INT32_MAX - 65536, DKV_ESHAPE, "%s: %d rows", what, n);  // (a workgroup runs past the last)
   if (n == 0) return DKV_OK;
   DKV_REQUIRE(key && value && slots, DKV_EINVAL, "%s: null pointer", what);
   DKV_REQUIRE((((uintptr_t)key | (uintptr_t)value) & 15) == 0, DKV_EINVAL, "%s: rows must be 16-byte aligned", what);
@@ -373,7 +373,7 @@ extern "C" int dkv_page_assign(const dkv_pages_t* p, const int32_t* new_tokens, 
                                int64_t* positions, int32_t* cu, void* stream) {
   const int rc = check_pages(p, "dkv_page_assign");
   if (rc) return rc;
-  DKV_REQUIRE(rows >= 0, DKV_ESHAPE, "dkv_page_assign: %d rows", rows);
+  DKV_REQUIRE(rows >= 0 && rows <= INT32_MAX - 65536, DKV_ESHAPE, "dkv_page_assign: %d rows", rows);
   DKV_REQUIRE(new_tokens && cu && (rows == 0 || (slots && positions)), DKV_EINVAL, "dkv_page_assign: null pointer");
   PageArgs a = page_args(*p, new_tokens);
   a.slots = slots; a.positions = positions; a.cu = cu; a.rows = rows;

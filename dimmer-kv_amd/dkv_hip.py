@@ -621,6 +621,8 @@ def fp4_store(cache: Fp4Cache, key, value, slots) -> None:
         _expect("fp4_store", slots.device, (slots, "slots", torch.int64, (n,)), (key, "key", dtype, shape),
                 (value, "value", dtype, shape))
         ptr(slots)
+    if n >= 1 << 31:
+        raise ValueError(f"fp4_store: {n} rows")
     if n == 0:
         return
     key, key_at, key_row, key_head = _strided_rows(key)
@@ -639,6 +641,8 @@ def fp4_load(cache: Fp4Cache, slots, key, value) -> None:
         _expect("fp4_load", slots.device, (slots, "slots", torch.int64, (n,)), (key, "key", dtype, shape),
                 (value, "value", dtype, shape))
         ptr(slots), ptr(key), ptr(value)
+    if n >= 1 << 31:
+        raise ValueError(f"fp4_load: {n} rows")
     if n == 0:
         return
     with _on_gpu(index):
@@ -710,8 +714,8 @@ def adjust_logits(args: LogitsArgs, logits, tokens=None, lengths=None, reply=Non
     args.tokens = args.lengths = args.reply = None
     if tokens is not None:
         if tokens.dtype not in (torch.int32, torch.int64) or tokens.dim() != 2 or (
-                tokens.shape[1] > 1 and tokens.stride(1) != 1):
-            raise ValueError("adjust_logits: tokens must be int32 or int64 [rows, history] with contiguous rows")
+                tokens.shape[1] > 1 and tokens.stride(1) != 1) or tokens.shape[1] >= 1 << 31:
+            raise ValueError("adjust_logits: tokens must be int32 or int64 [rows, history < 2^31] with contiguous rows")
         history = tokens.shape[1]
         if tokens.shape[0] != rows or tokens.get_device() != index or not _like(lengths, (rows,), torch.int32, index):
             _expect("adjust_logits", logits.device, (tokens, "tokens", tokens.dtype, (rows, history)),

@@ -111,7 +111,7 @@ class PagedCache:
             most = max(0, *new) if most is None else most
         if rows is None:
             raise ValueError("assign: a GPU tensor of new tokens needs rows, the step's number of rows")
-        if rows < 0:
+        if not 0 <= rows < (1 << 31) - (1 << 16):
             raise ValueError(f"assign: {rows} rows")
         slots, positions = torch.empty(2, rows, dtype=torch.int64, device=self.device).unbind()
         step = Step(slots, positions, torch.empty(self.requests + 1, dtype=torch.int32, device=self.device), rows,
@@ -167,8 +167,8 @@ class PagedCache:
                     window: int | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
         """Attention of the step's queries [rows, q_heads, head_dim] (float32, float16 or bfloat16, any strides) over
         the pages of ``layer``, where the step's own keys and values lie already: causal, and over the last ``window``
-        tokens of each query's if given.  ``out`` (same shape and type, contiguous) keeps its rows behind the last
-        request; without it they are zeros."""
+        tokens of each query's if given.  ``out`` (same shape and type, contiguous; it may be the query) keeps
+        its rows behind the last request; without it they are zeros."""
         if not 0 <= layer < self.layers:
             raise ValueError(f"layer {layer} of {self.layers}")
         if query.dim() != 3 or query.shape[1] % self.kv_heads or query.shape[0] != step.rows:

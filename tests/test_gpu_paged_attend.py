@@ -303,3 +303,17 @@ def test_graph_and_streams():
         out.fill_(float("nan"))
         want = body()
         cache.trim(keep)
+
+
+@pytest.mark.parametrize("dim,lengths,new", [(64, [2900, 7], [1, 1]), (128, [700, 0, 40], [50, 3, 0]), (256, [1500], [20])])
+def test_bounds_and_the_queries_place(dim, lengths, new):
+    """Bounds that are too low, or far too high, change launches only; the result may take the queries' place."""
+    cache, step = build(lengths, new, 2, dim, 16, seed=3)
+    for longest in (1, max(lengths), 1 << 20):
+        for most in (1, max(new), 4000):
+            step.longest, step.most = longest, most
+            query = torch.randn(step.rows, 8, dim, device=DEV).bfloat16()
+            given = query.clone()
+            got = cache.attend_rows(0, query, step, out=query)
+            assert got.data_ptr() == query.data_ptr()
+            compare(cache, step, given, got, dim ** -0.5)

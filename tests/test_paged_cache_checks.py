@@ -172,3 +172,10 @@ def test_attention_workspace():
     none = attend_args(rows=0)
     assert lib.dkv_fp4_attend(ctypes.addressof(none), None, 0, None) == 0
     refused(lib.dkv_fp4_attend(None, None, 0, None), -1, "null arguments")
+
+
+def test_most_rows():
+    c = cache()
+    for call in (store(c, n=2**31 - 1), dkv_hip.lib().dkv_fp4_load(ctypes.addressof(c), P, 2**31 - 1, P, P, 1, None)):
+        refused(call, -2, "2147483647 rows")
+    refused(assign(pages(), rows=2**31 - 1), -2, "2147483647 rows")

@@ -79,3 +79,13 @@ def test_oracle():
     assert logits_ref.adjust([1.0, 1.0], [], 0, 1, 0, 0)[1] == 0
     assert logits_ref.adjust([1.0, np.nan], [], 0, 1, 0, 0)[1] == 1
     assert logits_ref.adjust([1.0, np.nan], [], 0, 1, 0, 0, allowed=[False, False])[1] == -1
+
+
+@pytest.mark.parametrize("change", [dict(tokens=P, lengths=P, history=2**31 - 2**16),
+                                    dict(bias_ids=P, bias_values=P, bias_cu=P, biases=2**31 - 1)])
+def test_longest_lists(change):
+    a = args(**change)
+    assert dkv_hip.lib().dkv_adjust_logits(ctypes.addressof(a), P, 1 << 20, None) == -2
+    assert "2^31 - 2^16" in dkv_hip.lib().dkv_last_error().decode()
+    a = args(**{k: v - 2**17 if type(v) is int and v > P else v for k, v in change.items()})
+    assert dkv_hip.lib().dkv_adjust_logits_workspace_bytes(ctypes.addressof(a)) > 0
