@@ -2,7 +2,8 @@
 pass over the logits (dkv_adjust_logits; include/dimmerkv.h states the arithmetic).
 
 ``ReplyControls`` holds the controls of a batch of replies on the GPU; ``apply`` takes the logits of a step and the
-tokens so far.  ``greedy_answer(..., controls=...)`` answers under them.
+tokens so far.  ``greedy_answer(..., controls=...)`` answers under them.  Calls on one object, its copies and graphs captured
+from them share words that their workgroups count on, and belong on one stream (or on streams the caller orders).
 """
 
 from __future__ import annotations
