@@ -121,12 +121,14 @@ __global__ __launch_bounds__(kThreads, 8) void adjust_logits_kernel(LogitsArgs a
   fetch(0);
   for (int x = tid * 4; x < S::kCountWords + (p.biases ? S::kBitWords : 0); x += kThreads * 4) *(uint4*)(lds + x) = make_uint4(0, 0, 0, 0);
   __syncthreads();
+  // (in 32 bits, an id's upper half being 0: of 64, the comparisons of every id with every stretch would show)
+  const uint32_t lowest = (uint32_t)max(first, 0L), within = (uint32_t)(min(first + kTokens, (long)vocab) - (long)lowest);
   for (int j0 = 0; j0 < length; j0 += kBatch * kThreads) {
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
-      const long at = (long)id[k] - first;
-      if (id[k] >= 0 && id[k] < vocab && (uint64_t)at < (uint64_t)kTokens)
-        Count::add(counts, (int)at, j0 + k * kThreads + tid >= reply);
+      const uint32_t from = (uint32_t)id[k] - lowest;
+      if ((sizeof(ID) == 4 || (uint32_t)((uint64_t)id[k] >> 32) == 0) && from < within)
+        Count::add(counts, (int)(from + (uint32_t)(lowest - first)), j0 + k * kThreads + tid >= reply);
     }
     fetch(j0 + kBatch * kThreads);
   }
