@@ -94,9 +94,13 @@ __global__ __launch_bounds__(kThreads, 8) void adjust_logits_kernel(LogitsArgs a
   const int tid = threadIdx.x, lane = tid & 63, vocab = p.vocab;
   // Eight rows at a time, so that a row's stretches run on one die and its second cache holds the history for all of them
   // (128 replies 37.7 us, 39.0 with the stretches on one die each).
-  const uint32_t id_of = blockIdx.x + blockIdx.y * gridDim.x, eight = id_of / (8 * gridDim.x), in_eight = id_of - eight * 8 * gridDim.x;
-  const uint32_t beside = min(8u, gridDim.y - 8 * eight);
-  const int stretch = (int)(in_eight / beside), row = (int)(8 * eight + in_eight - stretch * beside);
+  int stretch = blockIdx.x, row = 0;
+  if (gridDim.y > 1) {  // (a single row does without the divisions)
+    const uint32_t id_of = blockIdx.x + blockIdx.y * gridDim.x, eight = id_of / (8 * gridDim.x), in_eight = id_of - eight * 8 * gridDim.x;
+    const uint32_t beside = min(8u, gridDim.y - 8 * eight);
+    stretch = (int)(in_eight / beside);
+    row = (int)(8 * eight + in_eight - stretch * beside);
+  }
   const T* logits = (const T*)p.logits + row * p.logits_row;
   T* out = (T*)p.out + row * p.out_row;
   // Elements are numbered from the 16-byte line the row begins in; a row of any alignment is read in whole lines, and
