@@ -13,8 +13,8 @@
 // K is exact in bfloat16 and float16 alike, V in float16 (the exponents are clamped for that).  Queries go in as they are
 // (float32 as three bfloat16 pieces that add up to it).  The weights are rounded to float16, 2^-11 relative, and are held
 // times 2^8 so that weights down to 2^-22 of the row's reference keep that (smaller ones are off by 2^-33 of it): an eighth
-// of a bfloat16 result's own rounding, as much as a float16 one's.  Float16 results of up to 32 rows take a second piece of
-// the weights, and so do float32 results, held times 2^15.  Sums, maxima and accumulators are float32.
+// of a bfloat16 result's own rounding, but as much as a float16 one's.  So float16 results take a second piece of the
+// weights, and so do float32 results, held times 2^15.  Sums, maxima and accumulators are float32.
 // Measured: one token over 2K-32K tokens of 32 requests (8 KV heads of 128 dimensions, 617 MB of pages) 130 us, 4.7 TB/s
 // against a copy's 5.1: the memory bounds it.  2,048 query tokens of 24 heads over 16K tokens (387 GFLOP) 400-430 us, 0.93
 // PFLOP/s; a large library product makes 1.17.  There the vector units bound it (conversions, exponentials and the issue
@@ -238,9 +238,9 @@ __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_at
   using Op = Operand<T>;
   using frag = typename Op::frag;
   constexpr int kRows = 16 * NT, kSteps = D / 32, kLane = D / 16, kPieces = Op::kPieces;
-  // float16 pieces of a weight: a second one for float32 results, and for float16 ones where the memory is what bounds
-  // (the products of up to 32 rows are free there)
-  constexpr int kWeights = kPieces > 1 || (__is_same(T, half_t) && NT <= 2) ? 2 : 1;
+  // float16 pieces of a weight: a second one for float32 and float16 results.  One piece for float16 costs 464 us instead
+  // of 615 at 2,048 query tokens of 24 heads over 16K tokens of 128 dimensions, and rounds as much as the result does.
+  constexpr int kWeights = kPieces > 1 || __is_same(T, half_t) ? 2 : 1;
   // Weights are held times 2^kShift, against a reference that scores may pass by kSlack: 2^15 at the most, below the
   // largest float16.
   constexpr float kSlack = kPieces == 1 ? 7.0f : 0.0f, kShift = 15.0f - kSlack;

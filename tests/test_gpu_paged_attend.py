@@ -317,3 +317,26 @@ def test_bounds_and_the_queries_place(dim, lengths, new):
             got = cache.attend_rows(0, query, step, out=query)
             assert got.data_ptr() == query.data_ptr()
             compare(cache, step, given, got, dim ** -0.5)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("new", [1, 5, 40])
+def test_float16_weights_keep_their_low_bits(new, dim):
+    """Values of 1 give 1 whatever the weights are.  Against the reference of the first 512 tokens the others weigh
+    1 + 0.9 * 2^-11, which one float16 would round to 1: a mean of 1 - 0.8 * 2^-11, past half of the 2^-11 to the next
+    float16 below 1.  Weights that are off by 2^-22 leave it next to 1."""
+    from paged_cache import PagedCache
+
+    total = 4096
+    cache = PagedCache(1, 1, dim, total // 64 + 1, device=DEV)
+    steps = cache.assign([total - new]), cache.assign([new])
+    key = torch.zeros(total, 1, dim, device=DEV)
+    key[512:, 0, 0] = 1.0
+    value = torch.ones(total, 1, dim, device=DEV)
+    for step, rows in zip(steps, (slice(0, total - new), slice(total - new, total))):
+        cache.store(0, key[rows], value[rows], step)
+    steps[1].longest = 1  # no splits: one reference for all tokens
+    query = torch.zeros(new, 2, dim, device=DEV, dtype=torch.float16)
+    query[..., 0] = 1.0
+    out = cache.attend_rows(0, query, steps[1], scaling=float(np.log1p(0.9 * 2.0 ** -11)))
+    assert torch.equal(out, torch.ones_like(out))
