@@ -19,6 +19,7 @@
 // against a copy's 5.1: the memory bounds it.  2,048 query tokens of 24 heads over 16K tokens (387 GFLOP) 400-430 us, 0.93
 // PFLOP/s; a large library product makes 1.17.  There the vector units bound it (conversions, exponentials and the issue
 // slots that matrix instructions take from them), at two waves a SIMD.
+#include <float.h>
 #include <math.h>
 
 #include "dkv_device.h"
@@ -233,8 +234,10 @@ DKV_DEVICE void load_values(const AttendArgs& a, const Tiles<CH>& tiles, const L
   }
 }
 
+// (waves a SIMD: one row tile of 64 dimensions is small enough for three, 32 float32 requests of 8K tokens 44.7 us and 50.2
+// with two)
 template <int D, typename T, int NT, int CH, int kWaves>
-__global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_attend_kernel(AttendArgs a) {
+__global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : NT == 1 && D == 64 ? 3 : 2) void fp4_attend_kernel(AttendArgs a) {
   using Op = Operand<T>;
   using frag = typename Op::frag;
   constexpr int kRows = 16 * NT, kSteps = D / 32, kLane = D / 16, kPieces = Op::kPieces;
@@ -511,12 +514,25 @@ __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_at
       }
     }
 
+    // whether a row sees a token of this wave's chunks (the tokens are the same in every lane)
+    auto sees_some = [&](int nt) {
+      const int last = last_seen(nt), before = before_first(last);
+      bool some = false;
+      for (int c = __builtin_amdgcn_readfirstlane(c0 + wave); c < c1; c += kWaves)
+        for (int token = c * CH * 16; token < min((c + 1) * CH * 16, len); token += 16)
+          if ((uint32_t)as_scalar(table)[token >> a.shift] < (uint32_t)a.c.pages) some = some || (token <= last && token + 15 > before);
+      return some;
+    };
+
     // the waves' sums, 16 rows at a time and four waves at a time
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const float total = sum_xor32(sum_xor16(l[nt]));
-      // a row whose scores are all NaN has no maximum, but is not one that sees nothing
+      // A row whose scores are all NaN has no maximum, but is not one that sees nothing.  Nor is one whose scores are all
+      // -infinity (an infinite query): it goes below every row of scores, with a sum of 0, so that it is 0 / 0 if no token
+      // has more.
       if (m[nt] == -INFINITY && total != 0.0f) m[nt] = 0.0f;
+      if (__any(m[nt] == -INFINITY)) m[nt] = m[nt] == -INFINITY && sees_some(nt) ? -FLT_MAX : m[nt];
       if (g == 0) {
         stat[0][wave][nt * 16 + i] = m[nt];
         stat[1][wave][nt * 16 + i] = total;
@@ -573,9 +589,9 @@ __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_at
         const long out_row = (long)(q0 + token) * q_heads + h * a.groups + (r - token * a.groups);
         if (splits == 1) {
           T* out = (T*)a.out + out_row * D + part * kPart;
-          const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+          const float inverse = 1.0f / total;
 #pragma unroll
-          for (int j = 0; j < kPart; ++j) set_result(out[j], total == 0.0f ? 0.0f : acc[j] * inverse);
+          for (int j = 0; j < kPart; ++j) set_result(out[j], highest == -INFINITY ? 0.0f : acc[j] * inverse);
         } else {
           const long at = out_row * splits + split;
           float* out = a.part + at * D + part * kPart;
@@ -661,7 +677,7 @@ __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_at
             }
             T* out = (T*)a.out + out_row * D + dim;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) set_result(out[j], whole == 0.0f ? 0.0f : v[j] / whole);
+            for (int j = 0; j < 4; ++j) set_result(out[j], highest == -INFINITY ? 0.0f : v[j] / whole);
           }
           __syncthreads();
         }
@@ -677,7 +693,7 @@ __global__ __launch_bounds__(256) void fp4_join_kernel(AttendArgs a, int q_heads
   constexpr int kSet = D / 4, kSets = 256 / kSet;
   __shared__ float weight[kMaxSplits];
   __shared__ float4 sums[kSets][kSet];
-  __shared__ float whole;
+  __shared__ float whole;  // below 0: the row sees nothing
   const long row = blockIdx.x;
   if (row >= (long)min(max(a.cu[a.requests], 0), a.rows) * q_heads) return;
   const float2* ml = a.part_ml + row * a.splits;
@@ -699,7 +715,7 @@ __global__ __launch_bounds__(256) void fp4_join_kernel(AttendArgs a, int q_heads
       total += factor < 0.0f ? 0.0f : x[k].y * factor;
     }
     total = wave_sum(total);
-    if (threadIdx.x == 0) whole = total;
+    if (threadIdx.x == 0) whole = top == -INFINITY ? -1.0f : total;
   }
   __syncthreads();
   const int at = threadIdx.x % kSet, set = threadIdx.x / kSet;
@@ -723,7 +739,7 @@ __global__ __launch_bounds__(256) void fp4_join_kernel(AttendArgs a, int q_heads
   T* out = (T*)a.out + row * D + at * 4;
   const float v[4] = {acc.x, acc.y, acc.z, acc.w};
 #pragma unroll
-  for (int j = 0; j < 4; ++j) set_result(out[j], whole == 0.0f ? 0.0f : v[j] / whole);
+  for (int j = 0; j < 4; ++j) set_result(out[j], whole < 0.0f ? 0.0f : v[j] / whole);
 }
 
 // The same for few splits: a set of D / 4 threads per row.  49,152 rows of two splits: 13 us, 40 with a workgroup for
@@ -750,7 +766,7 @@ __global__ __launch_bounds__(256) void fp4_join_few_kernel(AttendArgs a, int q_h
   T* out = (T*)a.out + row * D + at * 4;
   const float v[4] = {acc.x, acc.y, acc.z, acc.w};
 #pragma unroll
-  for (int j = 0; j < 4; ++j) set_result(out[j], whole == 0.0f ? 0.0f : v[j] / whole);
+  for (int j = 0; j < 4; ++j) set_result(out[j], top == -INFINITY ? 0.0f : v[j] / whole);
 }
 
 struct Plan {

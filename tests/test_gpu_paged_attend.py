@@ -340,3 +340,30 @@ def test_float16_weights_keep_their_low_bits(new, dim):
     query[..., 0] = 1.0
     out = cache.attend_rows(0, query, steps[1], scaling=float(np.log1p(0.9 * 2.0 ** -11)))
     assert torch.equal(out, torch.ones_like(out))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("heads,total,new,window", [(1, 1, 1, None), (1, 700, 1, None), (1, 3000, 2, None), (1, 20000, 1, None),
+                                                    (1, 200, 50, None), (1, 200, 50, 20), (1, 6000, 300, None), (8, 5000, 700, None)])
+def test_scores_of_minus_infinity(heads, total, new, window, dtype):
+    """A row that sees tokens, all with scores of -infinity, is NaN (0 / 0), unlike one that sees none; other rows keep
+    their results, in one launch, joined in it or by the others."""
+    cache, step = build([total - new], [new], heads, 64, 64)
+    from paged_cache import Step
+
+    slots = cache.slots(0, 0, total)
+    key, value = cache.load(0, slots, torch.float32)
+    key[..., 0] = 1.0  # (a key of 0 would make NaN of itself)
+    cache.store(0, key, value, Step(slots, slots, step.cu, total, 1, 1))
+    assert (cache.load(0, slots, torch.float32)[0][..., 0] > 0).all()
+    query = torch.randn(new, 3 * heads, 64, device=DEV).to(TYPES[dtype])
+    clean = cache.attend_rows(0, query, step, window=window)
+    assert clean.isfinite().all()
+    rows = sorted({0, new // 2, new - 1})
+    query[rows, 1, 0] = -float("inf")
+    got = cache.attend_rows(0, query, step, window=window)
+    assert got[rows, 1].isnan().all()
+    got[rows, 1] = clean[rows, 1]
+    assert torch.equal(got, clean)
+    cache.table.fill_(-1)  # no page holds a token: nothing is seen
+    assert not cache.attend_rows(0, query, step, window=window).any()
