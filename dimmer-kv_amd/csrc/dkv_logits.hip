@@ -13,9 +13,13 @@
 
 #include "dkv_device.h"
 #include "dkv_fp4.h"
+#include "dkv_stretch.h"
 #include "dkv_host.h"
 
 namespace {
+
+using dkv::TokenRange;
+using dkv::tokens_of_stretch;
 
 constexpr int kThreads = 1024;
 
@@ -131,13 +135,13 @@ __global__ __launch_bounds__(kThreads, 8) void adjust_logits_kernel(LogitsArgs a
   for (int x = tid * 4; x < S::kCountWords + (p.biases ? S::kBitWords : 0); x += kThreads * 4) *(uint4*)(lds + x) = make_uint4(0, 0, 0, 0);
   __syncthreads();
   // (in 32 bits, an id's upper half being 0: of 64, the comparisons of every id with every stretch would show)
-  const uint32_t lowest = (uint32_t)max(first, 0L), within = (uint32_t)(min(first + kTokens, (long)vocab) - (long)lowest);
+  const TokenRange own = tokens_of_stretch(first, kTokens, vocab);
   for (int j0 = 0; j0 < length; j0 += kBatch * kThreads) {
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
-      const uint32_t from = (uint32_t)id[k] - lowest;
-      if ((sizeof(ID) == 4 || (uint32_t)((uint64_t)id[k] >> 32) == 0) && from < within)
-        Count::add(counts, (int)(from + (uint32_t)(lowest - first)), j0 + k * kThreads + tid >= reply);
+      const uint32_t from = (uint32_t)id[k] - own.lowest;
+      if ((sizeof(ID) == 4 || (uint32_t)((uint64_t)id[k] >> 32) == 0) && from < own.count)
+        Count::add(counts, (int)(from + (uint32_t)(own.lowest - first)), j0 + k * kThreads + tid >= reply);
     }
     fetch(j0 + kBatch * kThreads);
   }
@@ -307,7 +311,7 @@ struct Plan {
 Plan plan_of(const dkv_logits_args_t& p) {
   Plan plan;
   const int line = p.dtype == DKV_F32 ? 4 : 8, most = 16 / line;  // elements of a line; lines of 16,384
-  const auto chunks = [&](int lines) { return (int)(((long)p.vocab + line - 1 + kThreads * lines * line - 1) / (kThreads * lines * line)); };
+  const auto chunks = [&](int lines) { return dkv::stretches_of_row(p.vocab, line, kThreads * lines * line); };
   plan.counts16 = !p.tokens || p.history < 0x8000;
   plan.lines = plan.counts16 && (long)chunks(most) * p.rows >= 512 ? most : 1;
   plan.chunks = chunks(plan.lines);

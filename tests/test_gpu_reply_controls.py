@@ -232,3 +232,17 @@ def test_masks_change_under_a_graph(masks):
         graph.replay()
         want = torch.where(may, logits, -float("inf")).argmax(1)
         assert torch.equal(pick, want) and torch.equal(controls.apply(logits)[1], want)
+
+
+@pytest.mark.parametrize("rows,dtype,vocabs", [(2, "f16", (8185, 8186, 8191, 16383)), (2, "bf16", (8186, 8191, 32767)),
+                                               (2, "f32", (4093, 4094, 4095, 8191)), (64, "bf16", (131070, 131071)),
+                                               (64, "f32", (131070, 131071))])
+def test_vocabularies_below_a_stretch(rows, dtype, vocabs):
+    """The last stretch of a row begins past the vocabulary: it counts nothing, and the others count as ever."""
+    for vocab in vocabs:
+        print(f"[case] logits {rows}x{vocab} {dtype}", flush=True)
+        c = make_case(rows, vocab, 500, 6, True, dtype)
+        out, pick = apply(c)
+        for r in (0, 1, rows - 1):
+            one = {k: (v[r:r + 1] if k != "bias" else [v[r]]) for k, v in c.items()}
+            check(one, out[r:r + 1], pick[r:r + 1])

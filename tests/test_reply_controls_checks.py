@@ -89,3 +89,50 @@ def test_longest_lists(change):
     assert "2^31 - 2^16" in dkv_hip.lib().dkv_last_error().decode()
     a = args(**{k: v - 2**17 if type(v) is int and v > P else v for k, v in change.items()})
     assert dkv_hip.lib().dkv_adjust_logits_workspace_bytes(ctypes.addressof(a)) > 0
+
+
+STRETCHES = """
+#include "dkv_stretch.h"
+// How often the stretches of a row count each token (seen), and how many of their counters lie outside a stretch.
+extern "C" long count(long vocab, int line, int tokens, int shift, int* seen) {
+  long outside = 0;
+  for (int s = 0; s < dkv::stretches_of_row(vocab, line, tokens); ++s) {
+    const long first = (long)s * tokens - shift;
+    const dkv::TokenRange own = dkv::tokens_of_stretch(first, tokens, vocab);
+    for (long id = -2; id < vocab + 2; ++id) {
+      const uint32_t from = (uint32_t)id - own.lowest;
+      if (from >= own.count) continue;
+      const long at = (int)(from + (uint32_t)(own.lowest - first));
+      if (id < 0 || id >= vocab || at < 0 || at >= tokens) ++outside;
+      else ++seen[id];
+    }
+  }
+  return outside;
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def count(tmp_path_factory):
+    import subprocess
+    from pathlib import Path
+
+    here = tmp_path_factory.mktemp("stretch")
+    (here / "count.cpp").write_text(STRETCHES)
+    csrc = Path(dkv_hip.__file__).resolve().parent / "csrc"
+    subprocess.run(["g++", "-std=c++17", "-O1", "-shared", "-fPIC", f"-I{csrc}", "-o", here / "count.so", here / "count.cpp"], check=True)
+    call = ctypes.CDLL(str(here / "count.so")).count
+    call.restype, call.argtypes = ctypes.c_long, [ctypes.c_long, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_void_p]
+    return call
+
+
+@pytest.mark.parametrize("line,tokens", [(8, 64), (4, 64), (8, 8192), (8, 16384), (4, 4096), (4, 16384)])
+def test_stretches_count_their_own_tokens(count, line, tokens):
+    """Every token of the vocabulary is counted once and inside its stretch, wherever in a line the row begins; so also
+    where the last stretch begins past the vocabulary (a vocabulary just below a multiple of the stretch)."""
+    some = range(1, 200) if tokens == 64 else [tokens - x for x in range(-9, 10)] + [1, 2 * tokens - 1, 2 * tokens - line + 2]
+    for vocab in some:
+        for shift in range(line):
+            seen = np.zeros(vocab, np.int32)
+            assert count(vocab, line, tokens, shift, seen.ctypes.data) == 0, (vocab, shift)
+            assert (seen == 1).all(), (vocab, shift)
