@@ -135,7 +135,7 @@ __global__ __launch_bounds__(kThreads, 8) void adjust_logits_kernel(LogitsArgs a
   for (int x = tid * 4; x < S::kCountWords + (p.biases ? S::kBitWords : 0); x += kThreads * 4) *(uint4*)(lds + x) = make_uint4(0, 0, 0, 0);
   __syncthreads();
   // (in 32 bits, an id's upper half being 0: of 64, the comparisons of every id with every stretch would show)
-  const TokenRange own = tokens_of_stretch(first, kTokens, vocab);
+  const TokenRange own = tokens_of_stretch((int)first, kTokens, vocab);
   for (int j0 = 0; j0 < length; j0 += kBatch * kThreads) {
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {

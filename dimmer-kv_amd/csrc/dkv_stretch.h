@@ -19,8 +19,8 @@ DKV_EITHER int stretches_of_row(int64_t vocab, int line, int tokens) { return (i
 struct TokenRange {
   uint32_t lowest, count;
 };
-DKV_EITHER TokenRange tokens_of_stretch(int64_t first, int tokens, int64_t vocab) {
-  const int64_t lowest = first < 0 ? 0 : first, end = first + tokens < vocab ? first + tokens : vocab;
+DKV_EITHER TokenRange tokens_of_stretch(int32_t first, int32_t tokens, int32_t vocab) {  // (their sum is below 2^31)
+  const int32_t lowest = first > 0 ? first : 0, end = first + tokens < vocab ? first + tokens : vocab;
   return TokenRange{(uint32_t)lowest, (uint32_t)(end > lowest ? end - lowest : 0)};
 }
 
