@@ -154,11 +154,13 @@ __global__ __launch_bounds__(kThreads, 8) void adjust_logits_kernel(LogitsArgs a
   __syncthreads();
 
   const uint32_t* allowed = nullptr;
+  bool limited = false;  // (a mask past the last one allows nothing)
   if (p.allowed) {
     const int mask = p.allowed_row ? p.allowed_row[row] : row;
-    if (mask >= 0 && mask < p.masks) allowed = (const uint32_t*)p.allowed + (long)mask * p.words;
+    limited = mask >= 0;
+    if (limited && mask < p.masks) allowed = (const uint32_t*)p.allowed + (long)mask * p.words;
   }
-  const auto may = [&](int token) { return !allowed || ((allowed[token >> 5] >> (token & 31)) & 1); };
+  const auto may = [&](int token) { return !limited || (allowed && ((allowed[token >> 5] >> (token & 31)) & 1)); };
   uint64_t best = 0;
   float highest = -INFINITY;  // of best; above it all once that is a NaN
   const auto seen = [&](float x, int token) {
@@ -192,10 +194,10 @@ __global__ __launch_bounds__(kThreads, 8) void adjust_logits_kernel(LogitsArgs a
       T x[V];
       float z[V];
       __builtin_memcpy(x, &lines[k], 16);
-      if (allowed) {
+      if (limited) {
         const int word = (int)token >> 5, in = (int)token & 31;
-        bits = allowed[word] >> in;
-        if (in + V > 32) bits |= allowed[word + 1] << (32 - in);
+        bits = allowed ? allowed[word] >> in : 0;
+        if (allowed && in + V > 32) bits |= allowed[word + 1] << (32 - in);
 #pragma unroll
         for (int v = 0; v < V; ++v)
           if (!(((bits | with_bias) >> v) & 1)) set_logit(x[v], -INFINITY);

@@ -36,7 +36,8 @@ class ReplyControls:
         - ``bias``: added to logits; {token: value} for every row, a list of such dicts by row, or (ids int32,
           values float32, cu int32 [rows + 1]); of an id that a row lists twice the last value counts;
         - ``allowed``: bool [rows, vocab] or [1, vocab] (every row), or (words int32 [masks, ceil(vocab / 32)],
-          mask of each row int32 [rows], -1 for none).  ``allow`` changes it later.
+          mask of each row int32 [rows], -1 for none; a number past the masks allows nothing).  ``allow`` changes it
+          later.
 
         A captured ``apply`` reads the memory of its capture: bool masks given to ``allow`` later go into the memory of
         the first of their shape, so replays see them; tensors of a tuple on the GPU are read where they are, and theirs

@@ -563,7 +563,7 @@ typedef struct dkv_logits_args {
   const float* bias_values;  /* [biases] */
   const int32_t* bias_cu;    /* [rows + 1] where each row's biases begin */
   const int32_t* allowed;    /* [masks][words] bit t % 32 of word t / 32: token t may be picked; null: no mask */
-  const int32_t* allowed_row;/* [rows] which mask, -1 none; null: row r takes mask r */
+  const int32_t* allowed_row;/* [rows] which mask, below 0 none, past the last one nothing allowed; null: row r takes mask r */
   int64_t* pick;             /* [rows] or null */
   uint32_t* arrivals;        /* [rows] zero at first and left so, or null: with it the pick takes no second launch.  Calls */
                              /* that overlap need words of their own. */

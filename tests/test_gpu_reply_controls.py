@@ -246,3 +246,20 @@ def test_vocabularies_below_a_stretch(rows, dtype, vocabs):
         for r in (0, 1, rows - 1):
             one = {k: (v[r:r + 1] if k != "bias" else [v[r]]) for k, v in c.items()}
             check(one, out[r:r + 1], pick[r:r + 1])
+
+
+@pytest.mark.parametrize("vocab,biases", [(300, 0), (300, 3), (9000, 2)])
+def test_mask_numbers_past_the_masks(vocab, biases):
+    """A row whose mask number is past the masks may take nothing; one below 0 has no mask."""
+    from reply_controls import ReplyControls, pack_allowed
+
+    logits = torch.randn(5, vocab, device=DEV)
+    mask = torch.rand(2, vocab, device=DEV) < 0.5
+    controls = ReplyControls(5, vocab, bias={t * 7: 1.0 for t in range(biases)} or None,
+                             allowed=(pack_allowed(mask), int32([0, 2, -1, 2**31 - 1, -(2**31)])))
+    out, pick = controls.apply(logits, torch.arange(50, device=DEV).expand(5, 50))
+    free, best = ReplyControls(5, vocab, bias={t * 7: 1.0 for t in range(biases)} or None).apply(
+        logits, torch.arange(50, device=DEV).expand(5, 50))
+    assert (out[[1, 3]] == -float("inf")).all() and pick[[1, 3]].tolist() == [-1, -1]
+    assert torch.equal(out[[2, 4]], free[[2, 4]]) and torch.equal(pick[[2, 4]], best[[2, 4]])
+    assert torch.equal(out[0], torch.where(mask[0], free[0], -float("inf")))
