@@ -65,11 +65,14 @@ class ReplyControls:
             self.allow(allowed)
 
     def __copy__(self) -> "ReplyControls":
-        """The same controls, with masks of its own from now on."""
+        """The same controls, with masks of its own from now on: bool masks given to one do not reach the other."""
         other = ReplyControls.__new__(ReplyControls)
         other.__dict__.update(self.__dict__)
         other._args = dkv_hip.LogitsArgs.from_buffer_copy(self._args)
         other._held, other._masks = dict(self._held), {}
+        words = self._held.get("allowed")
+        if any(words is kept for kept in self._masks.values()):
+            other._hold("allowed", words.clone())
         return other
 
     def _hold(self, name: str, t: torch.Tensor) -> None:

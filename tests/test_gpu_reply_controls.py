@@ -263,3 +263,23 @@ def test_mask_numbers_past_the_masks(vocab, biases):
     assert (out[[1, 3]] == -float("inf")).all() and pick[[1, 3]].tolist() == [-1, -1]
     assert torch.equal(out[[2, 4]], free[[2, 4]]) and torch.equal(pick[[2, 4]], best[[2, 4]])
     assert torch.equal(out[0], torch.where(mask[0], free[0], -float("inf")))
+
+
+@pytest.mark.parametrize("masks", [1, 2])
+def test_a_copy_keeps_its_masks(masks):
+    """Bool masks given to controls after they were copied, or to the copy, are theirs alone."""
+    import copy
+
+    from reply_controls import ReplyControls
+
+    only = lambda token: (torch.arange(100, device=DEV) == token).expand(masks, 100)
+    logits = torch.randn(2, 100, device=DEV)
+    controls = ReplyControls(2, 100, allowed=only(7))
+    other = copy.copy(controls)
+    controls.allow(only(9))
+    assert other.apply(logits)[1].tolist() == [7, 7] and controls.apply(logits)[1].tolist() == [9, 9]
+    other.allow(only(11))
+    third = copy.copy(other)
+    other.allow(None)
+    assert controls.apply(logits)[1].tolist() == [9, 9] and third.apply(logits)[1].tolist() == [11, 11]
+    assert torch.equal(other.apply(logits)[1], logits.argmax(1))
