@@ -40,8 +40,9 @@ class ReplyControls:
           later.
 
         A captured ``apply`` reads the memory of its capture: bool masks given to ``allow`` later go into the memory of
-        the first of their shape, so replays see them; tensors of a tuple on the GPU are read where they are, and theirs
-        to change is the caller's."""
+        the first of their shape, so replays see them; words and mask numbers given as a tuple of GPU tensors are read
+        where they are, and so are the values of biases: the caller may change them.  Which tokens of which rows have a
+        bias is fixed here (ids and cu are copied: equal ids of a row are sorted out once)."""
         if rows < 0 or rows > 65535 or vocab < 1:
             raise ValueError(f"ReplyControls: {rows} rows (at most 65535) of {vocab} tokens")
         if torch.device(device).type != "cuda":
@@ -106,14 +107,14 @@ class ReplyControls:
                 or ids.shape != values.shape or cu.shape != (self.rows + 1,)):
             raise ValueError(f"ReplyControls: bias must be (int32 [n], float32 [n], int32 [{self.rows + 1}])")
         ids, values, cu = (t.to(self.device).contiguous() for t in (ids, values, cu))
-        for name, t in (("bias_ids", self._last_of_each(ids, cu)), ("bias_values", values), ("bias_cu", cu)):
+        for name, t in (("bias_ids", self._last_of_each(ids, cu)), ("bias_values", values), ("bias_cu", cu.clone())):
             self._hold(name, t)
         self._args.biases = ids.shape[0]
 
     def _last_of_each(self, ids: torch.Tensor, cu: torch.Tensor) -> torch.Tensor:
         """The ids with -1 for all but a row's last mention of each: a stable sort by row and id puts that one last."""
         if ids.numel() == 0:
-            return ids
+            return ids.clone()
         row = torch.searchsorted(cu, torch.arange(ids.numel(), dtype=torch.int32, device=self.device), right=True)
         key, place = torch.sort(row * (1 << 32) + ids, stable=True)
         last = torch.nn.functional.pad(key[1:] != key[:-1], (0, 1), value=True)

@@ -283,3 +283,20 @@ def test_a_copy_keeps_its_masks(masks):
     other.allow(None)
     assert controls.apply(logits)[1].tolist() == [9, 9] and third.apply(logits)[1].tolist() == [11, 11]
     assert torch.equal(other.apply(logits)[1], logits.argmax(1))
+
+
+def test_bias_lists_are_fixed():
+    """Ids and rows of a tuple of biases changed later have no part (rows could come to hold an id twice); values have."""
+    from reply_controls import ReplyControls
+
+    logits = torch.randn(2, 100, device=DEV)
+    ids, values, cu = int32([7, 8, 7, 50]), f32([1.0, 2.0, 4.0, 8.0]), int32([0, 2, 4])
+    controls = ReplyControls(2, 100, bias=(ids, values, cu))
+    ids.fill_(3)
+    cu.copy_(int32([0, 4, 4]))
+    want = logits.clone()
+    want[0, 7], want[0, 8], want[1, 7], want[1, 50] = want[0, 7] + 1, want[0, 8] + 2, want[1, 7] + 4, want[1, 50] + 8
+    assert torch.equal(controls.apply(logits)[0], want)
+    values.mul_(2.0)
+    out = controls.apply(logits)[0]
+    assert torch.equal(out[0, 7], logits[0, 7] + 2.0) and torch.equal(out[1, 50], logits[1, 50] + 16.0)
