@@ -196,7 +196,8 @@ class PagedContext:
     ``compressed_attention.CompressedContext`` for the ``dimmer`` hook.  Every forward's new keys and values are stored
     before they are attended to, in 4 bits as all others, so ``exact_cache`` (the cache the model updates) only carries
     them here: it starts empty.  Attention is causal, over all tokens or a layer's sliding window as the model's
-    configuration has it; the model's additive mask is not read."""
+    configuration has it; the model's additive mask is not read.  Models whose attention is more than that (a soft cap on
+    scores, sinks beside the keys, other kinds of layers) are refused."""
 
     def __init__(self, keys: list[torch.Tensor], values: list[torch.Tensor], model, page: int = 64, room: int = 1024):
         """Per-layer [1, kv_heads, tokens, head_dim] keys (RoPE applied) and values on the GPU, with room for ``room`` more
@@ -208,12 +209,13 @@ class PagedContext:
                              f"(got {len(keys)} and {len(values)} of {list(shape)})")
         if room < 0:
             raise ValueError(f"PagedContext: room {room}")
+        self._windows = self._layer_windows(model.config, len(keys))
+        self._refuse_more_than_scores(model)
         _, heads, tokens, dim = shape
         pages = max(1, -(-(tokens + room) // page))
         self.cache = PagedCache(len(keys), heads, dim, pages, page=page, device=first.device)
         self.capacity, self.tokens = pages * page, tokens
         self._model = model
-        self._windows = self._layer_windows(model.config, len(keys))
         step = self.cache.assign([tokens], longest=tokens)
         for layer, (key, value) in enumerate(zip(keys, values)):
             if key.shape != shape or value.shape != shape:
@@ -231,6 +233,15 @@ class PagedContext:
             if kind not in ("full_attention", "sliding_attention"):
                 raise ValueError(f"PagedContext: layers of {kind}")
         return [window if kind == "sliding_attention" else None for kind in kinds]
+
+    @staticmethod
+    def _refuse_more_than_scores(model) -> None:
+        """Refuse models whose attention is not a softmax of scaled scores over the keys alone: the hook is given their
+        soft cap (``softcap``) and sinks (``s_aux``), and would drop them."""
+        if getattr(model.config.get_text_config(decoder=True), "attn_logit_softcapping", None):
+            raise ValueError("PagedContext: the model's attention has a soft cap on its scores")
+        if any(getattr(module, "sinks", None) is not None for module in getattr(model, "modules", tuple)()):
+            raise ValueError("PagedContext: the model's attention has sinks beside its keys")
 
     def fresh_cache(self):
         """An empty cache for the model to update: one for every answer."""

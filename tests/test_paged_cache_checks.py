@@ -179,3 +179,27 @@ def test_most_rows():
     for call in (store(c, n=2**31 - 1), dkv_hip.lib().dkv_fp4_load(ctypes.addressof(c), P, 2**31 - 1, P, P, 1, None)):
         refused(call, -2, "2147483647 rows")
     refused(assign(pages(), rows=2**31 - 1), -2, "2147483647 rows")
+
+
+@pytest.mark.parametrize("family,words", [("Gemma2", "soft cap"), ("GptOss", "sinks")])
+def test_attention_of_more_than_scores_is_refused(family, words):
+    """Models whose attention has a soft cap or sinks, before anything is stored; without them such a model is taken (as far
+    as the GPU that this test does without)."""
+    import transformers
+    from paged_cache import PagedContext
+
+    sizes = dict(num_hidden_layers=2, hidden_size=64, intermediate_size=64, num_attention_heads=2, num_key_value_heads=1,
+                 head_dim=64, vocab_size=50)
+    if family == "GptOss":
+        sizes |= dict(num_local_experts=2, num_experts_per_tok=1)
+    config = getattr(transformers, f"{family}Config")(**sizes)
+    model = getattr(transformers, f"{family}ForCausalLM")(config)
+    caches = [torch.zeros(1, 1, 5, 64) for _ in range(2)]
+    with pytest.raises(ValueError, match=words):
+        PagedContext(caches, caches, model)
+    config.attn_logit_softcapping = None
+    for module in model.modules():
+        if hasattr(module, "sinks"):
+            module.sinks = None
+    with pytest.raises(ValueError, match="needs a GPU"):
+        PagedContext(caches, caches, model)
