@@ -221,7 +221,7 @@ class PagedContext:
             if key.shape != shape or value.shape != shape:
                 raise ValueError(f"layer {layer}: keys {list(key.shape)} and values {list(value.shape)}, not {list(shape)}")
             self.cache.store(layer, key[0].transpose(0, 1), value[0].transpose(0, 1), step)
-        self._step = None
+        self._step, self._next = None, 0  # of the forward that runs: its rows, and the layer it is at
         self.exact_cache = self.fresh_cache()
 
     @staticmethod
@@ -259,7 +259,7 @@ class PagedContext:
         if not 0 <= tokens <= self.tokens:
             raise ValueError(f"rewind to {tokens} of {self.tokens} tokens")
         self.cache.trim([tokens])
-        self.tokens, self._step = tokens, None
+        self.tokens, self._step, self._next = tokens, None, 0
         self.exact_cache = self.fresh_cache()
 
     def rebuilt(self, dtype: torch.dtype = torch.float16, tokens: int | None = None):
@@ -271,7 +271,8 @@ class PagedContext:
                 [value.transpose(0, 1).contiguous().unsqueeze(0) for _, value in rows])
 
     def attend(self, module, query, key, value, attention_mask, scaling):
-        """Same contract as an HF attention function: returns (output [1, T, H, D], None)."""
+        """Same contract as an HF attention function: returns (output [1, T, H, D], None).  A forward takes its layers in
+        turn; after one that stopped half way ``rewind`` has to forget its tokens, which some layers do not hold."""
         layer, c = module.layer_idx, self.cache
         batch, q_heads, new, _ = query.shape
         if batch != 1:
@@ -280,17 +281,23 @@ class PagedContext:
             raise ValueError("module.num_key_value_groups does not match the cache's KV heads")
         if key is None or key.shape[2] < new:
             raise ValueError("PagedContext needs the new tokens' keys in the model's cache")
-        if layer == 0:  # a forward begins: pages for its tokens
+        if layer != self._next or (self._step is not None and self._step.rows != new):
+            if self._step is None:
+                raise ValueError("PagedContext: a forward starts at layer 0")
+            raise ValueError(f"PagedContext: {new} tokens at layer {layer} where a forward of {self._step.rows} is at layer "
+                             f"{self._next}; rewind({self.tokens - self._step.rows}) forgets one that stopped there")
+        if self._step is None:  # a forward begins: pages for its tokens
             if self.tokens + new > self.capacity:
                 raise ValueError(f"{self.tokens} + {new} tokens pass the {self.capacity} the context has pages for")
             self._step = c.assign([new], longest=self.tokens + new)
             self.tokens += new
-        elif self._step is None or self._step.rows != new:
-            raise ValueError("PagedContext: a forward starts at layer 0")
         past = key.shape[2] - new
         c.store(layer, key[0, :, past:].transpose(0, 1), value[0, :, past:].transpose(0, 1), self._step)
-        return c.attend_rows(layer, query[0].transpose(0, 1), self._step, scaling=scaling,
-                             window=self._windows[layer]).unsqueeze(0), None
+        out = c.attend_rows(layer, query[0].transpose(0, 1), self._step, scaling=scaling, window=self._windows[layer])
+        self._next = layer + 1
+        if self._next == c.layers:
+            self._step, self._next = None, 0
+        return out.unsqueeze(0), None
 
 
 __all__ = ["PagedCache", "PagedContext", "Step"]

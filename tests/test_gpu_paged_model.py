@@ -254,3 +254,51 @@ def test_sliding_window_layers():
     config = LlamaConfig(layer_types=["full_attention", "chunked_attention"], attention_chunk_size=64, **shape)
     with pytest.raises(ValueError, match="chunked"):
         PagedContext(keys, values, SimpleNamespace(config=config))
+
+
+def test_a_forward_that_stops_half_way():
+    """Tokens that some layers do not hold are not answered over: the next forward is refused until rewind forgets them."""
+    from types import SimpleNamespace
+
+    from paged_cache import PagedContext
+    from transformers import LlamaConfig
+
+    config = LlamaConfig(num_hidden_layers=3, hidden_size=256, num_attention_heads=4, num_key_value_heads=2, head_dim=64)
+    g = torch.Generator(DEV).manual_seed(6)
+    rand = lambda *s: torch.randn(*s, generator=g, device=DEV)
+    keys, values = ([rand(1, 2, 30, 64) for _ in range(3)] for _ in range(2))
+    context = PagedContext(keys, values, SimpleNamespace(config=config))
+
+    def call(layer, new, broken=False):
+        query, key, value = rand(1, 4, new, 64), rand(1, 2, new, 64), rand(1, 2, new, 64)
+        module = SimpleNamespace(layer_idx=layer, num_key_value_groups=2)
+        have, _ = context.attend(module, query, key[..., :32] if broken else key, value, None, 0.125)
+        rows = [t.double().cpu().numpy() for t in context.cache.load(layer, context.cache.slots(0, 0, context.tokens), torch.float32)]
+        want = paged_ref.attend(query[0].transpose(0, 1).double().cpu().numpy(), *rows, 0.125)
+        # float32 sums of at most 40 terms of order 1
+        assert np.abs(have[0].double().cpu().numpy() - want).max() < 40 * 2.0 ** -20
+        assert rows[0].shape[0] == context.tokens
+
+    for layer in range(3):
+        call(layer, 3)
+    with pytest.raises(ValueError, match="starts at layer 0"):
+        call(1, 3)
+    call(0, 3)
+    with pytest.raises(ValueError, match=r"rewind\(33\)"):
+        call(2, 3)  # a layer left out
+    call(1, 3)
+    for new in (3, 1):
+        with pytest.raises(ValueError, match=r"rewind\(33\)"):
+            call(0, new)
+    context.rewind(33)
+    assert context.tokens == 33
+    with pytest.raises(ValueError):
+        call(0, 2, broken=True)  # stopped inside its first layer
+    with pytest.raises(ValueError, match=r"rewind\(33\)"):
+        call(0, 1)
+    for layer in range(3):  # tried again with as many tokens
+        call(layer, 2)
+    assert context.tokens == 35
+    for layer in range(3):
+        call(layer, 1)
+    context.cache.check()
