@@ -134,6 +134,8 @@ class PagedCache:
 
     def slots(self, request: int, start: int, stop: int) -> torch.Tensor:
         """Slots int64 of tokens start..stop - 1 that a request holds."""
+        if not 0 <= start <= stop <= self.table_pages * self.page:
+            raise ValueError(f"slots: tokens {start} to {stop} of a request of at most {self.table_pages * self.page}")
         at = torch.arange(start, stop, device=self.device)
         return self.table[request].long()[at // self.page] * self.page + at % self.page
 

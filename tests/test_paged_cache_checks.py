@@ -203,3 +203,23 @@ def test_attention_of_more_than_scores_is_refused(family, words):
             module.sinks = None
     with pytest.raises(ValueError, match="needs a GPU"):
         PagedContext(caches, caches, model)
+
+
+def host_cache(**change):
+    """A PagedCache's tables on the CPU, for what is decided before any kernel."""
+    from paged_cache import PagedCache
+
+    c = PagedCache.__new__(PagedCache)
+    fields = dict(device=torch.device("cpu"), requests=2, table_pages=3, page=16, layers=1, kv_heads=2, head_dim=64,
+                  table=torch.tensor([[4, 2, -1], [0, -1, -1]], dtype=torch.int32))
+    for name, value in (fields | change).items():
+        setattr(c, name, value)
+    return c
+
+
+def test_slots_past_the_table_are_refused():
+    c = host_cache()
+    assert c.slots(0, 14, 18).tolist() == [78, 79, 32, 33] and c.slots(1, 48, 48).numel() == 0
+    for start, stop in ((0, 49), (-1, 5), (5, 4), (48, 64)):
+        with pytest.raises(ValueError, match="slots"):
+            c.slots(0, start, stop)
