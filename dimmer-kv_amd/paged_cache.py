@@ -94,9 +94,10 @@ class PagedCache:
             self._attend.append(a)
 
     # ----- tables -----
-    def _counts(self, counts) -> torch.Tensor:
+    def _counts(self, counts, what: str) -> torch.Tensor:
         if not torch.is_tensor(counts):
-            counts = dkv_hip.to_device(list(counts), torch.int32, self.device)
+            return dkv_hip.to_device(list(counts), torch.int32, self.device)
+        self._here(counts, what)
         return counts
 
     def assign(self, new, rows: int | None = None, longest: int | None = None, most: int | None = None) -> Step:
@@ -116,13 +117,13 @@ class PagedCache:
         slots, positions = torch.empty(2, rows, dtype=torch.int64, device=self.device).unbind()
         step = Step(slots, positions, torch.empty(self.requests + 1, dtype=torch.int32, device=self.device), rows,
                     self.table_pages * self.page if longest is None else longest, rows if most is None else most)
-        dkv_hip.page_assign(self._pages, self._counts(new), rows, step.slots, step.positions, step.cu)
+        dkv_hip.page_assign(self._pages, self._counts(new, "assign"), rows, step.slots, step.positions, step.cu)
         return step
 
     def trim(self, keep) -> None:
         """Cut every request back to at most ``keep`` tokens (int32 [requests] on the GPU, or host numbers; 0 ends a
         request) and free the pages behind that."""
-        dkv_hip.page_trim(self._pages, self._counts(keep))
+        dkv_hip.page_trim(self._pages, self._counts(keep, "trim"))
 
     def check(self) -> None:
         """Wait for the GPU and raise if the last ``assign`` or ``trim`` was refused."""

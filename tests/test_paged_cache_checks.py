@@ -223,3 +223,15 @@ def test_slots_past_the_table_are_refused():
     for start, stop in ((0, 49), (-1, 5), (5, 4), (48, 64)):
         with pytest.raises(ValueError, match="slots"):
             c.slots(0, start, stop)
+
+
+def test_trim_refuses_counts_of_another_device(monkeypatch):
+    """The tables' GPU is the one to launch on; counts that lie elsewhere would be launched on theirs."""
+    launched = []
+    monkeypatch.setattr(dkv_hip, "page_trim", lambda pages, keep: launched.append(keep))
+    c = host_cache(_pages=None)
+    with pytest.raises(ValueError, match="trim: tensors must be on"):
+        c.trim(torch.zeros(2, dtype=torch.int32, device="meta"))
+    assert not launched
+    c.trim([1, 0])
+    assert launched[0].tolist() == [1, 0] and launched[0].dtype == torch.int32
