@@ -650,6 +650,19 @@ def fp4_load(cache: Fp4Cache, slots, key, value) -> None:
                                   stream_handle()), "dkv_fp4_load")
 
 
+def _query_meets(query, args, out) -> bool:
+    """Whether a contiguous ``out`` shares memory with the query rows that ``args`` names, other than in their place."""
+    rows, heads, dim = query.shape
+    size, at, to = query.element_size(), args.query, out.data_ptr()
+    if at == to and query.is_contiguous():
+        return False
+    token, head, end = args.query_token * size, args.query_head * size, to + out.numel() * size
+    if at >= end or at + (rows - 1) * token + (heads - 1) * head + dim * size <= to:
+        return False
+    start = at + (torch.arange(rows).unsqueeze(1) * token + torch.arange(heads) * head)
+    return bool(((start < end) & (start + dim * size > to)).any())
+
+
 def fp4_attend(args: Fp4AttendArgs, query, cu, out=None) -> torch.Tensor:
     """Attention of query [rows, q_heads, head_dim] (f32, f16 or bf16) over the pages of ``args`` (its cache, table and
     lengths, requests, width, scaling, window, longest and most set): out of the same shape and type, whose rows behind
@@ -671,6 +684,8 @@ def fp4_attend(args: Fp4AttendArgs, query, cu, out=None) -> torch.Tensor:
     if rows == 0:
         return out
     query, args.query, args.query_token, args.query_head = _strided_rows(query)
+    if not args.fill and _query_meets(query, args, out):
+        raise ValueError("fp4_attend: out lies over queries of other rows (it may be the query)")
     args.cu, args.out, args.rows, args.q_heads = cu.data_ptr(), out.data_ptr(), rows, q_heads
     where, library = ctypes.addressof(args), lib()
     need = library.dkv_fp4_attend_workspace_bytes(where)
@@ -681,6 +696,20 @@ def fp4_attend(args: Fp4AttendArgs, query, cu, out=None) -> torch.Tensor:
         _check(library.dkv_fp4_attend(where, workspace.data_ptr() if need > 16 else None, need, stream_handle()),
                "dkv_fp4_attend")
     return out
+
+
+def _rows_meet(a: int, a_row: int, b: int, b_row: int, rows: int, width: int) -> bool:
+    """Whether rows of ``width`` bytes from address ``b`` on, ``b_row`` apart, share memory with those from ``a`` on other
+    than row for row in place.  Each side's rows lie in order and apart."""
+    if (a == b and a_row == b_row) or a + (rows - 1) * a_row + width <= b or b + (rows - 1) * b_row + width <= a:
+        return False
+    start = b + torch.arange(rows) * b_row
+    below = torch.div(start - a, a_row, rounding_mode="floor")
+    for row in (below, below + 1):  # the rows of a that begin next to start
+        at = a + row.clamp(0, rows - 1) * a_row
+        if ((start < at + width) & (at < start + width)).any():
+            return True
+    return False
 
 
 def adjust_logits(args: LogitsArgs, logits, tokens=None, lengths=None, reply=None, out=None):
@@ -709,7 +738,10 @@ def adjust_logits(args: LogitsArgs, logits, tokens=None, lengths=None, reply=Non
             _expect("adjust_logits", logits.device, (out, "out", dtype, (rows, vocab)))
         if one != 1 or (rows > 1 and out_row < vocab):
             raise ValueError("adjust_logits: out needs rows of unit stride that do not overlap")
-        args.out_row = max(out_row, vocab)
+        args.out_row = max(out_row, vocab) if rows > 1 else args.logits_row
+        size = out.element_size()
+        if _rows_meet(args.logits, args.logits_row * size, out.data_ptr(), args.out_row * size, rows, vocab * size):
+            raise ValueError("adjust_logits: out lies over other logits than its own (it may be the logits)")
     args.out = out.data_ptr()
     args.tokens = args.lengths = args.reply = None
     if tokens is not None:

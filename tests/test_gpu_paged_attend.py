@@ -367,3 +367,15 @@ def test_scores_of_minus_infinity(heads, total, new, window, dtype):
     assert torch.equal(got, clean)
     cache.table.fill_(-1)  # no page holds a token: nothing is seen
     assert not cache.attend_rows(0, query, step, window=window).any()
+
+
+def test_results_over_other_queries_are_refused():
+    cache, step = build([50, 9], [2, 3], 2, 64, 16)
+    room = torch.randn(8, 6, 64, device=DEV)
+    given = room.clone()
+    want = cache.attend_rows(0, given[:5], step)
+    for out in (room[1:6], room.view(-1)[64:64 + 5 * 384].view(5, 6, 64)):
+        with pytest.raises(ValueError, match="other rows"):
+            cache.attend_rows(0, room[:5], step, out=out)
+    assert torch.equal(room, given)
+    assert torch.equal(cache.attend_rows(0, room[:5], step, out=room[:5]), want)

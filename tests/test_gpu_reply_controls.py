@@ -300,3 +300,19 @@ def test_bias_lists_are_fixed():
     values.mul_(2.0)
     out = controls.apply(logits)[0]
     assert torch.equal(out[0, 7], logits[0, 7] + 2.0) and torch.equal(out[1, 50], logits[1, 50] + 16.0)
+
+
+def test_results_over_other_logits_are_refused():
+    """A result may lie in its logits' place, or between their rows, but not over others'."""
+    from reply_controls import ReplyControls
+
+    wide = torch.randn(5, 700, device=DEV)
+    controls, given = ReplyControls(4, 300, repetition=2.0), wide.clone()
+    history = torch.arange(40, device=DEV).expand(4, 40)
+    want, _ = controls.apply(given[:4, :300], history)
+    for out in (wide[1:, :300], wide[:4, 1:301], wide.view(-1)[:1200].view(4, 300), wide[:4, 299:599]):
+        with pytest.raises(ValueError, match="other logits"):
+            controls.apply(wide[:4, :300], history, out=out)
+    assert torch.equal(wide, given)
+    for out in (wide[:4, 300:600], wide[1:, 301:601], wide[:4, :300]):
+        assert torch.equal(controls.apply(wide[:4, :300], history, out=out)[0], want)

@@ -235,3 +235,23 @@ def test_trim_refuses_counts_of_another_device(monkeypatch):
     assert not launched
     c.trim([1, 0])
     assert launched[0].tolist() == [1, 0] and launched[0].dtype == torch.int32
+
+
+def test_queries_under_the_result():
+    """Whether a result lies over queries other than in their place."""
+    size, heads, dim = 4, 2, 64
+
+    def meets(query, out):
+        a = dkv_hip.Fp4AttendArgs()
+        a.query, a.query_token, a.query_head = query.data_ptr(), query.stride(0), query.stride(1)
+        return dkv_hip._query_meets(query, a, out)
+
+    room = torch.zeros(12 * heads * dim)
+    rows = lambda first, n=4: room[first * heads * dim:(first + n) * heads * dim].view(n, heads, dim)
+    assert not meets(rows(2), rows(2)) and not meets(rows(0), rows(4)) and not meets(rows(4), rows(0))
+    assert meets(rows(2), rows(3)) and meets(rows(3), rows(2))
+    apart = room[:8 * heads * dim].view(4, 2, heads, dim)[:, 0]  # every second row
+    assert meets(apart, rows(0)) and meets(apart, rows(5)) and not meets(apart, rows(7))
+    assert not meets(apart[:2], rows(3, 2)) and not meets(apart[:2, :1], room[dim:dim * 3].view(2, 1, dim))
+    swapped = rows(0).view(heads, 4, dim).transpose(0, 1)  # heads before rows at the same address
+    assert meets(swapped, rows(0))

@@ -136,3 +136,21 @@ def test_stretches_count_their_own_tokens(count, line, tokens):
             seen = np.zeros(vocab, np.int32)
             assert count(vocab, line, tokens, shift, seen.ctypes.data) == 0, (vocab, shift)
             assert (seen == 1).all(), (vocab, shift)
+
+
+def test_rows_that_meet():
+    """Shared memory of two sets of rows, other than row for row in place, against a count of every byte."""
+    rng = np.random.RandomState(0)
+    met = 0
+    for _ in range(3000):
+        rows, width = int(rng.randint(1, 5)), int(rng.randint(1, 6))
+        a_row, b_row = (int(width + rng.randint(0, 8)) for _ in range(2))
+        a, b = 100, int(100 + rng.randint(-30, 31))
+        if rng.rand() < 0.3:
+            b_row = a_row
+        owner = {a + r * a_row + x: (r, x) for r in range(rows) for x in range(width)}
+        same = a == b and a_row == b_row
+        want = not same and any(b + r * b_row + x in owner for r in range(rows) for x in range(width))
+        assert dkv_hip._rows_meet(a, a_row, b, b_row, rows, width) == want
+        met += want
+    assert 500 < met < 2500
