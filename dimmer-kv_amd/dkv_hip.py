@@ -650,6 +650,26 @@ def fp4_load(cache: Fp4Cache, slots, key, value) -> None:
                                   stream_handle()), "dkv_fp4_load")
 
 
+class _Forward(torch.autograd.Function):
+    """A result of a recorded call of an operator without a backward pass: it requires a gradient as any result does, and
+    asking for it raises."""
+
+    @staticmethod
+    def forward(ctx, what, out, given):
+        ctx.what = what
+        ctx.mark_dirty(out)
+        return out
+
+    @staticmethod
+    def backward(ctx, grad):
+        raise RuntimeError(f"{ctx.what} has no backward pass")
+
+
+def _recorded(what: str, out, given):
+    """``out``, tied to ``given`` where autograd records."""
+    return _Forward.apply(what, out, given) if given.requires_grad and torch.is_grad_enabled() else out
+
+
 def _query_meets(query, args, out) -> bool:
     """Whether a contiguous ``out`` shares memory with the query rows that ``args`` names, other than in their place."""
     rows, heads, dim = query.shape
@@ -666,7 +686,8 @@ def _query_meets(query, args, out) -> bool:
 def fp4_attend(args: Fp4AttendArgs, query, cu, out=None) -> torch.Tensor:
     """Attention of query [rows, q_heads, head_dim] (f32, f16 or bf16) over the pages of ``args`` (its cache, table and
     lengths, requests, width, scaling, window, longest and most set): out of the same shape and type, whose rows behind
-    cu[requests] are left as they are; a new one, with zeros there, if it is None."""
+    cu[requests] are left as they are; a new one, with zeros there, if it is None.  There is no backward pass: a recorded
+    call's gradient raises."""
     index, dtype, shape = cu.get_device(), query.dtype, query.shape
     rows, q_heads, dim = shape
     args.query_dtype = dtype_code(dtype)
@@ -683,6 +704,7 @@ def fp4_attend(args: Fp4AttendArgs, query, cu, out=None) -> torch.Tensor:
         raise ValueError("fp4_attend: out must be contiguous and 16-byte aligned")
     if rows == 0:
         return out
+    given = query
     query, args.query, args.query_token, args.query_head = _strided_rows(query)
     if not args.fill and _query_meets(query, args, out):
         raise ValueError("fp4_attend: out lies over queries of other rows (it may be the query)")
@@ -695,7 +717,7 @@ def fp4_attend(args: Fp4AttendArgs, query, cu, out=None) -> torch.Tensor:
         workspace = torch.empty(need, dtype=torch.uint8, device=query.device) if need > 16 else None
         _check(library.dkv_fp4_attend(where, workspace.data_ptr() if need > 16 else None, need, stream_handle()),
                "dkv_fp4_attend")
-    return out
+    return _recorded("fp4_attend", out, given)
 
 
 def _rows_meet(a: int, a_row: int, b: int, b_row: int, rows: int, width: int) -> bool:
@@ -715,12 +737,13 @@ def _rows_meet(a: int, a_row: int, b: int, b_row: int, rows: int, width: int) ->
 def adjust_logits(args: LogitsArgs, logits, tokens=None, lengths=None, reply=None, out=None):
     """logits [rows, vocab] (f32, f16 or bf16) under the controls of ``args`` (its penalties, biases and masks set) ->
     (out of the same shape and type, pick int64 [rows]).  ``tokens`` [rows, history] int32 or int64 with lengths and
-    reply int32 [rows]; ``out`` may be the logits."""
+    reply int32 [rows]; ``out`` may be the logits.  There is no backward pass: a recorded call's gradient raises."""
     index, dtype, rows, vocab = logits.get_device(), logits.dtype, args.rows, args.vocab
     args.dtype = dtype_code(dtype)
     if index < 0 or logits.shape != (rows, vocab):
         _expect("adjust_logits", logits.device, (logits, "logits", dtype, (rows, vocab)))
         raise ValueError("dimmer-kv HIP kernels need GPU tensors (no CPU path)")
+    given = logits
     row, one = logits.stride()
     if one != 1 or (rows > 1 and row < vocab):
         if out is logits:
@@ -771,4 +794,4 @@ def adjust_logits(args: LogitsArgs, logits, tokens=None, lengths=None, reply=Non
     with _on_gpu(index):
         workspace = torch.empty(need, dtype=torch.uint8, device=logits.device)
         _check(library.dkv_adjust_logits(where, workspace.data_ptr(), need, stream_handle()), "dkv_adjust_logits")
-    return out, pick
+    return _recorded("adjust_logits", out, given), pick

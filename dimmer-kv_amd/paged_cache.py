@@ -170,8 +170,9 @@ class PagedCache:
                     window: int | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
         """Attention of the step's queries [rows, q_heads, head_dim] (float32, float16 or bfloat16, any strides) over
         the pages of ``layer``, where the step's own keys and values lie already: causal, and over the last ``window``
-        tokens of each query's if given.  ``out`` (same shape and type, contiguous; it may be the query) keeps
-        its rows behind the last request; without it they are zeros."""
+        tokens of each query's if given.  ``out`` (same shape and type, contiguous; it may be the query, but not lie over
+        other rows of it) keeps its rows behind the last request; without it they are zeros.  No backward pass: asking a
+        recorded call for its gradient raises."""
         if not 0 <= layer < self.layers:
             raise ValueError(f"layer {layer} of {self.layers}")
         if query.dim() != 3 or query.shape[1] % self.kv_heads or query.shape[0] != step.rows:

@@ -157,8 +157,9 @@ class ReplyControls:
               reply_start: torch.Tensor | None = None, out: torch.Tensor | None = None):
         """(adjusted logits, pick) of logits [rows, vocab] (float32, float16 or bfloat16).  Row r's history is the first
         ``lengths[r]`` of ``tokens`` [rows, history] (int64 or int32; all of them by default), its reply begins at
-        ``reply_start[r]`` (0 by default).  ``out`` may be ``logits``.  pick int64 [rows] is the largest logit's token,
-        the lowest of equals, -1 where no token is allowed."""
+        ``reply_start[r]`` (0 by default).  ``out`` may be ``logits``, but not lie over other rows of them.  pick int64
+        [rows] is the largest logit's token, the lowest of equals, -1 where no token is allowed.  No backward pass: asking
+        a recorded call for its gradient raises."""
         if logits.device != self.device:
             raise ValueError(f"ReplyControls: logits must be on {self.device} (got {logits.device})")
         if tokens is not None and lengths is None:

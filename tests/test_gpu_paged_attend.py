@@ -379,3 +379,21 @@ def test_results_over_other_queries_are_refused():
             cache.attend_rows(0, room[:5], step, out=out)
     assert torch.equal(room, given)
     assert torch.equal(cache.attend_rows(0, room[:5], step, out=room[:5]), want)
+
+
+@pytest.mark.parametrize("given", ["nothing", "a result", "the query's place"])
+def test_recorded_calls_have_no_gradient(given):
+    """Attention has no backward pass: a recorded call's result is the plain one, requires a gradient and refuses it."""
+    cache, step = build([50, 9], [2, 3], 2, 64, 16)
+    query = torch.randn(5, 6, 64, device=DEV)
+    want = cache.attend_rows(0, query, step)
+    assert not want.requires_grad
+    leaf = query.clone().requires_grad_()
+    rows = leaf * 1.0
+    out = {"nothing": None, "a result": torch.empty_like(query), "the query's place": rows}[given]
+    got = cache.attend_rows(0, rows, step, out=out)
+    assert got.requires_grad and torch.equal(got, want) and (out is None or got is out)
+    with pytest.raises(RuntimeError, match="no backward pass"):
+        got.sum().backward()
+    with torch.no_grad():
+        assert not cache.attend_rows(0, leaf, step).requires_grad

@@ -316,3 +316,20 @@ def test_results_over_other_logits_are_refused():
     assert torch.equal(wide, given)
     for out in (wide[:4, 300:600], wide[1:, 301:601], wide[:4, :300]):
         assert torch.equal(controls.apply(wide[:4, :300], history, out=out)[0], want)
+
+
+@pytest.mark.parametrize("given", ["nothing", "a result", "the logits' place"])
+def test_recorded_calls_have_no_gradient(given):
+    from reply_controls import ReplyControls
+
+    logits = torch.randn(3, 400, device=DEV)
+    controls = ReplyControls(3, 400, bias={5: 1.0})
+    want, best = controls.apply(logits)
+    assert not want.requires_grad
+    rows = logits.clone().requires_grad_() * 1.0
+    out = {"nothing": None, "a result": torch.empty_like(logits), "the logits' place": rows}[given]
+    got, pick = controls.apply(rows, out=out)
+    assert got.requires_grad and torch.equal(got, want) and torch.equal(pick, best) and (out is None or got is out)
+    with pytest.raises(RuntimeError, match="no backward pass"):
+        got.sum().backward()
+    assert not controls.apply(rows.detach())[0].requires_grad
