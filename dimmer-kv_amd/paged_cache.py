@@ -41,6 +41,7 @@ class Step:
 
 
 ARRIVAL_SETS = 256
+ARRIVAL_WORDS = 256  # of a set: a launch that joins its splits has fewer than 512 workgroups, two of them at least a word
 REFUSED = {1: "more new tokens than rows", 2: "a request passes its row of the block table", 3: "too few free pages"}
 
 
@@ -80,17 +81,16 @@ class PagedCache:
         self._layers = [dkv_hip.Fp4Cache(self.key_codes[i].data_ptr(), self.key_scales[i].data_ptr(),
                                          self.value_codes[i].data_ptr(), self.value_scales[i].data_ptr(), pages,
                                          kv_heads, page, head_dim) for i in range(layers)]
-        # Words that the workgroups of one attention call count themselves on (zero between calls): calls take turns over
-        # several sets, so that ones captured in graphs or queued on other streams do not meet on one.
-        self._set = max(1024, 2 * requests * kv_heads)
-        self._arrivals = torch.zeros(ARRIVAL_SETS, self._set, dtype=torch.int32, device=device)
-        self._turns = itertools.cycle(range(self._arrivals.data_ptr(), self._arrivals.data_ptr() + ARRIVAL_SETS * self._set * 4,
-                                            self._set * 4))
+        # Words that the workgroups of one attention call count themselves on (zero between calls).  Calls take turns over
+        # the sets, which come round again: calls on one cache are ordered, and the turns keep none apart for good.
+        self._arrivals = torch.zeros(ARRIVAL_SETS, ARRIVAL_WORDS, dtype=torch.int32, device=device)
+        start, step = self._arrivals.data_ptr(), ARRIVAL_WORDS * 4
+        self._turns = itertools.cycle(range(start, start + ARRIVAL_SETS * step, step))
         self._attend = []
         for cache in self._layers:
             a = dkv_hip.Fp4AttendArgs()
             a.cache, a.table, a.lengths = cache, self.table.data_ptr(), self.lengths.data_ptr()
-            a.requests, a.width, a.arrivals_count = requests, table_pages, self._set
+            a.requests, a.width, a.arrivals_count = requests, table_pages, ARRIVAL_WORDS
             self._attend.append(a)
 
     # ----- tables -----

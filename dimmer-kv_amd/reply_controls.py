@@ -51,7 +51,8 @@ class ReplyControls:
         self.device = torch.empty(0, device=device).device
         self._args = dkv_hip.LogitsArgs()
         self._args.rows, self._args.vocab = rows, vocab
-        # words that a call's workgroups count themselves on (zero between calls); calls take turns over several sets
+        # words that a call's workgroups count themselves on (zero between calls); calls take turns over the sets, which
+        # come round again: calls on one object are ordered
         self._arrivals = torch.zeros(ARRIVAL_SETS, max(rows, 1), dtype=torch.int32, device=device)
         start, step = self._arrivals.data_ptr(), self._arrivals.stride(0) * 4
         self._turns = itertools.cycle(range(start, start + ARRIVAL_SETS * step, step))

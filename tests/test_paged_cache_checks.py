@@ -255,3 +255,36 @@ def test_queries_under_the_result():
     assert not meets(apart[:2], rows(3, 2)) and not meets(apart[:2, :1], room[dim:dim * 3].view(2, 1, dim))
     swapped = rows(0).view(heads, 4, dim).transpose(0, 1)  # heads before rows at the same address
     assert meets(swapped, rows(0))
+
+
+def test_arrival_words_suffice():
+    """More words than a cache has make no other launch: its splits, as the workspace tells, are the same with 2^20."""
+    from paged_cache import ARRIVAL_WORDS
+
+    need = dkv_hip.lib().dkv_fp4_attend_workspace_bytes
+    splits = set()
+    for dim in (64, 128, 256):
+        for dtype in (0, 1, 2):
+            for requests, heads, groups in ((1, 1, 1), (1, 8, 4), (16, 8, 3), (32, 8, 1), (60, 4, 2), (300, 1, 7), (8192, 8, 1)):
+                for longest in (100, 1500, 6000, 40000, 1 << 20):
+                    for most in (1, 3, 9):
+                        sizes = [need(ctypes.addressof(attend_args(
+                            cache=cache(head_dim=dim, kv_heads=heads), requests=requests, q_heads=heads * groups, longest=longest,
+                            width=1 << 17, most=most, rows=requests * most, query_dtype=dtype, arrivals=P, arrivals_count=count)))
+                            for count in (ARRIVAL_WORDS, 1 << 20)]
+                        assert sizes[0] == sizes[1] >= 16
+                        splits.add((sizes[0] - 16) // (requests * most * heads * groups * (dim + 2) * 4))
+    assert len(splits) > 10
+
+
+def test_arrival_words_held(monkeypatch):
+    """The words of a cache do not grow with its requests (they took 134 MB at 8,192 requests of 8 KV heads)."""
+    import paged_cache
+
+    for name in ("zeros", "full", "arange"):  # what a cache allocates, on no device
+        make = getattr(torch, name)
+        monkeypatch.setattr(torch, name, lambda *a, make=make, **k: make(*a, **(k | {"device": "meta"})))
+    c = paged_cache.PagedCache(1, 8, 64, 16, requests=8192, table_pages=4, device="cuda")
+    assert c._arrivals.numel() * 4 <= 1 << 18
+    assert c.held_bytes() == sum(t.numel() * t.element_size() for t in (
+        c.key_codes, c.key_scales, c.value_codes, c.value_scales, c.table, c.lengths, c.free, c.free_count, c._state, c._arrivals))
