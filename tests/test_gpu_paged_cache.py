@@ -278,3 +278,49 @@ def test_past_32_bits():
     want = torch.einsum("ht,thd->hd", weights, torch.cat([value, value[:1]]).double())
     # float32: the weights' error, some 2^-17 (256 products of order 1, 4,101 sums), on values below 8
     assert (out[0].double() - want).abs().max() < 8 * 2.0 ** -17
+
+
+def page_bytes(cache, arrays, slots, key, value):
+    """The cache's four arrays of one layer as include/dimmerkv.h lays them out, after rows went into ``slots``."""
+    heads, dim, page = cache.kv_heads, cache.head_dim, cache.page
+    key_codes, key_scales, value_codes, value_scales = (a.cpu().numpy().reshape(-1).copy() for a in arrays)
+    lane_dims, lane_bytes = dim // 16, dim // 32
+    (kc, ks, _), (vc, vs, _) = paged_ref.quantize(key), paged_ref.quantize(value)
+    for row, slot in enumerate(slots):
+        if slot < 0:
+            continue
+        p, t = divmod(slot, page)
+        for h in range(heads):
+            hp = p * heads + h
+            for i in range(dim // 2):  # dimension 2i low, 2i + 1 high
+                key_codes[(hp * page + t) * (dim // 2) + i] = kc[row, h, 2 * i] | kc[row, h, 2 * i + 1] << 4
+                lane, within = divmod(2 * i, lane_dims)
+                value_codes[hp * page * (dim // 2) + t // 4 * (2 * dim) + (lane * 4 + t % 4) * lane_bytes + within // 2] = \
+                    vc[row, h, 2 * i] | vc[row, h, 2 * i + 1] << 4
+            for block in range(dim // 32):
+                key_scales[(hp * page + t) * (dim // 32) + block] = ks[row, h, block]
+                value_scales[hp * page * (dim // 32) + t // 4 * (dim // 8) + block * 4 + t % 4] = vs[row, h, block]
+    return key_codes, key_scales, value_codes, value_scales
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("heads,dim,page", [(2, 64, 16), (3, 128, 32), (1, 256, 16), (2, 256, 64)])
+def test_stored_bytes(heads, dim, page, dtype):
+    """Codes, their signs (of zeros too) and exponents byte by byte where the published form has them, in pages that held
+    other bytes, and not a byte outside the slots."""
+    print(f"[case] bytes heads={heads} dim={dim} page={page} {dtype}", flush=True)
+    n = 43
+    cache, _ = make(2, 5, 9, page, layers=2, heads=heads, dim=dim)
+    cache.free.copy_(torch.tensor([4, 7, 0, 8, 2, 6, 1, 3, 5], dtype=torch.int32))
+    step = cache.assign([23, n - 23 - 2], rows=n)
+    key, value = (torch.tensor(special_rows(n, heads, dim, seed), device=DEV).to(TYPES[dtype]) for seed in (3, 4))
+    key[5, 0, 3], value[30, heads - 1, dim - 1] = float("nan"), -float("inf")
+    g = torch.Generator(DEV).manual_seed(dim)
+    every = (cache.key_codes, cache.key_scales, cache.value_codes, cache.value_scales)
+    for a in every:
+        a.copy_(torch.randint(1, 256, a.shape, generator=g, device=DEV))
+    other = [a[0].clone() for a in every]
+    want = page_bytes(cache, [a[1] for a in every], step.slots.tolist(), key.double().cpu().numpy(), value.double().cpu().numpy())
+    cache.store(1, key, value, step)
+    for a, b, expected in zip(every, other, want):
+        assert torch.equal(a[0], b) and np.array_equal(a[1].cpu().numpy().reshape(-1), expected)
