@@ -109,7 +109,7 @@ class PagedCache:
         if not torch.is_tensor(new):
             new = [int(n) for n in new]
             rows = sum(max(n, 0) for n in new) if rows is None else rows
-            most = max(0, *new) if most is None else most
+            most = max([0, *new]) if most is None else most
         if rows is None:
             raise ValueError("assign: a GPU tensor of new tokens needs rows, the step's number of rows")
         if not 0 <= rows < (1 << 31) - (1 << 16):

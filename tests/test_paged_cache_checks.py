@@ -288,3 +288,14 @@ def test_arrival_words_held(monkeypatch):
     assert c._arrivals.numel() * 4 <= 1 << 18
     assert c.held_bytes() == sum(t.numel() * t.element_size() for t in (
         c.key_codes, c.key_scales, c.value_codes, c.value_scales, c.table, c.lengths, c.free, c.free_count, c._state, c._arrivals))
+
+
+def test_counts_of_other_requests_are_refused():
+    import paged_cache
+
+    c = host_cache(_pages=pages(requests=2))
+    for new in ([], [1], [1, 2, 3]):
+        with pytest.raises(ValueError):
+            paged_cache.PagedCache.assign(c, new)
+        with pytest.raises(ValueError):
+            c.trim(new)
