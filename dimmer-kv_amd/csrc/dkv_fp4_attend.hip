@@ -19,7 +19,6 @@
 // against a copy's 5.1: the memory bounds it.  2,048 query tokens of 24 heads over 16K tokens (387 GFLOP) 400-430 us, 0.93
 // PFLOP/s; a large library product makes 1.17.  There the vector units bound it (conversions, exponentials and the issue
 // slots that matrix instructions take from them), at two waves a SIMD.
-#include <float.h>
 #include <math.h>
 
 #include "dkv_device.h"
@@ -89,6 +88,19 @@ struct Operand<float> : Operand<dkv_bf16> {
   static constexpr int kPieces = 3;
 };
 
+// A row with an infinite query value has no finite score (that value's products are infinite, or NaN with a key of 0), so no
+// finite result where it sees a token.  Infinities become NaN, and the row's scores with them: those of -infinity alone
+// would pass for tokens that the row does not see.
+DKV_DEVICE void quiet(half8 (&q)[1]) { q[0] = __builtin_elementwise_fma(q[0], (half8)(half_t)0.0f, q[0]); }  // x + 0 * x
+DKV_DEVICE void quiet(bf16x8 (&q)[1]) {  // the bit below an exponent of all ones set
+  uint32_t w[4];
+  __builtin_memcpy(w, &q[0], 16);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] |= (((w[i] & 0x7f807f80u) + 0x00800080u) & 0x80008000u) >> 9;
+  __builtin_memcpy(&q[0], w, 16);
+}
+DKV_DEVICE void quiet(bf16x8 (&)[3]) {}  // (where they are cut into pieces)
+
 // 8 query values into kPieces operands.
 DKV_DEVICE uint4 signed_words(const void* p, uint32_t sign) {
   const uint4 w = *(const uint4*)p;
@@ -115,8 +127,8 @@ DKV_DEVICE void query_pieces(const float* p, bool negate, bf16x8 (&out)[3]) {
     const float left = x - __uint_as_float(a);
     const uint32_t b = __float_as_uint(left) & 0xffff0000u;
     const uint32_t c = __float_as_uint(left - __uint_as_float(b));
-    const bool finite = (a & 0x7f800000u) != 0x7f800000u;  // an infinity or NaN is one piece
-    words[0][i >> 1] |= (a >> 16 | (finite || !(__float_as_uint(x) & 0x7fffffu) ? 0u : 0x40u)) << (16 * (i & 1));
+    const bool finite = (a & 0x7f800000u) != 0x7f800000u;  // an infinity or NaN is one piece, a NaN
+    words[0][i >> 1] |= (a >> 16 | (finite ? 0u : 0x40u)) << (16 * (i & 1));
     words[1][i >> 1] |= (finite ? b >> 16 : 0u) << (16 * (i & 1));
     words[2][i >> 1] |= (finite ? c >> 16 : 0u) << (16 * (i & 1));
   }
@@ -234,10 +246,8 @@ DKV_DEVICE void load_values(const AttendArgs& a, const Tiles<CH>& tiles, const L
   }
 }
 
-// (waves a SIMD: one row tile of 64 dimensions is small enough for three, 32 float32 requests of 8K tokens 44.7 us and 50.2
-// with two)
 template <int D, typename T, int NT, int CH, int kWaves>
-__global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : NT == 1 && D == 64 ? 3 : 2) void fp4_attend_kernel(AttendArgs a) {
+__global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_attend_kernel(AttendArgs a) {
   using Op = Operand<T>;
   using frag = typename Op::frag;
   constexpr int kRows = 16 * NT, kSteps = D / 32, kLane = D / 16, kPieces = Op::kPieces;
@@ -301,6 +311,7 @@ __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : NT == 1 && D =
 #pragma unroll
           for (int s = 0; s < kSteps; ++s) {
             query_pieces(p + g * (D / 4) + s * 8, a.negate, q[0][0]);
+            quiet(q[0][0]);
             held[(nt * kSteps + s) * 64 + lane] = q[0][0][0];
           }
         }
@@ -337,6 +348,12 @@ __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : NT == 1 && D =
     load_keys<D, CH>(a, tiles, at, keys);
     load_values<D, CH>(a, tiles, at, values);
     entries = load_entries<CH>(a, table, chunk + kWaves < c1 ? len : 0, chunk + kWaves);
+    if constexpr (!kLean) {  // (here, so that the first chunk's loads do not wait for the queries')
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) quiet(q[nt][s]);
+    }
     for (; chunk < c1; chunk += kWaves) {
       const int later = load_entries<CH>(a, table, chunk + 2 * kWaves < c1 ? len : 0, chunk + 2 * kWaves);
       find_tiles<CH>(a, entries, chunk + kWaves < c1 ? len : 0, h, chunk + kWaves, next_tiles);
@@ -514,25 +531,12 @@ __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : NT == 1 && D =
       }
     }
 
-    // whether a row sees a token of this wave's chunks (the tokens are the same in every lane)
-    auto sees_some = [&](int nt) {
-      const int last = last_seen(nt), before = before_first(last);
-      bool some = false;
-      for (int c = __builtin_amdgcn_readfirstlane(c0 + wave); c < c1; c += kWaves)
-        for (int token = c * CH * 16; token < min((c + 1) * CH * 16, len); token += 16)
-          if ((uint32_t)as_scalar(table)[token >> a.shift] < (uint32_t)a.c.pages) some = some || (token <= last && token + 15 > before);
-      return some;
-    };
-
     // the waves' sums, 16 rows at a time and four waves at a time
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const float total = sum_xor32(sum_xor16(l[nt]));
-      // A row whose scores are all NaN has no maximum, but is not one that sees nothing.  Nor is one whose scores are all
-      // -infinity (an infinite query): it goes below every row of scores, with a sum of 0, so that it is 0 / 0 if no token
-      // has more.
+      // a row whose scores are all NaN has no maximum, but is not one that sees nothing
       if (m[nt] == -INFINITY && total != 0.0f) m[nt] = 0.0f;
-      if (__any(m[nt] == -INFINITY)) m[nt] = m[nt] == -INFINITY && sees_some(nt) ? -FLT_MAX : m[nt];
       if (g == 0) {
         stat[0][wave][nt * 16 + i] = m[nt];
         stat[1][wave][nt * 16 + i] = total;
@@ -589,9 +593,9 @@ __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : NT == 1 && D =
         const long out_row = (long)(q0 + token) * q_heads + h * a.groups + (r - token * a.groups);
         if (splits == 1) {
           T* out = (T*)a.out + out_row * D + part * kPart;
-          const float inverse = 1.0f / total;
+          const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
 #pragma unroll
-          for (int j = 0; j < kPart; ++j) set_result(out[j], highest == -INFINITY ? 0.0f : acc[j] * inverse);
+          for (int j = 0; j < kPart; ++j) set_result(out[j], total == 0.0f ? 0.0f : acc[j] * inverse);
         } else {
           const long at = out_row * splits + split;
           float* out = a.part + at * D + part * kPart;
@@ -677,7 +681,7 @@ __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : NT == 1 && D =
             }
             T* out = (T*)a.out + out_row * D + dim;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) set_result(out[j], highest == -INFINITY ? 0.0f : v[j] / whole);
+            for (int j = 0; j < 4; ++j) set_result(out[j], whole == 0.0f ? 0.0f : v[j] / whole);
           }
           __syncthreads();
         }
@@ -693,7 +697,7 @@ __global__ __launch_bounds__(256) void fp4_join_kernel(AttendArgs a, int q_heads
   constexpr int kSet = D / 4, kSets = 256 / kSet;
   __shared__ float weight[kMaxSplits];
   __shared__ float4 sums[kSets][kSet];
-  __shared__ float whole;  // below 0: the row sees nothing
+  __shared__ float whole;
   const long row = blockIdx.x;
   if (row >= (long)min(max(a.cu[a.requests], 0), a.rows) * q_heads) return;
   const float2* ml = a.part_ml + row * a.splits;
@@ -715,7 +719,7 @@ __global__ __launch_bounds__(256) void fp4_join_kernel(AttendArgs a, int q_heads
       total += factor < 0.0f ? 0.0f : x[k].y * factor;
     }
     total = wave_sum(total);
-    if (threadIdx.x == 0) whole = top == -INFINITY ? -1.0f : total;
+    if (threadIdx.x == 0) whole = total;
   }
   __syncthreads();
   const int at = threadIdx.x % kSet, set = threadIdx.x / kSet;
@@ -739,7 +743,7 @@ __global__ __launch_bounds__(256) void fp4_join_kernel(AttendArgs a, int q_heads
   T* out = (T*)a.out + row * D + at * 4;
   const float v[4] = {acc.x, acc.y, acc.z, acc.w};
 #pragma unroll
-  for (int j = 0; j < 4; ++j) set_result(out[j], whole < 0.0f ? 0.0f : v[j] / whole);
+  for (int j = 0; j < 4; ++j) set_result(out[j], whole == 0.0f ? 0.0f : v[j] / whole);
 }
 
 // The same for few splits: a set of D / 4 threads per row.  49,152 rows of two splits: 13 us, 40 with a workgroup for
@@ -766,7 +770,7 @@ __global__ __launch_bounds__(256) void fp4_join_few_kernel(AttendArgs a, int q_h
   T* out = (T*)a.out + row * D + at * 4;
   const float v[4] = {acc.x, acc.y, acc.z, acc.w};
 #pragma unroll
-  for (int j = 0; j < 4; ++j) set_result(out[j], top == -INFINITY ? 0.0f : v[j] / whole);
+  for (int j = 0; j < 4; ++j) set_result(out[j], whole == 0.0f ? 0.0f : v[j] / whole);
 }
 
 struct Plan {
