@@ -501,7 +501,7 @@ def greedy_answer(model, tokenizer, context: CompressedContext | None, cache, in
     masks instead of the plain argmax: the penalties' history is ``history`` (the context's token ids, if wanted), the
     question and the reply, and the reply's own tokens are the ones counted.  ``grammar`` (with controls) is called with
     the reply's tokens before each choice and returns a bool [vocabulary] mask of the tokens that may follow, or None
-    for all; the reply ends where it allows none."""
+    for all, in place of the controls' own masks; the reply ends where it allows none."""
     import dimmer
 
     if grammar is not None and controls is None:

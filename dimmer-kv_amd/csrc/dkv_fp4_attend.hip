@@ -15,10 +15,11 @@
 // times 2^8 so that weights down to 2^-22 of the row's reference keep that (smaller ones are off by 2^-33 of it): an eighth
 // of a bfloat16 result's own rounding, but as much as a float16 one's.  So float16 results take a second piece of the
 // weights, and so do float32 results, held times 2^15.  Sums, maxima and accumulators are float32.
-// Measured: one token over 2K-32K tokens of 32 requests (8 KV heads of 128 dimensions, 617 MB of pages) 130 us, 4.7 TB/s
-// against a copy's 5.1: the memory bounds it.  2,048 query tokens of 24 heads over 16K tokens (387 GFLOP) 400-430 us, 0.93
-// PFLOP/s; a large library product makes 1.17.  There the vector units bound it (conversions, exponentials and the issue
-// slots that matrix instructions take from them), at two waves a SIMD.
+// Measured: one token over 2K-32K tokens of 32 requests (8 KV heads of 128 dimensions, 617 MB of pages) 134 us a call, 4.6
+// TB/s against a copy's 5.1: the memory bounds it.  2,048 query tokens of 24 heads over 16K tokens (387 GFLOP) 414 us a call
+// with its join, 0.93 PFLOP/s; a large library product makes 1.17.  There the issue of vector instructions bounds it
+// (conversions, exponentials and the matrix instructions' own slots: 63 % of the SIMDs' cycles, the matrix cores 41 %), at
+// two waves a SIMD.
 #include <math.h>
 
 #include "dkv_device.h"

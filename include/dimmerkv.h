@@ -507,10 +507,10 @@ int dkv_fp4_load(const dkv_fp4_cache_t* c, const int64_t* slots, int32_t n, void
  * the last `window` of them.  out = softmax(scaling * q k^T) v per row and head,
  * query head x reading KV head x / (q_heads / kv_heads); a row that sees nothing
  * is 0; one with an infinite query value that sees some is NaN, as the formula has
- * it; a token a row does not see has no part in it, whatever its values.  Scores are float32,
- * for magnitudes below 2^26 (above, neighbours differ by 8 and more).  Rows
- * behind cu[requests] are left as they are, or zeroed with `fill`.  Entries of the
- * table that are no page count as tokens not seen. */
+ * it; a token a row does not see has no part in it, whatever its values.  Scores
+ * are float32, for magnitudes below 2^26 (above, neighbours differ by 8 and more).
+ * Rows behind cu[requests] are left as they are, or zeroed with `fill`.  Entries of
+ * the table that are no page count as tokens not seen. */
 typedef struct dkv_fp4_attend_args {
   dkv_fp4_cache_t cache;
   const int32_t* table;    /* [requests][width] */
