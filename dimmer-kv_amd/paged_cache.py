@@ -96,6 +96,9 @@ class PagedCache:
     # ----- tables -----
     def _counts(self, counts, what: str) -> torch.Tensor:
         if not torch.is_tensor(counts):
+            if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+                raise ValueError(f"{what}: host numbers in a captured step, whose replays would read memory given back; it "
+                                 "needs an int32 tensor on the GPU")
             return dkv_hip.to_device(list(counts), torch.int32, self.device)
         self._here(counts, what)
         return counts
@@ -121,8 +124,8 @@ class PagedCache:
         return step
 
     def trim(self, keep) -> None:
-        """Cut every request back to at most ``keep`` tokens (int32 [requests] on the GPU, or host numbers; 0 ends a
-        request) and free the pages behind that."""
+        """Cut every request back to at most ``keep`` tokens (int32 [requests] on the GPU, as a captured step needs, or host
+        numbers; 0 ends a request) and free the pages behind that."""
         dkv_hip.page_trim(self._pages, self._counts(keep, "trim"))
 
     def check(self) -> None:

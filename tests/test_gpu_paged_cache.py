@@ -324,3 +324,25 @@ def test_stored_bytes(heads, dim, page, dtype):
     cache.store(1, key, value, step)
     for a, b, expected in zip(every, other, want):
         assert torch.equal(a[0], b) and np.array_equal(a[1].cpu().numpy().reshape(-1), expected)
+
+
+def test_captured_steps_take_counts_on_the_gpu():
+    """Host numbers are refused while a step is captured; the capture goes on, and its replays are right."""
+    cache, ref = make(2, 6, 16, 16)
+    new, keep = int32([3, 2]), int32([1, 99])
+    cache.assign([20, 1]), ref.assign([20, 1], 21)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for call in (lambda: cache.assign([3, 2]), lambda: cache.trim([1, 99])):
+            with pytest.raises(ValueError, match="captured"):
+                call()
+        step = cache.assign(new, 5)
+        cache.trim(keep)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        check_step(step, ref.assign([3, 2], 5))
+        ref.trim([1, 99])
+        check_tables(cache, ref)
+        cache.assign([1, 0]), ref.assign([1, 0], 1)
+    cache.check()

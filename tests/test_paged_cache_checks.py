@@ -299,3 +299,18 @@ def test_counts_of_other_requests_are_refused():
             paged_cache.PagedCache.assign(c, new)
         with pytest.raises(ValueError):
             c.trim(new)
+
+
+def test_host_numbers_in_a_captured_step_are_refused(monkeypatch):
+    """A graph would hold the copy from host memory that is given back after the call."""
+    copies = []
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    monkeypatch.setattr(dkv_hip, "to_device", lambda *a: copies.append(a))
+    monkeypatch.setattr(dkv_hip, "page_trim", lambda *a: None)
+    c = host_cache(device=torch.device("cuda", 0), _pages=None)
+    with pytest.raises(ValueError, match="captured"):
+        c.trim([1, 0])
+    assert not copies
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    c.trim([1, 0])
+    assert len(copies) == 1
