@@ -666,7 +666,7 @@ class _Forward(torch.autograd.Function):
 
 
 def _recorded(what: str, out, given):
-    """``out``, tied to ``given`` where autograd records."""
+    """``out``, tied to ``given`` where autograd records: before it is written, as autograd refuses some places (a leaf's)."""
     return _Forward.apply(what, out, given) if given.requires_grad and torch.is_grad_enabled() else out
 
 
@@ -713,11 +713,12 @@ def fp4_attend(args: Fp4AttendArgs, query, cu, out=None) -> torch.Tensor:
     need = library.dkv_fp4_attend_workspace_bytes(where)
     if need == 0:
         _check(-2, "dkv_fp4_attend_workspace_bytes")
+    out = _recorded("fp4_attend", out, given)
     with _on_gpu(index):
         workspace = torch.empty(need, dtype=torch.uint8, device=query.device) if need > 16 else None
         _check(library.dkv_fp4_attend(where, workspace.data_ptr() if need > 16 else None, need, stream_handle()),
                "dkv_fp4_attend")
-    return _recorded("fp4_attend", out, given)
+    return out
 
 
 def _rows_meet(a: int, a_row: int, b: int, b_row: int, rows: int, width: int) -> bool:
@@ -791,7 +792,8 @@ def adjust_logits(args: LogitsArgs, logits, tokens=None, lengths=None, reply=Non
     if rows == 0:
         return out, pick
     args.pick = pick.data_ptr()
+    out = _recorded("adjust_logits", out, given)
     with _on_gpu(index):
         workspace = torch.empty(need, dtype=torch.uint8, device=logits.device)
         _check(library.dkv_adjust_logits(where, workspace.data_ptr(), need, stream_handle()), "dkv_adjust_logits")
-    return _recorded("adjust_logits", out, given), pick
+    return out, pick

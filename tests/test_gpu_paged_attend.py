@@ -397,3 +397,14 @@ def test_recorded_calls_have_no_gradient(given):
         got.sum().backward()
     with torch.no_grad():
         assert not cache.attend_rows(0, leaf, step).requires_grad
+
+
+def test_a_recorded_leaf_is_not_written():
+    """What autograd does not let change in place stays as it is."""
+    cache, step = build([50, 9], [2, 3], 2, 64, 16)
+    leaf = torch.randn(5, 6, 64, device=DEV).requires_grad_()
+    given = leaf.detach().clone()
+    for place in (leaf, leaf[:]):
+        with pytest.raises(RuntimeError, match="leaf"):
+            cache.attend_rows(0, leaf, step, out=place)
+    assert torch.equal(leaf, given)

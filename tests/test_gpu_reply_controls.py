@@ -333,3 +333,14 @@ def test_recorded_calls_have_no_gradient(given):
     with pytest.raises(RuntimeError, match="no backward pass"):
         got.sum().backward()
     assert not controls.apply(rows.detach())[0].requires_grad
+
+
+def test_a_recorded_leaf_is_not_written():
+    from reply_controls import ReplyControls
+
+    leaf = torch.randn(3, 400, device=DEV).requires_grad_()
+    given = leaf.detach().clone()
+    for place in (leaf, leaf[:]):
+        with pytest.raises(RuntimeError, match="leaf"):
+            ReplyControls(3, 400, bias={5: 1.0}).apply(leaf, out=place)
+    assert torch.equal(leaf, given)
