@@ -885,6 +885,125 @@ void launch_type(const AttendArgs& a, const Plan& plan, int q_heads, int dtype, 
   else launch<D, dkv_bf16>(a, plan, q_heads, st);
 }
 
+// ---------------------------------------------------------------------------
+// Shaped scores: a cap, a bias that falls with the distance, sinks, ranges of tokens.  A wave per query row: a lane scores
+// a token of 64, then the lanes are the row's dimensions and take the tokens' values in turn.
+// ---------------------------------------------------------------------------
+struct ShapedArgs {
+  AttendArgs a;
+  dkv_fp4_shape_t s;
+  float scaling;
+};
+
+template <int D, typename T>
+__global__ __launch_bounds__(256) void fp4_shaped_kernel(ShapedArgs p) {
+  const AttendArgs& a = p.a;
+  constexpr int kDims = D / 64;
+  __shared__ float query[4][D], weights[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int q_heads = a.c.kv_heads * a.groups;
+  const long row = (long)blockIdx.x * 4 + wave;
+  if (row >= (long)a.rows * q_heads) return;
+  const int t = (int)(row / q_heads), x = (int)(row % q_heads), h = x / a.groups;
+  T* out = (T*)a.out + row * D + lane * kDims;
+  const int end = min(max(a.cu[a.requests], 0), a.rows);
+  if (t >= end) {
+    if (a.fill) __builtin_memset(out, 0, kDims * sizeof(T));
+    return;
+  }
+  int b = 0, above = a.requests;  // the last request whose rows begin at t or before
+  while (above - b > 1) {
+    const int mid = (b + above) >> 1;
+    if (a.cu[mid] <= t) b = mid; else above = mid;
+  }
+  const int q0 = min(max(a.cu[b], 0), a.rows), q1 = min(max(a.cu[b + 1], q0), a.rows);
+  const int len = min(max(a.lengths[b], 0), a.width << a.shift);
+  const long at = (long)len - (q1 - q0) + (t - q0);
+  const long low = max(max(p.s.first ? (long)p.s.first[t] : 0L, at - a.window + 1), 0L);
+  const long high = min(p.s.last ? (long)p.s.last[t] : at, (long)len - 1);
+  const T* q = (const T*)a.query + t * a.query_token + x * a.query_head + lane * kDims;
+#pragma unroll
+  for (int j = 0; j < kDims; ++j) query[wave][lane * kDims + j] = load_as_float(q, j, sizeof(T) == 4 ? DKV_F32 : __is_same(T, half_t) ? DKV_F16 : DKV_BF16);
+  const float slope = p.s.slopes ? p.s.slopes[x] : 0.0f;
+  const int page = a.c.page;
+  float m = -INFINITY, l = 0.0f, acc[kDims] = {};
+  for (long base = low & ~63L; base <= high; base += 64) {
+    const long token = base + lane;
+    bool sees = token >= low && token <= high;
+    const int id = sees ? a.table[(long)b * a.width + (token >> a.shift)] : -1;
+    sees = sees && (uint32_t)id < (uint32_t)a.c.pages;
+    float z = -INFINITY;
+    if (sees) {
+      const long line = ((long)id * a.c.kv_heads + h) * page + (token & (page - 1));
+      z = 0.0f;
+      for (int block = 0; block < D / 32; ++block) {
+        const float e = exponent(a.c.key_scales[line * (D / 32) + block]);
+        const uint4 w = *(const uint4*)(a.c.key_codes + line * (D / 2) + block * 16);
+        const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float* qq = query[wave] + block * 32 + i * 8;
+          const floatx2 k0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(words[i], e, 0), k1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(words[i], e, 1);
+          const floatx2 k2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(words[i], e, 2), k3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(words[i], e, 3);
+          z += k0[0] * qq[0] + k0[1] * qq[1] + k1[0] * qq[2] + k1[1] * qq[3] + k2[0] * qq[4] + k2[1] * qq[5] + k3[0] * qq[6] + k3[1] * qq[7];
+        }
+      }
+      z *= p.scaling;
+      if (p.s.cap > 0.0f) z = p.s.cap * tanhf(z / p.s.cap);
+      z -= slope * fabsf((float)(token - at));
+    }
+    const uint64_t seen = __ballot(sees);
+    const float top = wave_max(z), higher = fmaxf(m, top);
+    const float factor = higher == -INFINITY ? 1.0f : expf(m - higher);
+    m = higher;
+    const float w = sees ? expf(z - m) : 0.0f;
+    l = l * factor + wave_sum(w);
+    weights[wave][lane] = w;
+#pragma unroll
+    for (int j = 0; j < kDims; ++j) acc[j] *= factor;
+    for (uint64_t left = seen; left; left &= left - 1) {
+      const int i = __builtin_ctzll(left);
+      const int other = __shfl(id, i);
+      const long in_page = (base + i) & (page - 1), head_page = (long)other * a.c.kv_heads + h;
+      const float weight = weights[wave][i];
+#pragma unroll
+      for (int j = 0; j < kDims; ++j) {
+        const int d = lane * kDims + j, byte = d / 2;
+        constexpr int kLane = D / 32;
+        const uint32_t code = a.c.value_codes[head_page * page * (D / 2) + (in_page >> 2) * (2 * D) + byte / kLane * (4 * kLane) +
+                                              (in_page & 3) * kLane + byte % kLane];
+        const float e = exponent(a.c.value_scales[head_page * page * (D / 32) + (in_page >> 2) * (D / 8) + d / 32 * 4 + (in_page & 3)]);
+        const floatx2 v = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, e, 0);
+        acc[j] = fmaf(weight, d & 1 ? v[1] : v[0], acc[j]);
+      }
+    }
+  }
+  float whole = l, scale = 1.0f;
+  if (p.s.sinks && whole != 0.0f) {
+    const float sink = p.s.sinks[x], higher = fmaxf(m, sink);
+    scale = expf(m - higher);
+    whole = whole * scale + expf(sink - higher);
+  }
+#pragma unroll
+  for (int j = 0; j < kDims; ++j) set_result(out[j], whole == 0.0f ? 0.0f : acc[j] * scale / whole);
+}
+
+template <int D>
+void launch_shaped(const ShapedArgs& p, int q_heads, int dtype, hipStream_t st) {
+  const dim3 grid((unsigned)(((long)p.a.rows * q_heads + 3) / 4)), block(256);
+  if (dtype == DKV_F32) hipLaunchKernelGGL((fp4_shaped_kernel<D, float>), grid, block, 0, st, p);
+  else if (dtype == DKV_F16) hipLaunchKernelGGL((fp4_shaped_kernel<D, half_t>), grid, block, 0, st, p);
+  else hipLaunchKernelGGL((fp4_shaped_kernel<D, dkv_bf16>), grid, block, 0, st, p);
+}
+
+int check_shape(const dkv_fp4_shape_t* s, const char* what) {
+  DKV_REQUIRE(s, DKV_EINVAL, "%s: null shape", what);
+  DKV_REQUIRE(s->cap >= 0.0f && s->cap < INFINITY, DKV_EINVAL, "%s: cap %g", what, s->cap);
+  DKV_REQUIRE((((uintptr_t)s->slopes | (uintptr_t)s->sinks) & 3) == 0 && (((uintptr_t)s->first | (uintptr_t)s->last) & 7) == 0, DKV_EINVAL,
+              "%s: misaligned slopes, sinks, first or last", what);
+  return DKV_OK;
+}
+
 }  // namespace
 
 extern "C" size_t dkv_fp4_attend_workspace_bytes(const dkv_fp4_attend_args_t* p) {
@@ -925,4 +1044,38 @@ extern "C" int dkv_fp4_attend(const dkv_fp4_attend_args_t* p, void* workspace, s
   else if (a.c.head_dim == 128) launch_type<128>(a, plan, p->q_heads, p->query_dtype, st);
   else launch_type<256>(a, plan, p->q_heads, p->query_dtype, st);
   return dkv::check_launch("dkv_fp4_attend");
+}
+
+extern "C" size_t dkv_fp4_attend_shaped_workspace_bytes(const dkv_fp4_attend_args_t* p, const dkv_fp4_shape_t* shape) {
+  const char* what = "dkv_fp4_attend_shaped_workspace_bytes";
+  if (check_attend(p, what) || check_shape(shape, what)) return 0;
+  return 16;
+}
+
+extern "C" int dkv_fp4_attend_shaped(const dkv_fp4_attend_args_t* p, const dkv_fp4_shape_t* shape, void* workspace,
+                                     size_t workspace_bytes, void* stream) {
+  const char* what = "dkv_fp4_attend_shaped";
+  int rc = check_attend(p, what);
+  if (!rc) rc = check_shape(shape, what);
+  if (rc) return rc;
+  if (p->rows == 0) return DKV_OK;
+  DKV_REQUIRE(p->table && p->lengths && p->cu && p->query && p->out, DKV_EINVAL, "%s: null pointer", what);
+  const int unit = p->query_dtype == DKV_F32 ? 4 : 8;
+  DKV_REQUIRE((((uintptr_t)p->query | (uintptr_t)p->out) & 15) == 0 && p->query_token % unit == 0 && p->query_head % unit == 0,
+              DKV_EINVAL, "%s: query rows and out must be 16-byte aligned", what);
+  ShapedArgs s{};
+  s.s = *shape; s.scaling = p->scaling;
+  AttendArgs& a = s.a;
+  a.c = p->cache;
+  a.table = p->table; a.lengths = p->lengths; a.cu = p->cu; a.query = p->query; a.out = p->out;
+  a.query_token = p->query_token; a.query_head = p->query_head;
+  a.requests = p->requests; a.width = p->width; a.shift = dkv::page_shift(p->cache.page); a.rows = p->rows;
+  a.groups = p->q_heads / p->cache.kv_heads;
+  a.window = p->window ? p->window : INT32_MAX;
+  a.fill = p->fill;
+  hipStream_t st = dkv::as_stream(stream);
+  if (a.c.head_dim == 64) launch_shaped<64>(s, p->q_heads, p->query_dtype, st);
+  else if (a.c.head_dim == 128) launch_shaped<128>(s, p->q_heads, p->query_dtype, st);
+  else launch_shaped<256>(s, p->q_heads, p->query_dtype, st);
+  return dkv::check_launch(what);
 }

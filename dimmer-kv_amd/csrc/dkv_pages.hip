@@ -281,6 +281,148 @@ __global__ __launch_bounds__(256) void fp4_store_kernel(StoreArgs a) {
   if ((o & 3) == 0) (value ? a.c.value_scales : a.c.key_scales)[scale_at<D>(value, head_page, at, o >> 2, page)] = (uint8_t)e;
 }
 
+// ---------------------------------------------------------------------------
+// Raw projections into the pages: keys rotated on the way, and the queries rotated beside them.  A lane takes the octet
+// of a row that the store's lane takes, and reads the octet its dimensions are paired with beside it.  A rotated key next
+// to the border of two codes must fall on the right side, and float32 products do not tell: the products are made in
+// float64, where they are exact and their sum is rounded once at 2^-53, and the sum is cut to float32 towards an odd last
+// bit, which keeps it on its side of every border that the codes, the exponents and the queries' types have.
+// ---------------------------------------------------------------------------
+struct AppendArgs {
+  dkv_fp4_cache_t c;
+  const void* rows[3];        // queries, keys, values
+  void* out;
+  int64_t token[3], head[3];  // strides in elements
+  int64_t out_token, out_head;
+  const int64_t* slots;
+  const int64_t* positions;
+  const float* cos;
+  const float* sin;
+  int64_t cos_row, sin_row;
+  int n, shift, q_heads, rotary, table_rows, fill;
+};
+
+// d cut to float32, its last bit set where that loses something: rounding the result once more to fewer bits, to either
+// side of a border of fewer bits, is rounding d.
+DKV_DEVICE float cut_to_odd(double d) {
+  const float f = (float)d;
+  const double back = (double)f;
+  if (!(back != d) || d != d) return f;
+  return __uint_as_float((__float_as_uint(f) - (fabs(back) > fabs(d) ? 1u : 0u)) | 1u);
+}
+
+template <typename T>
+DKV_DEVICE void store_rotated(T* p, const double (&x)[8]) {
+  if constexpr (__is_same(T, float)) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      ((float4*)p)[i] = make_float4((float)x[4 * i], (float)x[4 * i + 1], (float)x[4 * i + 2], (float)x[4 * i + 3]);
+  } else if constexpr (__is_same(T, half_t)) {
+    half8 h;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) h[i] = (half_t)cut_to_odd(x[i]);
+    *(half8*)p = h;
+  } else {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      w[i] = (uint32_t)float_to_bf16_bits(cut_to_odd(x[2 * i])) | (uint32_t)float_to_bf16_bits(cut_to_odd(x[2 * i + 1])) << 16;
+    *(uint4*)p = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+// A row's octet into its slot; e and the codes from the block's four lanes.
+template <int D>
+DKV_DEVICE void store_octet(const dkv_fp4_cache_t& c, int shift, bool value, long slot, int h, int o, const float (&x)[8]) {
+  uint32_t amax = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) amax = max(amax, __float_as_uint(x[i]) & 0x7fffffffu);
+  const uint32_t e = block_exponent(max_quad(amax));
+  uint32_t codes = 0;
+  if (e != DKV_FP4_NAN) {
+    const float scale = __uint_as_float(e << 23);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[0], x[1], scale, 0);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[2], x[3], scale, 1);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[4], x[5], scale, 2);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[6], x[7], scale, 3);
+  }
+  const int page = c.page, at = (int)(slot & (page - 1));
+  const long head_page = (slot >> shift) * c.kv_heads + h;
+  uint8_t* code = (value ? c.value_codes : c.key_codes) + code_at<D>(value, head_page, at, o, page);
+  if (D == 64 && value) {  // a lane's 4 dimensions are 2 bytes: an octet is two lanes, four tokens' bytes apart
+    *(uint16_t*)code = (uint16_t)codes;
+    *(uint16_t*)(code + 8) = (uint16_t)(codes >> 16);
+  } else {
+    *(uint32_t*)code = codes;
+  }
+  if ((o & 3) == 0) (value ? c.value_scales : c.key_scales)[scale_at<D>(value, head_page, at, o >> 2, page)] = (uint8_t)e;
+}
+
+template <int D, typename T, bool PAIRS>
+__global__ __launch_bounds__(256) void fp4_append_kernel(AppendArgs a) {
+  constexpr int kOct = D / 8, kTok = 256 / kOct;
+  const int o = threadIdx.x % kOct, t = blockIdx.x * kTok + threadIdx.x / kOct;
+  if (t >= a.n) return;
+  const int y = blockIdx.y, kind = y < a.q_heads ? 0 : y < a.q_heads + a.c.kv_heads ? 1 : 2;
+  const int h = kind == 0 ? y : kind == 1 ? y - a.q_heads : y - a.q_heads - a.c.kv_heads;
+  const T* row = (const T*)a.rows[kind] + t * a.token[kind] + h * a.head[kind];
+  const long slot = a.slots[t], position = a.positions[t];
+  const bool kept = slot >= 0 && slot < (long)a.c.pages << a.shift;  // the same for a row's lanes
+  float x[8];
+  if (kind == 2) {
+    if (!kept) return;
+    load8<T>(row + o * 8, x);
+    store_octet<D>(a.c, a.shift, true, slot, h, o, x);
+    return;
+  }
+  if (kind == 1 && !kept) return;
+  T* out = (T*)a.out + t * a.out_token + h * a.out_head + o * 8;
+  if (kind == 0 && position < 0) {
+    if (a.fill) __builtin_memset(out, 0, 8 * sizeof(T));
+    return;
+  }
+  load8<T>(row + o * 8, x);
+  const int half = a.rotary / 2, first = o * 8;
+  double r[8];
+  if (position < 0 || position >= a.table_rows) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = __builtin_nan("");
+  } else if (first >= a.rotary) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = x[i];
+  } else if constexpr (PAIRS) {
+    const float4 c = *(const float4*)(a.cos + position * a.cos_row + o * 4);
+    const float4 s = *(const float4*)(a.sin + position * a.sin_row + o * 4);
+    const double cs[4] = {c.x, c.y, c.z, c.w}, sn[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      r[2 * i] = x[2 * i] * cs[i] - x[2 * i + 1] * sn[i];
+      r[2 * i + 1] = x[2 * i + 1] * cs[i] + x[2 * i] * sn[i];
+    }
+  } else {
+    const bool low = first < half;
+    const int pair = low ? first : first - half;
+    float other[8], c[8], s[8];
+    load8<T>(row + (low ? first + half : pair), other);
+    load8<float>(a.cos + position * a.cos_row + pair, c);
+    load8<float>(a.sin + position * a.sin_row + pair, s);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = (double)x[i] * c[i] + (double)other[i] * (low ? -s[i] : s[i]);
+  }
+  if (kind == 0) {
+    store_rotated<T>((T*)out, r);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = cut_to_odd(r[i]);
+    store_octet<D>(a.c, a.shift, false, slot, h, o, x);
+  }
+}
+
+template <int D, typename T>
+constexpr auto append_halves = fp4_append_kernel<D, T, false>;
+template <int D, typename T>
+constexpr auto append_pairs = fp4_append_kernel<D, T, true>;
+
 struct LoadArgs {
   dkv_fp4_cache_t c;
   void* rows[2];  // [n][kv_heads][D]
@@ -425,4 +567,44 @@ extern "C" int dkv_fp4_load(const dkv_fp4_cache_t* c, const int64_t* slots, int3
   DKV_FP4_BY_SHAPE(fp4_load_kernel, c->head_dim, dtype, dim3((n + tok - 1) / tok, c->kv_heads, 2), dim3(256), 0,
                    dkv::as_stream(stream), a);
   return dkv::check_launch("dkv_fp4_load");
+}
+
+extern "C" int dkv_fp4_append(const dkv_fp4_append_args_t* p, void* stream) {
+  const char* what = "dkv_fp4_append";
+  DKV_REQUIRE(p, DKV_EINVAL, "%s: null arguments", what);
+  const int rc = check_rows(&p->cache, p->key, p->value, p->dtype, p->slots, p->rows, what);
+  if (rc) return rc;
+  const int dim = p->cache.head_dim;
+  DKV_REQUIRE(p->rotary >= 16 && p->rotary <= dim && p->rotary % 16 == 0, DKV_ESHAPE,
+              "%s: %d rotated dimensions of %d (a multiple of 16)", what, p->rotary, dim);
+  DKV_REQUIRE(p->table_rows > 0, DKV_ESHAPE, "%s: tables of %d rows", what, p->table_rows);
+  DKV_REQUIRE(p->q_heads >= 0 && (p->query != nullptr || p->q_heads == 0), DKV_EINVAL, "%s: %d heads of null queries", what, p->q_heads);
+  DKV_REQUIRE((int64_t)p->q_heads + 2 * p->cache.kv_heads <= 65535, DKV_ESHAPE, "%s: %d query heads and %d KV heads", what,
+              p->q_heads, p->cache.kv_heads);
+  if (p->rows == 0) return DKV_OK;
+  DKV_REQUIRE(p->positions && p->cos && p->sin && (p->q_heads == 0 || p->out), DKV_EINVAL, "%s: null pointer", what);
+  DKV_REQUIRE((((uintptr_t)p->query | (uintptr_t)p->out | (uintptr_t)p->cos | (uintptr_t)p->sin) & 15) == 0, DKV_EINVAL,
+              "%s: rows and tables must be 16-byte aligned", what);
+  const int unit = p->dtype == DKV_F32 ? 4 : 8;
+  DKV_REQUIRE(p->key_token % unit == 0 && p->key_head % unit == 0 && p->value_token % unit == 0 && p->value_head % unit == 0 &&
+                  p->cos_row % 4 == 0 && p->sin_row % 4 == 0,
+              DKV_EINVAL, "%s: row strides must be multiples of 16 bytes", what);
+  DKV_REQUIRE(p->q_heads == 0 || (p->query_token % unit == 0 && p->query_head % unit == 0 && p->out_token % unit == 0 &&
+                                  p->out_head % unit == 0),
+              DKV_EINVAL, "%s: row strides must be multiples of 16 bytes", what);
+  AppendArgs a{};
+  a.c = p->cache;
+  a.rows[0] = p->query; a.rows[1] = p->key; a.rows[2] = p->value; a.out = p->out;
+  a.token[0] = p->query_token; a.token[1] = p->key_token; a.token[2] = p->value_token;
+  a.head[0] = p->query_head; a.head[1] = p->key_head; a.head[2] = p->value_head;
+  a.out_token = p->out_token; a.out_head = p->out_head;
+  a.slots = p->slots; a.positions = p->positions;
+  a.cos = p->cos; a.sin = p->sin; a.cos_row = p->cos_row; a.sin_row = p->sin_row;
+  a.n = p->rows; a.shift = dkv::page_shift(p->cache.page);
+  a.q_heads = p->q_heads; a.rotary = p->rotary; a.table_rows = p->table_rows; a.fill = p->fill;
+  const int tok = 256 / (dim / 8);
+  const dim3 grid((p->rows + tok - 1) / tok, p->q_heads + 2 * p->cache.kv_heads), block(256);
+  if (p->interleaved) DKV_FP4_BY_SHAPE(append_pairs, dim, p->dtype, grid, block, 0, dkv::as_stream(stream), a);
+  else DKV_FP4_BY_SHAPE(append_halves, dim, p->dtype, grid, block, 0, dkv::as_stream(stream), a);
+  return dkv::check_launch(what);
 }

@@ -32,8 +32,9 @@ EXPORTS = [
     "dkv_gather_cold", "dkv_refine_rows", "dkv_wire_pack", "dkv_wire_unpack", "dkv_attend_layer_noalloc",
     "dkv_quantize8", "dkv_quantize8_rungs", "dkv_centered_rows", "dkv_matmul_f32_workspace_bytes", "dkv_matmul_f32",
     "dkv_ladder_errors", "dkv_ladder_code", "dkv_rows_to_caches", "dkv_copy_tokens", "dkv_outside_tokens", "dkv_project_caches", "dkv_live_groups",
-    "dkv_page_assign", "dkv_page_trim", "dkv_fp4_store", "dkv_fp4_load",
-    "dkv_fp4_attend_workspace_bytes", "dkv_fp4_attend", "dkv_adjust_logits_workspace_bytes", "dkv_adjust_logits",
+    "dkv_page_assign", "dkv_page_trim", "dkv_fp4_store", "dkv_fp4_load", "dkv_fp4_append",
+    "dkv_fp4_attend_workspace_bytes", "dkv_fp4_attend", "dkv_fp4_attend_shaped_workspace_bytes", "dkv_fp4_attend_shaped",
+    "dkv_adjust_logits_workspace_bytes", "dkv_adjust_logits",
 ]
 NOALLOC_MAX_BYTES = 64 << 20  # DKV_NOALLOC_MAX_BYTES: the static workspace of dkv_attend_layer_noalloc
 
@@ -96,6 +97,21 @@ class Fp4AttendArgs(ctypes.Structure):
                 ("scaling", c_f32), ("fill", c_i32), ("arrivals", c_vp), ("arrivals_count", c_i32)]
 
 
+class Fp4Shape(ctypes.Structure):
+    """dkv_fp4_shape_t."""
+    _fields_ = [("slopes", c_vp), ("sinks", c_vp), ("first", c_vp), ("last", c_vp), ("cap", c_f32)]
+
+
+class Fp4AppendArgs(ctypes.Structure):
+    """dkv_fp4_append_args_t."""
+    _fields_ = [("cache", Fp4Cache)]
+    _fields_ += [(name, c_vp) for name in ("query", "key", "value", "out")]
+    _fields_ += [(f"{name}_{stride}", c_i64) for name in ("query", "key", "value", "out") for stride in ("token", "head")]
+    _fields_ += [(name, c_vp) for name in ("slots", "positions", "cos", "sin")]
+    _fields_ += [("cos_row", c_i64), ("sin_row", c_i64)]
+    _fields_ += [(name, c_i32) for name in ("table_rows", "rotary", "interleaved", "dtype", "rows", "q_heads", "fill")]
+
+
 class LogitsArgs(ctypes.Structure):
     """dkv_logits_args_t."""
     _fields_ = [(name, c_vp) for name in ("logits", "out", "tokens", "lengths", "reply", "repetition", "presence", "frequency",
@@ -124,7 +140,7 @@ def lib() -> ctypes.CDLL:
         handle.dkv_last_error.restype = ctypes.c_char_p
         for name in ("dkv_attend_workspace_bytes", "dkv_score_workspace_bytes", "dkv_topk_workspace_bytes",
                      "dkv_matmul_f32_workspace_bytes", "dkv_fp4_attend_workspace_bytes",
-                     "dkv_adjust_logits_workspace_bytes"):
+                     "dkv_fp4_attend_shaped_workspace_bytes", "dkv_adjust_logits_workspace_bytes"):
             getattr(handle, name).restype = c_sz
         handle.dkv_topk_workspace_bytes.argtypes = [c_i32]
         handle.dkv_page_assign.argtypes = [c_vp, c_vp, c_i32, c_vp, c_vp, c_vp, c_vp]
@@ -132,6 +148,9 @@ def lib() -> ctypes.CDLL:
         handle.dkv_fp4_store.argtypes = [c_vp, c_vp, c_vp, c_i32, c_i64, c_i64, c_i64, c_i64, c_vp, c_i32, c_vp]
         handle.dkv_fp4_attend_workspace_bytes.argtypes = [c_vp]
         handle.dkv_fp4_attend.argtypes = [c_vp, c_vp, c_sz, c_vp]
+        handle.dkv_fp4_attend_shaped_workspace_bytes.argtypes = [c_vp, c_vp]
+        handle.dkv_fp4_attend_shaped.argtypes = [c_vp, c_vp, c_vp, c_sz, c_vp]
+        handle.dkv_fp4_append.argtypes = [c_vp, c_vp]
         handle.dkv_adjust_logits_workspace_bytes.argtypes = [c_vp]
         handle.dkv_adjust_logits.argtypes = [c_vp, c_vp, c_sz, c_vp]
         handle.dkv_fp4_load.argtypes = [c_vp, c_vp, c_i32, c_vp, c_vp, c_i32, c_vp]
@@ -665,9 +684,14 @@ class _Forward(torch.autograd.Function):
         raise RuntimeError(f"{ctx.what} has no backward pass")
 
 
-def _recorded(what: str, out, given):
-    """``out``, tied to ``given`` where autograd records: before it is written, as autograd refuses some places (a leaf's)."""
-    return _Forward.apply(what, out, given) if given.requires_grad and torch.is_grad_enabled() else out
+def _recorded(what: str, out, *given):
+    """``out``, tied to what is ``given`` where autograd records: before it is written, as autograd refuses some places (a
+    leaf's)."""
+    if torch.is_grad_enabled():
+        for t in given:
+            if t is not None and t.requires_grad:
+                return _Forward.apply(what, out, t)
+    return out
 
 
 def _query_meets(query, args, out) -> bool:
@@ -683,10 +707,38 @@ def _query_meets(query, args, out) -> bool:
     return bool(((start < end) & (start + dim * size > to)).any())
 
 
-def fp4_attend(args: Fp4AttendArgs, query, cu, out=None) -> torch.Tensor:
+def _rows_meet_rows(a, b) -> bool:
+    """Whether rows ``a`` and ``b`` [n, heads, dim] (contiguous dimensions, one type) share memory."""
+    spans = []
+    for t in (a, b):
+        (rows, heads, dim), (row, head, _) = t.shape, t.stride()
+        spans.append((t.data_ptr(), row, head, (heads - 1) * head + dim, (rows - 1) * row))
+    size = a.element_size()
+    (a_at, a_row, _, a_span, a_long), (b_at, b_row, _, b_span, b_long) = spans
+    if a_at >= b_at + (b_long + b_span) * size or b_at >= a_at + (a_long + a_span) * size:
+        return False
+    if a_row == b_row and a_row > 0:  # columns of one matrix
+        ahead = (b_at - a_at) // size % a_row
+        if a_span <= ahead and ahead + b_span <= a_row:
+            return False
+    starts = [at + size * (torch.arange(t.shape[0]).unsqueeze(1) * row + torch.arange(t.shape[1]) * head).flatten()
+              for t, (at, row, head, _, _) in zip((a, b), spans)]
+    mine = starts[0].sort().values
+    width = a.shape[2] * size
+    near = torch.searchsorted(mine, starts[1])
+    for place in (near - 1, near):  # the rows of a that begin next to one of b
+        inside = (place >= 0) & (place < mine.numel())
+        other = mine[place.clamp(0, mine.numel() - 1)]
+        if (inside & (other < starts[1] + width) & (starts[1] < other + width)).any():
+            return True
+    return False
+
+
+def fp4_attend(args: Fp4AttendArgs, query, cu, out=None, shape_of=None) -> torch.Tensor:
     """Attention of query [rows, q_heads, head_dim] (f32, f16 or bf16) over the pages of ``args`` (its cache, table and
     lengths, requests, width, scaling, window, longest and most set): out of the same shape and type, whose rows behind
-    cu[requests] are left as they are; a new one, with zeros there, if it is None.  There is no backward pass: a recorded
+    cu[requests] are left as they are; a new one, with zeros there, if it is None.  ``shape_of``: (cap, slopes, sinks, first,
+    last) of shaped scores, each None where there is none (dkv_fp4_attend_shaped).  There is no backward pass: a recorded
     call's gradient raises."""
     index, dtype, shape = cu.get_device(), query.dtype, query.shape
     rows, q_heads, dim = shape
@@ -702,6 +754,7 @@ def fp4_attend(args: Fp4AttendArgs, query, cu, out=None) -> torch.Tensor:
     elif not _like(out, shape, dtype, index) or out.data_ptr() % 16:
         _expect("fp4_attend", cu.device, (out, "out", dtype, shape))
         raise ValueError("fp4_attend: out must be contiguous and 16-byte aligned")
+    shaped = None if shape_of is None else _fp4_shape(index, rows, q_heads, *shape_of)
     if rows == 0:
         return out
     given = query
@@ -710,15 +763,112 @@ def fp4_attend(args: Fp4AttendArgs, query, cu, out=None) -> torch.Tensor:
         raise ValueError("fp4_attend: out lies over queries of other rows (it may be the query)")
     args.cu, args.out, args.rows, args.q_heads = cu.data_ptr(), out.data_ptr(), rows, q_heads
     where, library = ctypes.addressof(args), lib()
-    need = library.dkv_fp4_attend_workspace_bytes(where)
+    if shaped is None:
+        need = library.dkv_fp4_attend_workspace_bytes(where)
+    else:
+        need = library.dkv_fp4_attend_shaped_workspace_bytes(where, ctypes.addressof(shaped))
     if need == 0:
         _check(-2, "dkv_fp4_attend_workspace_bytes")
-    out = _recorded("fp4_attend", out, given)
+    out = _recorded("fp4_attend", out, given) if shaped is None else _recorded("fp4_attend", out, given, *shape_of[1:3])
     with _on_gpu(index):
         workspace = torch.empty(need, dtype=torch.uint8, device=query.device) if need > 16 else None
-        _check(library.dkv_fp4_attend(where, workspace.data_ptr() if need > 16 else None, need, stream_handle()),
-               "dkv_fp4_attend")
+        at = workspace.data_ptr() if need > 16 else None
+        if shaped is None:
+            _check(library.dkv_fp4_attend(where, at, need, stream_handle()), "dkv_fp4_attend")
+        else:
+            _check(library.dkv_fp4_attend_shaped(where, ctypes.addressof(shaped), at, need, stream_handle()), "dkv_fp4_attend_shaped")
     return out
+
+
+def _fp4_shape(index: int, rows: int, q_heads: int, cap, slopes, sinks, first, last) -> Fp4Shape:
+    shape = Fp4Shape()
+    if cap is not None:
+        if not 0.0 < cap <= 3.0e38:
+            raise ValueError(f"fp4_attend: cap {cap} must be above 0 and finite")
+        shape.cap = cap
+    for name, t, dtype, count in (("slopes", slopes, torch.float32, q_heads), ("sinks", sinks, torch.float32, q_heads),
+                                  ("first", first, torch.int64, rows), ("last", last, torch.int64, rows)):
+        if t is None:
+            continue
+        if not _like(t, (count,), dtype, index):
+            raise ValueError(f"fp4_attend: {name} must be contiguous {dtype} [{count}] on the cache's GPU (got {t.dtype} "
+                             f"{list(t.shape)} on {t.device})")
+        if count:
+            setattr(shape, name, t.data_ptr())
+    return shape
+
+
+def fp4_append(cache: Fp4Cache, query, key, value, slots, positions, cos, sin, interleaved: bool = False, out=None):
+    """Rows key and value [n, kv_heads, head_dim] into slots int64 [n], the keys rotated to positions int64 [n] by the tables
+    cos and sin float32 [table rows, rotary / 2] -> query [n, q_heads, head_dim] rotated (None for None): into ``out``, the
+    query itself or contiguous memory apart from all rows, whose rows of negative positions are left as they are; a new
+    one, with zeros there, if it is None.  There is no backward pass: a recorded call's gradient raises."""
+    index, n, dtype = slots.get_device(), slots.shape[0], key.dtype
+    shape, code = (n, cache.kv_heads, cache.head_dim), dtype_code(dtype)
+    if not (index >= 0 and _like(slots, (n,), torch.int64, index) and _like(positions, (n,), torch.int64, index)
+            and key.shape == shape and value.shape == shape and value.dtype == dtype and key.get_device() == index
+            and value.get_device() == index):
+        _expect("fp4_append", slots.device, (slots, "slots", torch.int64, (n,)), (positions, "positions", torch.int64, (n,)),
+                (key, "key", dtype, shape), (value, "value", dtype, shape))
+        ptr(slots), ptr(positions)
+    for t, name in ((cos, "cos"), (sin, "sin")):
+        if (t.dtype != torch.float32 or t.dim() != 2 or t.shape != cos.shape or t.get_device() != index or t.stride(1) != 1
+                or t.stride(0) % 4 or t.data_ptr() % 16 or not 0 < t.shape[0] < 1 << 31):
+            raise ValueError(f"fp4_append: {name} must be float32 [positions, rotary / 2] on the cache's GPU, rows 16-byte "
+                             f"aligned (got {t.dtype} {list(t.shape)}, strides {list(t.stride())}, on {t.device})")
+    if 2 * cos.shape[1] > cache.head_dim or cos.shape[1] % 8 or cos.shape[1] == 0:
+        raise ValueError(f"fp4_append: {2 * cos.shape[1]} rotated dimensions of {cache.head_dim} (a multiple of 16)")
+    if n >= 1 << 31:
+        raise ValueError(f"fp4_append: {n} rows")
+    args = Fp4AppendArgs()
+    given = query
+    if query is None:
+        if out is not None:
+            raise ValueError("fp4_append: out without queries")
+    else:
+        wide = (n, query.shape[1] if query.dim() == 3 else -1, cache.head_dim)
+        if query.shape != wide or query.dtype != dtype or query.get_device() != index:
+            _expect("fp4_append", slots.device, (query, "query", dtype, wide))
+        args.fill = out is None
+        if out is None:
+            out = torch.empty(wide, dtype=dtype, device=query.device)
+        elif out.shape != wide or out.dtype != dtype or out.get_device() != index:
+            _expect("fp4_append", slots.device, (out, "out", dtype, wide))
+    if n == 0:
+        return out
+    key, args.key, args.key_token, args.key_head = _strided_rows(key)
+    value, args.value, args.value_token, args.value_head = _strided_rows(value)
+    if query is not None and query.shape[1]:
+        query, args.query, args.query_token, args.query_head = _strided_rows(query)
+        if not args.fill:
+            in_place = out.data_ptr() == args.query and out.stride() == query.stride()
+            if not in_place and (not out.is_contiguous() or out.data_ptr() % 16):
+                raise ValueError("fp4_append: out must be the query (rows 16-byte aligned), or contiguous and 16-byte aligned")
+            if (_rows_lie_over(out) or any(_rows_meet_rows(out, t) for t in (key, value))
+                    or (not in_place and _query_meets(query, args, out))):
+                raise ValueError("fp4_append: out lies over other rows of the queries, or over keys or values")
+        args.out, args.out_token, args.out_head = out.data_ptr(), out.stride(0), out.stride(1)
+        args.q_heads = query.shape[1]
+        out = _recorded("fp4_append", out, given, cos, sin)
+    args.cache, args.slots, args.positions = cache, slots.data_ptr(), positions.data_ptr()
+    args.cos, args.sin, args.cos_row, args.sin_row = cos.data_ptr(), sin.data_ptr(), cos.stride(0), sin.stride(0)
+    args.table_rows, args.rotary = cos.shape[0], 2 * cos.shape[1]
+    args.interleaved, args.dtype, args.rows = bool(interleaved), code, n
+    with _on_gpu(index):
+        _check(lib().dkv_fp4_append(ctypes.addressof(args), stream_handle()), "dkv_fp4_append")
+    return out
+
+
+def _rows_lie_over(t) -> bool:
+    """Whether rows of ``t`` [n, heads, dim] (contiguous dimensions) may share memory with each other: they do not where one
+    of the two strides steps over all that the other reaches."""
+    sizes = sorted((stride, count) for count, stride in zip(t.shape[:2], t.stride()[:2]) if count > 1)
+    reach = t.shape[2]
+    for stride, count in sizes:
+        if stride < reach:
+            return True
+        reach = (count - 1) * stride + reach
+    return False
 
 
 def _rows_meet(a: int, a_row: int, b: int, b_row: int, rows: int, width: int) -> bool:

@@ -159,6 +159,19 @@ class PagedCache:
         self._here(step.slots, "store")
         dkv_hip.fp4_store(self._layer(layer), key, value, step.slots)
 
+    def append(self, layer: int, query: torch.Tensor | None, key: torch.Tensor, value: torch.Tensor, step: Step,
+               cos: torch.Tensor, sin: torch.Tensor, interleaved: bool = False, out: torch.Tensor | None = None):
+        """``store`` for raw projections: the step's keys are rotated to their positions on the way into the pages of
+        ``layer``, and its queries [rows, q_heads, head_dim] with them (None: there are none), all of one type and any
+        strides -> the rotated queries.  ``cos`` and ``sin``: float32 [positions, n], n a multiple of 8; the first 2n
+        dimensions are rotated, i with i + n, or 2i with 2i + 1 if ``interleaved``.  Results are rounded once: a key's code
+        is the nearest to the exact value.  ``out`` may be the query itself (a view of a fused projection, say), or
+        contiguous memory apart from the rows given; its rows behind the last request are left as they are, without it
+        they are zeros.  A position past the tables makes its keys and queries NaN.  No backward pass: asking a recorded
+        call for its gradient raises."""
+        self._here(step.slots, "append")
+        return dkv_hip.fp4_append(self._layer(layer), query, key, value, step.slots, step.positions, cos, sin, interleaved, out)
+
     def load(self, layer: int, slots: torch.Tensor, dtype: torch.dtype = torch.float16):
         """(keys, values) [n, kv_heads, head_dim] held in ``slots`` (int64 [n]); zeros for negative slots.  Every value
         is exact in the three types."""
@@ -170,12 +183,22 @@ class PagedCache:
         return key, value
 
     def attend_rows(self, layer: int, query: torch.Tensor, step: Step, scaling: float | None = None,
-                    window: int | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+                    window: int | None = None, out: torch.Tensor | None = None, cap: float | None = None,
+                    slopes: torch.Tensor | None = None, sinks: torch.Tensor | None = None,
+                    first: torch.Tensor | None = None, last: torch.Tensor | None = None) -> torch.Tensor:
         """Attention of the step's queries [rows, q_heads, head_dim] (float32, float16 or bfloat16, any strides) over
         the pages of ``layer``, where the step's own keys and values lie already: causal, and over the last ``window``
         tokens of each query's if given.  ``out`` (same shape and type, contiguous; it may be the query, but not lie over
-        other rows of it) keeps its rows behind the last request; without it they are zeros.  No backward pass: asking a
-        recorded call for its gradient raises."""
+        other rows of it) keeps its rows behind the last request; without it they are zeros.
+
+        Scores may be shaped: ``cap`` c makes a score z c tanh(z / c); ``slopes`` float32 [q_heads] take slope * distance off
+        it; ``sinks`` float32 [q_heads] are the score of one more token without a value.  ``first`` and ``last`` (int64
+        [rows]) are the tokens of its request between which a row may see (0 and its own position by default, tokens that
+        the request does not hold never): a document's first token for the rows of documents packed into one request,
+        ``torch.maximum(step.positions, prefix - 1)`` for a prefix that sees itself both ways.  A window counts from the
+        row's own position all the same, and a row that sees nothing is 0.
+
+        No backward pass: asking a recorded call for its gradient raises."""
         if not 0 <= layer < self.layers:
             raise ValueError(f"layer {layer} of {self.layers}")
         if query.dim() != 3 or query.shape[1] % self.kv_heads or query.shape[0] != step.rows:
@@ -189,7 +212,8 @@ class PagedCache:
         args.window = window or 0
         args.arrivals = next(self._turns)
         args.longest, args.most = min(max(step.longest, 1), (1 << 31) - 1), min(max(step.most, 1), (1 << 31) - 1)
-        return dkv_hip.fp4_attend(args, query, step.cu, out)
+        shape = (cap, slopes, sinks, first, last)
+        return dkv_hip.fp4_attend(args, query, step.cu, out, None if all(s is None for s in shape) else shape)
 
     def held_bytes(self) -> int:
         """GPU memory of the pages of all layers, the tables and the free list."""

@@ -501,6 +501,44 @@ int dkv_fp4_store(const dkv_fp4_cache_t* c, const void* key, const void* value, 
 int dkv_fp4_load(const dkv_fp4_cache_t* c, const int64_t* slots, int32_t n, void* key, void* value, int32_t dtype,
                  void* stream);
 
+/* The same for raw projections: keys rotated to their positions before they are cut to codes, values as they are, and
+ * the queries rotated on the way (a null query: none).  Pair i < rotary / 2 of row t at positions[t] is dimensions i and
+ * i + rotary / 2, or 2i and 2i + 1 if `interleaved`; (x, y) becomes (x cos - y sin, y cos + x sin) with cos and sin of
+ * row positions[t] of the tables, and dimensions from `rotary` on stay.  Each result is rounded once: a key's code is the
+ * nearest to the exact value, and so is a query in its type.  Rows without a slot store nothing; rows of a negative
+ * position leave out as it is, or zero with `fill`; a position past the tables makes keys and queries NaN.  out may be the
+ * query in place, else it lies apart from query, key and value. */
+typedef struct dkv_fp4_append_args {
+  dkv_fp4_cache_t cache;
+  const void* query;       /* row t, head x at query + t * query_token + x * query_head elements; all rows 16-byte aligned */
+  const void* key;
+  const void* value;
+  void* out;               /* the query's type */
+  int64_t query_token;
+  int64_t query_head;
+  int64_t key_token;
+  int64_t key_head;
+  int64_t value_token;
+  int64_t value_head;
+  int64_t out_token;
+  int64_t out_head;
+  const int64_t* slots;     /* [rows] */
+  const int64_t* positions; /* [rows] */
+  const float* cos;         /* [table_rows][rotary / 2], cos_row elements apart, rows 16-byte aligned */
+  const float* sin;
+  int64_t cos_row;
+  int64_t sin_row;
+  int32_t table_rows;
+  int32_t rotary;           /* a multiple of 16 up to head_dim */
+  int32_t interleaved;
+  int32_t dtype;            /* of query, key, value and out */
+  int32_t rows;
+  int32_t q_heads;
+  int32_t fill;
+} dkv_fp4_append_args_t;
+
+int dkv_fp4_append(const dkv_fp4_append_args_t* p, void* stream);
+
 /* Attention of the newest tokens of every request over its pages: request b's
  * rows cu[b] .. cu[b+1]-1 of query are its last tokens (stored before), row i of n
  * at position lengths[b] - n + i, and sees tokens up to its own and, with a window,
@@ -536,6 +574,23 @@ typedef struct dkv_fp4_attend_args {
 
 size_t dkv_fp4_attend_workspace_bytes(const dkv_fp4_attend_args_t* p);
 int dkv_fp4_attend(const dkv_fp4_attend_args_t* p, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Attention of shaped scores over the same pages.  For a query at position p (as above) and a token t it sees,
+ *   z = scaling q.k;  z = cap tanh(z / cap)  (cap > 0);  z = z - slopes[x] |p - t|
+ * and out = sum_t e^z v / (sum_t e^z + e^sinks[x]) for query head x.  A row sees the tokens from first[row] (0 if null)
+ * to last[row] (p if null), of the window's (from p - window + 1 on) and of those the request holds; a row that sees
+ * nothing is 0.  NaN and infinities as above; a cap makes an infinite score the cap. */
+typedef struct dkv_fp4_shape {
+  const float* slopes;     /* [q_heads] or null */
+  const float* sinks;      /* [q_heads] or null */
+  const int64_t* first;    /* [rows] or null */
+  const int64_t* last;     /* [rows] or null */
+  float cap;               /* 0: none */
+} dkv_fp4_shape_t;
+
+size_t dkv_fp4_attend_shaped_workspace_bytes(const dkv_fp4_attend_args_t* p, const dkv_fp4_shape_t* shape);
+int dkv_fp4_attend_shaped(const dkv_fp4_attend_args_t* p, const dkv_fp4_shape_t* shape, void* workspace, size_t workspace_bytes,
+                          void* stream);
 
 /* ---- logits of replies ------------------------------------------------------
  * No counterpart in the reference, whose answers take the argmax as it is.  For

@@ -100,3 +100,51 @@ def attend(query, keys, values, scaling: float, window: int | None = None):
             weights = np.exp(scores - scores.max())
             out[i, h] = (weights / weights.sum()) @ values[first:position + 1, kv]
     return out
+
+
+def rotate(rows, positions, cos, sin, interleaved: bool = False):
+    """Rows [n, H, D] rotated to their positions in float64: pair i of the first 2 * cos.shape[1] dimensions is i and
+    i + cos.shape[1], or 2i and 2i + 1 if ``interleaved``; NaN where the tables have no row for a position."""
+    rows = np.array(rows, dtype=np.float64)
+    pairs = cos.shape[1]
+    for t, position in enumerate(positions):
+        if not 0 <= position < len(cos):
+            rows[t] = np.nan
+            continue
+        for i in range(pairs):
+            one, two = (2 * i, 2 * i + 1) if interleaved else (i, i + pairs)
+            x, y = rows[t, :, one].copy(), rows[t, :, two].copy()
+            c, s = float(cos[position, i]), float(sin[position, i])
+            rows[t, :, one], rows[t, :, two] = x * c - y * s, y * c + x * s
+    return rows
+
+
+def attend_shaped(query, keys, values, scaling: float, window: int | None = None, cap: float | None = None, slopes=None,
+                  sinks=None, first=None, last=None):
+    """``attend`` of shaped scores: capped, less slopes[h] times the distance, beside a sink of sinks[h], over the tokens
+    from first[i] to last[i] (0 and the row's own position by default) that there are."""
+    query, keys, values = (np.asarray(a, dtype=np.float64) for a in (query, keys, values))
+    n, q_heads, _ = query.shape
+    total, kv_heads, _ = keys.shape
+    out = np.zeros(query.shape)
+    for i in range(n):
+        position = total - n + i
+        low = 0 if first is None else max(0, int(first[i]))
+        if window is not None:
+            low = max(low, position - window + 1)
+        high = min(position if last is None else int(last[i]), total - 1)
+        if high < low:
+            continue
+        at = np.arange(low, high + 1)
+        for h in range(q_heads):
+            kv = h // (q_heads // kv_heads)
+            scores = keys[at, kv] @ query[i, h] * scaling
+            if cap is not None:
+                scores = cap * np.tanh(scores / cap)
+            if slopes is not None:
+                scores = scores - float(slopes[h]) * np.abs(position - at)
+            top = scores.max() if sinks is None else max(scores.max(), float(sinks[h]))
+            weights = np.exp(scores - top)
+            whole = weights.sum() + (0.0 if sinks is None else np.exp(float(sinks[h]) - top))
+            out[i, h] = (weights / whole) @ values[at, kv]
+    return out
