@@ -50,6 +50,19 @@ struct AttendArgs {
   int negate;   // scaling < 0: the queries change sign
 };
 
+// Shaped scores.  They are made in units of log2 e, in place of the products: cap tanh(z / cap), less the slope's share of
+// the distance; the sink joins a row's sum where its result is made.
+struct ShapedArgs : AttendArgs {
+  const float* slopes;   // [q_heads]
+  const float* sinks;    // [q_heads]
+  const int64_t* first;  // [rows]
+  const int64_t* last;   // [rows]
+  float reach;           // |scaling| / cap: what a product is of the cap
+  float cap;             // cap * log2 e, or 0
+  float small[5];        // cap times the coefficients of tanh(u) / u in u^2
+};
+constexpr float kLog2e = 1.44269504088896340736f;
+
 DKV_DEVICE void set_result(float& y, float x) { y = x; }
 DKV_DEVICE void set_result(half_t& y, float x) { y = (half_t)x; }
 DKV_DEVICE void set_result(dkv_bf16& y, float x) { y.bits = float_to_bf16_bits(x); }
@@ -107,15 +120,15 @@ DKV_DEVICE uint4 signed_words(const void* p, uint32_t sign) {
   const uint4 w = *(const uint4*)p;
   return make_uint4(w.x ^ sign, w.y ^ sign, w.z ^ sign, w.w ^ sign);
 }
-DKV_DEVICE void query_pieces(const half_t* p, bool negate, half8 (&out)[1]) {
+DKV_DEVICE void query_pieces(const half_t* p, bool negate, half8 (&out)[1], bool = false) {
   const uint4 w = signed_words(p, negate ? 0x80008000u : 0u);
   __builtin_memcpy(&out[0], &w, 16);
 }
-DKV_DEVICE void query_pieces(const dkv_bf16* p, bool negate, bf16x8 (&out)[1]) {
+DKV_DEVICE void query_pieces(const dkv_bf16* p, bool negate, bf16x8 (&out)[1], bool = false) {
   const uint4 w = signed_words(p, negate ? 0x80008000u : 0u);
   __builtin_memcpy(&out[0], &w, 16);
 }
-DKV_DEVICE void query_pieces(const float* p, bool negate, bf16x8 (&out)[3]) {
+DKV_DEVICE void query_pieces(const float* p, bool negate, bf16x8 (&out)[3], bool infinite = false) {
   const uint32_t sign = negate ? 0x80000000u : 0u;
   const uint4 first = signed_words(p, sign), second = signed_words(p + 4, sign);
   const uint32_t value[8] = {first.x, first.y, first.z, first.w, second.x, second.y, second.z, second.w};
@@ -129,7 +142,8 @@ DKV_DEVICE void query_pieces(const float* p, bool negate, bf16x8 (&out)[3]) {
     const uint32_t b = __float_as_uint(left) & 0xffff0000u;
     const uint32_t c = __float_as_uint(left - __uint_as_float(b));
     const bool finite = (a & 0x7f800000u) != 0x7f800000u;  // an infinity or NaN is one piece, a NaN
-    words[0][i >> 1] |= (a >> 16 | (finite ? 0u : 0x40u)) << (16 * (i & 1));
+    const bool stays = finite || (infinite && x == x);     // (or the infinity, where a cap makes something of it)
+    words[0][i >> 1] |= (a >> 16 | (stays ? 0u : 0x40u)) << (16 * (i & 1));
     words[1][i >> 1] |= (finite ? b >> 16 : 0u) << (16 * (i & 1));
     words[2][i >> 1] |= (finite ? c >> 16 : 0u) << (16 * (i & 1));
   }
@@ -150,12 +164,36 @@ DKV_DEVICE float larger(float a, float b, float c) {
   return d;
 }
 
+// cap * tanh(u) for |u| <= 1/2: u times a polynomial in u^2, whose coefficients hold the cap (6e-8 off, relative).
+DKV_DEVICE float small_tanh(float u, const float (&c)[5]) {
+  const float z = u * u;
+  return u * fmaf(fmaf(fmaf(fmaf(c[4], z, c[3]), z, c[2]), z, c[1]), z, c[0]);
+}
+// cap * tanh(u) with 1 - 2 / (1 + e^2u), whose error is the cap's size: for scores that reach far into it.
+DKV_DEVICE float large_tanh(float u, float cap) {
+  return fmaf(-2.0f * cap, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(u * (2.0f * kLog2e))), cap);
+}
+
+// What a row's sums are worth beside its sink: (factor of the sums, their whole), weights held times 2^shift.
+DKV_DEVICE float2 beside_sink(float top, float total, const float* sinks, int head, float shift) {
+  if (!sinks || total == 0.0f) return make_float2(1.0f, total);
+  const float sink = sinks[head] * kLog2e, higher = fmaxf(top, sink), factor = __builtin_amdgcn_exp2f(top - higher);
+  return make_float2(factor, fmaf(total, factor, __builtin_amdgcn_exp2f(sink - higher + shift)));
+}
+
 DKV_DEVICE float exponent(uint32_t byte) { return __uint_as_float(byte << 23); }
 
 // The tables are read through the scalar cache: an index the same in every lane costs no vector load, and no wait for the
 // page loads on their way.
 typedef const __attribute__((address_space(4))) int32_t* scalar_ints;
 DKV_DEVICE scalar_ints as_scalar(const int32_t* p) { return (scalar_ints)(uintptr_t)p; }
+
+// The largest magnitude of three floats (a NaN loses).
+DKV_DEVICE float larger_size(float a, float b, float c) {
+  float d;
+  asm("v_max3_f32 %0, |%1|, |%2|, |%3|" : "=v"(d) : "v"(a), "v"(b), "v"(c));
+  return d;
+}
 
 // One chunk in this lane, CH tiles of 16 tokens: codes and exponents, and which tiles hold something (the same in every
 // lane).
@@ -247,17 +285,23 @@ DKV_DEVICE void load_values(const AttendArgs& a, const Tiles<CH>& tiles, const L
   }
 }
 
-template <int D, typename T, int NT, int CH, int kWaves>
-__global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_attend_kernel(AttendArgs a) {
+// Weights are held times 2^kShift, against a reference that scores may pass by kSlack: 2^15 at the most, below the largest
+// float16.
+template <typename T>
+constexpr float kSlackOf = Operand<T>::kPieces == 1 ? 7.0f : 0.0f;
+template <typename T>
+constexpr float kShiftOf = 15.0f - kSlackOf<T>;
+
+template <int D, typename T, int NT, int CH, int kWaves, typename Args>
+__global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_attend_kernel(Args a) {
+  constexpr bool kShaped = __is_same(Args, ShapedArgs);
   using Op = Operand<T>;
   using frag = typename Op::frag;
   constexpr int kRows = 16 * NT, kSteps = D / 32, kLane = D / 16, kPieces = Op::kPieces;
   // float16 pieces of a weight: a second one for float32 and float16 results.  One piece for float16 costs 464 us instead
   // of 615 at 2,048 query tokens of 24 heads over 16K tokens of 128 dimensions, and rounds as much as the result does.
   constexpr int kWeights = kPieces > 1 || __is_same(T, half_t) ? 2 : 1;
-  // Weights are held times 2^kShift, against a reference that scores may pass by kSlack: 2^15 at the most, below the
-  // largest float16.
-  constexpr float kSlack = kPieces == 1 ? 7.0f : 0.0f, kShift = 15.0f - kSlack;
+  constexpr float kSlack = kSlackOf<T>, kShift = kShiftOf<T>;
   constexpr int kStride = D + 4;                  // a row of sums in LDS
   constexpr bool kJoins = NT <= 2 && kWaves == 4;  // may join its splits itself (sums hold 6 floats a thread)
   // With 64 rows the accumulators leave no registers for the queries and a second chunk, and two waves a SIMD matter more
@@ -266,7 +310,10 @@ __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_at
   __shared__ frag held[kLean ? NT * kSteps * 64 : 1];
   __shared__ float sums[4 * 16 * kStride];
   __shared__ float stat[2][kWaves][kRows];
+  __shared__ int2 ranges[kShaped ? kWaves : 1][kShaped ? kRows : 1];  // tokens that a row sees, a copy for each wave
 
+  bool capped = false;
+  if constexpr (kShaped) capped = a.cap > 0.0f;
   const int h = blockIdx.x, b = blockIdx.z, split = blockIdx.y % a.splits, blocks = gridDim.y / a.splits;
   __shared__ int last;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
@@ -302,6 +349,14 @@ __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_at
     // the last token a row sees, and the one before the first (made where a chunk has a mask, and not held)
     auto last_seen = [&](int nt) { return first_position + min(row0 + nt * 16 + i, n_rows - 1) / a.groups; };
     auto before_first = [&](int last) { return (int)max((long)last - a.window, -1L); };
+    // (the one before the first token a row sees, the last one)
+    auto seen_by = [&](int nt) {
+      if constexpr (kShaped) {
+        if (a.first || a.last) return ranges[wave][nt * 16 + i];
+      }
+      const int last = last_seen(nt);
+      return make_int2(before_first(last), last);
+    };
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int r = min(row0 + nt * 16 + i, n_rows - 1);  // (rows past the last one repeat it, and go nowhere)
@@ -312,19 +367,57 @@ __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_at
 #pragma unroll
           for (int s = 0; s < kSteps; ++s) {
             query_pieces(p + g * (D / 4) + s * 8, a.negate, q[0][0]);
-            quiet(q[0][0]);
+            if (!kShaped || !capped) quiet(q[0][0]);
             held[(nt * kSteps + s) * 64 + lane] = q[0][0][0];
           }
         }
       } else {
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) query_pieces(p + g * (D / 4) + s * 8, a.negate, q[nt][s]);
+        for (int s = 0; s < kSteps; ++s) query_pieces(p + g * (D / 4) + s * 8, a.negate, q[nt][s], kShaped && capped);
       }
     }
     if constexpr (kLean) __syncthreads();
-    const int low_position = first_position + row0 / a.groups, high_position = first_position + (row1 - 1) / a.groups;
-    const int begin = (int)max((long)low_position - a.window + 1, 0L), end = high_position + 1;  // tokens some row sees
-    const int all_from = (int)max((long)high_position - a.window + 1, 0L);                       // and all rows, from here
+    int low_position = first_position + row0 / a.groups, high_position = first_position + (row1 - 1) / a.groups;
+    int begin = (int)max((long)low_position - a.window + 1, 0L), end = high_position + 1;  // tokens some row sees
+    int all_from = (int)max((long)high_position - a.window + 1, 0L);  // and all rows, from here to low_position
+    int place[kShaped ? NT : 1];     // a row's position and slope
+    float slope[kShaped ? NT : 1];
+    if constexpr (kShaped) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const int r = min(row0 + nt * 16 + i, n_rows - 1), token = r / a.groups;
+        place[nt] = first_position + token;
+        slope[nt] = a.slopes ? a.slopes[h * a.groups + (r - token * a.groups)] * -kLog2e : 0.0f;
+      }
+      if (a.first || a.last) {
+        int lowest = INT32_MAX, highest = -1, from = 0, to = INT32_MAX;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const int64_t row = q0 + (place[nt] - first_position);
+          const long low = max(a.first ? (long)a.first[row] : 0L, max((long)place[nt] - a.window + 1, 0L));
+          const long high = min(a.last ? (long)a.last[row] : (long)place[nt], (long)len - 1);
+          const bool some = low <= high;  // (a row that sees nothing has no say in where the block begins and ends)
+          const int2 range = some ? make_int2((int)low - 1, (int)high) : make_int2(INT32_MAX, -1);
+          if (g == 0) ranges[wave][nt * 16 + i] = range;
+          lowest = min(lowest, some ? (int)low : INT32_MAX);
+          highest = max(highest, range.y);
+          from = max(from, some ? (int)low : INT32_MAX);
+          to = min(to, range.y);
+        }
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int x = 1; x < 16; x <<= 1) {
+          lowest = min(lowest, __shfl_xor(lowest, x));
+          highest = max(highest, __shfl_xor(highest, x));
+          from = max(from, __shfl_xor(from, x));
+          to = min(to, __shfl_xor(to, x));
+        }
+        begin = __builtin_amdgcn_readfirstlane(min(lowest, highest + 1));
+        end = __builtin_amdgcn_readfirstlane(highest) + 1;
+        all_from = __builtin_amdgcn_readfirstlane(from);
+        low_position = __builtin_amdgcn_readfirstlane(to);
+      }
+    }
     const int chunk_begin = begin / (16 * CH), chunk_end = max((end + 16 * CH - 1) / (16 * CH), chunk_begin);
     const long chunks = end > begin ? chunk_end - chunk_begin : 0;
     // as many chunks a split as the plan gives (so that a short request takes few), or what covers them all
@@ -353,7 +446,8 @@ __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_at
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) quiet(q[nt][s]);
+        for (int s = 0; s < kSteps; ++s)
+          if (!kShaped || !capped) quiet(q[nt][s]);
     }
     for (; chunk < c1; chunk += kWaves) {
       const int later = load_entries<CH>(a, table, chunk + 2 * kWaves < c1 ? len : 0, chunk + 2 * kWaves);
@@ -410,17 +504,52 @@ __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_at
       }
 
       const int base = chunk * CH * 16;
+      float scale = a.scale;
+      if constexpr (kShaped) {
+        if (capped) {
+          scale = 1.0f;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float size = 0.0f;
+#pragma unroll
+            for (int t = 0; t < CH; ++t) size = larger_size(larger_size(size, s[nt][t][0], s[nt][t][1]), s[nt][t][2], s[nt][t][3]);
+            const bool far = __any(size * a.reach > 0.5f);
+#pragma unroll
+            for (int t = 0; t < CH; ++t)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                const float u = s[nt][t][r] * a.reach;
+                float y;
+                if (!far) y = small_tanh(u, a.small);
+                else if (kPieces == 1) y = large_tanh(u, a.cap);
+                else y = fabsf(u) <= 0.5f ? small_tanh(u, a.small) : large_tanh(u, a.cap);
+                s[nt][t][r] = y;
+              }
+          }
+        }
+        if (a.slopes) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const float ahead = (float)(base + g * 4 - place[nt]);  // (whole numbers where distances are below 2^24)
+#pragma unroll
+            for (int t = 0; t < CH; ++t)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) s[nt][t][r] = fmaf(s[nt][t][r], scale, slope[nt] * fabsf(ahead + (float)(t * 16 + r)));
+          }
+          scale = 1.0f;
+        }
+      }
       const bool masked = !tiles.whole || base + CH * 16 > low_position + 1 || base < all_from;
       if (masked) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          const int last = last_seen(nt), before = before_first(last);
+          const int2 seen = seen_by(nt);
 #pragma unroll
           for (int t = 0; t < CH; ++t)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
               const int token = base + t * 16 + g * 4 + r;
-              if (!tiles.valid[t] || token > last || token <= before) s[nt][t][r] = -INFINITY;
+              if (!tiles.valid[t] || token > seen.y || token <= seen.x) s[nt][t][r] = -INFINITY;
             }
         }
         // what lies behind the request is stale: its values become zeros
@@ -439,8 +568,8 @@ __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_at
         float top = s[nt][0][0];
 #pragma unroll
         for (int t = 0; t < CH; ++t) top = larger(larger(top, s[nt][t][0], s[nt][t][1]), s[nt][t][2], s[nt][t][3]);
-        if (__any(top * a.scale > m[nt] + kSlack)) {
-          const float higher = larger(m[nt], max_xor32(max_xor16(top)) * a.scale);
+        if (__any(top * scale > m[nt] + kSlack)) {
+          const float higher = larger(m[nt], max_xor32(max_xor16(top)) * scale);
           const float factor = __builtin_amdgcn_exp2f(m[nt] - (higher == -INFINITY ? 0.0f : higher));
           l[nt] *= factor;
 #pragma unroll
@@ -452,7 +581,7 @@ __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_at
         for (int t = 0; t < CH; ++t) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const float p = __builtin_amdgcn_exp2f(fmaf(s[nt][t][r], a.scale, shift));
+            const float p = __builtin_amdgcn_exp2f(fmaf(s[nt][t][r], scale, shift));
             l[nt] += p;
             w[nt][t / 2][0][(t & 1) * 4 + r] = (half_t)p;
             if constexpr (kWeights == 2) w[nt][t / 2][1][(t & 1) * 4 + r] = (half_t)(p - (float)(half_t)p);
@@ -478,12 +607,12 @@ __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_at
             for (int x = 0; x < 8; ++x) is_bad[x] = (bad[x >> 2] >> (8 * (x & 3) + 7)) & 1 ? (half_t)1.0f : (half_t)0.0f;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-              const int last = last_seen(nt), before = before_first(last);
+              const int2 seen = seen_by(nt);
               half8 sees;
 #pragma unroll
               for (int x = 0; x < 8; ++x) {
                 const int token = base + (2 * u + (x >> 2)) * 16 + g * 4 + (x & 3);
-                sees[x] = token <= last && token > before ? (half_t)1.0f : (half_t)0.0f;
+                sees[x] = token <= seen.y && token > seen.x ? (half_t)1.0f : (half_t)0.0f;
               }
               const floatx4 hit = __builtin_amdgcn_mfma_f32_16x16x32_f16(is_bad, sees, floatx4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
 #pragma unroll
@@ -594,7 +723,13 @@ __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_at
         const long out_row = (long)(q0 + token) * q_heads + h * a.groups + (r - token * a.groups);
         if (splits == 1) {
           T* out = (T*)a.out + out_row * D + part * kPart;
-          const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+          float inverse;
+          if constexpr (kShaped) {
+            const float2 beside = beside_sink(highest, total, a.sinks, h * a.groups + (r - token * a.groups), kShift);
+            inverse = total == 0.0f ? 0.0f : beside.x / beside.y;
+          } else {
+            inverse = total == 0.0f ? 0.0f : 1.0f / total;
+          }
 #pragma unroll
           for (int j = 0; j < kPart; ++j) set_result(out[j], total == 0.0f ? 0.0f : acc[j] * inverse);
         } else {
@@ -681,6 +816,12 @@ __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_at
               for (int j = 0; j < 4; ++j) v[j] = fmaf(other[j], f, v[j]);
             }
             T* out = (T*)a.out + out_row * D + dim;
+            if constexpr (kShaped) {
+              const float2 beside = beside_sink(highest, whole, a.sinks, h * a.groups + (r - token * a.groups), kShift);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) v[j] *= beside.x;
+              whole = beside.y;
+            }
 #pragma unroll
             for (int j = 0; j < 4; ++j) set_result(out[j], whole == 0.0f ? 0.0f : v[j] / whole);
           }
@@ -693,12 +834,12 @@ __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_at
 
 // The splits of a row joined: a workgroup per row, D / 4 threads for its dimensions in fours, the splits dealt out to the
 // 256 / (D / 4) sets of them and their sums added in LDS.
-template <int D, typename T>
-__global__ __launch_bounds__(256) void fp4_join_kernel(AttendArgs a, int q_heads) {
+template <int D, typename T, typename Args>
+__global__ __launch_bounds__(256) void fp4_join_kernel(Args a, int q_heads) {
   constexpr int kSet = D / 4, kSets = 256 / kSet;
   __shared__ float weight[kMaxSplits];
   __shared__ float4 sums[kSets][kSet];
-  __shared__ float whole;
+  __shared__ float whole, ours;
   const long row = blockIdx.x;
   if (row >= (long)min(max(a.cu[a.requests], 0), a.rows) * q_heads) return;
   const float2* ml = a.part_ml + row * a.splits;
@@ -720,6 +861,11 @@ __global__ __launch_bounds__(256) void fp4_join_kernel(AttendArgs a, int q_heads
       total += factor < 0.0f ? 0.0f : x[k].y * factor;
     }
     total = wave_sum(total);
+    if constexpr (__is_same(Args, ShapedArgs)) {
+      const float2 beside = beside_sink(top, total, a.sinks, (int)(row % q_heads), kShiftOf<T>);
+      if (threadIdx.x == 0) ours = beside.x;
+      total = beside.y;
+    }
     if (threadIdx.x == 0) whole = total;
   }
   __syncthreads();
@@ -742,15 +888,18 @@ __global__ __launch_bounds__(256) void fp4_join_kernel(AttendArgs a, int q_heads
     acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
   }
   T* out = (T*)a.out + row * D + at * 4;
-  const float v[4] = {acc.x, acc.y, acc.z, acc.w};
+  float v[4] = {acc.x, acc.y, acc.z, acc.w};
+  if constexpr (__is_same(Args, ShapedArgs))
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] *= ours;
 #pragma unroll
   for (int j = 0; j < 4; ++j) set_result(out[j], whole == 0.0f ? 0.0f : v[j] / whole);
 }
 
 // The same for few splits: a set of D / 4 threads per row.  49,152 rows of two splits: 13 us, 40 with a workgroup for
 // each row.
-template <int D, typename T>
-__global__ __launch_bounds__(256) void fp4_join_few_kernel(AttendArgs a, int q_heads) {
+template <int D, typename T, typename Args>
+__global__ __launch_bounds__(256) void fp4_join_few_kernel(Args a, int q_heads) {
   constexpr int kSet = D / 4, kSets = 256 / kSet;
   const int at = threadIdx.x % kSet;
   const long row = (long)blockIdx.x * kSets + threadIdx.x / kSet;
@@ -769,7 +918,13 @@ __global__ __launch_bounds__(256) void fp4_join_few_kernel(AttendArgs a, int q_h
     acc.x = fmaf(v.x, w, acc.x); acc.y = fmaf(v.y, w, acc.y); acc.z = fmaf(v.z, w, acc.z); acc.w = fmaf(v.w, w, acc.w);
   }
   T* out = (T*)a.out + row * D + at * 4;
-  const float v[4] = {acc.x, acc.y, acc.z, acc.w};
+  float v[4] = {acc.x, acc.y, acc.z, acc.w};
+  if constexpr (__is_same(Args, ShapedArgs)) {
+    const float2 beside = beside_sink(top, whole, a.sinks, (int)(row % q_heads), kShiftOf<T>);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] *= beside.x;
+    whole = beside.y;
+  }
 #pragma unroll
   for (int j = 0; j < 4; ++j) set_result(out[j], whole == 0.0f ? 0.0f : v[j] / whole);
 }
@@ -856,175 +1011,53 @@ size_t part_bytes(const dkv_fp4_attend_args_t& p, const Plan& plan) {
   return (size_t)p.rows * p.q_heads * plan.splits * (p.cache.head_dim * sizeof(float) + sizeof(float2));
 }
 
-template <int D, typename T>
-void launch(const AttendArgs& a, const Plan& plan, int q_heads, hipStream_t st) {
+template <int D, typename T, typename Args>
+void launch(const Args& a, const Plan& plan, int q_heads, hipStream_t st) {
   const dim3 grid(a.c.kv_heads, plan.blocks * plan.splits, a.requests), block(plan.waves * 64);
   constexpr bool wide = D < 256 && sizeof(T) == 2;
   if (plan.tiles == 1) {
-    if (plan.waves == 8) hipLaunchKernelGGL((fp4_attend_kernel<D, T, 1, D == 256 ? 2 : 4, 8>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((fp4_attend_kernel<D, T, 1, D == 256 ? 2 : 4, 4>), grid, block, 0, st, a);
+    if (plan.waves == 8) hipLaunchKernelGGL((fp4_attend_kernel<D, T, 1, D == 256 ? 2 : 4, 8, Args>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((fp4_attend_kernel<D, T, 1, D == 256 ? 2 : 4, 4, Args>), grid, block, 0, st, a);
   } else if (plan.tiles == 2) {
-    if constexpr (D < 256 || sizeof(T) == 2) hipLaunchKernelGGL((fp4_attend_kernel<D, T, 2, 2, 4>), grid, block, 0, st, a);
+    if constexpr (D < 256 || sizeof(T) == 2) hipLaunchKernelGGL((fp4_attend_kernel<D, T, 2, 2, 4, Args>), grid, block, 0, st, a);
   } else {
-    if constexpr (wide) hipLaunchKernelGGL((fp4_attend_kernel<D, T, 4, 2, 4>), grid, block, 0, st, a);
+    if constexpr (wide) hipLaunchKernelGGL((fp4_attend_kernel<D, T, 4, 2, 4, Args>), grid, block, 0, st, a);
   }
   const long rows = (long)a.rows * q_heads;
   if (plan.splits == 1 || a.arrivals) return;
   if (plan.splits > kFewSplits) {
-    hipLaunchKernelGGL((fp4_join_kernel<D, T>), dim3((unsigned)rows), dim3(256), 0, st, a, q_heads);
+    hipLaunchKernelGGL((fp4_join_kernel<D, T, Args>), dim3((unsigned)rows), dim3(256), 0, st, a, q_heads);
   } else {
     constexpr int kSets = 1024 / D;
-    hipLaunchKernelGGL((fp4_join_few_kernel<D, T>), dim3((unsigned)((rows + kSets - 1) / kSets)), dim3(256), 0, st, a, q_heads);
+    hipLaunchKernelGGL((fp4_join_few_kernel<D, T, Args>), dim3((unsigned)((rows + kSets - 1) / kSets)), dim3(256), 0, st, a, q_heads);
   }
 }
 
-template <int D>
-void launch_type(const AttendArgs& a, const Plan& plan, int q_heads, int dtype, hipStream_t st) {
+template <int D, typename Args>
+void launch_type(const Args& a, const Plan& plan, int q_heads, int dtype, hipStream_t st) {
   if (dtype == DKV_F32) launch<D, float>(a, plan, q_heads, st);
   else if (dtype == DKV_F16) launch<D, half_t>(a, plan, q_heads, st);
   else launch<D, dkv_bf16>(a, plan, q_heads, st);
 }
 
-// ---------------------------------------------------------------------------
-// Shaped scores: a cap, a bias that falls with the distance, sinks, ranges of tokens.  A wave per query row: a lane scores
-// a token of 64, then the lanes are the row's dimensions and take the tokens' values in turn.
-// ---------------------------------------------------------------------------
-struct ShapedArgs {
-  AttendArgs a;
-  dkv_fp4_shape_t s;
-  float scaling;
-};
-
-template <int D, typename T>
-__global__ __launch_bounds__(256) void fp4_shaped_kernel(ShapedArgs p) {
-  const AttendArgs& a = p.a;
-  constexpr int kDims = D / 64;
-  __shared__ float query[4][D], weights[4][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int q_heads = a.c.kv_heads * a.groups;
-  const long row = (long)blockIdx.x * 4 + wave;
-  if (row >= (long)a.rows * q_heads) return;
-  const int t = (int)(row / q_heads), x = (int)(row % q_heads), h = x / a.groups;
-  T* out = (T*)a.out + row * D + lane * kDims;
-  const int end = min(max(a.cu[a.requests], 0), a.rows);
-  if (t >= end) {
-    if (a.fill) __builtin_memset(out, 0, kDims * sizeof(T));
-    return;
-  }
-  int b = 0, above = a.requests;  // the last request whose rows begin at t or before
-  while (above - b > 1) {
-    const int mid = (b + above) >> 1;
-    if (a.cu[mid] <= t) b = mid; else above = mid;
-  }
-  const int q0 = min(max(a.cu[b], 0), a.rows), q1 = min(max(a.cu[b + 1], q0), a.rows);
-  const int len = min(max(a.lengths[b], 0), a.width << a.shift);
-  const long at = (long)len - (q1 - q0) + (t - q0);
-  const long low = max(max(p.s.first ? (long)p.s.first[t] : 0L, at - a.window + 1), 0L);
-  const long high = min(p.s.last ? (long)p.s.last[t] : at, (long)len - 1);
-  const T* q = (const T*)a.query + t * a.query_token + x * a.query_head + lane * kDims;
-#pragma unroll
-  for (int j = 0; j < kDims; ++j) query[wave][lane * kDims + j] = load_as_float(q, j, sizeof(T) == 4 ? DKV_F32 : __is_same(T, half_t) ? DKV_F16 : DKV_BF16);
-  const float slope = p.s.slopes ? p.s.slopes[x] : 0.0f;
-  const int page = a.c.page;
-  float m = -INFINITY, l = 0.0f, acc[kDims] = {};
-  for (long base = low & ~63L; base <= high; base += 64) {
-    const long token = base + lane;
-    bool sees = token >= low && token <= high;
-    const int id = sees ? a.table[(long)b * a.width + (token >> a.shift)] : -1;
-    sees = sees && (uint32_t)id < (uint32_t)a.c.pages;
-    float z = -INFINITY;
-    if (sees) {
-      const long line = ((long)id * a.c.kv_heads + h) * page + (token & (page - 1));
-      z = 0.0f;
-      for (int block = 0; block < D / 32; ++block) {
-        const float e = exponent(a.c.key_scales[line * (D / 32) + block]);
-        const uint4 w = *(const uint4*)(a.c.key_codes + line * (D / 2) + block * 16);
-        const uint32_t words[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float* qq = query[wave] + block * 32 + i * 8;
-          const floatx2 k0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(words[i], e, 0), k1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(words[i], e, 1);
-          const floatx2 k2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(words[i], e, 2), k3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(words[i], e, 3);
-          z += k0[0] * qq[0] + k0[1] * qq[1] + k1[0] * qq[2] + k1[1] * qq[3] + k2[0] * qq[4] + k2[1] * qq[5] + k3[0] * qq[6] + k3[1] * qq[7];
-        }
-      }
-      z *= p.scaling;
-      if (p.s.cap > 0.0f) z = p.s.cap * tanhf(z / p.s.cap);
-      z -= slope * fabsf((float)(token - at));
-    }
-    const uint64_t seen = __ballot(sees);
-    const float top = wave_max(z), higher = fmaxf(m, top);
-    const float factor = higher == -INFINITY ? 1.0f : expf(m - higher);
-    m = higher;
-    const float w = sees ? expf(z - m) : 0.0f;
-    l = l * factor + wave_sum(w);
-    weights[wave][lane] = w;
-#pragma unroll
-    for (int j = 0; j < kDims; ++j) acc[j] *= factor;
-    for (uint64_t left = seen; left; left &= left - 1) {
-      const int i = __builtin_ctzll(left);
-      const int other = __shfl(id, i);
-      const long in_page = (base + i) & (page - 1), head_page = (long)other * a.c.kv_heads + h;
-      const float weight = weights[wave][i];
-#pragma unroll
-      for (int j = 0; j < kDims; ++j) {
-        const int d = lane * kDims + j, byte = d / 2;
-        constexpr int kLane = D / 32;
-        const uint32_t code = a.c.value_codes[head_page * page * (D / 2) + (in_page >> 2) * (2 * D) + byte / kLane * (4 * kLane) +
-                                              (in_page & 3) * kLane + byte % kLane];
-        const float e = exponent(a.c.value_scales[head_page * page * (D / 32) + (in_page >> 2) * (D / 8) + d / 32 * 4 + (in_page & 3)]);
-        const floatx2 v = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, e, 0);
-        acc[j] = fmaf(weight, d & 1 ? v[1] : v[0], acc[j]);
-      }
-    }
-  }
-  float whole = l, scale = 1.0f;
-  if (p.s.sinks && whole != 0.0f) {
-    const float sink = p.s.sinks[x], higher = fmaxf(m, sink);
-    scale = expf(m - higher);
-    whole = whole * scale + expf(sink - higher);
-  }
-#pragma unroll
-  for (int j = 0; j < kDims; ++j) set_result(out[j], whole == 0.0f ? 0.0f : acc[j] * scale / whole);
-}
-
-template <int D>
-void launch_shaped(const ShapedArgs& p, int q_heads, int dtype, hipStream_t st) {
-  const dim3 grid((unsigned)(((long)p.a.rows * q_heads + 3) / 4)), block(256);
-  if (dtype == DKV_F32) hipLaunchKernelGGL((fp4_shaped_kernel<D, float>), grid, block, 0, st, p);
-  else if (dtype == DKV_F16) hipLaunchKernelGGL((fp4_shaped_kernel<D, half_t>), grid, block, 0, st, p);
-  else hipLaunchKernelGGL((fp4_shaped_kernel<D, dkv_bf16>), grid, block, 0, st, p);
-}
-
 int check_shape(const dkv_fp4_shape_t* s, const char* what) {
   DKV_REQUIRE(s, DKV_EINVAL, "%s: null shape", what);
-  DKV_REQUIRE(s->cap >= 0.0f && s->cap < INFINITY, DKV_EINVAL, "%s: cap %g", what, s->cap);
+  DKV_REQUIRE(s->cap == 0.0f || (s->cap >= 1e-30f && s->cap <= 1e30f), DKV_EINVAL, "%s: cap %g (0, or 1e-30 to 1e30)", what, s->cap);
   DKV_REQUIRE((((uintptr_t)s->slopes | (uintptr_t)s->sinks) & 3) == 0 && (((uintptr_t)s->first | (uintptr_t)s->last) & 7) == 0, DKV_EINVAL,
               "%s: misaligned slopes, sinks, first or last", what);
   return DKV_OK;
 }
 
-}  // namespace
-
-extern "C" size_t dkv_fp4_attend_workspace_bytes(const dkv_fp4_attend_args_t* p) {
-  if (check_attend(p, "dkv_fp4_attend_workspace_bytes")) return 0;
-  return part_bytes(*p, plan_of(*p)) + 16;
-}
-
-extern "C" int dkv_fp4_attend(const dkv_fp4_attend_args_t* p, void* workspace, size_t workspace_bytes, void* stream) {
-  const int rc = check_attend(p, "dkv_fp4_attend");
-  if (rc) return rc;
-  if (p->rows == 0) return DKV_OK;
-  DKV_REQUIRE(p->table && p->lengths && p->cu && p->query && p->out, DKV_EINVAL, "dkv_fp4_attend: null pointer");
+// The arguments that every launch of a call shares, or why there is none.
+int attend_args(const dkv_fp4_attend_args_t* p, const Plan& plan, void* workspace, size_t workspace_bytes, AttendArgs& a, const char* what) {
+  DKV_REQUIRE(p->table && p->lengths && p->cu && p->query && p->out, DKV_EINVAL, "%s: null pointer", what);
   const int unit = p->query_dtype == DKV_F32 ? 4 : 8;
   DKV_REQUIRE((((uintptr_t)p->query | (uintptr_t)p->out) & 15) == 0 && p->query_token % unit == 0 && p->query_head % unit == 0,
-              DKV_EINVAL, "dkv_fp4_attend: query rows and out must be 16-byte aligned");
-  const Plan plan = plan_of(*p);
+              DKV_EINVAL, "%s: query rows and out must be 16-byte aligned", what);
   const size_t need = part_bytes(*p, plan);
-  DKV_REQUIRE(need == 0 || workspace, DKV_EINVAL, "dkv_fp4_attend: null workspace");
-  DKV_REQUIRE(need <= workspace_bytes, DKV_EWORKSPACE, "dkv_fp4_attend: workspace %zu < %zu bytes", workspace_bytes, need);
-  DKV_REQUIRE(((uintptr_t)workspace & 15) == 0, DKV_EINVAL, "dkv_fp4_attend: workspace must be 16-byte aligned");
-  AttendArgs a{};
+  DKV_REQUIRE(need == 0 || workspace, DKV_EINVAL, "%s: null workspace", what);
+  DKV_REQUIRE(need <= workspace_bytes, DKV_EWORKSPACE, "%s: workspace %zu < %zu bytes", what, workspace_bytes, need);
+  DKV_REQUIRE(((uintptr_t)workspace & 15) == 0, DKV_EINVAL, "%s: workspace must be 16-byte aligned", what);
   a.c = p->cache;
   a.table = p->table; a.lengths = p->lengths; a.cu = p->cu; a.query = p->query; a.out = p->out;
   a.part = (float*)workspace;
@@ -1036,20 +1069,42 @@ extern "C" int dkv_fp4_attend(const dkv_fp4_attend_args_t* p, void* workspace, s
   a.window = p->window ? p->window : INT32_MAX;
   a.splits = plan.splits; a.share = plan.share; a.fill = p->fill;
   // a positive factor keeps the order of the scores; one of 0 weighs every token the same, as the smallest does
-  a.scale = fmaxf(fabsf(p->scaling) * 1.44269504088896340736f, 1.1754944e-38f);
+  a.scale = fmaxf(fabsf(p->scaling) * kLog2e, 1.1754944e-38f);
   if (p->scaling != p->scaling) a.scale = p->scaling;
   a.negate = p->scaling < 0.0f;
+  return DKV_OK;
+}
+
+template <typename Args>
+int launch_attend(const Args& a, const Plan& plan, const dkv_fp4_attend_args_t* p, void* stream, const char* what) {
   hipStream_t st = dkv::as_stream(stream);
   if (a.c.head_dim == 64) launch_type<64>(a, plan, p->q_heads, p->query_dtype, st);
   else if (a.c.head_dim == 128) launch_type<128>(a, plan, p->q_heads, p->query_dtype, st);
   else launch_type<256>(a, plan, p->q_heads, p->query_dtype, st);
-  return dkv::check_launch("dkv_fp4_attend");
+  return dkv::check_launch(what);
+}
+
+}  // namespace
+
+extern "C" size_t dkv_fp4_attend_workspace_bytes(const dkv_fp4_attend_args_t* p) {
+  if (check_attend(p, "dkv_fp4_attend_workspace_bytes")) return 0;
+  return part_bytes(*p, plan_of(*p)) + 16;
+}
+
+extern "C" int dkv_fp4_attend(const dkv_fp4_attend_args_t* p, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check_attend(p, "dkv_fp4_attend");
+  if (rc) return rc;
+  if (p->rows == 0) return DKV_OK;
+  const Plan plan = plan_of(*p);
+  AttendArgs a{};
+  rc = attend_args(p, plan, workspace, workspace_bytes, a, "dkv_fp4_attend");
+  return rc ? rc : launch_attend(a, plan, p, stream, "dkv_fp4_attend");
 }
 
 extern "C" size_t dkv_fp4_attend_shaped_workspace_bytes(const dkv_fp4_attend_args_t* p, const dkv_fp4_shape_t* shape) {
   const char* what = "dkv_fp4_attend_shaped_workspace_bytes";
   if (check_attend(p, what) || check_shape(shape, what)) return 0;
-  return 16;
+  return part_bytes(*p, plan_of(*p)) + 16;
 }
 
 extern "C" int dkv_fp4_attend_shaped(const dkv_fp4_attend_args_t* p, const dkv_fp4_shape_t* shape, void* workspace,
@@ -1059,23 +1114,18 @@ extern "C" int dkv_fp4_attend_shaped(const dkv_fp4_attend_args_t* p, const dkv_f
   if (!rc) rc = check_shape(shape, what);
   if (rc) return rc;
   if (p->rows == 0) return DKV_OK;
-  DKV_REQUIRE(p->table && p->lengths && p->cu && p->query && p->out, DKV_EINVAL, "%s: null pointer", what);
-  const int unit = p->query_dtype == DKV_F32 ? 4 : 8;
-  DKV_REQUIRE((((uintptr_t)p->query | (uintptr_t)p->out) & 15) == 0 && p->query_token % unit == 0 && p->query_head % unit == 0,
-              DKV_EINVAL, "%s: query rows and out must be 16-byte aligned", what);
-  ShapedArgs s{};
-  s.s = *shape; s.scaling = p->scaling;
-  AttendArgs& a = s.a;
-  a.c = p->cache;
-  a.table = p->table; a.lengths = p->lengths; a.cu = p->cu; a.query = p->query; a.out = p->out;
-  a.query_token = p->query_token; a.query_head = p->query_head;
-  a.requests = p->requests; a.width = p->width; a.shift = dkv::page_shift(p->cache.page); a.rows = p->rows;
-  a.groups = p->q_heads / p->cache.kv_heads;
-  a.window = p->window ? p->window : INT32_MAX;
-  a.fill = p->fill;
-  hipStream_t st = dkv::as_stream(stream);
-  if (a.c.head_dim == 64) launch_shaped<64>(s, p->q_heads, p->query_dtype, st);
-  else if (a.c.head_dim == 128) launch_shaped<128>(s, p->q_heads, p->query_dtype, st);
-  else launch_shaped<256>(s, p->q_heads, p->query_dtype, st);
-  return dkv::check_launch(what);
+  const Plan plan = plan_of(*p);
+  ShapedArgs a{};
+  rc = attend_args(p, plan, workspace, workspace_bytes, a, what);
+  if (rc) return rc;
+  a.slopes = shape->slopes; a.sinks = shape->sinks; a.first = shape->first; a.last = shape->last;
+  if (shape->cap > 0.0f) {
+    a.cap = shape->cap * kLog2e;
+    // (tanh(u) / u - 1) / u^2 interpolated at the four Chebyshev nodes of u^2 from 0 to 1/4
+    const float c[5] = {1.0f, -0.33333310f, 0.13330476f, -0.053387109f, 0.017988745f};
+    for (int i = 0; i < 5; ++i) a.small[i] = a.cap * c[i];
+    a.reach = fminf(fabsf(p->scaling) / shape->cap, 3e38f);
+    if (p->scaling != p->scaling) a.reach = p->scaling;
+  }
+  return launch_attend(a, plan, p, stream, what);
 }

@@ -783,8 +783,8 @@ def fp4_attend(args: Fp4AttendArgs, query, cu, out=None, shape_of=None) -> torch
 def _fp4_shape(index: int, rows: int, q_heads: int, cap, slopes, sinks, first, last) -> Fp4Shape:
     shape = Fp4Shape()
     if cap is not None:
-        if not 0.0 < cap <= 3.0e38:
-            raise ValueError(f"fp4_attend: cap {cap} must be above 0 and finite")
+        if not 1e-30 <= cap <= 1e30:
+            raise ValueError(f"fp4_attend: cap {cap} must be from 1e-30 to 1e30")
         shape.cap = cap
     for name, t, dtype, count in (("slopes", slopes, torch.float32, q_heads), ("sinks", sinks, torch.float32, q_heads),
                                   ("first", first, torch.int64, rows), ("last", last, torch.int64, rows)):

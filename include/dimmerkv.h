@@ -585,7 +585,7 @@ typedef struct dkv_fp4_shape {
   const float* sinks;      /* [q_heads] or null */
   const int64_t* first;    /* [rows] or null */
   const int64_t* last;     /* [rows] or null */
-  float cap;               /* 0: none */
+  float cap;               /* 0: none; else from 1e-30 to 1e30 */
 } dkv_fp4_shape_t;
 
 size_t dkv_fp4_attend_shaped_workspace_bytes(const dkv_fp4_attend_args_t* p, const dkv_fp4_shape_t* shape);
