@@ -151,18 +151,10 @@ DKV_DEVICE void query_pieces(const float* p, bool negate, bf16x8 (&out)[3], bool
   for (int k = 0; k < 3; ++k) __builtin_memcpy(&out[k], words[k], 16);
 }
 
-// The larger of two floats (a NaN loses), without the quieting that the compiler puts before fmaxf.
-DKV_DEVICE float larger(float a, float b) {
-  float c;
-  asm("v_max_f32 %0, %1, %2" : "=v"(c) : "v"(a), "v"(b));
-  return c;
-}
-
-DKV_DEVICE float larger(float a, float b, float c) {
-  float d;
-  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));
-  return d;
-}
+// The largest of three floats, without the quieting that the compiler puts before fmaxf (a NaN wins: its row is NaN anyway).
+// By a builtin and not in assembly: what it reads has just left a matrix instruction, and only the compiler knows how long
+// the vector instructions behind one have to wait.
+DKV_DEVICE float larger(float a, float b, float c) { return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c); }
 
 // cap * tanh(u) for |u| <= 1/2: u times a polynomial in u^2, whose coefficients hold the cap (6e-8 off, relative).
 DKV_DEVICE float small_tanh(float u, const float (&c)[5]) {
@@ -188,12 +180,8 @@ DKV_DEVICE float exponent(uint32_t byte) { return __uint_as_float(byte << 23); }
 typedef const __attribute__((address_space(4))) int32_t* scalar_ints;
 DKV_DEVICE scalar_ints as_scalar(const int32_t* p) { return (scalar_ints)(uintptr_t)p; }
 
-// The largest magnitude of three floats (a NaN loses).
-DKV_DEVICE float larger_size(float a, float b, float c) {
-  float d;
-  asm("v_max3_f32 %0, |%1|, |%2|, |%3|" : "=v"(d) : "v"(a), "v"(b), "v"(c));
-  return d;
-}
+// The largest magnitude of three floats; a NaN loses (it may be a token's that the row does not see).
+DKV_DEVICE float larger_size(float a, float b, float c) { return fmaxf(fmaxf(fabsf(a), fabsf(b)), fabsf(c)); }
 
 // One chunk in this lane, CH tiles of 16 tokens: codes and exponents, and which tiles hold something (the same in every
 // lane).
@@ -569,7 +557,7 @@ __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_at
 #pragma unroll
         for (int t = 0; t < CH; ++t) top = larger(larger(top, s[nt][t][0], s[nt][t][1]), s[nt][t][2], s[nt][t][3]);
         if (__any(top * scale > m[nt] + kSlack)) {
-          const float higher = larger(m[nt], max_xor32(max_xor16(top)) * scale);
+          const float higher = fmaxf(m[nt], max_xor32(max_xor16(top)) * scale);
           const float factor = __builtin_amdgcn_exp2f(m[nt] - (higher == -INFINITY ? 0.0f : higher));
           l[nt] *= factor;
 #pragma unroll

@@ -408,3 +408,33 @@ def test_a_recorded_leaf_is_not_written():
         with pytest.raises(RuntimeError, match="leaf"):
             cache.attend_rows(0, leaf, step, out=place)
     assert torch.equal(leaf, given)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("total,new", [(40, 1), (600, 1), (64, 64), (3000, 20)])
+def test_scores_of_the_last_products(total, new, dim, dtype):
+    """Scores that are large in the last matrix instruction of a tile alone, one tile after the other: read before that has
+    ended they would be 0, and the weights, against a reference of 0, infinite.  All tokens but one score 0 and that one
+    e^60 times their weight, so the result is its value, but for total values of 6 at the most that weigh e^-60 each."""
+    from paged_cache import PagedCache
+
+    cache = PagedCache(1, 1, dim, -(-total // 64) + 1, device=DEV)
+    cache.assign([total - new])
+    step = cache.assign([new])
+    slots = cache.slots(0, 0, total)
+    from paged_cache import Step
+
+    steps = dim // 32
+    dims = [g * (dim // 4) + (steps - 1) * 8 + j for g in range(4) for j in range(8)]  # the last step's
+    value = torch.arange(total, device=DEV).remainder(6).float()[:, None, None].expand(total, 1, dim).contiguous()
+    query = torch.zeros(new, 2, dim, device=DEV, dtype=TYPES[dtype])
+    query[..., dims] = 1.0
+    for at in {0, 3, 17, total // 2, total - new}:
+        key = torch.zeros(total, 1, dim, device=DEV)
+        key[at, 0, dims] = 6.0
+        cache.store(0, key, value, Step(slots, slots, step.cu, total, 1, 1))
+        held = cache.load(0, slots[at:at + 1], torch.float32)[1][0, 0, 0].item()
+        out = cache.attend_rows(0, query, step, scaling=60.0 / (6.0 * len(dims)))
+        seen = step.positions >= at
+        assert (out[seen].float() - held).abs().max() <= 2.0 ** -8 * held + 6 * total * np.exp(-60.0), (at, out[seen].float().max())
