@@ -63,9 +63,27 @@ struct ShapedArgs : AttendArgs {
 };
 constexpr float kLog2e = 1.44269504088896340736f;
 
+struct alignas(16) RowShape {  // of a query row: it sees the tokens behind `before` up to `last`
+  int before, last, position;
+  float slope;  // * -log2 e
+};
+
 DKV_DEVICE void set_result(float& y, float x) { y = x; }
 DKV_DEVICE void set_result(half_t& y, float x) { y = (half_t)x; }
 DKV_DEVICE void set_result(dkv_bf16& y, float x) { y.bits = float_to_bf16_bits(x); }
+
+DKV_DEVICE void store_results(half_t* p, const float (&x)[8]) {
+  half8 y;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] = (half_t)x[i];
+  *(half8*)p = y;
+}
+DKV_DEVICE void store_results(dkv_bf16* p, const float (&x)[8]) {
+  bf16x8 y;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] = (__bf16)x[i];
+  *(bf16x8*)p = y;
+}
 
 template <typename T>
 struct Operand;  // what a query type's products are made of
@@ -180,8 +198,8 @@ DKV_DEVICE float exponent(uint32_t byte) { return __uint_as_float(byte << 23); }
 typedef const __attribute__((address_space(4))) int32_t* scalar_ints;
 DKV_DEVICE scalar_ints as_scalar(const int32_t* p) { return (scalar_ints)(uintptr_t)p; }
 
-// The largest magnitude of three floats; a NaN loses (it may be a token's that the row does not see).
-DKV_DEVICE float larger_size(float a, float b, float c) { return fmaxf(fmaxf(fabsf(a), fabsf(b)), fabsf(c)); }
+// The same of magnitudes.
+DKV_DEVICE float larger_size(float a, float b, float c) { return larger(fabsf(a), fabsf(b), fabsf(c)); }
 
 // One chunk in this lane, CH tiles of 16 tokens: codes and exponents, and which tiles hold something (the same in every
 // lane).
@@ -296,9 +314,9 @@ __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_at
   // (one fills the other's waits): queries lie in LDS, and a chunk's loads follow the last use of the one before.
   constexpr bool kLean = NT == 4;
   __shared__ frag held[kLean ? NT * kSteps * 64 : 1];
-  __shared__ float sums[4 * 16 * kStride];
+  __shared__ float sums[kWaves == 1 ? 1 : (kWaves < 4 ? kWaves : 4) * 16 * kStride];
   __shared__ float stat[2][kWaves][kRows];
-  __shared__ int2 ranges[kShaped ? kWaves : 1][kShaped ? kRows : 1];  // tokens that a row sees, a copy for each wave
+  __shared__ RowShape rows_of[kShaped ? kWaves : 1][kShaped ? kRows : 1];  // a copy for each wave
 
   bool capped = false;
   if constexpr (kShaped) capped = a.cap > 0.0f;
@@ -337,11 +355,8 @@ __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_at
     // the last token a row sees, and the one before the first (made where a chunk has a mask, and not held)
     auto last_seen = [&](int nt) { return first_position + min(row0 + nt * 16 + i, n_rows - 1) / a.groups; };
     auto before_first = [&](int last) { return (int)max((long)last - a.window, -1L); };
-    // (the one before the first token a row sees, the last one)
-    auto seen_by = [&](int nt) {
-      if constexpr (kShaped) {
-        if (a.first || a.last) return ranges[wave][nt * 16 + i];
-      }
+    auto seen_by = [&](int nt) {  // (the one before the first token a row sees, the last one)
+      if constexpr (kShaped) return make_int2(rows_of[wave][nt * 16 + i].before, rows_of[wave][nt * 16 + i].last);
       const int last = last_seen(nt);
       return make_int2(before_first(last), last);
     };
@@ -351,7 +366,7 @@ __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_at
       const int token = r / a.groups;
       const T* p = (const T*)a.query + (q0 + token) * a.query_token + (h * a.groups + r - token * a.groups) * a.query_head;
       if constexpr (kLean) {
-        if (nt == wave) {
+        if (nt % kWaves == wave) {
 #pragma unroll
           for (int s = 0; s < kSteps; ++s) {
             query_pieces(p + g * (D / 4) + s * 8, a.negate, q[0][0]);
@@ -368,31 +383,27 @@ __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_at
     int low_position = first_position + row0 / a.groups, high_position = first_position + (row1 - 1) / a.groups;
     int begin = (int)max((long)low_position - a.window + 1, 0L), end = high_position + 1;  // tokens some row sees
     int all_from = (int)max((long)high_position - a.window + 1, 0L);  // and all rows, from here to low_position
-    int place[kShaped ? NT : 1];     // a row's position and slope
-    float slope[kShaped ? NT : 1];
+    const int least_position = low_position;
     if constexpr (kShaped) {
+      int lowest = INT32_MAX, highest = -1, from = 0, to = INT32_MAX;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const int r = min(row0 + nt * 16 + i, n_rows - 1), token = r / a.groups;
-        place[nt] = first_position + token;
-        slope[nt] = a.slopes ? a.slopes[h * a.groups + (r - token * a.groups)] * -kLog2e : 0.0f;
+        const int r = min(row0 + nt * 16 + i, n_rows - 1), token = r / a.groups, position = first_position + token;
+        const long low = max(a.first ? (long)a.first[q0 + token] : 0L, max((long)position - a.window + 1, 0L));
+        const long high = min(a.last ? (long)a.last[q0 + token] : (long)position, (long)len - 1);
+        // A row that sees nothing has no say in where the block begins and ends, nor in which chunks are masked: what it
+        // gathers in the others is dropped with its sums.
+        const bool some = low <= high;
+        const RowShape row = {some ? (int)low - 1 : INT32_MAX, some ? (int)high : -1, position,
+                              a.slopes ? a.slopes[h * a.groups + (r - token * a.groups)] * -kLog2e : 0.0f};
+        if (g == 0) rows_of[wave][nt * 16 + i] = row;
+        lowest = min(lowest, some ? (int)low : INT32_MAX);
+        highest = max(highest, row.last);
+        from = max(from, some ? (int)low : 0);
+        to = min(to, some ? row.last : INT32_MAX);
       }
+      __builtin_amdgcn_wave_barrier();
       if (a.first || a.last) {
-        int lowest = INT32_MAX, highest = -1, from = 0, to = INT32_MAX;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          const int64_t row = q0 + (place[nt] - first_position);
-          const long low = max(a.first ? (long)a.first[row] : 0L, max((long)place[nt] - a.window + 1, 0L));
-          const long high = min(a.last ? (long)a.last[row] : (long)place[nt], (long)len - 1);
-          const bool some = low <= high;  // (a row that sees nothing has no say in where the block begins and ends)
-          const int2 range = some ? make_int2((int)low - 1, (int)high) : make_int2(INT32_MAX, -1);
-          if (g == 0) ranges[wave][nt * 16 + i] = range;
-          lowest = min(lowest, some ? (int)low : INT32_MAX);
-          highest = max(highest, range.y);
-          from = max(from, some ? (int)low : INT32_MAX);
-          to = min(to, range.y);
-        }
-        __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int x = 1; x < 16; x <<= 1) {
           lowest = min(lowest, __shfl_xor(lowest, x));
@@ -469,6 +480,9 @@ __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_at
       if constexpr (kLean)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) lean[0][nt] = held[(nt * kSteps) * 64 + lane];
+      // (a wave in its products goes first, so that the other one of the SIMD makes its weights meanwhile: 603 -> 586 us for
+      // 2,048 capped query tokens of 24 heads over 16K tokens)
+      if constexpr (kShaped && kLean) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int st = 0; st < kSteps; ++st) {
         if constexpr (kLean) __builtin_amdgcn_sched_barrier(0);
@@ -491,46 +505,79 @@ __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_at
         __builtin_amdgcn_sched_barrier(0);
       }
 
+      if constexpr (kShaped && kLean) __builtin_amdgcn_s_setprio(0);
       const int base = chunk * CH * 16;
+      const bool masked = !tiles.whole || base + CH * 16 > low_position + 1 || base < all_from;
       float scale = a.scale;
-      if constexpr (kShaped) {
-        if (capped) {
-          scale = 1.0f;
+      bool made = false;
+      if constexpr (kShaped) {  // shaped scores in place of the products
+        made = capped || a.slopes;
+        if (made) scale = 1.0f;
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            float size = 0.0f;
-#pragma unroll
-            for (int t = 0; t < CH; ++t) size = larger_size(larger_size(size, s[nt][t][0], s[nt][t][1]), s[nt][t][2], s[nt][t][3]);
-            const bool far = __any(size * a.reach > 0.5f);
+        for (int nt = 0; nt < NT && made; ++nt) {
+          RowShape row;
+          if (masked || a.slopes) row = rows_of[wave][nt * 16 + i];
+          uint32_t hidden = 0;
+          if (masked) {  // (what a row does not see may be anything: nothing is made of it)
 #pragma unroll
             for (int t = 0; t < CH; ++t)
 #pragma unroll
               for (int r = 0; r < 4; ++r) {
-                const float u = s[nt][t][r] * a.reach;
-                float y;
-                if (!far) y = small_tanh(u, a.small);
-                else if (kPieces == 1) y = large_tanh(u, a.cap);
-                else y = fabsf(u) <= 0.5f ? small_tanh(u, a.small) : large_tanh(u, a.cap);
-                s[nt][t][r] = y;
+                const int token = base + t * 16 + g * 4 + r;
+                if (!tiles.valid[t] || token > row.last || token <= row.before) {
+                  hidden |= 1u << (t * 4 + r);
+                  s[nt][t][r] = 0.0f;
+                }
               }
           }
-        }
-        if (a.slopes) {
+          if (capped) {
+            float size = 0.0f;
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            const float ahead = (float)(base + g * 4 - place[nt]);  // (whole numbers where distances are below 2^24)
+            for (int t = 0; t < CH; ++t) size = larger_size(larger_size(size, s[nt][t][0], s[nt][t][1]), s[nt][t][2], s[nt][t][3]);
+            if (!__any(size * a.reach > 0.5f)) {
+#pragma unroll
+              for (int t = 0; t < CH; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[nt][t][r] = small_tanh(s[nt][t][r] * a.reach, a.small);
+            } else {
+#pragma unroll
+              for (int t = 0; t < CH; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                  const float u = s[nt][t][r] * a.reach, y = large_tanh(u, a.cap);
+                  s[nt][t][r] = kPieces == 1 || fabsf(u) > 0.5f ? y : small_tanh(u, a.small);
+                }
+            }
+          }
+          if (a.slopes) {
+            const float ahead = (float)(base + g * 4 - row.position), factor = capped ? 1.0f : a.scale;
+            // Where no token is ahead of a row, distances need no magnitude: a lane's differ by constants.  (Float32 results
+            // take each distance as the whole number that it is, below 2^24.)
+            if (kPieces == 1 && base + CH * 16 <= least_position + 1) {
+              const float bias = -row.slope * ahead;
+#pragma unroll
+              for (int t = 0; t < CH; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[nt][t][r] = fmaf(s[nt][t][r], factor, fmaf(-row.slope, (float)(t * 16 + r), bias));
+            } else {
+#pragma unroll
+              for (int t = 0; t < CH; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[nt][t][r] = fmaf(s[nt][t][r], factor, row.slope * fabsf(ahead + (float)(t * 16 + r)));
+            }
+          }
+          if (masked)
 #pragma unroll
             for (int t = 0; t < CH; ++t)
 #pragma unroll
-              for (int r = 0; r < 4; ++r) s[nt][t][r] = fmaf(s[nt][t][r], scale, slope[nt] * fabsf(ahead + (float)(t * 16 + r)));
-          }
-          scale = 1.0f;
+              for (int r = 0; r < 4; ++r)
+                if (hidden & (1u << (t * 4 + r))) s[nt][t][r] = -INFINITY;
+          if constexpr (kLean) __builtin_amdgcn_sched_barrier(0);
         }
       }
-      const bool masked = !tiles.whole || base + CH * 16 > low_position + 1 || base < all_from;
       if (masked) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
+        for (int nt = 0; nt < NT && !made; ++nt) {
           const int2 seen = seen_by(nt);
 #pragma unroll
           for (int t = 0; t < CH; ++t)
@@ -626,6 +673,7 @@ __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_at
           odd[x] = two[1];
         }
       };
+      if constexpr (kShaped && kLean) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int turn = 0; turn < kTurns; ++turn) {
         if constexpr (kLean) __builtin_amdgcn_sched_barrier(0);
@@ -640,6 +688,7 @@ __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_at
             o[nt][j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, w[nt][u][p], o[nt][j + 1], 0, 0, 0);
           }
       }
+      if constexpr (kShaped && kLean) __builtin_amdgcn_s_setprio(0);
       tiles = next_tiles;
       if constexpr (kLean) {
         load_values<D, CH>(a, tiles, at, values);
@@ -649,10 +698,36 @@ __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_at
       }
     }
 
+    if constexpr (kWaves == 1) {  // nothing to add up: a lane has a quarter of its rows' dimensions
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float total = sum_xor32(sum_xor16(l[nt]));
+        if (rows_of[wave][nt * 16 + i].last < 0) m[nt] = -INFINITY, total = 0.0f;
+        if (m[nt] == -INFINITY && total != 0.0f) m[nt] = 0.0f;
+        const int r = row0 + nt * 16 + i;
+        if (r >= n_rows) continue;
+        const int token = r / a.groups, head = h * a.groups + (r - token * a.groups);
+        const float2 beside = beside_sink(m[nt], total, a.sinks, head, kShift);
+        const float inverse = total == 0.0f ? 0.0f : beside.x / beside.y;
+        T* out = (T*)a.out + ((long)(q0 + token) * q_heads + head) * D + g * (D / 4);
+#pragma unroll
+        for (int d = 0; d < D / 4; d += 8) {
+          float x[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) x[k] = total == 0.0f ? 0.0f : o[nt][(d + k) % kLane][(d + k) / kLane] * inverse;
+          store_results(out + d, x);
+        }
+      }
+      continue;
+    }
+
     // the waves' sums, 16 rows at a time and four waves at a time
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const float total = sum_xor32(sum_xor16(l[nt]));
+      float total = sum_xor32(sum_xor16(l[nt]));
+      if constexpr (kShaped) {
+        if (rows_of[wave][nt * 16 + i].last < 0) m[nt] = -INFINITY, total = 0.0f;
+      }
       // a row whose scores are all NaN has no maximum, but is not one that sees nothing
       if (m[nt] == -INFINITY && total != 0.0f) m[nt] = 0.0f;
       if (g == 0) {
@@ -704,7 +779,7 @@ __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_at
           total += mx == -INFINITY ? 0.0f : stat[1][x][nt * 16 + row] * __builtin_amdgcn_exp2f(mx - highest);
         }
 #pragma unroll
-        for (int x = 0; x < 4; ++x)
+        for (int x = 0; x < (kWaves < 4 ? kWaves : 4); ++x)
 #pragma unroll
           for (int j = 0; j < kPart; ++j) acc[j] += sums[(x * 16 + row) * kStride + part * kPart + j];
         const int token = r / a.groups;
@@ -919,7 +994,7 @@ __global__ __launch_bounds__(256) void fp4_join_few_kernel(Args a, int q_heads) 
 
 struct Plan {
   int tiles;   // 16-row tiles a workgroup takes
-  int waves;   // of a workgroup
+  int waves;   // of a workgroup: 1, 2, 4 or 8
   int blocks;  // row blocks a request is given
   int splits;
   int share;   // 16-token tiles a split takes at the least
@@ -928,7 +1003,7 @@ struct Plan {
 
 constexpr long kWorkgroups = 512;  // of four waves: what the card holds at two waves a SIMD
 
-Plan plan_of(const dkv_fp4_attend_args_t& p) {
+Plan plan_of(const dkv_fp4_attend_args_t& p, const dkv_fp4_shape_t* shape = nullptr) {
   Plan plan;
   const long groups = p.q_heads / p.cache.kv_heads, rows = (long)(p.most < 1 ? 1 : p.most) * groups;
   const bool narrow = p.query_dtype == DKV_F32 || p.cache.head_dim == 256;
@@ -940,7 +1015,7 @@ Plan plan_of(const dkv_fp4_attend_args_t& p) {
   if (p.window) longest = min(longest, (long)p.window + plan.tiles * 16 / groups + 16);
   // Workgroups enough for the card, of 256 tokens at the least; of 1,024 where that makes more than the card holds at
   // once, so that requests of different lengths even out.
-  const long fill = (kWorkgroups + each - 1) / each, even = p.requests > 1 ? (8 * kWorkgroups + each - 1) / each : 1;
+  const long fill = (kWorkgroups + each - 1) / each, even = p.requests > 1 && !(shape && plan.tiles == 4) ? (8 * kWorkgroups + each - 1) / each : 1;
   const long wanted = max(min(fill, (longest + 255) / 256), min(even, (longest + 1023) / 1024));
   // Short requests of few rows are not split: eight waves take them in two turns, four where requests alone fill the card.
   // In a captured graph, 8 KV heads of 128 bfloat16 dimensions: 700 tokens of 32 requests 9.1 us against 13.5 split and
@@ -948,10 +1023,20 @@ Plan plan_of(const dkv_fp4_attend_args_t& p) {
   // 14.1 against 9.0.  Called from Python the second launch costs 3 us more.
   const long brief = p.cache.head_dim < 256 ? 1024 : p.query_dtype == DKV_F32 ? 256 : 512;
   plan.waves = plan.tiles == 1 && longest <= (each >= 256 ? 2 * brief : brief) ? 8 : 4;
-  plan.splits = plan.waves == 8 ? 1 : (int)min(max(wanted, 1L), (long)kMaxSplits);
+  // Many blocks of 64 rows: fewer waves take each, as joining them is what a short range costs most.  With starts of their
+  // own rows see few tokens each (documents), but not the same number, and two waves even out what one would be left with.
+  // 32 query heads of 8 KV heads, by four, two and one waves: 8,192 tokens of 64 float16 dimensions (4,096 blocks) that see
+  // one token 90, 55 and 29 us, 768 at the most 126, 100 and 93, documents of 80 to 2,300 tokens 169, 146 and 188, all
+  // tokens 553, 552 and 542; 2,048 tokens (1,024 blocks) 768 at the most 34, 30 and 36, all 50, 53 and 77; 16,384 tokens of
+  // 128 bfloat16 dimensions (8,192 blocks) 768 at the most 309, 270 and 186, all 2,075, 2,103 and 1,956.
+  if (shape && plan.tiles == 4) {
+    if (each >= 8192 || (longest <= 1024 && !shape->first && each >= 2048)) plan.waves = 1;
+    else if (shape->first && each >= 1024) plan.waves = 2;
+  }
+  plan.splits = plan.waves != 4 ? 1 : (int)min(max(wanted, 1L), (long)kMaxSplits);
   // Blocks of 64 rows that fill the card once and a half leave half of it idle at the end: two or three splits where that
   // makes fuller rounds, by more than the join costs.
-  if (plan.splits == 1 && plan.tiles == 4 && longest >= 4096) {
+  if (plan.splits == 1 && plan.tiles == 4 && plan.waves == 4 && longest >= 4096 && !(shape && shape->first)) {
     const auto rounds = [&](long x) { return (double)((each * x + kWorkgroups - 1) / kWorkgroups) / x; };
     for (int x = 2; x <= 3; ++x)
       if (rounds(x) < 0.85 * rounds(plan.splits)) plan.splits = x;
@@ -1009,7 +1094,13 @@ void launch(const Args& a, const Plan& plan, int q_heads, hipStream_t st) {
   } else if (plan.tiles == 2) {
     if constexpr (D < 256 || sizeof(T) == 2) hipLaunchKernelGGL((fp4_attend_kernel<D, T, 2, 2, 4, Args>), grid, block, 0, st, a);
   } else {
-    if constexpr (wide) hipLaunchKernelGGL((fp4_attend_kernel<D, T, 4, 2, 4, Args>), grid, block, 0, st, a);
+    if constexpr (wide) {
+      if constexpr (__is_same(Args, ShapedArgs)) {
+        if (plan.waves == 1) hipLaunchKernelGGL((fp4_attend_kernel<D, T, 4, 2, 1, Args>), grid, block, 0, st, a);
+        if (plan.waves == 2) hipLaunchKernelGGL((fp4_attend_kernel<D, T, 4, 2, 2, Args>), grid, block, 0, st, a);
+      }
+      if (plan.waves == 4) hipLaunchKernelGGL((fp4_attend_kernel<D, T, 4, 2, 4, Args>), grid, block, 0, st, a);
+    }
   }
   const long rows = (long)a.rows * q_heads;
   if (plan.splits == 1 || a.arrivals) return;
@@ -1092,7 +1183,7 @@ extern "C" int dkv_fp4_attend(const dkv_fp4_attend_args_t* p, void* workspace, s
 extern "C" size_t dkv_fp4_attend_shaped_workspace_bytes(const dkv_fp4_attend_args_t* p, const dkv_fp4_shape_t* shape) {
   const char* what = "dkv_fp4_attend_shaped_workspace_bytes";
   if (check_attend(p, what) || check_shape(shape, what)) return 0;
-  return part_bytes(*p, plan_of(*p)) + 16;
+  return part_bytes(*p, plan_of(*p, shape)) + 16;
 }
 
 extern "C" int dkv_fp4_attend_shaped(const dkv_fp4_attend_args_t* p, const dkv_fp4_shape_t* shape, void* workspace,
@@ -1102,7 +1193,7 @@ extern "C" int dkv_fp4_attend_shaped(const dkv_fp4_attend_args_t* p, const dkv_f
   if (!rc) rc = check_shape(shape, what);
   if (rc) return rc;
   if (p->rows == 0) return DKV_OK;
-  const Plan plan = plan_of(*p);
+  const Plan plan = plan_of(*p, shape);
   ShapedArgs a{};
   rc = attend_args(p, plan, workspace, workspace_bytes, a, what);
   if (rc) return rc;

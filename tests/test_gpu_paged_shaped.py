@@ -43,8 +43,8 @@ def formula(q, k, v, scaling, position, low, high, cap, slope, sink):
 
 
 def compare(cache, step, query, got, scaling=None, window=None, cap=None, slopes=None, sinks=None, first=None, last=None,
-            layer=0, heads=None):
-    """Every row and head (or the query heads given) against the formula, with the bound above."""
+            layer=0, heads=None, some=None):
+    """Every row and head (or the query heads, and the rows of a request, given) against the formula, with the bound above."""
     lengths, cu, dtype, dim = cache.lengths.tolist(), step.cu.tolist(), query.dtype, cache.head_dim
     scaling = dim ** -0.5 if scaling is None else scaling
     slopes, sinks, first, last = (None if t is None else t.double().cpu().numpy() if t.is_floating_point() else t.tolist()
@@ -56,7 +56,7 @@ def compare(cache, step, query, got, scaling=None, window=None, cap=None, slopes
             continue
         keys, values = (t.double().cpu().numpy() for t in cache.load(layer, cache.slots(b, 0, total), torch.float32))
         q, have = (t[lo:hi].double().cpu().numpy() for t in (query, got))
-        for i in range(hi - lo):
+        for i in range(hi - lo) if some is None else sorted({min(x, hi - lo - 1) for x in some}):
             position = total - (hi - lo) + i
             low = 0 if first is None else max(first[lo + i], 0)
             low = low if window is None else max(low, position - window + 1)
@@ -99,7 +99,7 @@ def shape_of(kind, rows, heads, step, lengths):
     return made
 
 
-def run(kind, lengths, new, heads=2, groups=3, dim=64, page=16, dtype="bf16", seed=0, reach=3.0, only=None, scaling=None):
+def run(kind, lengths, new, heads=2, groups=3, dim=64, page=16, dtype="bf16", seed=0, reach=3.0, only=None, some=None, scaling=None):
     print(f"[case] shaped {kind} {lengths} + {new} heads={heads}x{groups} dim={dim} page={page} {dtype}", flush=True)
     cache, step = build(lengths, new, heads, dim, page, seed)
     g = torch.Generator(DEV).manual_seed(seed + 1)
@@ -107,7 +107,7 @@ def run(kind, lengths, new, heads=2, groups=3, dim=64, page=16, dtype="bf16", se
     made = shape_of(kind, step.rows, heads * groups, step, lengths)
     got = cache.attend_rows(0, query, step, scaling=scaling, **made)
     assert got.shape == query.shape and got.dtype == query.dtype
-    compare(cache, step, query, got, scaling=scaling, heads=only, **made)
+    compare(cache, step, query, got, scaling=scaling, heads=only, some=some, **made)
     return cache, step, query, made, got
 
 
@@ -144,6 +144,33 @@ def test_long(kind, dim, dtype):
     run(kind, [20000], [2], heads=2, groups=2, dim=dim, page=64, dtype=dtype)
     run(kind, [3000, 5, 2000], [3, 1, 2], heads=1, groups=2, dim=dim, page=64, dtype=dtype)
     run(kind, [5000], [200], heads=8, groups=4, dim=dim, page=64, dtype=dtype, only=[0, 13, 31])
+
+
+@pytest.mark.parametrize("kind,heads,new", [("documents+sinks", 8, [2200]), ("documents+cap6+slopes", 8, [2100, 0, 300]),
+                                            ("cap9+window500", 8, [4200]), ("slopes+window64+sinks", 8, [4100, 40]),
+                                            ("cap12+sinks", 16, [8210]), ("slopes+prefix700", 16, [8210]), ("documents", 16, [8210])])
+@pytest.mark.parametrize("dim,dtype", [(64, "f16"), (128, "bf16"), (64, "bf16"), (128, "f16")])
+def test_many_blocks(kind, heads, new, dim, dtype):
+    """Prompts of so many blocks of 64 rows that two waves, or one, take each: rows around blocks, tiles and the ends."""
+    run(kind, [0] * len(new), new, heads=heads, groups=4, dim=dim, page=64, dtype=dtype, only=[0, 5, 4 * heads - 1],
+        some=[0, 1, 15, 16, 17, 39, 500, 699, 700, 701, 1039, 2079, 2199, new[0] // 2, new[0] - 17, new[0] - 1])
+
+
+@pytest.mark.parametrize("kind", ["documents+sinks", "window300+cap7"])
+def test_many_blocks_against_few(kind):
+    """Every row of a launch of one or two waves a block against the same rows in a launch of four, to what two roundings of
+    the results and the orders of sums may differ (twice 2^-8, and 2^-9 for weights of one float16)."""
+    cache, step = build([0], [4200], 8, 64, 64)
+    query = torch.randn(step.rows, 32, 64, generator=torch.Generator(DEV).manual_seed(5), device=DEV).bfloat16()
+    made = shape_of(kind, step.rows, 32, step, [0])
+    want = cache.attend_rows(0, query, step, **made)
+    from paged_cache import Step
+
+    other = Step(step.slots, step.positions, step.cu, step.rows, step.longest, 100)  # a bound on rows that shapes fewer blocks
+    got = cache.attend_rows(0, query, other, **made)
+    assert torch.equal(want.any(-1), got.any(-1))  # rows that see nothing
+    size = cache.load(0, step.slots, torch.float32)[1].abs().max().item()
+    assert (got.float() - want.float()).abs().max().item() <= (2.0 ** -7 + 2.0 ** -9) * size
 
 
 @pytest.mark.parametrize("cap", [1e-3, 0.4, 3.0, 1e4, 1e9])
