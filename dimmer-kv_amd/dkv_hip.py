@@ -803,60 +803,72 @@ def fp4_append(cache: Fp4Cache, query, key, value, slots, positions, cos, sin, i
     cos and sin float32 [table rows, rotary / 2] -> query [n, q_heads, head_dim] rotated (None for None): into ``out``, the
     query itself or contiguous memory apart from all rows, whose rows of negative positions are left as they are; a new
     one, with zeros there, if it is None.  There is no backward pass: a recorded call's gradient raises."""
-    index, n, dtype = slots.get_device(), slots.shape[0], key.dtype
-    shape, code = (n, cache.kv_heads, cache.head_dim), dtype_code(dtype)
+    index, n, dtype, dim = slots.get_device(), slots.shape[0], key.dtype, cache.head_dim
+    shape, code = (n, cache.kv_heads, dim), dtype_code(dtype)
     if not (index >= 0 and _like(slots, (n,), torch.int64, index) and _like(positions, (n,), torch.int64, index)
             and key.shape == shape and value.shape == shape and value.dtype == dtype and key.get_device() == index
             and value.get_device() == index):
         _expect("fp4_append", slots.device, (slots, "slots", torch.int64, (n,)), (positions, "positions", torch.int64, (n,)),
                 (key, "key", dtype, shape), (value, "value", dtype, shape))
         ptr(slots), ptr(positions)
-    for t, name in ((cos, "cos"), (sin, "sin")):
-        if (t.dtype != torch.float32 or t.dim() != 2 or t.shape != cos.shape or t.get_device() != index or t.stride(1) != 1
-                or t.stride(0) % 4 or t.data_ptr() % 16 or not 0 < t.shape[0] < 1 << 31):
-            raise ValueError(f"fp4_append: {name} must be float32 [positions, rotary / 2] on the cache's GPU, rows 16-byte "
-                             f"aligned (got {t.dtype} {list(t.shape)}, strides {list(t.stride())}, on {t.device})")
-    if 2 * cos.shape[1] > cache.head_dim or cos.shape[1] % 8 or cos.shape[1] == 0:
-        raise ValueError(f"fp4_append: {2 * cos.shape[1]} rotated dimensions of {cache.head_dim} (a multiple of 16)")
+    table_rows, pairs, cos_at, cos_row = _angles("cos", cos, index)
+    sin_rows, sin_pairs, sin_at, sin_row = _angles("sin", sin, index)
+    if sin_rows != table_rows or sin_pairs != pairs:
+        raise ValueError(f"fp4_append: sin must be as cos is, {list(cos.shape)} (got {list(sin.shape)})")
+    if 2 * pairs > dim or pairs % 8 or pairs == 0:
+        raise ValueError(f"fp4_append: {2 * pairs} rotated dimensions of {dim} (a multiple of 16)")
     if n >= 1 << 31:
         raise ValueError(f"fp4_append: {n} rows")
-    args = Fp4AppendArgs()
-    given = query
-    if query is None:
-        if out is not None:
-            raise ValueError("fp4_append: out without queries")
-    else:
-        wide = (n, query.shape[1] if query.dim() == 3 else -1, cache.head_dim)
+    given, fill, q_heads = query, out is None, 0
+    if query is not None:
+        q_heads = query.shape[1] if query.dim() == 3 else -1
+        wide = (n, q_heads, dim)
         if query.shape != wide or query.dtype != dtype or query.get_device() != index:
             _expect("fp4_append", slots.device, (query, "query", dtype, wide))
-        args.fill = out is None
-        if out is None:
+        if fill:
             out = torch.empty(wide, dtype=dtype, device=query.device)
         elif out.shape != wide or out.dtype != dtype or out.get_device() != index:
             _expect("fp4_append", slots.device, (out, "out", dtype, wide))
+    elif not fill:
+        raise ValueError("fp4_append: out without queries")
     if n == 0:
         return out
-    key, args.key, args.key_token, args.key_head = _strided_rows(key)
-    value, args.value, args.value_token, args.value_head = _strided_rows(value)
-    if query is not None and query.shape[1]:
-        query, args.query, args.query_token, args.query_head = _strided_rows(query)
-        if not args.fill:
-            in_place = out.data_ptr() == args.query and out.stride() == query.stride()
-            if not in_place and (not out.is_contiguous() or out.data_ptr() % 16):
-                raise ValueError("fp4_append: out must be the query (rows 16-byte aligned), or contiguous and 16-byte aligned")
-            if (_rows_lie_over(out) or any(_rows_meet_rows(out, t) for t in (key, value))
-                    or (not in_place and _query_meets(query, args, out))):
-                raise ValueError("fp4_append: out lies over other rows of the queries, or over keys or values")
-        args.out, args.out_token, args.out_head = out.data_ptr(), out.stride(0), out.stride(1)
-        args.q_heads = query.shape[1]
+    key, key_at, key_row, key_head = _strided_rows(key)
+    value, value_at, value_row, value_head = _strided_rows(value)
+    query_at = query_row = query_head = out_at = out_row = out_head = 0
+    if q_heads:
+        query, query_at, query_row, query_head = _strided_rows(query)
+        out_at, out_row, out_head = out.data_ptr(), q_heads * dim, dim
+        if not fill:
+            out_row, out_head, _ = out.stride()
+            _check_append_place(out, query, query_at, key, value)
         out = _recorded("fp4_append", out, given, cos, sin)
-    args.cache, args.slots, args.positions = cache, slots.data_ptr(), positions.data_ptr()
-    args.cos, args.sin, args.cos_row, args.sin_row = cos.data_ptr(), sin.data_ptr(), cos.stride(0), sin.stride(0)
-    args.table_rows, args.rotary = cos.shape[0], 2 * cos.shape[1]
-    args.interleaved, args.dtype, args.rows = bool(interleaved), code, n
+    args = Fp4AppendArgs(cache, query_at, key_at, value_at, out_at, query_row, query_head, key_row, key_head, value_row, value_head,
+                         out_row, out_head, slots.data_ptr(), positions.data_ptr(), cos_at, sin_at, cos_row, sin_row, table_rows,
+                         2 * pairs, bool(interleaved), code, n, q_heads, fill)
     with _on_gpu(index):
         _check(lib().dkv_fp4_append(ctypes.addressof(args), stream_handle()), "dkv_fp4_append")
     return out
+
+
+def _angles(name: str, t, index: int):
+    """(rows, pairs, address, row stride) of a table of cosines or sines."""
+    shape, stride, at = t.shape, t.stride(), t.data_ptr()
+    if (t.dtype != torch.float32 or len(shape) != 2 or t.get_device() != index or stride[1] != 1 or stride[0] % 4 or at % 16
+            or not 0 < shape[0] < 1 << 31):
+        raise ValueError(f"fp4_append: {name} must be float32 [positions, rotary / 2] on the cache's GPU, rows 16-byte "
+                         f"aligned (got {t.dtype} {list(shape)}, strides {list(stride)}, on {t.device})")
+    return shape[0], shape[1], at, stride[0]
+
+
+def _check_append_place(out, query, query_at: int, key, value) -> None:
+    """Refuse a place for rotated queries that the launch would read elsewhere."""
+    in_place = out.data_ptr() == query_at and out.stride() == query.stride()
+    if not in_place and (not out.is_contiguous() or out.data_ptr() % 16):
+        raise ValueError("fp4_append: out must be the query (rows 16-byte aligned), or contiguous and 16-byte aligned")
+    if (_rows_lie_over(out) or _rows_meet_rows(out, key) or _rows_meet_rows(out, value)
+            or (not in_place and _rows_meet_rows(out, query))):
+        raise ValueError("fp4_append: out lies over other rows of the queries, or over keys or values")
 
 
 def _rows_lie_over(t) -> bool:
