@@ -51,6 +51,9 @@ def dimmer_attention(module, query, key, value, attention_mask, scaling, dropout
     # query head h reads KV head h // groups; the key operand is made contiguous before the product
     keys_t = key.repeat_interleave(groups, dim=1).transpose(-1, -2).contiguous()
     logits = torch.matmul(query, keys_t).mul_(scaling)
+    cap, sinks = kwargs.get("softcap"), kwargs.get("s_aux")  # of models that have them
+    if cap is not None:
+        logits = torch.tanh(logits / cap) * cap
     if attention_mask is not None:
         logits = logits + attention_mask
     evicted = STATE.evicted.get(module.layer_idx)
@@ -58,7 +61,11 @@ def dimmer_attention(module, query, key, value, attention_mask, scaling, dropout
         # tokens appended after the context (the question, the reply) are never hidden
         hidden = F.pad(evicted.repeat_interleave(groups, dim=0), (0, logits.shape[-1] - evicted.shape[1]))
         logits = logits.masked_fill(hidden[None, :, None, :], torch.finfo(logits.dtype).min)
+    if sinks is not None:
+        logits = torch.cat([logits, sinks.to(logits.dtype).view(1, -1, 1, 1).expand(*logits.shape[:3], 1)], dim=-1)
     probs = torch.softmax(logits, dim=-1, dtype=torch.float32)
+    if sinks is not None:
+        probs = probs[..., :-1]
     if STATE.scoring:
         layer = module.layer_idx
         received = _per_kv_head(probs[0].sum(dim=1), groups)

@@ -184,7 +184,7 @@ class Methods:
             raise ValueError("fp4 needs Methods(..., model=model) for the model's cache configuration.")
         from paged_cache import PagedContext
 
-        stored, seconds = self._timed(lambda: PagedContext(keys, values, self._model))
+        stored, seconds = self._timed(lambda: PagedContext(keys, values, self._model, shaped=True))
         tokens, dtype = keys[0].shape[2], keys[0].dtype
         per_token = torch.full((tokens,), float(stored.token_bytes()), device=self.device)
         return Compressed(None, None, None, tokens * stored.token_bytes(), seconds, token_bytes=per_token, stored=stored,

@@ -13,6 +13,9 @@ the GPU or reads from it, so a step can be captured in a HIP graph.  A step of a
     out = cache.attend_rows(layer, query, step)       # and the queries over all of them
     cache.trim(keep)                                  # finished requests, refused drafts
 
+``append`` in the place of ``store`` takes raw projections and rotates keys and queries to their positions on the way, and
+``attend_rows`` takes scores that are capped, biased by distance, joined by sinks or masked by ranges of tokens.
+
 Calls on one cache share its tables and belong on one stream (or on streams the caller orders).
 
 ``PagedContext`` is the cache of one conversation behind a Hugging Face model: an attention context like
@@ -227,12 +230,14 @@ class PagedContext:
     ``compressed_attention.CompressedContext`` for the ``dimmer`` hook.  Every forward's new keys and values are stored
     before they are attended to, in 4 bits as all others, so ``exact_cache`` (the cache the model updates) only carries
     them here: it starts empty.  Attention is causal, over all tokens or a layer's sliding window as the model's
-    configuration has it; the model's additive mask is not read.  Models whose attention is more than that (a soft cap on
-    scores, sinks beside the keys, other kinds of layers) are refused."""
+    configuration has it; the model's additive mask is not read.  Models whose attention is more than that are refused (other
+    kinds of layers), or taken with ``shaped`` (a soft cap on scores, sinks beside the keys)."""
 
-    def __init__(self, keys: list[torch.Tensor], values: list[torch.Tensor], model, page: int = 64, room: int = 1024):
+    def __init__(self, keys: list[torch.Tensor], values: list[torch.Tensor], model, page: int = 64, room: int = 1024,
+                 shaped: bool = False):
         """Per-layer [1, kv_heads, tokens, head_dim] keys (RoPE applied) and values on the GPU, with room for ``room`` more
-        tokens."""
+        tokens.  ``shaped``: attention takes the soft cap of the model's configuration and its layers' sinks as they are now;
+        without it a model that has either is refused."""
         first = keys[0]
         shape = first.shape
         if len(keys) != len(values) or len(shape) != 4 or shape[0] != 1:
@@ -241,7 +246,8 @@ class PagedContext:
         if room < 0:
             raise ValueError(f"PagedContext: room {room}")
         self._windows = self._layer_windows(model.config, len(keys))
-        self._refuse_more_than_scores(model)
+        if not shaped:
+            self._refuse_more_than_scores(model)
         _, heads, tokens, dim = shape
         pages = max(1, -(-(tokens + room) // page))
         self.cache = PagedCache(len(keys), heads, dim, pages, page=page, device=first.device)
@@ -252,6 +258,7 @@ class PagedContext:
             if key.shape != shape or value.shape != shape:
                 raise ValueError(f"layer {layer}: keys {list(key.shape)} and values {list(value.shape)}, not {list(shape)}")
             self.cache.store(layer, key[0].transpose(0, 1), value[0].transpose(0, 1), step)
+        self._shapes = self._layer_shapes(model, len(keys), first.device)
         self._step, self._next = None, 0  # of the forward that runs: its rows, and the layer it is at
         self.exact_cache = self.fresh_cache()
 
@@ -273,6 +280,16 @@ class PagedContext:
             raise ValueError("PagedContext: the model's attention has a soft cap on its scores")
         if any(getattr(module, "sinks", None) is not None for module in getattr(model, "modules", tuple)()):
             raise ValueError("PagedContext: the model's attention has sinks beside its keys")
+
+    @staticmethod
+    def _layer_shapes(model, layers: int, device) -> list[dict]:
+        """What ``attend_rows`` takes for the shapes of each layer's scores."""
+        cap = getattr(model.config.get_text_config(decoder=True), "attn_logit_softcapping", None)
+        shapes = [{} if not cap else {"cap": cap} for _ in range(layers)]
+        for module in getattr(model, "modules", tuple)():
+            if getattr(module, "sinks", None) is not None and 0 <= getattr(module, "layer_idx", -1) < layers:
+                shapes[module.layer_idx]["sinks"] = module.sinks.detach().to(device, torch.float32).contiguous()
+        return shapes
 
     def fresh_cache(self):
         """An empty cache for the model to update: one for every answer."""
@@ -324,7 +341,8 @@ class PagedContext:
             self.tokens += new
         past = key.shape[2] - new
         c.store(layer, key[0, :, past:].transpose(0, 1), value[0, :, past:].transpose(0, 1), self._step)
-        out = c.attend_rows(layer, query[0].transpose(0, 1), self._step, scaling=scaling, window=self._windows[layer])
+        out = c.attend_rows(layer, query[0].transpose(0, 1), self._step, scaling=scaling, window=self._windows[layer],
+                            **self._shapes[layer])
         self._next = layer + 1
         if self._next == c.layers:
             self._step, self._next = None, 0

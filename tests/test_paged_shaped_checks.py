@@ -169,3 +169,61 @@ def test_oracle_shaped_scores():
     some = paged_ref.attend_shaped(query, keys, values, 0.0, first=[2, 5, -4], last=[4, 4, 100])
     assert np.allclose(some[0], values[2:5].mean(0)[[0, 0, 1, 1]]) and not some[1].any()
     assert np.allclose(some[2], values.mean(0)[[0, 0, 1, 1]])
+
+
+def small_model(family, layers=2, window=None, seed=0):
+    """A random model whose scores are capped (Gemma2), or joined by sinks (GptOss), with its sliding layers as they are."""
+    import transformers
+
+    torch.manual_seed(seed)
+    sizes = dict(num_hidden_layers=layers, hidden_size=64, intermediate_size=64, num_attention_heads=4, num_key_value_heads=2,
+                 head_dim=64, vocab_size=50, pad_token_id=0)
+    if window:
+        sizes |= dict(sliding_window=window)
+    if family == "GptOss":
+        sizes |= dict(num_local_experts=2, num_experts_per_tok=1)
+    else:
+        sizes |= dict(attn_logit_softcapping=3.0, query_pre_attn_scalar=16)
+    model = getattr(transformers, f"{family}ForCausalLM")(getattr(transformers, f"{family}Config")(**sizes)).float().eval()
+    with torch.no_grad():  # scores that reach the cap, and sinks that take their part
+        for layer in model.model.layers:
+            for projection in (layer.self_attn.q_proj, layer.self_attn.k_proj):
+                projection.weight.mul_(8.0)
+            if family == "GptOss":
+                layer.self_attn.sinks.normal_(1.0, 2.0)
+    return model
+
+
+@pytest.mark.parametrize("family", ["Gemma2", "GptOss"])
+def test_the_hook_keeps_caps_and_sinks(family):
+    """The hook's own attention is the model's."""
+    import dimmer
+
+    model = small_model(family, window=16)
+    ids = torch.randint(0, 50, (1, 40), generator=torch.Generator().manual_seed(1))
+    model.set_attn_implementation("eager")
+    with torch.no_grad():
+        want = model(input_ids=ids).logits
+    dimmer.install(model)
+    with torch.no_grad():
+        got = model(input_ids=ids).logits
+    assert torch.allclose(got, want, atol=1e-5, rtol=1e-5), float((got - want).abs().max())
+
+
+@pytest.mark.parametrize("family", ["Gemma2", "GptOss"])
+def test_contexts_of_shaped_scores(family):
+    """Such a model is taken with ``shaped`` (as far as the GPU that this test does without), each layer with its own shape."""
+    from paged_cache import PagedContext
+
+    model = small_model(family)
+    caches = [torch.zeros(1, 2, 5, 64) for _ in range(2)]
+    with pytest.raises(ValueError, match="soft cap|sinks"):
+        PagedContext(caches, caches, model)
+    with pytest.raises(ValueError, match="needs a GPU"):
+        PagedContext(caches, caches, model, shaped=True)
+    shapes = PagedContext._layer_shapes(model, 2, "cpu")
+    if family == "Gemma2":
+        assert shapes == [{"cap": 3.0}] * 2
+    else:
+        for shape, layer in zip(shapes, model.model.layers):
+            assert list(shape) == ["sinks"] and torch.equal(shape["sinks"], layer.self_attn.sinks) and not shape["sinks"].requires_grad
