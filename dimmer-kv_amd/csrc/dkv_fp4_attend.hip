@@ -59,8 +59,15 @@ struct ShapedArgs : AttendArgs {
   const int64_t* last;   // [rows]
   float reach;           // |scaling| / cap: what a product is of the cap
   float cap;             // cap * log2 e, or 0
+  float steep;           // 2 log2 e * reach where every capped score is made as 2 cap * (-1 / (1 + e^2u)) + cap, else 0
+  float factor, lift;    // a made score times `factor` plus `lift` is the score where slopes are taken off it,
+  float offset;          // and times `scale` plus `offset` where its weight is made
   float small[5];        // cap times the coefficients of tanh(u) / u in u^2
 };
+// Kernels of their own for a cap and for slopes (with a cap or without): what the others do not need costs them registers,
+// and a branch in the chunks' loop as much as some ten instructions.
+struct CappedArgs : ShapedArgs {};
+struct BiasedArgs : ShapedArgs {};
 constexpr float kLog2e = 1.44269504088896340736f;
 
 struct alignas(16) RowShape {  // of a query row: it sees the tokens behind `before` up to `last`
@@ -300,7 +307,7 @@ constexpr float kShiftOf = 15.0f - kSlackOf<T>;
 
 template <int D, typename T, int NT, int CH, int kWaves, typename Args>
 __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_attend_kernel(Args a) {
-  constexpr bool kShaped = __is_same(Args, ShapedArgs);
+  constexpr bool kShaped = !__is_same(Args, AttendArgs), kSlopes = __is_same(Args, BiasedArgs), kMade = kSlopes || __is_same(Args, CappedArgs);
   using Op = Operand<T>;
   using frag = typename Op::frag;
   constexpr int kRows = 16 * NT, kSteps = D / 32, kLane = D / 16, kPieces = Op::kPieces;
@@ -318,8 +325,8 @@ __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_at
   __shared__ float stat[2][kWaves][kRows];
   __shared__ RowShape rows_of[kShaped ? kWaves : 1][kShaped ? kRows : 1];  // a copy for each wave
 
-  bool capped = false;
-  if constexpr (kShaped) capped = a.cap > 0.0f;
+  bool capped = kMade && !kSlopes;
+  if constexpr (kSlopes) capped = a.cap > 0.0f;
   const int h = blockIdx.x, b = blockIdx.z, split = blockIdx.y % a.splits, blocks = gridDim.y / a.splits;
   __shared__ int last;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
@@ -370,13 +377,13 @@ __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_at
 #pragma unroll
           for (int s = 0; s < kSteps; ++s) {
             query_pieces(p + g * (D / 4) + s * 8, a.negate, q[0][0]);
-            if (!kShaped || !capped) quiet(q[0][0]);
+            if (!capped) quiet(q[0][0]);
             held[(nt * kSteps + s) * 64 + lane] = q[0][0][0];
           }
         }
       } else {
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) query_pieces(p + g * (D / 4) + s * 8, a.negate, q[nt][s], kShaped && capped);
+        for (int s = 0; s < kSteps; ++s) query_pieces(p + g * (D / 4) + s * 8, a.negate, q[nt][s], capped);
       }
     }
     if constexpr (kLean) __syncthreads();
@@ -395,7 +402,7 @@ __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_at
         // gathers in the others is dropped with its sums.
         const bool some = low <= high;
         const RowShape row = {some ? (int)low - 1 : INT32_MAX, some ? (int)high : -1, position,
-                              a.slopes ? a.slopes[h * a.groups + (r - token * a.groups)] * -kLog2e : 0.0f};
+                              kSlopes ? a.slopes[h * a.groups + (r - token * a.groups)] * -kLog2e : 0.0f};
         if (g == 0) rows_of[wave][nt * 16 + i] = row;
         lowest = min(lowest, some ? (int)low : INT32_MAX);
         highest = max(highest, row.last);
@@ -446,7 +453,7 @@ __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_at
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int s = 0; s < kSteps; ++s)
-          if (!kShaped || !capped) quiet(q[nt][s]);
+          if (!capped) quiet(q[nt][s]);
     }
     for (; chunk < c1; chunk += kWaves) {
       const int later = load_entries<CH>(a, table, chunk + 2 * kWaves < c1 ? len : 0, chunk + 2 * kWaves);
@@ -508,76 +515,136 @@ __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_at
       if constexpr (kShaped && kLean) __builtin_amdgcn_s_setprio(0);
       const int base = chunk * CH * 16;
       const bool masked = !tiles.whole || base + CH * 16 > low_position + 1 || base < all_from;
-      float scale = a.scale;
-      bool made = false;
-      if constexpr (kShaped) {  // shaped scores in place of the products
-        made = capped || a.slopes;
-        if (made) scale = 1.0f;
+      const float scale = a.scale;
+      if constexpr (kMade) {  // shaped scores in place of the products
+        // Those of a chunk that is all seen, where all is made by one rule, without a branch.  (Paths that a type does not take
+        // are left out: the loop is as fast as its code is short, 525 us for the capped question and 588 with another path.)
+        const bool behind = kPieces == 1 && base + CH * 16 <= least_position + 1;  // no token is ahead of a row
+        constexpr bool kSteep = __is_same(T, dkv_bf16);
+        if (!kSlopes && kSteep && !masked && a.steep > 0.0f) {
 #pragma unroll
-        for (int nt = 0; nt < NT && made; ++nt) {
-          RowShape row;
-          if (masked || a.slopes) row = rows_of[wave][nt * 16 + i];
-          uint32_t hidden = 0;
-          if (masked) {  // (what a row does not see may be anything: nothing is made of it)
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int t = 0; t < CH; ++t)
 #pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                const int token = base + t * 16 + g * 4 + r;
-                if (!tiles.valid[t] || token > row.last || token <= row.before) {
-                  hidden |= 1u << (t * 4 + r);
-                  s[nt][t][r] = 0.0f;
-                }
-              }
-          }
-          if (capped) {
+              for (int r = 0; r < 4; ++r) s[nt][t][r] = __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(s[nt][t][r] * a.steep));
+        } else if (!kSlopes && !kSteep && !masked && kPieces == 1) {
+          bool far = false;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
             float size = 0.0f;
 #pragma unroll
             for (int t = 0; t < CH; ++t) size = larger_size(larger_size(size, s[nt][t][0], s[nt][t][1]), s[nt][t][2], s[nt][t][3]);
-            if (!__any(size * a.reach > 0.5f)) {
+            far = far || size * a.reach > 0.5f;
+          }
+          if (__any(far)) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int t = 0; t < CH; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[nt][t][r] = large_tanh(s[nt][t][r] * a.reach, a.cap);
+          } else {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
               for (int t = 0; t < CH; ++t)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) s[nt][t][r] = small_tanh(s[nt][t][r] * a.reach, a.small);
-            } else {
+          }
+        } else if (kSlopes && !masked && !behind && !capped) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const RowShape row = rows_of[wave][nt * 16 + i];
+            const float ahead = (float)(base + g * 4 - row.position);
+#pragma unroll
+            for (int t = 0; t < CH; ++t)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) s[nt][t][r] = fmaf(s[nt][t][r], a.factor, row.slope * fabsf(ahead + (float)(t * 16 + r)));
+          }
+        } else if (kSlopes && !masked && !capped) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const RowShape row = rows_of[wave][nt * 16 + i];
+            const float bias = -row.slope * (float)(base + g * 4 - row.position);
+#pragma unroll
+            for (int t = 0; t < CH; ++t)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) s[nt][t][r] = fmaf(s[nt][t][r], a.factor, fmaf(-row.slope, (float)(t * 16 + r), bias));
+          }
+        } else {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            RowShape row;
+            if (masked || kSlopes) row = rows_of[wave][nt * 16 + i];
+            uint32_t hidden = 0;
+            if (masked) {  // (what a row does not see may be anything: nothing is made of it)
 #pragma unroll
               for (int t = 0; t < CH; ++t)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                  const float u = s[nt][t][r] * a.reach, y = large_tanh(u, a.cap);
-                  s[nt][t][r] = kPieces == 1 || fabsf(u) > 0.5f ? y : small_tanh(u, a.small);
+                  const int token = base + t * 16 + g * 4 + r;
+                  if (!tiles.valid[t] || token > row.last || token <= row.before) {
+                    hidden |= 1u << (t * 4 + r);
+                    s[nt][t][r] = 0.0f;
+                  }
                 }
             }
-          }
-          if (a.slopes) {
-            const float ahead = (float)(base + g * 4 - row.position), factor = capped ? 1.0f : a.scale;
-            // Where no token is ahead of a row, distances need no magnitude: a lane's differ by constants.  (Float32 results
-            // take each distance as the whole number that it is, below 2^24.)
-            if (kPieces == 1 && base + CH * 16 <= least_position + 1) {
-              const float bias = -row.slope * ahead;
+            if (kSteep && a.steep > 0.0f) {
 #pragma unroll
               for (int t = 0; t < CH; ++t)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) s[nt][t][r] = fmaf(s[nt][t][r], factor, fmaf(-row.slope, (float)(t * 16 + r), bias));
-            } else {
+                for (int r = 0; r < 4; ++r) s[nt][t][r] = __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(s[nt][t][r] * a.steep));
+            } else if (capped) {
+              float size = 0.0f;
 #pragma unroll
-              for (int t = 0; t < CH; ++t)
+              for (int t = 0; t < CH; ++t) size = larger_size(larger_size(size, s[nt][t][0], s[nt][t][1]), s[nt][t][2], s[nt][t][3]);
+              if (!__any(size * a.reach > 0.5f)) {
 #pragma unroll
-                for (int r = 0; r < 4; ++r) s[nt][t][r] = fmaf(s[nt][t][r], factor, row.slope * fabsf(ahead + (float)(t * 16 + r)));
+                for (int t = 0; t < CH; ++t)
+#pragma unroll
+                  for (int r = 0; r < 4; ++r) s[nt][t][r] = small_tanh(s[nt][t][r] * a.reach, a.small);
+              } else {
+#pragma unroll
+                for (int t = 0; t < CH; ++t)
+#pragma unroll
+                  for (int r = 0; r < 4; ++r) {
+                    const float u = s[nt][t][r] * a.reach, y = large_tanh(u, a.cap);
+                    s[nt][t][r] = kPieces == 1 || fabsf(u) > 0.5f ? y : small_tanh(u, a.small);
+                  }
+              }
             }
+            if constexpr (kSlopes) {
+              const float ahead = (float)(base + g * 4 - row.position);
+              // Where no token is ahead of a row, distances need no magnitude: a lane's differ by constants.  (Float32 results
+              // take each distance as the whole number that it is, below 2^24.)
+              if (behind) {
+                const float bias = fmaf(-row.slope, ahead, a.lift);
+#pragma unroll
+                for (int t = 0; t < CH; ++t)
+#pragma unroll
+                  for (int r = 0; r < 4; ++r) s[nt][t][r] = fmaf(s[nt][t][r], a.factor, fmaf(-row.slope, (float)(t * 16 + r), bias));
+              } else {
+#pragma unroll
+                for (int t = 0; t < CH; ++t)
+#pragma unroll
+                  for (int r = 0; r < 4; ++r)
+                    s[nt][t][r] = fmaf(s[nt][t][r], a.factor, fmaf(row.slope, fabsf(ahead + (float)(t * 16 + r)), a.lift));
+              }
+            }
+            if (masked)
+#pragma unroll
+              for (int t = 0; t < CH; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                  if (hidden & (1u << (t * 4 + r))) s[nt][t][r] = -INFINITY;
+            if constexpr (kLean) __builtin_amdgcn_sched_barrier(0);
           }
-          if (masked)
-#pragma unroll
-            for (int t = 0; t < CH; ++t)
-#pragma unroll
-              for (int r = 0; r < 4; ++r)
-                if (hidden & (1u << (t * 4 + r))) s[nt][t][r] = -INFINITY;
-          if constexpr (kLean) __builtin_amdgcn_sched_barrier(0);
         }
       }
       if (masked) {
 #pragma unroll
-        for (int nt = 0; nt < NT && !made; ++nt) {
+        for (int nt = 0; nt < NT && !kMade; ++nt) {
           const int2 seen = seen_by(nt);
 #pragma unroll
           for (int t = 0; t < CH; ++t)
@@ -603,15 +670,18 @@ __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_at
         float top = s[nt][0][0];
 #pragma unroll
         for (int t = 0; t < CH; ++t) top = larger(larger(top, s[nt][t][0], s[nt][t][1]), s[nt][t][2], s[nt][t][3]);
-        if (__any(top * scale > m[nt] + kSlack)) {
-          const float higher = fmaxf(m[nt], max_xor32(max_xor16(top)) * scale);
+        float offset = 0.0f;
+        if constexpr (kMade) offset = a.offset;
+        if (__any((kMade ? fmaf(top, scale, offset) : top * scale) > m[nt] + kSlack)) {
+          const float highest = max_xor32(max_xor16(top)), higher = fmaxf(m[nt], kMade ? fmaf(highest, scale, offset) : highest * scale);
           const float factor = __builtin_amdgcn_exp2f(m[nt] - (higher == -INFINITY ? 0.0f : higher));
           l[nt] *= factor;
 #pragma unroll
           for (int j = 0; j < kLane; ++j) o[nt][j] *= factor;
           m[nt] = higher;
         }
-        const float shift = kShift - (m[nt] == -INFINITY ? 0.0f : m[nt]);
+        float shift = kShift - (m[nt] == -INFINITY ? 0.0f : m[nt]);
+        if constexpr (kMade) shift += offset;
 #pragma unroll
         for (int t = 0; t < CH; ++t) {
 #pragma unroll
@@ -1084,6 +1154,11 @@ size_t part_bytes(const dkv_fp4_attend_args_t& p, const Plan& plan) {
   return (size_t)p.rows * p.q_heads * plan.splits * (p.cache.head_dim * sizeof(float) + sizeof(float2));
 }
 
+template <typename Args>
+struct JoinOf { typedef ShapedArgs type; };
+template <>
+struct JoinOf<AttendArgs> { typedef AttendArgs type; };
+
 template <int D, typename T, typename Args>
 void launch(const Args& a, const Plan& plan, int q_heads, hipStream_t st) {
   const dim3 grid(a.c.kv_heads, plan.blocks * plan.splits, a.requests), block(plan.waves * 64);
@@ -1095,7 +1170,7 @@ void launch(const Args& a, const Plan& plan, int q_heads, hipStream_t st) {
     if constexpr (D < 256 || sizeof(T) == 2) hipLaunchKernelGGL((fp4_attend_kernel<D, T, 2, 2, 4, Args>), grid, block, 0, st, a);
   } else {
     if constexpr (wide) {
-      if constexpr (__is_same(Args, ShapedArgs)) {
+      if constexpr (!__is_same(Args, AttendArgs)) {
         if (plan.waves == 1) hipLaunchKernelGGL((fp4_attend_kernel<D, T, 4, 2, 1, Args>), grid, block, 0, st, a);
         if (plan.waves == 2) hipLaunchKernelGGL((fp4_attend_kernel<D, T, 4, 2, 2, Args>), grid, block, 0, st, a);
       }
@@ -1104,11 +1179,13 @@ void launch(const Args& a, const Plan& plan, int q_heads, hipStream_t st) {
   }
   const long rows = (long)a.rows * q_heads;
   if (plan.splits == 1 || a.arrivals) return;
+  using Join = typename JoinOf<Args>::type;
+  const Join& join = a;
   if (plan.splits > kFewSplits) {
-    hipLaunchKernelGGL((fp4_join_kernel<D, T, Args>), dim3((unsigned)rows), dim3(256), 0, st, a, q_heads);
+    hipLaunchKernelGGL((fp4_join_kernel<D, T, Join>), dim3((unsigned)rows), dim3(256), 0, st, join, q_heads);
   } else {
     constexpr int kSets = 1024 / D;
-    hipLaunchKernelGGL((fp4_join_few_kernel<D, T, Args>), dim3((unsigned)((rows + kSets - 1) / kSets)), dim3(256), 0, st, a, q_heads);
+    hipLaunchKernelGGL((fp4_join_few_kernel<D, T, Join>), dim3((unsigned)((rows + kSets - 1) / kSets)), dim3(256), 0, st, join, q_heads);
   }
 }
 
@@ -1194,17 +1271,37 @@ extern "C" int dkv_fp4_attend_shaped(const dkv_fp4_attend_args_t* p, const dkv_f
   if (rc) return rc;
   if (p->rows == 0) return DKV_OK;
   const Plan plan = plan_of(*p, shape);
-  ShapedArgs a{};
+  BiasedArgs a{};
   rc = attend_args(p, plan, workspace, workspace_bytes, a, what);
   if (rc) return rc;
   a.slopes = shape->slopes; a.sinks = shape->sinks; a.first = shape->first; a.last = shape->last;
   if (shape->cap > 0.0f) {
     a.cap = shape->cap * kLog2e;
+    a.scale = 1.0f;
     // (tanh(u) / u - 1) / u^2 interpolated at the four Chebyshev nodes of u^2 from 0 to 1/4
     const float c[5] = {1.0f, -0.33333310f, 0.13330476f, -0.053387109f, 0.017988745f};
     for (int i = 0; i < 5; ++i) a.small[i] = a.cap * c[i];
     a.reach = fminf(fabsf(p->scaling) / shape->cap, 3e38f);
     if (p->scaling != p->scaling) a.reach = p->scaling;
+    // Scores off by the rounding of the cap and not by their own: 12 * 2^-24 of it at the most, and of 128 at the most that
+    // is below 2^-13, where the weights of bfloat16 results are float16 and off by 2^-12.
+    if (p->query_dtype == DKV_BF16 && shape->cap <= 128.0f) {
+      a.steep = fmaxf(a.reach * (2.0f * kLog2e), 1.1754944e-38f);
+      a.scale = 2.0f * a.cap;
+      a.offset = a.cap;
+    }
   }
-  return launch_attend(a, plan, p, stream, what);
+  if (a.slopes) {
+    a.factor = a.scale;
+    a.lift = a.offset;
+    a.scale = 1.0f;
+    a.offset = 0.0f;
+  }
+  if (a.slopes) return launch_attend(a, plan, p, stream, what);
+  if (a.cap > 0.0f) {
+    CappedArgs capped{};
+    (ShapedArgs&)capped = a;
+    return launch_attend(capped, plan, p, stream, what);
+  }
+  return launch_attend((const ShapedArgs&)a, plan, p, stream, what);
 }

@@ -8,7 +8,8 @@ sum p_t d_t and the sums' own n 2^-24.  s_t in units of 2^-24: D + 8 roundings o
 the exponent's argument and two units of the exponential (2 |z| + 32), three of the bias and its sum (3 |bias|), and a
 capped score's: cap tanh(u) of a float32 u is 8 |z| off at the most where it is a polynomial times u, and where it is
 cap - 2 cap / (1 + e^2u) the parts of that are cap in size: 12 cap, taken only if a score reaches half of the cap, so
-12 min(cap, 2 max |z|).  The smallest weights are subnormal float16, as in test_gpu_paged_attend.  A float16 result below
+12 min(cap, 2 max |z|).  Bfloat16 results take the second form under every cap up to 128, whose 12 * 128 * 2^-24 is less than
+the 2^-12 that w has above half a step of a float16.  The smallest weights are subnormal float16, as in test_gpu_paged_attend.  A float16 result below
 2^-14 is subnormal too: its steps are 2^-24 whatever its size, so its rounding is off by 2^-25 and not by 2^-11 |ref|."""
 
 from __future__ import annotations
