@@ -1286,7 +1286,8 @@ extern "C" int dkv_fp4_attend_shaped(const dkv_fp4_attend_args_t* p, const dkv_f
     // Scores off by the rounding of the cap and not by their own: 12 * 2^-24 of it at the most, and of 128 at the most that
     // is below 2^-13, where the weights of bfloat16 results are float16 and off by 2^-12.
     if (p->query_dtype == DKV_BF16 && shape->cap <= 128.0f) {
-      a.steep = fmaxf(a.reach * (2.0f * kLog2e), 1.1754944e-38f);
+      a.steep = a.reach * (2.0f * kLog2e);
+      if (a.steep < 1.1754944e-38f) a.steep = 1.1754944e-38f;  // (no scale; a NaN stays one, and goes the other way)
       a.scale = 2.0f * a.cap;
       a.offset = a.cap;
     }

@@ -248,6 +248,7 @@ class PagedContext:
         self._windows = self._layer_windows(model.config, len(keys))
         if not shaped:
             self._refuse_more_than_scores(model)
+        self._shapes = self._layer_shapes(model, len(keys), first.device)
         _, heads, tokens, dim = shape
         pages = max(1, -(-(tokens + room) // page))
         self.cache = PagedCache(len(keys), heads, dim, pages, page=page, device=first.device)
@@ -258,7 +259,6 @@ class PagedContext:
             if key.shape != shape or value.shape != shape:
                 raise ValueError(f"layer {layer}: keys {list(key.shape)} and values {list(value.shape)}, not {list(shape)}")
             self.cache.store(layer, key[0].transpose(0, 1), value[0].transpose(0, 1), step)
-        self._shapes = self._layer_shapes(model, len(keys), first.device)
         self._step, self._next = None, 0  # of the forward that runs: its rows, and the layer it is at
         self.exact_cache = self.fresh_cache()
 
@@ -287,8 +287,12 @@ class PagedContext:
         cap = getattr(model.config.get_text_config(decoder=True), "attn_logit_softcapping", None)
         shapes = [{} if not cap else {"cap": cap} for _ in range(layers)]
         for module in getattr(model, "modules", tuple)():
-            if getattr(module, "sinks", None) is not None and 0 <= getattr(module, "layer_idx", -1) < layers:
-                shapes[module.layer_idx]["sinks"] = module.sinks.detach().to(device, torch.float32).contiguous()
+            if getattr(module, "sinks", None) is None:
+                continue
+            layer = getattr(module, "layer_idx", None)
+            if layer is None or not 0 <= layer < layers:
+                raise ValueError(f"PagedContext: sinks of layer {layer}, where the caches have {layers}")
+            shapes[layer]["sinks"] = module.sinks.detach().to(device, torch.float32).contiguous()
         return shapes
 
     def fresh_cache(self):

@@ -193,6 +193,14 @@ def test_scalings(scaling):
     run("slopes+sinks", [77, 300], [1, 30], scaling=scaling, dtype="bf16")
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_a_scale_that_is_no_number(dtype):
+    cache, step = build([77, 300], [1, 30], 1, 64, 16)
+    query = torch.randn(31, 2, 64, device=DEV).to(TYPES[dtype])
+    for made in (dict(cap=5.0), dict(cap=5.0, slopes=numbers(2, 1)), dict(slopes=numbers(2, 1)), dict(sinks=numbers(2, 1))):
+        assert cache.attend_rows(0, query, step, scaling=float("nan"), **made).isnan().all()
+
+
 @pytest.mark.parametrize("new", [1, 45])
 def test_slopes_and_sinks_of_any_size(new):
     cache, step = build([400], [new], 1, 64, 16)

@@ -227,3 +227,5 @@ def test_contexts_of_shaped_scores(family):
     else:
         for shape, layer in zip(shapes, model.model.layers):
             assert list(shape) == ["sinks"] and torch.equal(shape["sinks"], layer.self_attn.sinks) and not shape["sinks"].requires_grad
+        with pytest.raises(ValueError, match="sinks of layer 1"):
+            PagedContext(caches[:1], caches[:1], model, shaped=True)
