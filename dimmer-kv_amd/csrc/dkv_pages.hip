@@ -288,8 +288,9 @@ __global__ __launch_bounds__(256) void fp4_store_kernel(StoreArgs a) {
 // queries and 10^6 keys) the exact sum rounds to the same; where a wave holds one that does not, it makes them all again in
 // float64: products of float32 are exact there, and the sum's last bits are cut towards an odd one, which keeps it on its
 // side of every border of fewer bits.  Float32 rows go that way at once.
-// The pass is the memory's: 16,384 rows of 24 + 8 + 8 heads of 128 bfloat16 dimensions (294 MB) 53 us, 5.5 TB/s, against 102
-// with float64 for all and a head a thread; 64 rows of 32 + 8 + 8 heads of 64 float16 dimensions 4.1 us, which is latency.
+// The pass is the memory's: 16,384 rows of 24 + 8 + 8 heads of 128 bfloat16 dimensions (294 MB) 64 us among other passes (4.6
+// TB/s) and 53 where a graph repeats it, against 102 there with float64 for all and a head a thread; 64 rows of 32 + 8 + 8
+// heads of 64 float16 dimensions 4.1 us, which is latency.
 // A lane takes an octet of dimensions, and the one it is rotated with where all dimensions are in halves, so that nothing
 // is read twice; it keeps its angles for all the heads that it takes.
 // ---------------------------------------------------------------------------
