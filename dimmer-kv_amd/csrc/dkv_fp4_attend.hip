@@ -1091,8 +1091,10 @@ Plan plan_of(const dkv_fp4_attend_args_t& p, const dkv_fp4_shape_t* shape = null
   long longest = p.longest < 1 ? 1 : p.longest;  // the tokens a row block may see
   if (p.window) longest = min(longest, (long)p.window + plan.tiles * 16 / groups + 16);
   // Workgroups enough for the card, of 256 tokens at the least; of 1,024 where that makes more than the card holds at
-  // once, so that requests of different lengths even out.
-  const long fill = (kWorkgroups + each - 1) / each, even = p.requests > 1 && !(shape && plan.tiles == 4) ? (8 * kWorkgroups + each - 1) / each : 1;
+  // once, so that requests of different lengths even out.  (Shaped prompts of 64-row blocks do not: their blocks are many and
+  // of different lengths anyway, and the join is another launch: two prompts of 4,001 tokens 165 us, 234 in three splits.)
+  const bool evens = p.requests > 1 && !(shape && plan.tiles == 4);
+  const long fill = (kWorkgroups + each - 1) / each, even = evens ? (8 * kWorkgroups + each - 1) / each : 1;
   const long wanted = max(min(fill, (longest + 255) / 256), min(even, (longest + 1023) / 1024));
   // Short requests of few rows are not split: eight waves take them in two turns, four where requests alone fill the card.
   // In a captured graph, 8 KV heads of 128 bfloat16 dimensions: 700 tokens of 32 requests 9.1 us against 13.5 split and

@@ -157,6 +157,36 @@ def test_many_blocks(kind, heads, new, dim, dtype):
         some=[0, 1, 15, 16, 17, 39, 500, 699, 700, 701, 1039, 2079, 2199, new[0] // 2, new[0] - 17, new[0] - 1])
 
 
+@pytest.mark.parametrize("heads,kind,dim,dtype", [(2, "window100+cap5+sinks", 64, "bf16"), (1, "documents+window90", 64, "f16"),
+                                                  (2, "slopes+window70", 128, "bf16")])
+def test_more_blocks_than_a_launch(heads, kind, dim, dtype):
+    """Prompts of more than 4,096 blocks of rows: a workgroup takes several, one after the other."""
+    new = 40000
+    run(kind, [0], [new], heads=heads, groups=8, dim=dim, page=64, dtype=dtype, only=[0, 8 * heads - 1],
+        some=[0, 1, 17, 99, 100, 3615, 7232, 7233, 8191, 8192, 20000, 32767, 32768, new - 2, new - 1])
+
+
+def test_pages_past_32_bits():
+    """Rows appended to, and attended to in, pages whose codes lie past 2^32 bytes."""
+    from paged_cache import PagedCache, Step
+    from test_gpu_paged_append import check, inputs, tables
+
+    page, heads, dim = 64, 8, 256
+    pages = (1 << 32) // (heads * page * dim // 2) + 5
+    cache = PagedCache(1, heads, dim, pages, page=page, requests=1, table_pages=2, device=DEV)
+    cache.table.copy_(torch.tensor([[pages - 1, pages - 3]], dtype=torch.int32))
+    cache.lengths.fill_(100)
+    slots = cache.slots(0, 0, 100)
+    assert int(slots.min()) * heads * dim // 2 > 1 << 32
+    step = Step(slots, torch.arange(100, device=DEV), torch.tensor([0, 100], dtype=torch.int32, device=DEV), 100, 100, 100)
+    query, key, value = inputs(100, 16, heads, dim, "bf16")
+    cos, sin = tables(100, dim // 2)
+    turned = cache.append(0, query, key, value, step, cos, sin)
+    check(cache, step, query, key, value, turned, cos, sin)
+    made = dict(cap=6.0, sinks=numbers(16, 2))
+    compare(cache, step, turned, cache.attend_rows(0, turned, step, **made), heads=[0, 15], some=[0, 50, 99], **made)
+
+
 @pytest.mark.parametrize("kind", ["documents+sinks", "window300+cap7"])
 def test_many_blocks_against_few(kind):
     """Every row of a launch of one or two waves a block against the same rows in a launch of four, to what two roundings of
