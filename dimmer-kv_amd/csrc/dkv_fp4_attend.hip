@@ -328,7 +328,8 @@ __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_at
   // (one fills the other's waits): queries lie in LDS, and a chunk's loads follow the last use of the one before.
   constexpr bool kLean = NT == 4;
   __shared__ frag held[kLean ? NT * kSteps * 64 : 1];
-  __shared__ float sums[kWaves == 1 ? 1 : (kWaves < 4 ? kWaves : 4) * 16 * kStride];
+  __shared__ float sums[kWaves < 4 ? 1 : 4 * 16 * kStride];
+  __shared__ floatx4 given[kWaves == 2 ? 2 * kLane * 64 : 1];  // a tile's sums that each of two waves gives the other
   __shared__ float stat[2][kWaves][kRows];
   __shared__ RowShape rows_of[kShaped ? kWaves : 1][kShaped ? kRows : 1];  // a copy for each wave
 
@@ -775,24 +776,69 @@ __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_at
       }
     }
 
-    if constexpr (kWaves == 1) {  // nothing to add up: a lane has a quarter of its rows' dimensions
+    if constexpr (kWaves <= 2) {  // a lane has a quarter of its rows' dimensions, and writes them
+      float total[NT];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        float total = sum_xor32(sum_xor16(l[nt]));
-        if (rows_of[wave][nt * 16 + i].last < 0) m[nt] = -INFINITY, total = 0.0f;
-        if (m[nt] == -INFINITY && total != 0.0f) m[nt] = 0.0f;
+        total[nt] = sum_xor32(sum_xor16(l[nt]));
+        if (rows_of[wave][nt * 16 + i].last < 0) m[nt] = -INFINITY, total[nt] = 0.0f;
+        if (m[nt] == -INFINITY && total[nt] != 0.0f) m[nt] = 0.0f;
+      }
+      auto put = [&](int nt) {
         const int r = row0 + nt * 16 + i;
-        if (r >= n_rows) continue;
+        if (r >= n_rows) return;
         const int token = r / a.groups, head = h * a.groups + (r - token * a.groups);
-        const float2 beside = beside_sink(m[nt], total, a.sinks, head, kShift);
-        const float inverse = total == 0.0f ? 0.0f : beside.x / beside.y;
+        const float2 beside = beside_sink(m[nt], total[nt], a.sinks, head, kShift);
+        const float inverse = total[nt] == 0.0f ? 0.0f : beside.x / beside.y;
         T* out = (T*)a.out + ((long)(q0 + token) * q_heads + head) * D + g * (D / 4);
 #pragma unroll
         for (int d = 0; d < D / 4; d += 8) {
           float x[8];
 #pragma unroll
-          for (int k = 0; k < 8; ++k) x[k] = total == 0.0f ? 0.0f : o[nt][(d + k) % kLane][(d + k) / kLane] * inverse;
+          for (int k = 0; k < 8; ++k) x[k] = total[nt] == 0.0f ? 0.0f : o[nt][(d + k) % kLane][(d + k) / kLane] * inverse;
           store_results(out + d, x);
+        }
+      };
+      if constexpr (kWaves == 1) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) put(nt);
+      } else {
+        // Two waves: each finishes half of the tiles, and gives the other its sums of the rest, lane by lane.
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          if (g == 0) {
+            stat[0][wave][nt * 16 + i] = m[nt];
+            stat[1][wave][nt * 16 + i] = total[nt];
+          }
+        __syncthreads();
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const float other = stat[0][1 - wave][nt * 16 + i], top = fmaxf(m[nt], other);
+          const float factor = m[nt] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[nt] - top);
+#pragma unroll
+          for (int j = 0; j < kLane; ++j) o[nt][j] *= factor;
+          total[nt] = total[nt] * factor +
+                      (other == -INFINITY ? 0.0f : stat[1][1 - wave][nt * 16 + i] * __builtin_amdgcn_exp2f(other - top));
+          m[nt] = top;
+        }
+        auto give = [&](int nt) {
+#pragma unroll
+          for (int j = 0; j < kLane; ++j) given[(wave * kLane + j) * 64 + lane] = o[nt][j];
+        };
+        auto take = [&](int nt) {
+#pragma unroll
+          for (int j = 0; j < kLane; ++j) o[nt][j] += given[((1 - wave) * kLane + j) * 64 + lane];
+          put(nt);
+        };
+        const int side = __builtin_amdgcn_readfirstlane(wave);
+#pragma unroll
+        for (int x = 0; x < NT / 2; ++x) {
+          if (side == 0) give(NT / 2 + x);
+          else give(x);
+          __syncthreads();
+          if (side == 0) take(x);
+          else take(NT / 2 + x);
+          __syncthreads();
         }
       }
       continue;
@@ -856,7 +902,7 @@ __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_at
           total += mx == -INFINITY ? 0.0f : stat[1][x][nt * 16 + row] * __builtin_amdgcn_exp2f(mx - highest);
         }
 #pragma unroll
-        for (int x = 0; x < (kWaves < 4 ? kWaves : 4); ++x)
+        for (int x = 0; x < 4; ++x)
 #pragma unroll
           for (int j = 0; j < kPart; ++j) acc[j] += sums[(x * 16 + row) * kStride + part * kPart + j];
         const int token = r / a.groups;
@@ -1105,12 +1151,13 @@ Plan plan_of(const dkv_fp4_attend_args_t& p, const dkv_fp4_shape_t* shape = null
   // Many blocks of 64 rows: fewer waves take each, as joining them is what a short range costs most.  With starts of their
   // own rows see few tokens each (documents), but not the same number, and two waves even out what one would be left with.
   // 32 query heads of 8 KV heads, by four, two and one waves: 8,192 tokens of 64 float16 dimensions (4,096 blocks) that see
-  // one token 90, 55 and 29 us, 768 at the most 126, 100 and 93, documents of 80 to 2,300 tokens 169, 146 and 188, all
-  // tokens 553, 552 and 542; 2,048 tokens (1,024 blocks) 768 at the most 34, 30 and 36, all 50, 53 and 77; 16,384 tokens of
-  // 128 bfloat16 dimensions (8,192 blocks) 768 at the most 309, 270 and 186, all 2,075, 2,103 and 1,956.
+  // one token 90, 48 and 29 us, 768 at the most 126, 100 and 93, documents of 80 to 2,300 tokens 169, 134 and 188, all
+  // tokens 553, 514 and 542; 2,048 tokens (1,024 blocks) 768 at the most 34, 25 and 36, all 50, 47 and 77.  By four waves
+  // and one, 16,384 tokens of 128 bfloat16 dimensions (8,192 blocks) 768 at the most 309 and 186, all 2,075 and 1,956.  Few
+  // blocks that see much stay with four: 4,096 tokens of 24 heads after 12,288 (1,536 blocks) 647 us, by two waves 837.
   if (shape && plan.tiles == 4) {
     if (each >= 8192 || (longest <= 1024 && !shape->first && each >= 2048)) plan.waves = 1;
-    else if (shape->first && each >= 1024) plan.waves = 2;
+    else if (shape->first && each >= (longest <= 8192 ? 1024 : 4096)) plan.waves = 2;
   }
   plan.splits = plan.waves != 4 ? 1 : (int)min(max(wanted, 1L), (long)kMaxSplits);
   // Blocks of 64 rows that fill the card once and a half leave half of it idle at the end: two or three splits where that
