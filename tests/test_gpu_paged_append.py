@@ -69,6 +69,9 @@ def test_shapes(dim, rotary, interleaved, dtype):
     got = cache.append(0, query, key, value, step, cos, sin, interleaved=interleaved)
     assert got.shape == query.shape and got.dtype == query.dtype
     check(cache, step, query, key, value, got, cos, sin, interleaved)
+    place = query.clone()  # the queries' own
+    assert cache.append(0, place, key, value, step, cos, sin, interleaved=interleaved, out=place) is place
+    assert torch.equal(place, got)
 
 
 @pytest.mark.parametrize("heads,q_heads", [(1, 1), (1, 7), (3, 3), (8, 32), (5, 40)])
