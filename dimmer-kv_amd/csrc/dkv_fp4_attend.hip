@@ -69,6 +69,7 @@ struct ShapedArgs : AttendArgs {
   float factor, lift;    // a made score times `factor` plus `lift` is the score where slopes are taken off it,
   float offset;          // and times `scale` plus `offset` where its weight is made
   float small[5];        // cap times the coefficients of tanh(u) / u in u^2
+  int apart;             // each score takes its own form of the cap: the error of a large one would show in a small score
 };
 // Kernels of their own for a cap and for slopes (with a cap or without): what the others do not need costs them registers,
 // and a branch in the chunks' loop as much as some ten instructions.
@@ -536,7 +537,7 @@ __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_at
             for (int t = 0; t < CH; ++t)
 #pragma unroll
               for (int r = 0; r < 4; ++r) s[nt][t][r] = __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(s[nt][t][r] * a.steep));
-        } else if (!kSlopes && !kSteep && !masked && kPieces == 1) {
+        } else if (!kSlopes && !kSteep && !masked && kPieces == 1 && !a.apart) {
           bool far = false;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
@@ -607,19 +608,43 @@ __global__ __launch_bounds__(kWaves * 64, NT == 2 && D > 64 ? 1 : 2) void fp4_at
               float size = 0.0f;
 #pragma unroll
               for (int t = 0; t < CH; ++t) size = larger_size(larger_size(size, s[nt][t][0], s[nt][t][1]), s[nt][t][2], s[nt][t][3]);
-              if (!__any(size * a.reach > 0.5f)) {
+              const bool far = __any(size * a.reach > 0.5f);
+              // Which form a type takes where is a matter of registers: with the loop of small scores first, as the others have
+              // it, bfloat16 tokens of 64 dimensions take 172 and two waves a SIMD, and 161 and three as it is.
+              if (!kSteep && !far) {
 #pragma unroll
                 for (int t = 0; t < CH; ++t)
 #pragma unroll
                   for (int r = 0; r < 4; ++r) s[nt][t][r] = small_tanh(s[nt][t][r] * a.reach, a.small);
-              } else {
+              } else if (kSlopes && !kSteep && kPieces == 1 && !a.apart) {
 #pragma unroll
                 for (int t = 0; t < CH; ++t)
 #pragma unroll
+                  for (int r = 0; r < 4; ++r) s[nt][t][r] = large_tanh(s[nt][t][r] * a.reach, a.cap);
+              } else if (!kSteep) {
+#pragma unroll
+                for (int t = 0; t < CH; ++t) {
+#pragma unroll
                   for (int r = 0; r < 4; ++r) {
                     const float u = s[nt][t][r] * a.reach, y = large_tanh(u, a.cap);
-                    s[nt][t][r] = kPieces == 1 || fabsf(u) > 0.5f ? y : small_tanh(u, a.small);
+                    s[nt][t][r] = fabsf(u) > 0.5f ? y : small_tanh(u, a.small);
                   }
+                  if constexpr (kPieces == 1) __builtin_amdgcn_sched_barrier(0);
+                }
+              } else {
+#pragma unroll
+                for (int t = 0; t < CH; ++t) {
+                  float u[4];
+#pragma unroll
+                  for (int r = 0; r < 4; ++r) {
+                    u[r] = s[nt][t][r] * a.reach;
+                    s[nt][t][r] = small_tanh(u[r], a.small);
+                  }
+                  if (far) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) s[nt][t][r] = fabsf(u[r]) > 0.5f ? large_tanh(u[r], a.cap) : s[nt][t][r];
+                  }
+                }
               }
             }
             if constexpr (kSlopes) {
@@ -1340,8 +1365,10 @@ extern "C" int dkv_fp4_attend_shaped(const dkv_fp4_attend_args_t* p, const dkv_f
     a.reach = fminf(fabsf(p->scaling) / shape->cap, 3e38f);
     if (p->scaling != p->scaling) a.reach = p->scaling;
     // Scores off by the rounding of the cap and not by their own: 12 * 2^-24 of it at the most, and of 128 at the most that
-    // is below 2^-13, where the weights of bfloat16 results are float16 and off by 2^-12.
-    if (p->query_dtype == DKV_BF16 && shape->cap <= 128.0f) {
+    // is below 2^-13, where the weights of bfloat16 results are float16 and off by 2^-12, and float16 results by 2^-12 at the
+    // least.
+    a.apart = shape->cap > 128.0f;
+    if (p->query_dtype == DKV_BF16 && !a.apart) {
       a.steep = a.reach * (2.0f * kLog2e);
       if (a.steep < 1.1754944e-38f) a.steep = 1.1754944e-38f;  // (no scale; a NaN stays one, and goes the other way)
       a.scale = 2.0f * a.cap;

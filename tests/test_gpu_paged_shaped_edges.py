@@ -1,0 +1,41 @@
+"""Shaped scores where one row or input could spoil another's."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from test_gpu_paged_attend import DEV, TYPES, build
+from test_gpu_paged_shaped import compare, numbers
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("kind", ["", "slopes", "sinks+first"])
+@pytest.mark.parametrize("old,new,dim", [(59, 1, 64), (300, 40, 64), (300, 40, 128), (130, 3, 256)])
+@pytest.mark.parametrize("dtype,cap", [(dtype, cap) for dtype in ("f32", "f16", "bf16") for cap in (200.0, 1e4, 1e5)] +
+                         [("f32", 1e6), ("bf16", 1e6)])
+def test_caps_beside_rows_that_reach_them(dtype, cap, old, new, dim, kind):
+    """Heads whose scores pass four fifths of the cap, up and down, in the tiles of heads whose scores are about 1.  The bound
+    is compare's: a row whose own scores stay within half of its cap is off by the size of those and not of the cap, for
+    caps above 128 whatever the type.  (The far heads' scores at ten tokens are z = 0.8 cap, of some 0.1 cap at the others.)"""
+    print(f"[case] caps beside {kind} {old}+{new} dim={dim} cap={cap} {dtype}", flush=True)
+    cache, step = build([old], [new], 1, dim, 16, seed=3)
+    keys = cache.load(0, cache.slots(0, 0, old + new), torch.float32)[0][:, 0]
+    g = torch.Generator(DEV).manual_seed(1)
+    query = torch.randn(new, 4, dim, generator=g, device=DEV) * (0.8 / dim ** 0.5)
+    ten = torch.arange(10, device=DEV) * (old // 10) + 3
+    near = keys[ten].double().cpu()  # the shortest vector of these ten scores
+    far = (near.T @ torch.linalg.solve(near @ near.T, torch.full((10,), 0.8 * cap, dtype=torch.float64))).float().to(DEV)
+    query[:, 0], query[:, 2] = far, -far
+    query = query.to(TYPES[dtype])
+    assert query.isfinite().all()
+    z = query.double() @ keys.double().T
+    assert (z[:, [0, 2]].abs().amax(-1) > 0.7 * cap).all() and (z[:, [1, 3]].abs() < 6.0).all()
+    made = dict(cap=cap)
+    if "slopes" in kind:
+        made["slopes"] = torch.tensor([0.5, 0.01, 0.002, 0.0], device=DEV)
+    if "sinks" in kind:
+        made["sinks"], made["first"] = numbers(4, 5), (step.positions - 250).clamp(min=0)
+    got = cache.attend_rows(0, query, step, scaling=1.0, **made)
+    compare(cache, step, query, got, scaling=1.0, **made)
