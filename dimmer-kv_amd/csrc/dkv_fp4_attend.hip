@@ -201,8 +201,12 @@ DKV_DEVICE float large_tanh(float u, float cap) {
 // What a row's sums are worth beside its sink: (factor of the sums, their whole), weights held times 2^shift.
 DKV_DEVICE float2 beside_sink(float top, float total, const float* sinks, int head, float shift) {
   if (!sinks || total == 0.0f) return make_float2(1.0f, total);
-  const float sink = sinks[head] * kLog2e, higher = fmaxf(top, sink), factor = __builtin_amdgcn_exp2f(top - higher);
-  return make_float2(factor, fmaf(total, factor, __builtin_amdgcn_exp2f(sink - higher + shift)));
+  const float sink = sinks[head] * kLog2e, higher = fmaxf(top, sink);
+  // A sink so far above the row's scores that they have no share; past 2^23 its own would be e to the rounding of its units,
+  // and an infinite one no number.
+  const bool all = sink > top + 256.0f;
+  const float factor = all ? 0.0f : __builtin_amdgcn_exp2f(top - higher);
+  return make_float2(factor, fmaf(total, factor, __builtin_amdgcn_exp2f(all ? shift : sink - higher + shift)));
 }
 
 DKV_DEVICE float exponent(uint32_t byte) { return __uint_as_float(byte << 23); }

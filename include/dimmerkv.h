@@ -579,7 +579,8 @@ int dkv_fp4_attend(const dkv_fp4_attend_args_t* p, void* workspace, size_t works
  *   z = scaling q.k;  z = cap tanh(z / cap)  (cap > 0);  z = z - slopes[x] |p - t|
  * and out = sum_t e^z v / (sum_t e^z + e^sinks[x]) for query head x.  A row sees the tokens from first[row] (0 if null)
  * to last[row] (p if null), of the window's (from p - window + 1 on) and of those the request holds; a row that sees
- * nothing is 0.  NaN and infinities as above; a cap makes an infinite score the cap. */
+ * nothing is 0, and so is one whose sink is +infinity.  NaN and infinities as above; a cap makes an infinite score the
+ * cap. */
 typedef struct dkv_fp4_shape {
   const float* slopes;     /* [q_heads] or null */
   const float* sinks;      /* [q_heads] or null */

@@ -39,3 +39,22 @@ def test_caps_beside_rows_that_reach_them(dtype, cap, old, new, dim, kind):
         made["sinks"], made["first"] = numbers(4, 5), (step.positions - 250).clamp(min=0)
     got = cache.attend_rows(0, query, step, scaling=1.0, **made)
     compare(cache, step, query, got, scaling=1.0, **made)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("dim,heads,old,new", [(64, 1, 59, 1), (128, 1, 9000, 2), (64, 2, 20000, 1), (64, 1, 300, 45), (256, 1, 300, 45),
+                                               (64, 8, 0, 2100), (64, 16, 0, 6600)])
+def test_sinks_past_all_scores(dim, heads, old, new, dtype):
+    """A sink of +infinity, or one that is finite and past all scores by any amount, takes all: rows are 0, as
+    sum e^z v / (sum e^z + e^s) is; a sink that is no number makes its rows NaN; other heads' are as without."""
+    print(f"[case] sinks past all {old}+{new} dim={dim} heads={heads} {dtype}", flush=True)
+    cache, step = build([old], [new], heads, dim, 64)
+    query = torch.randn(new, 5 * heads, dim, generator=torch.Generator(DEV).manual_seed(2), device=DEV).to(TYPES[dtype])
+    first = torch.zeros_like(step.positions)
+    mild = torch.tensor([-1.0, -1.0, -1.0, -1.0, 0.5], device=DEV).repeat(heads)
+    for large in ((float("inf"), 3.4e38, 2.5e38), (1e4, 7.77e8, 3.3e12), (1.23e17, 5.4e29, 2.3e38)):
+        sinks = torch.tensor([*large, float("nan"), 0.5], device=DEV).repeat(heads)
+        for made in (dict(), dict(cap=5.0), dict(first=first), dict(slopes=torch.full_like(sinks, 0.1))):
+            got = cache.attend_rows(0, query, step, sinks=sinks, **made).unflatten(1, (heads, 5))
+            want = cache.attend_rows(0, query, step, sinks=mild, **made).unflatten(1, (heads, 5))
+            assert not got[:, :, :3].any() and got[:, :, 3].isnan().all() and torch.equal(got[:, :, 4], want[:, :, 4])
