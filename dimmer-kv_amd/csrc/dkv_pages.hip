@@ -286,8 +286,8 @@ __global__ __launch_bounds__(256) void fp4_store_kernel(StoreArgs a) {
 // border of two codes must fall on the right side, and float32 sums do not tell: so each sum of 16-bit rows is made in
 // float32 with a bound on its error, and rounded from both ends of that.  Where the two agree (all but one of some 10^4
 // queries and 10^6 keys) the exact sum rounds to the same; where a wave holds one that does not, it makes them all again in
-// float64: products of float32 are exact there, and the sum's last bits are cut towards an odd one, which keeps it on its
-// side of every border of fewer bits.  Float32 rows go that way at once.
+// float64: products of float32 are exact there, and what the sum loses, and its cut to float32, set the last bit, which keeps
+// it on its side of every border of fewer bits.  Float32 rows go that way at once.
 // The pass is the memory's: 16,384 rows of 24 + 8 + 8 heads of 128 bfloat16 dimensions (294 MB) 64 us among other passes (4.6
 // TB/s) and 53 where a graph repeats it, against 102 there with float64 for all and a head a thread; 64 rows of 32 + 8 + 8
 // heads of 64 float16 dimensions 4.1 us, which is latency.
@@ -308,15 +308,6 @@ struct AppendArgs {
   int n, shift, q_heads, rotary, table_rows, fill;
   int each;  // heads that a thread takes, of the queries', the keys' and the values' in turn
 };
-
-// d cut to float32, its last bit set where that loses something: rounding the result once more to fewer bits, to either
-// side of a border of fewer bits, is rounding d.
-DKV_DEVICE float cut_to_odd(double d) {
-  const float f = (float)d;
-  const double back = (double)f;
-  if (!(back != d) || d != d) return f;
-  return __uint_as_float((__float_as_uint(f) - (fabs(back) > fabs(d) ? 1u : 0u)) | 1u);
-}
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
@@ -352,7 +343,34 @@ struct Turn {
       off[i] = fmaf(fabsf(product) + fabsf(r[i]), 0x1.8p-23f, 0x1p-140f);
     }
   }
-  DKV_DEVICE double exact(int i) const { return (double)x[i] * c[i] + (double)y[i] * s[i]; }
+  // What a sum in float64 lacks of its two products, which are exact there.
+  DKV_DEVICE double lacks(int i, double sum) const {
+    const double one = (double)x[i] * c[i], two = (double)y[i] * s[i], took = sum - one;
+    return (one - (sum - took)) + (two - took);
+  }
+  // The exact sum cut to float32, its last bit set where that loses something: rounding the result once more to fewer bits, to
+  // either side of a border of fewer bits, is rounding the exact one.  What float64 lacks is asked for only where float32 seems
+  // to hold the sum: the five additions for all eight at once would take registers that there are not (16,384 rows 130 us
+  // instead of 82, with their load).
+  DKV_DEVICE float cut_to_odd(int i) const {
+    const double sum = (double)x[i] * c[i] + (double)y[i] * s[i];
+    const float f = (float)sum;
+    double rest = sum - (double)f;
+    if (__builtin_expect(rest == 0.0, 0)) rest = lacks(i, sum);
+    if (!(fabs(rest) > 0.0)) return f;  // (nor of infinities)
+    return __uint_as_float((__float_as_uint(f) - (signbit(rest) != signbit(f) ? 1u : 0u)) | 1u);
+  }
+  // The exact sum rounded to float32.  A sum in float64 that lies between two floats is on its side of their middle, or on it
+  // (the 28 last bits are zero), where a last bit that is set tells the side.
+  DKV_DEVICE float nearest(int i) const {
+    const double sum = (double)x[i] * c[i] + (double)y[i] * s[i];
+    long bits = __double_as_longlong(sum);
+    if (__builtin_expect(!(bits & 0xfffffff), 0)) {
+      const double rest = lacks(i, sum);
+      if (fabs(rest) > 0.0) bits += (rest > 0.0) == (sum > 0.0) ? 1 : -1;
+    }
+    return (float)__longlong_as_double(bits);
+  }
 };
 
 template <typename T>
@@ -365,14 +383,14 @@ DKV_DEVICE void put_query(T* p, const Turn& turn) {
     uint4 w = rounded(low, T());
     if (__any(differ(w, rounded(high, T())))) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) r[i] = cut_to_odd(turn.exact(i));
+      for (int i = 0; i < 8; ++i) r[i] = turn.cut_to_odd(i);
       w = rounded(r, T());
     }
     *(uint4*)p = w;
   } else {
 #pragma unroll
     for (int i = 0; i < 8; i += 4)
-      *(float4*)(p + i) = make_float4((float)turn.exact(i), (float)turn.exact(i + 1), (float)turn.exact(i + 2), (float)turn.exact(i + 3));
+      *(float4*)(p + i) = make_float4(turn.nearest(i), turn.nearest(i + 1), turn.nearest(i + 2), turn.nearest(i + 3));
   }
 }
 
@@ -429,7 +447,7 @@ DKV_DEVICE void put_key(const dkv_fp4_cache_t& c, int shift, long slot, int h, i
     if (!__any(!certain)) return place_octet<D>(c, shift, false, slot, h, o, codes, e);
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) r[i] = cut_to_odd(turn.exact(i));
+  for (int i = 0; i < 8; ++i) r[i] = turn.cut_to_odd(i);
   put_octet<D>(c, shift, false, slot, h, o, r);
 }
 
