@@ -333,6 +333,7 @@ DKV_DEVICE bool differ(uint4 a, uint4 b) { return ((a.x ^ b.x) | (a.y ^ b.y) | (
 // One octet: x c + y s, y with its partners and s with the sign of its side.
 struct Turn {
   float x[8], y[8], c[8], s[8];
+  bool stays;  // the octet is not rotated: c is 1 (or NaN), y 0 and s -0, so that sums are x, the sign of a zero too
   // The sums in float32, and by how much they may be off: 2^-24 of the product that is rounded and of the sum, three times that for
   // the roundings of the bounds that are made with it.
   DKV_DEVICE void sums(float (&r)[8], float (&off)[8]) const {
@@ -340,7 +341,7 @@ struct Turn {
     for (int i = 0; i < 8; ++i) {
       const float product = y[i] * s[i];
       r[i] = fmaf(x[i], c[i], product);
-      off[i] = fmaf(fabsf(product) + fabsf(r[i]), 0x1.8p-23f, 0x1p-140f);
+      off[i] = stays ? 0.0f : fmaf(fabsf(product) + fabsf(r[i]), 0x1.8p-23f, 0x1p-140f);
     }
   }
   // What a sum in float64 lacks of its two products, which are exact there.
@@ -356,7 +357,7 @@ struct Turn {
     const double sum = (double)x[i] * c[i] + (double)y[i] * s[i];
     const float f = (float)sum;
     double rest = sum - (double)f;
-    if (__builtin_expect(rest == 0.0, 0)) rest = lacks(i, sum);
+    if (__builtin_expect(rest == 0.0 && !stays, 0)) rest = lacks(i, sum);
     if (!(fabs(rest) > 0.0)) return f;  // (nor of infinities)
     return __uint_as_float((__float_as_uint(f) - (signbit(rest) != signbit(f) ? 1u : 0u)) | 1u);
   }
@@ -365,7 +366,7 @@ struct Turn {
   DKV_DEVICE float nearest(int i) const {
     const double sum = (double)x[i] * c[i] + (double)y[i] * s[i];
     long bits = __double_as_longlong(sum);
-    if (__builtin_expect(!(bits & 0xfffffff), 0)) {
+    if (__builtin_expect(!(bits & 0xfffffff) && !stays, 0)) {
       const double rest = lacks(i, sum);
       if (fabs(rest) > 0.0) bits += (rest > 0.0) == (sum > 0.0) ? 1 : -1;
     }
@@ -381,7 +382,7 @@ DKV_DEVICE void put_query(T* p, const Turn& turn) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) low[i] = r[i] - off[i], high[i] = r[i] + off[i];
     uint4 w = rounded(low, T());
-    if (__any(differ(w, rounded(high, T())))) {
+    if (__any(!turn.stays && differ(w, rounded(high, T())))) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) r[i] = turn.cut_to_odd(i);
       w = rounded(r, T());
@@ -443,7 +444,7 @@ DKV_DEVICE void put_key(const dkv_fp4_cache_t& c, int shift, long slot, int h, i
     const uint32_t e = block_exponent(max_quad(__float_as_uint(most) & 0x7fffffffu));
     const uint32_t codes = octet_codes(low, min(e, 254u));
     const bool certain = e != DKV_FP4_NAN && e == block_exponent(max_quad(__float_as_uint(least) & 0x7fffffffu)) &&
-                         codes == octet_codes(high, min(e, 254u));
+                         (turn.stays || codes == octet_codes(high, min(e, 254u)));
     if (!__any(!certain)) return place_octet<D>(c, shift, false, slot, h, o, codes, e);
   }
 #pragma unroll
@@ -465,6 +466,7 @@ __global__ __launch_bounds__(256, 4) void fp4_append_kernel(AppendArgs a) {
   const int half = a.rotary / 2, first = o * 8;
   const bool turns = LAYOUT == kWholeHalves || first < a.rotary, low = LAYOUT == kWholeHalves || first < half;
   Turn turn;
+  turn.stays = !turns;
   if (turns && y0 < values) {
     const bool known = position >= 0 && position < a.table_rows;  // (else the row becomes NaN)
     if constexpr (LAYOUT == kPairs) {
@@ -491,7 +493,7 @@ __global__ __launch_bounds__(256, 4) void fp4_append_kernel(AppendArgs a) {
   } else if (y0 < values) {
     const float stays = position >= 0 && position < a.table_rows ? 1.0f : __builtin_nanf("");
 #pragma unroll
-    for (int i = 0; i < 8; ++i) turn.c[i] = stays, turn.s[i] = 0.0f;
+    for (int i = 0; i < 8; ++i) turn.c[i] = stays, turn.s[i] = -0.0f;
   }
   for (int y = y0; y < y1; ++y) {
     const int kind = y < keys ? 0 : y < values ? 1 : 2, h = kind == 0 ? y : kind == 1 ? y - keys : y - values;

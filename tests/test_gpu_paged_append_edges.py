@@ -7,7 +7,7 @@ from fractions import Fraction
 import pytest
 import torch
 
-from test_gpu_paged_append import make
+from test_gpu_paged_append import inputs, make, tables
 from test_gpu_paged_attend import DEV, TYPES
 
 pytestmark = pytest.mark.gpu
@@ -103,3 +103,36 @@ def test_queries_whose_sums_pass_64_bits(interleaved, dtype):
         assert len(large) >= 32
         have = got[t, 0].double().tolist()
         assert [nearest(exact[i], bits) for i in large] == [have[i] for i in large], t
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dim,rotary", [(64, 32), (64, 48), (128, 32), (128, 64), (128, 96), (256, 16), (256, 64), (256, 192)])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_dimensions_that_stay(dtype, dim, rotary, interleaved):
+    """Blocks of dimensions behind the rotated ones hold the bytes that store writes, the sign of zeros and values on the
+    border of two codes among them; the queries' dimensions there keep their bits."""
+    cache, step = make([40], 2, dim)
+    query, key, value = inputs(40, 4, 2, dim, dtype, 3)
+    ties = torch.tensor([0.0, -0.0, 0.25, -0.25, 0.75, 1.25, -1.75, 2.5, 3.5, -5.0, 6.0], device=DEV)
+    for t in (query, key):
+        t[::2, :, rotary:] = ties[torch.arange(t[::2, :, rotary:].numel(), device=DEV) % 11].view_as(t[::2, :, rotary:]).to(t.dtype)
+        t[5] = -0.0
+    cos, sin = tables(40, rotary // 2)
+    got = cache.append(0, query, key, value, step, cos, sin, interleaved=interleaved)
+    bits = {2: torch.int16, 4: torch.int32}[query.element_size()]
+    assert torch.equal(got[..., rotary:].contiguous().view(bits), query[..., rotary:].contiguous().view(bits))
+    keys = cache.load(0, step.slots, torch.float32)[0]
+    codes, scales = cache.key_codes.clone(), cache.key_scales.clone()
+    cache.store(0, key, value, step)
+    stored = cache.load(0, step.slots, torch.float32)[0]
+    whole = -(-rotary // 32) * 32  # the first block that nothing of is rotated
+    if whole < dim:
+        assert torch.equal(keys[..., whole:].contiguous().view(torch.int32), stored[..., whole:].contiguous().view(torch.int32))
+        page = cache.page
+        for a, b, width, at in ((codes, cache.key_codes, dim // 2, whole // 2), (scales, cache.key_scales, dim // 32, whole // 32)):
+            a, b = (t[0].view(-1, 2, page, width)[..., at:] for t in (a, b))
+            assert torch.equal(a, b)
+    if rotary % 32:  # a block of both: a zero keeps its sign whatever the block's exponent
+        part = key[..., rotary:whole].float()
+        zero = part == 0
+        assert zero.any() and torch.equal(keys[..., rotary:whole][zero].signbit(), part[zero].signbit())
