@@ -377,12 +377,17 @@ struct Turn {
 template <typename T>
 DKV_DEVICE void put_query(T* p, const Turn& turn) {
   if constexpr (sizeof(T) == 2) {
-    float r[8], off[8], low[8], high[8];
+    float r[8], off[8], low[8], high[8], most = 0.0f;
     turn.sums(r, off);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) low[i] = r[i] - off[i], high[i] = r[i] + off[i];
+    for (int i = 0; i < 8; ++i) {
+      low[i] = r[i] - off[i];
+      high[i] = r[i] + off[i];
+      most = __builtin_elementwise_maximum(most, off[i]);
+    }
     uint4 w = rounded(low, T());
-    if (__any(!turn.stays && differ(w, rounded(high, T())))) {
+    // (An infinity beside a product past float32 may be NaN at both ends, and no bound tells.)
+    if (__any(!turn.stays && (differ(w, rounded(high, T())) || !(most < INFINITY)))) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) r[i] = turn.cut_to_odd(i);
       w = rounded(r, T());

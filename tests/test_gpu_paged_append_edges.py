@@ -136,3 +136,16 @@ def test_dimensions_that_stay(dtype, dim, rotary, interleaved):
         part = key[..., rotary:whole].float()
         zero = part == 0
         assert zero.any() and torch.equal(keys[..., rotary:whole][zero].signbit(), part[zero].signbit())
+
+
+@pytest.mark.parametrize("x,y,want", [(float("inf"), 3e38, (float("inf"), float("inf"))),
+                                      (3e38, -float("inf"), (float("inf"), -float("inf")))])
+def test_infinities_beside_products_past_float32(x, y, want):
+    """An infinite query beside a finite product that float32 does not hold is infinite, not NaN: x - 1.5 y, y + 1.5 x."""
+    cache, step = make([4], 1, 64)
+    query = torch.ones(4, 1, 64, device=DEV).bfloat16()
+    query[1, 0, 3], query[1, 0, 35] = x, y
+    cos, sin = torch.ones(4, 32, device=DEV), torch.full((4, 32), 1.5, device=DEV)
+    got = cache.append(0, query, query, query, step, cos, sin).float()
+    assert (got[1, 0, 3].item(), got[1, 0, 35].item()) == want
+    assert got.isinf().sum() == 2 and not got.isnan().any()
