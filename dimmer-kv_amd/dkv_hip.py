@@ -674,7 +674,7 @@ class _Forward(torch.autograd.Function):
     asking for it raises."""
 
     @staticmethod
-    def forward(ctx, what, out, given):
+    def forward(ctx, what, out, *given):
         ctx.what = what
         ctx.mark_dirty(out)
         return out
@@ -685,12 +685,12 @@ class _Forward(torch.autograd.Function):
 
 
 def _recorded(what: str, out, *given):
-    """``out``, tied to what is ``given`` where autograd records: before it is written, as autograd refuses some places (a
+    """``out``, tied to all that is ``given`` where autograd records: before it is written, as autograd refuses some places (a
     leaf's)."""
     if torch.is_grad_enabled():
-        for t in given:
-            if t is not None and t.requires_grad:
-                return _Forward.apply(what, out, t)
+        given = [t for t in given if t is not None and t.requires_grad]
+        if given:
+            return _Forward.apply(what, out, *given)
     return out
 
 

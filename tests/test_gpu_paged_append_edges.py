@@ -149,3 +149,15 @@ def test_infinities_beside_products_past_float32(x, y, want):
     got = cache.append(0, query, query, query, step, cos, sin).float()
     assert (got[1, 0, 3].item(), got[1, 0, 35].item()) == want
     assert got.isinf().sum() == 2 and not got.isnan().any()
+
+
+def test_every_recorded_input_refuses_its_gradient():
+    cache, step = make([5], 2, 64)
+    query, key, value = inputs(5, 4, 2, 64, "f32")
+    cos, sin = tables(8, 32)
+    for t in (query, cos, sin):
+        t.requires_grad_()
+    got = cache.append(0, query, key, value, step, cos, sin)
+    for t in (query, cos, sin):
+        with pytest.raises(RuntimeError, match="no backward pass"):
+            torch.autograd.grad(got.sum(), t, allow_unused=True, retain_graph=True)

@@ -58,3 +58,14 @@ def test_sinks_past_all_scores(dim, heads, old, new, dtype):
             got = cache.attend_rows(0, query, step, sinks=sinks, **made).unflatten(1, (heads, 5))
             want = cache.attend_rows(0, query, step, sinks=mild, **made).unflatten(1, (heads, 5))
             assert not got[:, :, :3].any() and got[:, :, 3].isnan().all() and torch.equal(got[:, :, 4], want[:, :, 4])
+
+
+def test_every_recorded_input_refuses_its_gradient():
+    cache, step = build([50, 9], [2, 3], 2, 64, 16)
+    given = [torch.randn(5, 6, 64, device=DEV), numbers(6, 1), numbers(6, 2).abs()]
+    for t in given:
+        t.requires_grad_()
+    got = cache.attend_rows(0, given[0], step, sinks=given[1], slopes=given[2])
+    for t in given:
+        with pytest.raises(RuntimeError, match="no backward pass"):
+            torch.autograd.grad(got.sum(), t, allow_unused=True, retain_graph=True)
