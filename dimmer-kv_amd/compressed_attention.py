@@ -84,7 +84,11 @@ class CompressedContext:
     - ``CompressedContext(tables, key, value, positions, q_heads, cu_seqlens=None,
       exact_cache=None)`` over packed streams (``prog@``, and ragged batches): ``cu_seqlens``
       (int32 [B+1]) splits the streams into B conversations for a fused varlen decode.
+
+    Scores are scaled products: the hook refuses models that cap them or have sinks.
     """
+
+    takes_shapes = False
 
     def __init__(self, *args, **kwargs):
         from kvtc import KVTCCodec

@@ -4,7 +4,8 @@ scripts/dimmer.py: ``STATE`` :24-35, ``dimmer_attention`` :45-77, ``install`` :8
 
 With ``STATE.compressed`` set (a ``CompressedContext``), every attention call of the model goes to
 ``CompressedContext.attend``, which runs the HIP kernels over the packed codes; this is the
-dispatch the reference makes at scripts/dimmer.py:47-48.  Without it the hook is ordinary eager
+dispatch the reference makes at scripts/dimmer.py:47-48.  A context whose ``takes_shapes`` is false
+attends by plain scores, and calls of a model that caps them or has sinks raise.  Without it the hook is ordinary eager
 attention over the cache the model holds, with the reference's two side duties: hiding evicted
 (layer, KV head, token) slots, and recording the attention each token receives (the H2O sum over
 all queries and the SnapKV sum over the last ``window`` queries) while ``STATE.scoring`` is on.
@@ -45,13 +46,16 @@ def _per_kv_head(received: torch.Tensor, groups: int) -> torch.Tensor:
 def dimmer_attention(module, query, key, value, attention_mask, scaling, dropout=0.0, **kwargs):
     """HF attention function: ``query`` [B, q_heads, q, D], ``key``/``value`` [B, kv_heads, k, D];
     returns (output [B, q, q_heads, D], None) (scripts/dimmer.py:45-77)."""
+    cap, sinks = kwargs.get("softcap"), kwargs.get("s_aux")  # of models that have them
     if STATE.compressed is not None:
+        if not getattr(STATE.compressed, "takes_shapes", True) and (cap is not None or sinks is not None):
+            raise ValueError(f"{type(STATE.compressed).__name__}: the model's attention has "
+                             f"{'a soft cap on its scores' if cap is not None else 'sinks beside its keys'}, and the context's has not")
         return STATE.compressed.attend(module, query, key, value, attention_mask, scaling)
     groups = module.num_key_value_groups
     # query head h reads KV head h // groups; the key operand is made contiguous before the product
     keys_t = key.repeat_interleave(groups, dim=1).transpose(-1, -2).contiguous()
     logits = torch.matmul(query, keys_t).mul_(scaling)
-    cap, sinks = kwargs.get("softcap"), kwargs.get("s_aux")  # of models that have them
     if cap is not None:
         logits = torch.tanh(logits / cap) * cap
     if attention_mask is not None:

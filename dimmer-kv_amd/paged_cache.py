@@ -238,6 +238,7 @@ class PagedContext:
         """Per-layer [1, kv_heads, tokens, head_dim] keys (RoPE applied) and values on the GPU, with room for ``room`` more
         tokens.  ``shaped``: attention takes the soft cap of the model's configuration and its layers' sinks as they are now;
         without it a model that has either is refused."""
+        self.takes_shapes = shaped
         first = keys[0]
         shape = first.shape
         if len(keys) != len(values) or len(shape) != 4 or shape[0] != 1:

@@ -6,6 +6,61 @@ import pytest
 import torch
 
 import dkv_hip
+from test_paged_shaped_checks import small_model
+
+
+class Plain:
+    """A context that says what scores it takes, and counts its calls."""
+
+    def __init__(self, takes_shapes=None):
+        self.calls = 0
+        if takes_shapes is not None:
+            self.takes_shapes = takes_shapes
+
+    def attend(self, module, query, key, value, attention_mask, scaling):
+        self.calls += 1
+        return torch.zeros_like(query).transpose(1, 2), None
+
+
+@pytest.mark.parametrize("family,words", [("Gemma2", "soft cap"), ("GptOss", "sinks")])
+def test_contexts_of_plain_scores_refuse_others(family, words):
+    """A context that attends by plain scores raises for a model whose scores are more, rather than answer by another formula;
+    one that takes them, or does not say, is called."""
+    import dimmer
+    from compressed_attention import CompressedContext
+
+    assert not CompressedContext.takes_shapes
+    model = small_model(family)
+    dimmer.install(model)
+    ids = torch.randint(0, 50, (1, 7), generator=torch.Generator().manual_seed(1))
+    for takes, refused in ((False, True), (True, False), (None, False)):
+        context = Plain(takes)
+        dimmer.STATE.compressed = context
+        try:
+            with torch.no_grad():
+                if refused:
+                    with pytest.raises(ValueError, match=words):
+                        model(input_ids=ids)
+                else:
+                    model(input_ids=ids)
+        finally:
+            dimmer.STATE.compressed = None
+        assert context.calls == (0 if refused else 2)
+
+
+def test_a_plain_model_is_taken():
+    """Models that hand the hook no cap and no sinks, or None for them, are served as before."""
+    import dimmer
+
+    context = Plain(False)
+    module = torch.nn.Module()
+    dimmer.STATE.compressed = context
+    try:
+        for more in ({}, dict(softcap=None), dict(s_aux=None, sliding_window=5)):
+            dimmer.dimmer_attention(module, torch.zeros(1, 2, 3, 8), torch.zeros(1, 2, 3, 8), torch.zeros(1, 2, 3, 8), None, 1.0, **more)
+    finally:
+        dimmer.STATE.compressed = None
+    assert context.calls == 3
 
 
 def test_every_recorded_input_refuses_its_gradient():
