@@ -703,7 +703,7 @@ def _query_meets(query, args, out) -> bool:
     token, head, end = args.query_token * size, args.query_head * size, to + out.numel() * size
     if at >= end or at + (rows - 1) * token + (heads - 1) * head + dim * size <= to:
         return False
-    start = at + (torch.arange(rows).unsqueeze(1) * token + torch.arange(heads) * head)
+    start = at + (torch.arange(rows, device="cpu").unsqueeze(1) * token + torch.arange(heads, device="cpu") * head)
     return bool(((start < end) & (start + dim * size > to)).any())
 
 
@@ -721,7 +721,9 @@ def _rows_meet_rows(a, b) -> bool:
         ahead = (b_at - a_at) // size % a_row
         if a_span <= ahead and ahead + b_span <= a_row:
             return False
-    starts = [at + size * (torch.arange(t.shape[0]).unsqueeze(1) * row + torch.arange(t.shape[1]) * head).flatten()
+    # (on the host whatever the default device is: an answer of the GPU's would have to be waited for)
+    starts = [at + size * (torch.arange(t.shape[0], device="cpu").unsqueeze(1) * row
+                           + torch.arange(t.shape[1], device="cpu") * head).flatten()
               for t, (at, row, head, _, _) in zip((a, b), spans)]
     mine = starts[0].sort().values
     width = a.shape[2] * size
@@ -888,7 +890,7 @@ def _rows_meet(a: int, a_row: int, b: int, b_row: int, rows: int, width: int) ->
     than row for row in place.  Each side's rows lie in order and apart."""
     if (a == b and a_row == b_row) or a + (rows - 1) * a_row + width <= b or b + (rows - 1) * b_row + width <= a:
         return False
-    start = b + torch.arange(rows) * b_row
+    start = b + torch.arange(rows, device="cpu") * b_row
     below = torch.div(start - a, a_row, rounding_mode="floor")
     for row in (below, below + 1):  # the rows of a that begin next to start
         at = a + row.clamp(0, rows - 1) * a_row

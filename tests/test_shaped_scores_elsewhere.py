@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import dkv_hip
-from test_paged_shaped_checks import small_model
+from test_paged_shaped_checks import rows_of, small_model
 
 
 class Plain:
@@ -72,3 +72,19 @@ def test_every_recorded_input_refuses_its_gradient():
     assert dkv_hip._recorded("this", plain, plain, None) is plain
     with torch.no_grad():
         assert not dkv_hip._recorded("this", torch.ones(3), first).requires_grad
+
+
+def test_places_are_compared_on_the_host():
+    """Whatever torch's default device is: a GPU's answer would have to be waited for, which a captured call may not."""
+    storage = torch.zeros(4000)
+    a, b = (rows_of(storage, at, 5, 3, 8, 40, 80) for at in (0, 16))
+    args = dkv_hip.Fp4AttendArgs()
+    args.query, args.query_token, args.query_head = b.data_ptr(), 40, 80
+    out = rows_of(storage, 100, 5, 3, 8, 24, 8)
+
+    def answers():
+        return dkv_hip._rows_meet_rows(a, b), dkv_hip._query_meets(b, args, out), dkv_hip._rows_meet(0, 40, 16, 56, 5, 24)
+
+    want = answers()
+    with torch.device("meta"):
+        assert answers() == want
