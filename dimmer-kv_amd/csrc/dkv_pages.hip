@@ -521,6 +521,7 @@ __global__ __launch_bounds__(256, 4) void fp4_append_kernel(AppendArgs a) {
     }
     if constexpr (LAYOUT == kHalves) {
       if (turns) load8<T>(row + (low ? first + half : first - half), other);
+      __builtin_amdgcn_wave_barrier();  // a row is one wave's: in place, no lane writes before its partner has read
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) turn.x[i] = x[i], turn.y[i] = LAYOUT == kPairs ? (turns ? x[i ^ 1] : 0.0f) : other[i];
