@@ -151,6 +151,23 @@ def test_infinities_beside_products_past_float32(x, y, want):
     assert got.isinf().sum() == 2 and not got.isnan().any()
 
 
+def test_layers_beside_the_one_that_is_written():
+    """Appends to a layer leave the codes and exponents of the others as they are, whatever they held."""
+    cache, step = make([300, 41], 4, 64, page=64, layers=3)
+    query, key, value = inputs(step.rows, 8, 4, 64, "f16")
+    cos, sin = tables(300, 32)
+    names = ("key_codes", "key_scales", "value_codes", "value_scales")
+    for name in names:
+        t = getattr(cache, name)
+        t.copy_(torch.randint(0, 255, t.shape, dtype=torch.uint8, generator=torch.Generator().manual_seed(1)))
+    before = {name: getattr(cache, name).clone() for name in names}
+    cache.append(1, query, key, value, step, cos, sin)
+    for name in names:
+        held = getattr(cache, name)
+        assert torch.equal(held[0], before[name][0]) and torch.equal(held[2], before[name][2])
+        assert not torch.equal(held[1], before[name][1])
+
+
 def test_every_recorded_input_refuses_its_gradient():
     cache, step = make([5], 2, 64)
     query, key, value = inputs(5, 4, 2, 64, "f32")
