@@ -293,7 +293,7 @@ class PagedContext:
             layer = getattr(module, "layer_idx", None)
             if layer is None or not 0 <= layer < layers:
                 raise ValueError(f"PagedContext: sinks of layer {layer}, where the caches have {layers}")
-            shapes[layer]["sinks"] = module.sinks.detach().to(device, torch.float32).contiguous()
+            shapes[layer]["sinks"] = module.sinks.detach().to(device, torch.float32, copy=True).contiguous()
         return shapes
 
     def fresh_cache(self):

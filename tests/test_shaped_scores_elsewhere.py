@@ -63,6 +63,19 @@ def test_a_plain_model_is_taken():
     assert context.calls == 3
 
 
+def test_a_context_keeps_the_sinks_it_was_made_with():
+    """As its documents say: sinks that are changed in place later are not the context's."""
+    from paged_cache import PagedContext
+
+    model = small_model("GptOss")
+    shapes = PagedContext._layer_shapes(model, 2, "cpu")
+    held = [shape["sinks"].clone() for shape in shapes]
+    with torch.no_grad():
+        for layer in model.model.layers:
+            layer.self_attn.sinks.add_(1.0)
+    assert all(torch.equal(shape["sinks"], was) for shape, was in zip(shapes, held))
+
+
 def test_every_recorded_input_refuses_its_gradient():
     first, second, plain = torch.zeros(3, requires_grad=True), torch.zeros(3, requires_grad=True), torch.zeros(3)
     out = dkv_hip._recorded("this", torch.ones(3), first, None, plain, second)
