@@ -284,13 +284,16 @@ __global__ __launch_bounds__(256) void fp4_store_kernel(StoreArgs a) {
 // ---------------------------------------------------------------------------
 // Raw projections into the pages: keys rotated on the way, and the queries rotated beside them.  A rotated key next to the
 // border of two codes must fall on the right side, and float32 sums do not tell: so each sum of 16-bit rows is made in
-// float32 with a bound on its error, and rounded from both ends of that.  Where the two agree (all but one of some 10^4
-// queries and 10^6 keys) the exact sum rounds to the same; where a wave holds one that does not, it makes them all again in
-// float64: products of float32 are exact there, and what the sum loses, and its cut to float32, set the last bit, which keeps
-// it on its side of every border of fewer bits.  Float32 rows go that way at once.
+// float32 with a bound on its error, and rounded from both ends of that.  Where the two agree the exact sum rounds to the same;
+// where a wave's 512 hold one that does not, it makes them all again in float64: products of float32 are exact there, and
+// what the sum loses, and its cut to float32, set the last bit, which keeps it on its side of every border of fewer bits.  Of
+// rotated normal numbers that is one float16 query in 1,300 and one bfloat16 in 9,000 (a third and a twentieth of the
+// waves), and one key in some 10^5 (less than a wave in a thousand).  Dimensions that are not rotated have no bound to fail.
+// Float32 rows are summed in float64 at once.
 // The pass is the memory's: 16,384 rows of 24 + 8 + 8 heads of 128 bfloat16 dimensions (294 MB) 64 us among other passes (4.6
-// TB/s) and 53 where a graph repeats it, against 102 there with float64 for all and a head a thread; 64 rows of 32 + 8 + 8
-// heads of 64 float16 dimensions 4.1 us, which is latency.
+// TB/s) and 57 where a graph repeats it (float16 55, 8,192 float32 rows 60), against 102 there with float64 for all and a head
+// a thread.  With half of the dimensions rotated 77 and 82 (an octet a lane, whose partner is read twice), in neighbouring
+// pairs 66 and 71.  64 rows of 32 + 8 + 8 heads of 64 float16 dimensions 4.5 us, which is latency.
 // A lane takes an octet of dimensions, and the one it is rotated with where all dimensions are in halves, so that nothing
 // is read twice; it keeps its angles for all the heads that it takes.
 // ---------------------------------------------------------------------------
@@ -334,14 +337,14 @@ DKV_DEVICE bool differ(uint4 a, uint4 b) { return ((a.x ^ b.x) | (a.y ^ b.y) | (
 struct Turn {
   float x[8], y[8], c[8], s[8];
   bool stays;  // the octet is not rotated: c is 1 (or NaN), y 0 and s -0, so that sums are x, the sign of a zero too
-  // The sums in float32, and by how much they may be off: 2^-24 of the product that is rounded and of the sum, three times that for
-  // the roundings of the bounds that are made with it.
+  // The sums in float32, and by how much their ends r - off and r + off have to lie apart from them: 2^-24 of the product that is
+  // rounded, of the sum, and of the sum once more for the rounding of the end itself; 2^-20 of that more for the roundings in off.
   DKV_DEVICE void sums(float (&r)[8], float (&off)[8]) const {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float product = y[i] * s[i];
       r[i] = fmaf(x[i], c[i], product);
-      off[i] = stays ? 0.0f : fmaf(fabsf(product) + fabsf(r[i]), 0x1.8p-23f, 0x1p-140f);
+      off[i] = stays ? 0.0f : fmaf(fmaf(2.0f, fabsf(r[i]), fabsf(product)), 0x1.00001p-24f, 0x1p-140f);
     }
   }
   // What a sum in float64 lacks of its two products, which are exact there.
