@@ -24,7 +24,7 @@
 // Shaped scores go through the same kernels: a product z becomes cap tanh(z / cap), less slope |p - t|, where its tile lies in
 // registers, a row's range of tokens takes the place of "up to its own position", and the sink's e^s joins the sum of a row
 // where its result is made.  The tanh costs four instructions a score (two of them at half rate) beside the softmax's six, and
-// vector issue is what bounds prompts: 2,048 query tokens of 24 heads over 16K tokens 527 us with a cap, 403 with sinks alone.
+// vector issue is what bounds prompts: 2,048 query tokens of 24 heads over 16K tokens 526 us with a cap (float16 701), 400 with sinks alone.
 // One token over 2K-32K tokens of 32 requests takes 140 us with a cap (4.2 TB/s).
 #include <math.h>
 
@@ -1184,6 +1184,7 @@ Plan plan_of(const dkv_fp4_attend_args_t& p, const dkv_fp4_shape_t* shape = null
   // tokens 553, 514 and 542; 2,048 tokens (1,024 blocks) 768 at the most 34, 25 and 36, all 50, 47 and 77.  By four waves
   // and one, 16,384 tokens of 128 bfloat16 dimensions (8,192 blocks) 768 at the most 309 and 186, all 2,075 and 1,956.  Few
   // blocks that see much stay with four: 4,096 tokens of 24 heads after 12,288 (1,536 blocks) 647 us, by two waves 837.
+  // (Measured on single requests; of several `each` counts as many blocks as the largest has.)
   if (shape && plan.tiles == 4) {
     if (each >= 8192 || (longest <= 1024 && !shape->first && each >= 2048)) plan.waves = 1;
     else if (shape->first && each >= (longest <= 8192 ? 1024 : 4096)) plan.waves = 2;
